@@ -125,6 +125,34 @@ int infer_hip_gemm_w8a16(const int8_t* weight, const uint16_t* scales,
                          const uint16_t* input, uint16_t* output, int tokens,
                          int out_features, int in_features, hipStream_t stream);
 
+/* ---- 4-bit weights (W4A16) -----------------------------------------------
+ * No reference counterpart (its formats are int8 and BF16): the decode
+ * Linear on weights of half the int8 bytes, for one token or a few.
+ *   Y[t,n] = bf16(sum_g s[n,g] (sum_{k in group g} q[n,k] X[t,k]) + bias[n])
+ * with q in [-8, 7], group_size 32, 64 or 128 dividing in_features, BF16
+ * scales, FP32 sums and 1 to 16 tokens ([tokens, in_features] in,
+ * [tokens, out_features] out).  weight, scales and input are 16-byte
+ * aligned.
+ *
+ * The weights are laid out once, in tiles of 16 rows by 128 columns that a
+ * wave reads as one contiguous KiB: weight holds
+ * [ceil(N/16)][ceil(K/128)][4][16][4] dwords, dword (b, r, i) of a tile row
+ * r's columns 32 i + 8 b .. + 7 as q + 8 in nibbles (lowest first) of
+ * columns 0 2 4 6 1 3 5 7; rows and columns past the matrix hold q = 0.
+ * scales are [ceil(N/16)][K / group_size][16], zero past the matrix.
+ * infer_hip_w4a16_pack makes both from row-major q [N][K] (one int8 each)
+ * and BF16 scales [N][K / group_size], in host memory and without a GPU, into
+ * infer_hip_w4a16_weight_bytes bytes and infer_hip_w4a16_scale_count words
+ * (both 0 for shapes that are not supported). */
+size_t infer_hip_w4a16_weight_bytes(int out_features, int in_features);
+size_t infer_hip_w4a16_scale_count(int out_features, int in_features, int group_size);
+int infer_hip_w4a16_pack(const int8_t* values, const uint16_t* scales, int group_size,
+                         int out_features, int in_features, uint8_t* packed_weight,
+                         uint16_t* packed_scales);
+int infer_hip_gemv_w4a16(const uint8_t* weight, const uint16_t* scales, int group_size,
+                         const uint16_t* bias, const uint16_t* input, uint16_t* output,
+                         int tokens, int out_features, int in_features, hipStream_t stream);
+
 /* ---- Explicit MFMA tile selection --------------------------------------
  * No reference counterpart (the reference picks its WMMA tile from M and N
  * divisibility, src/cuda/kernels.cu:1606-1622, 1665-1681).  The same

@@ -36,6 +36,10 @@ EXPORTED_SYMBOLS = (
     "infer_hip_lm_head_workspace_entries",
     "infer_hip_gemv_w8a16",
     "infer_hip_gemm_w8a16",
+    "infer_hip_w4a16_weight_bytes",
+    "infer_hip_w4a16_scale_count",
+    "infer_hip_w4a16_pack",
+    "infer_hip_gemv_w4a16",
     "infer_hip_gemm_tile_count",
     "infer_hip_gemm_w8a16_tile",
     "infer_hip_gemm_bf16_tile",
@@ -136,6 +140,8 @@ def load() -> ctypes.CDLL:
         "infer_hip_lm_head_bf16_noalloc": [p, p, p, p, p, i, i, p],
         "infer_hip_gemv_w8a16": [p, p, i, p, p, p, i, i, p],
         "infer_hip_gemm_w8a16": [p, p, i, p, p, p, i, i, i, p],
+        "infer_hip_gemv_w4a16": [p, p, i, p, p, p, i, i, i, p],
+        "infer_hip_w4a16_pack": [p, p, i, i, i, p, p],
         "infer_hip_gemm_w8a16_tile": [p, p, i, p, p, p, i, i, i, i, p],
         "infer_hip_gemm_bf16_tile": [p, p, p, p, i, i, i, i, p],
         "infer_hip_gemm_w8a16_ws": [p, p, i, p, p, p, i, i, i, p, ctypes.c_size_t, p],
@@ -145,6 +151,10 @@ def load() -> ctypes.CDLL:
         fn = getattr(lib, name)
         fn.argtypes = args
         fn.restype = i
+    lib.infer_hip_w4a16_weight_bytes.argtypes = [i, i]
+    lib.infer_hip_w4a16_weight_bytes.restype = ctypes.c_size_t
+    lib.infer_hip_w4a16_scale_count.argtypes = [i, i, i]
+    lib.infer_hip_w4a16_scale_count.restype = ctypes.c_size_t
     lib.infer_hip_gemm_tile_count.argtypes = []
     lib.infer_hip_gemm_tile_count.restype = i
     lib.infer_hip_gemm_workspace_bytes.argtypes = [i, i, i]
@@ -254,6 +264,58 @@ def gemm_w8a16(weight, scales, group_size, bias, input, output, tokens,
                                        _ptr(bias), _ptr(input), _ptr(output),
                                        tokens, out_features, in_features,
                                        _stream(stream)))
+
+
+def quantize_w4a16(weight, group_size: int = 64):
+    """FP32 weights [N, K] (numpy) -> (int8 values in [-7, 7], BF16 scale words
+    [N, K / group_size]) as the W8A16 exporter quantises: s = max|w| / 7 of a
+    row's group in FP32 (0 -> 1), values rint(w / s), s stored as BF16."""
+    import numpy as np
+
+    import synthetic
+    w = np.ascontiguousarray(weight, dtype=np.float32)
+    if w.ndim != 2 or group_size not in (32, 64, 128) or w.shape[1] % group_size or not w.size:
+        raise InferError(INVALID_ARGUMENT,
+                         f"quantize_w4a16: {w.shape} in groups of {group_size} (32, 64 or 128, "
+                         "dividing K)")
+    if not np.isfinite(w).all():
+        raise InferError(INVALID_ARGUMENT, "quantize_w4a16: weights must be finite")
+    blocks = w.reshape(w.shape[0], -1, group_size)
+    s = (np.abs(blocks).max(axis=2) / np.float32(7)).astype(np.float32)
+    s = np.where(s == 0, np.float32(1), s)
+    q = np.clip(np.rint(blocks / s[:, :, None]), -7, 7).astype(np.int8).reshape(w.shape)
+    return q, synthetic.float32_to_bf16_bits(s)
+
+
+def pack_w4a16(values, scales, group_size: int):
+    """Row-major int8 values in [-8, 7] [N, K] and BF16 scale words
+    [N, K / group_size] (numpy) -> the packed (weight bytes, scale words) that
+    gemv_w4a16 takes (infer_hip_w4a16_pack; host only)."""
+    import numpy as np
+    values = np.ascontiguousarray(values)
+    scales = np.ascontiguousarray(scales)
+    if values.dtype != np.int8 or values.ndim != 2 or scales.dtype != np.uint16:
+        raise InferError(INVALID_ARGUMENT, "pack_w4a16: int8 values [N, K] and uint16 scale words")
+    n, k = values.shape
+    lib = load()
+    count = lib.infer_hip_w4a16_scale_count(n, k, group_size)
+    if count == 0 or scales.shape != (n, k // group_size):
+        raise InferError(INVALID_ARGUMENT,
+                         f"pack_w4a16: values {values.shape}, scales {scales.shape}, group "
+                         f"{group_size} (32, 64 or 128, dividing K)")
+    packed = np.empty(lib.infer_hip_w4a16_weight_bytes(n, k), np.uint8)
+    tiled = np.empty(count, np.uint16)
+    _check(lib.infer_hip_w4a16_pack(values.ctypes.data, scales.ctypes.data, group_size, n, k,
+                                    packed.ctypes.data, tiled.ctypes.data))
+    return packed, tiled
+
+
+def gemv_w4a16(weight, scales, group_size, bias, input, output, tokens, out_features,
+               in_features, stream=None):
+    """1 to 16 tokens by packed 4-bit weights (infer_hip_gemv_w4a16)."""
+    _check(load().infer_hip_gemv_w4a16(_ptr(weight), _ptr(scales), group_size, _ptr(bias),
+                                       _ptr(input), _ptr(output), tokens, out_features,
+                                       in_features, _stream(stream)))
 
 
 # MFMA workgroup tiles (rows x columns of Y) of the explicit-tile entries.

@@ -1,0 +1,156 @@
+"""infer_hip_gemv_w4a16 against 64 bits: group sizes, token counts, rows that
+do not fill a tile, columns that do not fill one, values at the ends of their
+range, activations that are huge, infinite or NaN, captured graphs."""
+import math
+
+import pytest
+import torch
+
+import w4_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+
+def make(n, k, group, tokens, seed, bias=False):
+    g = torch.Generator().manual_seed(seed)
+    q = torch.randint(-8, 8, (n, k), generator=g, dtype=torch.int8)
+    s = ((torch.rand((n, k // group), generator=g) + 0.1) * 0.02).to(torch.bfloat16)
+    s[::3] *= -1  # nothing asks scales to be positive
+    x = torch.randn((tokens, k), generator=g).to(torch.bfloat16)
+    b = torch.randn(n, generator=g).to(torch.bfloat16) if bias else None
+    return q, s, x, b
+
+
+def run(hip, dev, q, s, group, b, x, spare=3):
+    n, k = q.shape
+    tokens = x.shape[0]
+    packed, tiled = ref.pack(q, s)
+    out = torch.full((tokens + spare, n), 5.0, dtype=torch.bfloat16, device=dev)
+    hip.gemv_w4a16(packed.to(dev), tiled.to(dev), group, None if b is None else b.to(dev),
+                   x.to(dev), out, tokens, n, k)
+    got = out.cpu()
+    assert (got[tokens:] == 5).all()
+    return got[:tokens]
+
+
+def check(got, y, bound):
+    err = (got.double() - y).abs()
+    assert (err <= y.abs() * 2.0 ** -8 + bound * (1 + 2.0 ** -8)).all(), float(err.max())
+
+
+@pytest.mark.parametrize("n,k,group", [
+    (1, 32, 32), (15, 32, 32), (16, 64, 64), (17, 96, 32), (33, 128, 128), (100, 192, 64),
+    (257, 160, 32), (896, 896, 64), (896, 896, 128), (130, 4864, 64), (896, 4864, 128),
+    (70, 8960, 32), (1000, 1088, 64), (4864, 896, 32), (5000, 1536, 128), (513, 9088, 64),
+    (20, 33 * 128, 128), (48, 20480, 64)])
+@pytest.mark.parametrize("tokens", [1, 2, 5, 16])
+def test_product(hip, dev, n, k, group, tokens):
+    q, s, x, b = make(n, k, group, tokens, n + k + tokens, bias=tokens % 2 == 1)
+    check(run(hip, dev, q, s, group, b, x), *ref.product(q, s, group, b, x))
+
+
+@pytest.mark.parametrize("tokens", list(range(1, 17)))
+def test_every_token_count(hip, dev, tokens):
+    q, s, x, b = make(50, 384, 64, tokens, tokens, bias=True)
+    check(run(hip, dev, q, s, 64, b, x), *ref.product(q, s, 64, b, x))
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_many_rows(hip, dev, group):
+    """As many rows as a vocabulary, not a multiple of anything."""
+    q, s, x, b = make(151931, 256, group, 3, group)
+    check(run(hip, dev, q, s, group, b, x), *ref.product(q, s, group, b, x))
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_every_value_at_every_column(hip, dev, group):
+    """One-hot activations read single weights back: exact."""
+    n, k = 40, 256
+    q = ((torch.arange(n)[:, None] * 5 + torch.arange(k)[None] * 3) % 16 - 8).to(torch.int8)
+    s = torch.exp2(torch.arange(n * (k // group)).view(n, -1) % 7 - 3.0).to(torch.bfloat16)
+    want = q.double() * s.double().repeat_interleave(group, dim=1)
+    for at in range(0, k, 16):
+        x = torch.zeros((16, k), dtype=torch.bfloat16)
+        x[torch.arange(16), at + torch.arange(16)] = 1
+        got = run(hip, dev, q, s, group, None, x)
+        assert torch.equal(got.double(), want[:, at:at + 16].t())
+
+
+@pytest.mark.parametrize("value", [-8, 7, 0])
+def test_constant_weights(hip, dev, value):
+    q = torch.full((37, 512), value, dtype=torch.int8)
+    _, s, x, _ = make(37, 512, 64, 4, 1)
+    check(run(hip, dev, q, s, 64, None, x), *ref.product(q, s, 64, None, x))
+
+
+@pytest.mark.parametrize("special", [math.inf, -math.inf, math.nan, 3.0e38, -3.3e38])
+@pytest.mark.parametrize("tokens", [1, 3])
+def test_activations_at_the_ends_of_their_range(hip, dev, special, tokens):
+    """The last token holds one such value: as the sum's definition in FP32
+    says, and the other tokens are not touched."""
+    q, s, x, b = make(50, 1024, 64, tokens, 8, bias=True)
+    q[:20, 700] = torch.arange(20, dtype=torch.int8) % 16 - 8
+    x[-1, 700] = special
+    got = run(hip, dev, q, s, 64, b, x).double()
+    if tokens > 1:
+        y, bound = ref.product(q, s, 64, b, x[:-1])
+        check(got[:-1], y, bound)
+    w = q[:, 700].double() * s[:, 700 // 64].double()
+    if math.isfinite(special):
+        y = ref.product(q, s, 64, b, x)[0][-1]
+        # sums of exact products: the large one's rounding is 2^-24 of it
+        tol = y.abs() * 2.0 ** -8 + abs(special) * w.abs() * 2.0 ** -20 + 1.0
+        assert ((got[-1] - y).abs() <= tol).all()
+        return
+    want = special * w  # 0 x inf is NaN
+    assert torch.equal(got[-1].isnan(), want.isnan())
+    assert torch.equal(got[-1][~want.isnan()], want[~want.isnan()])
+
+
+@pytest.mark.parametrize("tokens", [1, 8])
+def test_quantised_weights(hip, dev, tokens):
+    """FP32 weights through the quantiser and the packer to the product, within
+    the quantiser's half step of the FP32 product."""
+    import numpy as np
+    g = torch.Generator().manual_seed(5)
+    w = torch.randn((300, 896), generator=g) * 0.02
+    x = torch.randn((tokens, 896), generator=g).to(torch.bfloat16)
+    for group in (32, 64, 128):
+        q, s = hip.quantize_w4a16(w.numpy(), group)
+        packed, tiled = hip.pack_w4a16(q, s, group)
+        out = torch.empty((tokens, 300), dtype=torch.bfloat16, device=dev)
+        hip.gemv_w4a16(torch.from_numpy(packed).to(dev),
+                       torch.from_numpy(tiled.view(np.int16)).view(torch.bfloat16).to(dev), group,
+                       None, x.to(dev), out, tokens, 300, 896)
+        sb = torch.from_numpy(s.view(np.int16)).view(torch.bfloat16)
+        y, bound = ref.product(torch.from_numpy(q), sb, group, None, x)
+        check(out.cpu(), y, bound)
+        # a weight is off by half a step (s / 2) and its scale's rounding (7 s 2^-8)
+        step = sb.double().repeat_interleave(group, dim=1) * (0.5 + 7 * 2.0 ** -8) * (1 + 2.0 ** -7)
+        far = (y - x.double() @ w.double().t()).abs()
+        assert (far <= x.double().abs() @ step.t()).all()
+
+
+def test_captured(hip, dev):
+    q, s, x, b = make(896, 4864, 64, 4, 3, bias=True)
+    packed, tiled = (t.to(dev) for t in ref.pack(q, s))
+    dx, db = x.to(dev), b.to(dev)
+    out = torch.zeros((4, 896), dtype=torch.bfloat16, device=dev)
+    graph = torch.cuda.CUDAGraph()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        hip.gemv_w4a16(packed, tiled, 64, db, dx, out, 4, 896, 4864)
+    torch.cuda.current_stream().wait_stream(side)
+    with torch.cuda.graph(graph):
+        hip.gemv_w4a16(packed, tiled, 64, db, dx, out, 4, 896, 4864)
+    for seed in range(3):
+        x = torch.randn((4, 4864), generator=torch.Generator().manual_seed(seed)).to(torch.bfloat16)
+        dx.copy_(x)
+        out.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        check(out.cpu(), *ref.product(q, s, 64, b, x))
+        eager = torch.empty_like(out)
+        hip.gemv_w4a16(packed, tiled, 64, db, dx, eager, 4, 896, 4864)
+        assert torch.equal(out.view(torch.int16), eager.view(torch.int16))
