@@ -123,10 +123,10 @@ int infer_hip_kv_pages_load(const infer_hip_kv_pages* pages, const infer_hip_kv_
  *
  * The work of all sequences is cut into equal parts over the chip on the
  * device, from the lengths, and the parts of a head joined in a fixed order:
- * results do not change from run to run.  workspace: device memory of
- * infer_hip_attention_paged_decode_workspace_bytes, 16-byte aligned, zeroed once
- * before its first use (every call leaves it ready for the next); calls that
- * share one must not overlap. */
+ * results do not change from run to run.  lengths must not change while the
+ * call runs.  workspace: device memory of
+ * infer_hip_attention_paged_decode_workspace_bytes, 16-byte aligned, holding
+ * nothing between calls; calls that share one must not overlap. */
 size_t infer_hip_attention_paged_decode_workspace_bytes(int num_sequences, int num_heads,
                                                         int num_kv_heads, int head_dim);
 int infer_hip_attention_paged_decode(const infer_hip_kv_pages* pages,

@@ -203,77 +203,687 @@ __global__ __launch_bounds__(kThreads) void kv_load_kernel(KvLoadArgs a) {
 }
 
 // -------------------------------------------------------------- attention --
+//
+// out[s][h] = sum_j p_j v_j / sum_j p_j, p_j = 2^(log2(e) q.k_j / sqrt(d) - m).
+//
+// Work.  A unit is a (sequence, KV head, block of at most 16 query heads) and
+// has ceil(length / 32) tiles of 32 keys.  All tiles of a call, in the order
+// (sequence, unit, tile), are cut into equal pieces, one a workgroup, from the
+// lengths on the device: the load is even whatever the lengths, and a graph
+// captured once follows them.  A workgroup's waves cut its piece again; each
+// walks its tiles alone, without barriers.  A unit that ends inside one wave is
+// written by it, one inside a workgroup is joined there through LDS, and one
+// over several by a second launch, in the order of its tiles.  (Joined inside
+// the launch by the last workgroup to arrive, in two levels of 16, 131001 keys
+// of two KV heads took 42 us against 35: coherent stores, an atomic and the loads
+// of what other XCDs wrote cost 4 us a level under load.)  Where the tables
+// leave room for short sequences only, the cuts move to the units' ends
+// instead and the second launch is left out.
+//
+// Tile.  S = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_bf16.  With lane =
+// 16 g + r: S's lanes hold head r's scores of keys 4 g .. + 3 of the tile's two
+// halves of 16, which is the layout P^T is read in if the contraction over keys
+// runs in that order, so P never moves between lanes; V^T's lanes read their
+// eight keys' dimensions r D / 16 .. and pair them up in registers.  Keys and
+// values go from memory to registers once, the next tile's while this one is
+// multiplied.  8-bit elements become BF16 exactly; their scales go onto the
+// scores and the weights.  A weight is the sum of two BF16 numbers (2^-17 of it
+// is lost): one alone rounds as coarsely as the output and made the error
+// 1.35 times the output rounding's own; maxima, sums and O are FP32.
 
-// The plain form of the kernel: a workgroup per (query head, sequence), each
-// wave every fourth key with its own running maximum and sum (a lane holds
-// D / 64 dimensions), the four states joined through LDS.
-template <int F, int D>
-__global__ __launch_bounds__(kThreads) void paged_attention_kernel(PagedAttnArgs a) {
-  constexpr int N = D / 64;
-  const int head = blockIdx.x, seq = blockIdx.y;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int g = head / (a.heads / a.pool.kv_heads);
-  const int n = min(a.lengths[seq], a.table.max_pages << a.pool.page_shift);
-  const uint16_t* qp = a.q + seq * a.q_stride + static_cast<size_t>(head) * D + N * lane;
-  float q[N], acc[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    q[i] = bf16_to_f32(qp[i]) * (1.0f / sqrtf(static_cast<float>(D)));
-    acc[i] = 0.0f;
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+
+constexpr int kTileKeys = 32;
+constexpr int kHeadBlock = 16;       // query heads of a unit at most
+constexpr int kJoinThreads = 512;    // of the join, and the parts a thread has in flight
+constexpr int kJoinBatch = 8;
+constexpr float kRescaleSlack = 6.0f;  // p <= 2^6 before the maximum is moved
+
+// A uniform 32-bit word that nothing writes while the kernel runs, through the
+// scalar cache.
+__device__ __forceinline__ int scalar_word(const int* p) {
+  return *(const __attribute__((address_space(4))) int*)(reinterpret_cast<uintptr_t>(p));
+}
+
+template <int N>
+struct Words;
+template <>
+struct Words<4> {
+  uint32_t w[1];
+  __device__ __forceinline__ void load(const uint8_t* p) { w[0] = gload(reinterpret_cast<const uint32_t*>(p)); }
+};
+template <>
+struct Words<8> {
+  uint32_t w[2];
+  __device__ __forceinline__ void load(const uint8_t* p) {
+    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+    const u32x2 v = gload(reinterpret_cast<const u32x2*>(p));
+    w[0] = v.x;
+    w[1] = v.y;
   }
-  float m = -FLT_MAX, l = 0.0f;
-  for (int p = wave; p < n; p += kThreads / kWave) {
-    const int page =
-        a.table.pages[static_cast<size_t>(seq) * a.table.stride + (p >> a.pool.page_shift)];
-    if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.pool.num_pages)) {
-      l = __uint_as_float(0x7FC00000u);
-      break;
-    }
-    const size_t at = pool_row(a.pool, page, g, p & ((1 << a.pool.page_shift) - 1));
-    float k[N], v[N];
+};
+template <>
+struct Words<16> {
+  uint32_t w[4];
+  __device__ __forceinline__ void load(const uint8_t* p) {
+    const uint4 v = load_global16(p);
+    w[0] = v.x;
+    w[1] = v.y;
+    w[2] = v.z;
+    w[3] = v.w;
+  }
+};
+
+// Low (high) halves of two dwords: a's in bits 0-15.
+__device__ __forceinline__ uint32_t low_halves(uint32_t a, uint32_t b) {
+  return __builtin_amdgcn_perm(b, a, 0x05040100u);
+}
+__device__ __forceinline__ uint32_t high_halves(uint32_t a, uint32_t b) {
+  return __builtin_amdgcn_perm(b, a, 0x07060302u);
+}
+
+// Byte b of w, an int8, as the FP32 whose high half is its BF16.
+template <int B>
+__device__ __forceinline__ uint32_t int8_f32(uint32_t w) {
+  return __float_as_uint(B == 0 ? sbyte0(w) : B == 1 ? sbyte1(w) : B == 2 ? sbyte2(w) : sbyte3(w));
+}
+
+// Two FP8 of a dword (its low or high half) as a BF16 pair.
+template <bool HIGH>
+__device__ __forceinline__ uint32_t fp8_pair(uint32_t w) {
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, HIGH));
+}
+
+// Eight 8-bit elements in order as BF16.
+template <int F>
+__device__ __forceinline__ bf16x8_t widen8(uint32_t lo, uint32_t hi) {
+  uint4 r;
+  if (F == kInt8) {
+    r.x = high_halves(int8_f32<0>(lo), int8_f32<1>(lo));
+    r.y = high_halves(int8_f32<2>(lo), int8_f32<3>(lo));
+    r.z = high_halves(int8_f32<0>(hi), int8_f32<1>(hi));
+    r.w = high_halves(int8_f32<2>(hi), int8_f32<3>(hi));
+  } else {
+    r.x = fp8_pair<false>(lo);
+    r.y = fp8_pair<true>(lo);
+    r.z = fp8_pair<false>(hi);
+    r.w = fp8_pair<true>(hi);
+  }
+  return __builtin_bit_cast(bf16x8_t, r);
+}
+
+// V^T fragments of a lane: frag[j] = dimension j of eight keys, key e in
+// element e, from the keys' words.
+template <int F, int D, int N>
+__device__ __forceinline__ void turn_values(const Words<N> (&v)[8], bf16x8_t (&frag)[D / 16]) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const size_t e = at * D + N * lane + i;
+  for (int w = 0; w < N / 4; ++w) {
+    uint32_t out[F == kBf16 ? 2 : 4][4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t a = v[2 * e].w[w], b = v[2 * e + 1].w[w];
       if (F == kBf16) {
-        k[i] = bf16_to_f32(static_cast<const uint16_t*>(a.pool.key)[e]);
-        v[i] = bf16_to_f32(static_cast<const uint16_t*>(a.pool.value)[e]);
+        out[0][e] = low_halves(a, b);
+        out[1][e] = high_halves(a, b);
+      } else if (F == kInt8) {
+        out[0][e] = high_halves(int8_f32<0>(a), int8_f32<0>(b));
+        out[1][e] = high_halves(int8_f32<1>(a), int8_f32<1>(b));
+        out[2][e] = high_halves(int8_f32<2>(a), int8_f32<2>(b));
+        out[3][e] = high_halves(int8_f32<3>(a), int8_f32<3>(b));
       } else {
-        float x[8];
-        dequantise8<F>(make_uint2(static_cast<const uint8_t*>(a.pool.key)[e], 0), a.pool.key_scales[at], x);
-        k[i] = x[0];
-        dequantise8<F>(make_uint2(static_cast<const uint8_t*>(a.pool.value)[e], 0), a.pool.value_scales[at], x);
-        v[i] = x[0];
+        const uint32_t al = fp8_pair<false>(a), bl = fp8_pair<false>(b);
+        const uint32_t ah = fp8_pair<true>(a), bh = fp8_pair<true>(b);
+        out[0][e] = low_halves(al, bl);
+        out[1][e] = high_halves(al, bl);
+        out[2][e] = low_halves(ah, bh);
+        out[3][e] = high_halves(ah, bh);
       }
     }
-    float s = 0.0f;
+    constexpr int per = F == kBf16 ? 2 : 4;
 #pragma unroll
-    for (int i = 0; i < N; ++i) s = fmaf(q[i], k[i], s);
-    s = wave_sum(s);
-    const float top = fmaxf(m, s), old = expf(m - top), w = expf(s - top);
-    m = top;
-    l = l * old + w;
-#pragma unroll
-    for (int i = 0; i < N; ++i) acc[i] = acc[i] * old + w * v[i];
+    for (int j = 0; j < per; ++j) {
+      frag[w * per + j] = __builtin_bit_cast(
+          bf16x8_t, make_uint4(out[j][0], out[j][1], out[j][2], out[j][3]));
+    }
   }
-  __shared__ float sm[4], sl[4], sa[4][D];
-  if (lane == 0) {
-    sm[wave] = m;
-    sl[wave] = l;
+}
+
+// Over the four lanes r, 16 + r, 32 + r, 48 + r.
+__device__ __forceinline__ float groups_max(float v) {
+  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v), false, false);
+  v = fmaxf(__int_as_float(a[0]), __int_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
+  return fmaxf(__int_as_float(b[0]), __int_as_float(b[1]));
+}
+__device__ __forceinline__ float groups_sum(float v) {
+  v = swap16_sum(v, v);
+  return swap32_sum(v, v);
+}
+
+// Inclusive prefix sums over the wave.
+__device__ __forceinline__ int wave_scan(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, true);  // row_shr:1, 2, 4, 8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, true);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // row_bcast:15, 31
+  return v + __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+}
+
+// Tiles of the walk a wave takes, of all in `waves` equal parts.
+__device__ __forceinline__ int piece_of(int total, int waves) {
+  return max(1, (total + waves - 1) / waves);
+}
+
+// Four dimensions of the output from O and the sum of the weights (0: no keys).
+__device__ __forceinline__ void store_out(uint16_t* out, f32x4_t o, float sum) {
+  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  store_global8(out, make_uint2(pack2_bf16(o[0] * inv, o[1] * inv),
+                                pack2_bf16(o[2] * inv, o[3] * inv)));
+}
+
+__device__ __forceinline__ int tiles_of(int n) { return (n + kTileKeys - 1) / kTileKeys; }
+
+// One tile of the walk (wave-uniform).
+struct TileAt {
+  int seq, unit;    // unit: KV head * head blocks + head block
+  int kvh, block;
+  int tile, tiles;  // of the unit
+  int n;            // length of the sequence
+};
+
+// A part of a unit that is not whole: which tiles, and where the unit lies in
+// the walk.
+struct PartTag {
+  int first;  // the unit's first tile in the walk
+  int tiles;
+  int seq, unit;
+  int begin, end;  // the part's tiles; end 0: no part
+};
+
+// W waves a workgroup; HB: room for that many query heads of a unit in LDS.
+template <int F, int D, int W, int HB>
+__global__ __launch_bounds__(W * kWave, 2) void paged_attention_kernel(PagedAttnArgs a) {
+  constexpr int ES = F == kBf16 ? 2 : 1;
+  constexpr int RB = D * ES;       // bytes of a row
+  constexpr int KC = RB / 64;      // 16-byte pieces of a key per lane
+  constexpr int VB = RB / 16;      // bytes of a value row per lane
+  constexpr int NQ = D / 32;       // MFMA steps of q.k
+  constexpr int NO = D / 16;       // dimensions of O per lane and register row
+  // the states of parts of units: O [2 W][HB][D], then (maximum, sum)
+  __shared__ __align__(16) float smem[2 * W * HB * (D + 2)];
+  __shared__ PartTag tags[2 * W];
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int r = lane & 15, g = lane >> 4;
+  const int units = a.units, cap = a.table.max_pages << a.pool.page_shift;
+  const int heads_per_kv = a.heads / a.pool.kv_heads;
+  const int hb = min(heads_per_kv, kHeadBlock);  // query heads of a full unit
+  const int mask = (1 << a.pool.page_shift) - 1;
+
+  // ---- the wave's part of the walk.  Lane i: sequence i's tiles, and those of
+  // all up to it (of the first 64 sequences).
+  auto length = [&](int i) {
+    return i < a.table.sequences ? max(0, min(a.lengths[i], cap)) : 0;
+  };
+  const int n_first = length(lane), upto_first = wave_scan(tiles_of(n_first));
+  int total = __builtin_amdgcn_readlane(upto_first, kWave - 1);
+  if (a.table.sequences > kWave) {
+    int more = 0;
+    for (int i = kWave + lane; i < a.table.sequences; i += kWave) more += tiles_of(length(i));
+    total += __builtin_amdgcn_readlane(wave_scan(more), kWave - 1);
   }
+  total *= units;
+  // Where tile x < total of the walk lies.
+  auto locate = [&](int x) {
+    TileAt at{};
+    int n = n_first, upto = upto_first;
+    for (int base = 0, run = 0; base < a.table.sequences; base += kWave) {
+      if (base > 0) {
+        n = length(base + lane);
+        upto = wave_scan(tiles_of(n));
+      }
+      const unsigned long long hit = __ballot((run + upto) * units > x);
+      if (hit) {
+        const int i = __builtin_ctzll(hit);
+        at.seq = base + i;
+        at.n = __builtin_amdgcn_readlane(n, i);
+        at.tiles = tiles_of(at.n);
+        const unsigned rest = x - (run + __builtin_amdgcn_readlane(upto, i) - at.tiles) * units;
+        at.unit = rest / static_cast<unsigned>(at.tiles);
+        at.tile = rest - at.unit * at.tiles;
+        at.kvh = HB == 8 ? at.unit : at.unit / a.head_blocks;
+        at.block = HB == 8 ? 0 : at.unit - at.kvh * a.head_blocks;
+        break;
+      }
+      run += __builtin_amdgcn_readlane(upto, kWave - 1);
+    }
+    return at;
+  };
+  const int piece = piece_of(total, a.waves) * W;
+  int group_start = min(total, static_cast<int>(blockIdx.x) * piece);
+  int group_end = min(total, group_start + piece);
+  if (a.whole) {  // to the nearer end of the unit that a cut is in
+    auto moved = [&](int x) {
+      if (x >= total) return total;
+      const TileAt at = locate(x);
+      return 2 * at.tile <= at.tiles ? x - at.tile : x - at.tile + at.tiles;
+    };
+    group_start = moved(group_start);
+    group_end = moved(group_end);
+  }
+  const int chunk = (group_end - group_start + W - 1) / W;
+  const int start = min(group_end, group_start + wave * chunk);
+  const int end = min(group_end, start + chunk);
+
+  if (lane < 2) tags[2 * wave + lane].end = 0;
+
+  if (start < end) {
+    const TileAt at = locate(start);
+
+    auto advance = [&](TileAt& t) {
+      if (++t.tile < t.tiles) return;
+      t.tile = 0;
+      if (HB == 8 || ++t.block == a.head_blocks) {
+        t.block = 0;
+        ++t.kvh;
+      }
+      if (++t.unit < units) return;
+      t.unit = 0;
+      t.kvh = 0;
+      do {  // a later tile exists, so a later sequence with keys does
+        ++t.seq;
+        t.n = max(0, min(scalar_word(a.lengths + t.seq), cap));
+        t.tiles = tiles_of(t.n);
+      } while (t.tiles == 0 && t.seq + 1 < a.table.sequences);
+    };
+
+    bf16x8_t q[NQ], q_next[NQ];
+    auto load_q = [&](const TileAt& t, bf16x8_t (&to)[NQ]) {
+      const int h = t.kvh * heads_per_kv + min(t.block * kHeadBlock + r, heads_per_kv - 1);
+      const uint16_t* p = a.q + t.seq * a.q_stride + static_cast<size_t>(h) * D;
 #pragma unroll
-  for (int i = 0; i < N; ++i) sa[wave][N * lane + i] = acc[i];
+      for (int m = 0; m < NQ; ++m) {
+        const int dim = F == kBf16 ? 32 * m + 8 * g : 64 * (m >> 1) + 16 * g + 8 * (m & 1);
+        to[m] = __builtin_bit_cast(bf16x8_t, load_global16(p + dim));
+      }
+    };
+
+    // A tile's two halves of 16 keys each lie in one page.  Rows of a half past
+    // the sequence's end are read with it (the page is there) and dropped; a
+    // second half wholly past the end reads the first again.
+    const bool small_pages = a.pool.page_shift == 4;
+    const uint32_t page_rows = static_cast<uint32_t>(a.pool.kv_heads) << a.pool.page_shift;
+    int e0 = 0, e1 = 0;  // page entries of the tile to be loaded next
+    auto look_up = [&](const TileAt& t) {
+      const int* row = a.table.pages + static_cast<size_t>(t.seq) * a.table.stride;
+      e0 = scalar_word(row + (t.tile * kTileKeys >> a.pool.page_shift));
+      if (small_pages) {
+        e1 = scalar_word(row + (t.tile * 2 + (t.tile * kTileKeys + 16 < t.n ? 1 : 0)));
+      }
+    };
+    size_t row[2];  // of the pool, the halves' first keys
+    bool bad;       // a page is not in the pool
+    auto find_rows = [&](const TileAt& t) {
+      const uint32_t pages = a.pool.num_pages;
+      const bool two = t.tile * kTileKeys + 16 < t.n;
+      const uint32_t head_row = static_cast<uint32_t>(t.kvh) << a.pool.page_shift;
+      bad = static_cast<uint32_t>(e0) >= pages;
+      row[0] = static_cast<size_t>(bad ? 0 : e0) * page_rows + head_row + (t.tile * kTileKeys & mask);
+      row[1] = row[0] + (two ? 16 : 0);
+      if (small_pages) {
+        const bool bad1 = static_cast<uint32_t>(e1) >= pages;
+        row[1] = static_cast<size_t>(bad1 ? 0 : e1) * page_rows + head_row;
+        bad = bad || bad1;
+      }
+    };
+
+    uint4 k[2][KC];
+    Words<VB> v[8];
+    f32x4_t ks[2], vs[2];
+    const uint32_t k_off = r * RB + 16 * g, v_off = 4 * g * RB + r * VB;
+    auto load_keys = [&] {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint8_t* base = static_cast<const uint8_t*>(a.pool.key) + row[h] * RB;
+#pragma unroll
+        for (int c = 0; c < KC; ++c) k[h][c] = load_global16(base + k_off + 64 * c);
+        if (F != kBf16) {
+          ks[h] = gload(reinterpret_cast<const f32x4_t*>(a.pool.key_scales + row[h]) + g);
+        }
+      }
+    };
+    auto load_values = [&] {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint8_t* base = static_cast<const uint8_t*>(a.pool.value) + row[h] * RB;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[4 * h + i].load(base + v_off + i * RB);
+        if (F != kBf16) {
+          vs[h] = gload(reinterpret_cast<const f32x4_t*>(a.pool.value_scales + row[h]) + g);
+        }
+      }
+    };
+
+    const float scale = 1.44269504088896340736f / sqrtf(static_cast<float>(D));
+    f32x4_t acc[NO];
+    float m = -FLT_MAX, l = 0.0f;
+#pragma unroll
+    for (int j = 0; j < NO; ++j) acc[j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+
+    TileAt next = at;
+    look_up(next);
+    load_q(next, q);
+    find_rows(next);
+    load_keys();
+    load_values();
+    int begin = at.tile;  // of the part of the current unit
+    bool first_part = true, part_bad = bad;
+    TileAt t = at;
+    if (start + 1 < end) {
+      advance(next);
+      look_up(next);
+    }
+
+    for (int idx = start; idx < end; ++idx) {
+      const bool more = idx + 1 < end;
+      // S of both halves, times the keys' scales
+      float s[8];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        f32x4_t d{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+          if (F == kBf16) {
+            d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, k[h][c]), q[c],
+                                                        d, 0, 0, 0);
+          } else {
+            d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen8<F>(k[h][c].x, k[h][c].y), q[2 * c],
+                                                        d, 0, 0, 0);
+            d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen8<F>(k[h][c].z, k[h][c].w),
+                                                        q[2 * c + 1], d, 0, 0, 0);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[4 * h + i] = F == kBf16 ? d[i] : d[i] * ks[h][i];
+      }
+      const bool unit_ends = more && next.tile == 0;
+      if (more) {
+        find_rows(next);
+        load_keys();
+        if (unit_ends) load_q(next, q_next);
+      }
+      const int keys = t.n - t.tile * kTileKeys;  // that the sequence holds
+      if (keys < kTileKeys) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (16 * (e >> 2) + 4 * g + (e & 3) >= keys) s[e] = -INFINITY;
+        }
+      }
+      float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])),
+                        fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+      top = groups_max(top) * scale;
+      if (__any(top > m + kRescaleSlack)) {
+        const float up = fmaxf(m, top), old = __builtin_amdgcn_exp2f(m - up);
+        m = up;
+        l *= old;
+#pragma unroll
+        for (int j = 0; j < NO; ++j) acc[j] *= old;
+      }
+      float p[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        p[e] = __builtin_amdgcn_exp2f(fmaf(s[e], scale, -m));
+        l += p[e];
+        if (F != kBf16) p[e] *= vs[e >> 2][e & 3];
+      }
+      if (keys < kTileKeys) {  // what is read past the end counts for nothing
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if (16 * (e >> 2) + 4 * g + (e & 3) >= keys) {
+            p[e] = 0.0f;
+#pragma unroll
+            for (int w = 0; w < VB / 4; ++w) v[e].w[w] = 0;
+          }
+        }
+      }
+      const uint4 hi = pack8(p);
+      float rest[8];
+      unpack8(hi, rest);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) rest[e] = p[e] - rest[e];
+      const bf16x8_t p_hi = __builtin_bit_cast(bf16x8_t, hi);
+      const bf16x8_t p_lo = __builtin_bit_cast(bf16x8_t, pack8(rest));
+      bf16x8_t vf[NO];
+      turn_values<F, D, VB>(v, vf);
+#pragma unroll
+      for (int j = 0; j < NO; ++j) {
+        acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[j], p_hi, acc[j], 0, 0, 0);
+      }
+#pragma unroll
+      for (int j = 0; j < NO; ++j) {
+        acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[j], p_lo, acc[j], 0, 0, 0);
+      }
+      if (more) load_values();
+      if (!more || unit_ends) {
+        float sum_l = groups_sum(l);
+        if (part_bad) sum_l = __uint_as_float(0x7FC00000u);
+        const int h = t.block * kHeadBlock + r;
+        if (begin == 0 && t.tile + 1 == t.tiles) {
+          if (h < heads_per_kv) {
+            const float inv = sum_l == 0.0f ? 0.0f : 1.0f / sum_l;
+            uint16_t* out = a.out + (static_cast<size_t>(t.seq) * a.heads + t.kvh * heads_per_kv + h) * D +
+                            4 * g * NO;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t w[NO / 2];
+#pragma unroll
+              for (int j = 0; j < NO / 2; ++j) w[j] = pack2_bf16(acc[2 * j][i] * inv, acc[2 * j + 1][i] * inv);
+              if constexpr (NO == 8) {
+                store_global16(out + i * NO, make_uint4(w[0], w[1], w[2], w[3]));
+              } else {
+                store_global8(out + i * NO, make_uint2(w[0], w[1]));
+              }
+            }
+          }
+        } else {
+          const int slot = 2 * wave + (first_part ? 0 : 1);
+          if (r < hb) {
+            float* rec = smem + (slot * HB + r) * D + 4 * g * NO;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+#pragma unroll
+              for (int j = 0; j < NO; ++j) rec[i * NO + j] = acc[j][i];
+            }
+            if (g == 0) {
+              float* ml = smem + 2 * W * HB * D + (slot * HB + r) * 2;
+              ml[0] = m;
+              ml[1] = sum_l;
+            }
+          }
+          if (lane == 0) {
+            tags[slot] = PartTag{idx - t.tile, t.tiles, t.seq, t.unit, begin, t.tile + 1};
+          }
+        }
+        first_part = false;
+        begin = 0;
+        part_bad = false;
+        m = -FLT_MAX;
+        l = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NO; ++j) acc[j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int i = 0; i < NQ; ++i) q[i] = q_next[i];
+      }
+      if (more) {
+        part_bad = part_bad || bad;
+        t = next;
+        if (idx + 2 < end) {
+          advance(next);
+          look_up(next);
+        }
+      }
+    }
+  }
+
+  // ---- empty sequences
+  if (a.table.sequences > kWave || __ballot(lane < a.table.sequences && n_first == 0)) {
+    for (int s = blockIdx.x; s < a.table.sequences; s += gridDim.x) {
+      if (scalar_word(a.lengths + s) > 0) continue;
+      uint16_t* out = a.out + static_cast<size_t>(s) * a.heads * D;
+      for (int e = threadIdx.x; e < a.heads * (D / 8); e += W * kWave) {
+        store_global16(out + 8 * e, make_uint4(0, 0, 0, 0));
+      }
+    }
+  }
+  if (group_start >= group_end) return;  // the whole workgroup
   __syncthreads();
-  if (threadIdx.x >= D) return;
-  float top = sm[0];
-  for (int w = 1; w < 4; ++w) top = fmaxf(top, sm[w]);
-  float sum = 0.0f, total = 0.0f;
-  for (int w = 0; w < 4; ++w) {
-    const float e = expf(sm[w] - top);
-    sum += e * sa[w][threadIdx.x];
-    total += e * sl[w];
+
+  // ---- the workgroup's parts: neighbours of one unit together
+  const float* ml_at = smem + 2 * W * HB * D;
+  {
+    const PartTag mine = tags[lane & (2 * W - 1)];
+    const uint32_t there = static_cast<uint32_t>(__ballot(lane < 2 * W && mine.end != 0));
+    const uint32_t before = there & ((1u << (lane & 31)) - 1u);
+    const int previous = __shfl(mine.first, before ? 31 - __builtin_clz(before) : 0);
+    const uint32_t starts = static_cast<uint32_t>(__ballot(
+        lane < 2 * W && mine.end != 0 && (before == 0 || previous != mine.first)));
+    const int runs = __builtin_popcount(starts), per_run = hb * (D / 4);
+    for (int x = threadIdx.x; x < runs * per_run; x += W * kWave) {
+      const int run = x / per_run, e = x - run * per_run;
+      uint32_t left = starts;
+      for (int i = 0; i < run; ++i) left &= left - 1;
+      const int i = __builtin_ctz(left);
+      left &= left - 1;
+      const uint32_t in = there & ~((1u << i) - 1u) & (left ? (left & -left) - 1u : ~0u);
+      const int last = 31 - __builtin_clz(in);
+      const PartTag tag = tags[i];
+      const bool whole = tag.begin == 0 && tags[last].end == tag.tiles;
+      const int kvh = HB == 8 ? tag.unit : tag.unit / a.head_blocks;
+      const int block = HB == 8 ? 0 : tag.unit - kvh * a.head_blocks;
+      const int h = e / (D / 4), d = 4 * (e % (D / 4));
+      const int head = block * kHeadBlock + h;
+      if (head >= heads_per_kv) continue;
+      float top = -FLT_MAX, sum_l = 0.0f;
+      for (uint32_t w = in; w; w &= w - 1) {
+        top = fmaxf(top, ml_at[(__builtin_ctz(w) * HB + h) * 2]);
+      }
+      f32x4_t o{0.0f, 0.0f, 0.0f, 0.0f};
+      for (uint32_t w = in; w; w &= w - 1) {
+        const int at = __builtin_ctz(w) * HB + h;
+        const float f = __builtin_amdgcn_exp2f(ml_at[at * 2] - top);
+        sum_l += f * ml_at[at * 2 + 1];
+        o += f * *reinterpret_cast<const f32x4_t*>(smem + at * D + d);
+      }
+      if (whole) {
+        store_out(a.out + (static_cast<size_t>(tag.seq) * a.heads + kvh * heads_per_kv + head) * D + d,
+                  o, sum_l);
+      } else {
+        const int side = tag.begin == 0 ? 1 : 0;  // 1: the unit's first workgroup
+        float* rec = a.records + (static_cast<size_t>(blockIdx.x * 2 + side) * hb + h) * (D + 4);
+        *reinterpret_cast<f32x4_t*>(rec + d) = o;
+        if (d == 0) *reinterpret_cast<f32x4_t*>(rec + D) = f32x4_t{top, sum_l, 0.0f, 0.0f};
+      }
+    }
   }
-  a.out[(static_cast<size_t>(seq) * a.heads + head) * D + threadIdx.x] =
-      f32_to_bf16(total == 0.0f ? 0.0f : sum / total);
+}
+
+// Joins the units that lie over several workgroups of the launch before: one
+// workgroup per (unit, sequence), or (a.join_heads 1) per query head of one.
+template <int D, int W>
+__global__ __launch_bounds__(kJoinThreads) void paged_attention_join_kernel(PagedAttnArgs a) {
+  __shared__ __align__(16) float smem[kJoinThreads * 6];
+  const int lane = threadIdx.x & 63;
+  const int seq = blockIdx.y;
+  const int cap = a.table.max_pages << a.pool.page_shift;
+  const int heads_per_kv = a.heads / a.pool.kv_heads;
+  const int hb = min(heads_per_kv, kHeadBlock);
+  int before = 0, all = 0, tiles = 0;
+  for (int i = lane; i < a.table.sequences; i += kWave) {
+    const int t = tiles_of(max(0, min(a.lengths[i], cap)));
+    all += t;
+    if (i < seq) before += t;
+    if (i == seq) tiles = t;
+  }
+  before = __builtin_amdgcn_readlane(wave_scan(before), kWave - 1);
+  all = __builtin_amdgcn_readlane(wave_scan(all), kWave - 1);
+  tiles = __builtin_amdgcn_readlane(wave_scan(tiles), kWave - 1);
+  const int piece = piece_of(all * a.units, a.waves) * W;
+  const int unit = a.join_heads ? blockIdx.x / hb : blockIdx.x;
+  const int first = before * a.units + unit * tiles;
+  const int from = first / piece, to = (first + tiles - 1) / piece;
+  if (tiles == 0 || from == to) return;
+  const int kvh = unit / a.head_blocks, block = unit - kvh * a.head_blocks;
+  const int h0 = a.join_heads ? blockIdx.x - unit * hb : 0;
+  const int live = min(hb, heads_per_kv - block * kHeadBlock);  // heads of the unit
+  if (h0 >= live) return;
+  const int items = (a.join_heads ? 1 : live) * (D / 4);
+
+  // The threads are as many rows of `items` as fit, row i taking parts i, i +
+  // rows, ...; what the rows found is joined through LDS.
+  const int rows = max(1, kJoinThreads / items), row = rows > 1 ? threadIdx.x / items : 0;
+  for (int e0 = 0; e0 < items; e0 += kJoinThreads) {
+    const int e = rows > 1 ? static_cast<int>(threadIdx.x) - row * items
+                           : e0 + static_cast<int>(threadIdx.x);
+    const bool busy = e < items && row < rows;
+    const int h = h0 + e / (D / 4), d = 4 * (e % (D / 4));
+    float top = -FLT_MAX, sum_l = 0.0f;
+    f32x4_t o{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int part = busy ? from + row : to + 1; part <= to; part += kJoinBatch * rows) {
+      f32x4_t x[kJoinBatch], ml[kJoinBatch];
+#pragma unroll
+      for (int b = 0; b < kJoinBatch; ++b) {
+        const int wg = part + b * rows;
+        x[b] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        ml[b] = f32x4_t{-FLT_MAX, 0.0f, 0.0f, 0.0f};
+        if (wg > to) continue;
+        const float* rec =
+            a.records + (static_cast<size_t>(wg * 2 + (wg == from ? 1 : 0)) * hb + h) * (D + 4);
+        x[b] = gload(reinterpret_cast<const f32x4_t*>(rec + d));
+        ml[b] = gload(reinterpret_cast<const f32x4_t*>(rec + D));
+      }
+      float next = top;
+#pragma unroll
+      for (int b = 0; b < kJoinBatch; ++b) next = fmaxf(next, ml[b][0]);
+      const float old = __builtin_amdgcn_exp2f(top - next);
+      top = next;
+      sum_l *= old;
+      o *= old;
+#pragma unroll
+      for (int b = 0; b < kJoinBatch; ++b) {
+        const float w = __builtin_amdgcn_exp2f(ml[b][0] - next);
+        sum_l += w * ml[b][1];
+        o += w * x[b];
+      }
+    }
+    if (rows > 1) {
+      float* mine = smem + (row * items + e) * 6;
+      if (busy) {
+        mine[0] = o[0];
+        mine[1] = o[1];
+        mine[2] = o[2];
+        mine[3] = o[3];
+        mine[4] = top;
+        mine[5] = sum_l;
+      }
+      __syncthreads();
+      for (int i = 1; i < rows && row == 0; ++i) {
+        const float* other = smem + (i * items + e) * 6;
+        const float next = fmaxf(top, other[4]);
+        const float old = __builtin_amdgcn_exp2f(top - next);
+        const float w = __builtin_amdgcn_exp2f(other[4] - next);
+        top = next;
+        sum_l = sum_l * old + w * other[5];
+        o = o * old + w * f32x4_t{other[0], other[1], other[2], other[3]};
+      }
+    }
+    if (busy && row == 0) {
+      const int head = kvh * heads_per_kv + block * kHeadBlock + h;
+      store_out(a.out + (static_cast<size_t>(seq) * a.heads + head) * D + d, o, sum_l);
+    }
+  }
 }
 
 }  // namespace
@@ -319,13 +929,85 @@ void launch_kv_load(const KvLoadArgs& a, hipStream_t stream) {
   });
 }
 
-size_t paged_attention_workspace_bytes(int, int, int, int) { return 256; }
+// Workgroups of the attention: 8 waves a CU, the registers' limit at head_dim
+// 128, in workgroups of 8 (of 4 where a unit has more than 8 query heads, whose
+// states fill the LDS).
+constexpr int kCus = 256;
+constexpr int kWholeTiles = 32;  // a unit of more is cut
 
-void launch_paged_attention(const PagedAttnArgs& a, hipStream_t stream) {
+struct PagedAttnShape {
+  int head_blocks, units, waves_per_group, groups, record_floats;
+};
+
+static PagedAttnShape paged_attention_shape(int heads, int kv_heads, int head_dim) {
+  PagedAttnShape s{};
+  const int per_kv = heads / kv_heads;
+  s.head_blocks = (per_kv + kHeadBlock - 1) / kHeadBlock;
+  s.units = kv_heads * s.head_blocks;
+  s.waves_per_group = per_kv <= 8 ? 8 : 4;
+  s.groups = 8 / s.waves_per_group * kCus;
+  s.record_floats = (per_kv < kHeadBlock ? per_kv : kHeadBlock) * (head_dim + 4);
+  return s;
+}
+
+size_t paged_attention_workspace_bytes(int, int heads, int kv_heads, int head_dim) {
+  const PagedAttnShape s = paged_attention_shape(heads, kv_heads, head_dim);
+  return static_cast<size_t>(s.groups) * 2 * s.record_floats * sizeof(float);
+}
+
+// Tiles of a sequence that fills its table.
+static long long most_tiles(const PagedAttnArgs& a) {
+  return ((static_cast<long long>(a.table.max_pages) << a.pool.page_shift) + kTileKeys - 1) /
+         kTileKeys;
+}
+
+bool paged_attention_supported(const PagedAttnArgs& a) {
+  const PagedAttnShape s = paged_attention_shape(a.heads, a.pool.kv_heads, a.pool.head_dim);
+  return static_cast<double>(most_tiles(a)) * a.table.sequences * s.units < 2147000000.0;
+}
+
+void launch_paged_attention(PagedAttnArgs a, hipStream_t stream) {
+  const PagedAttnShape s = paged_attention_shape(a.heads, a.pool.kv_heads, a.pool.head_dim);
+  a.head_blocks = s.head_blocks;
+  a.units = s.units;
+  // no more workgroups than the tables have tiles for, one a wave
+  const long long most = most_tiles(a) * a.table.sequences * s.units;
+  const long long wanted = (most + s.waves_per_group - 1) / s.waves_per_group;
+  const unsigned groups = static_cast<unsigned>(wanted < s.groups ? wanted : s.groups);
+  a.waves = groups * s.waves_per_group;
+  const long long pieces = static_cast<long long>(a.table.sequences) * s.units;
+  a.whole = most_tiles(a) <= (pieces <= s.groups ? kWholeTiles : kWholeTiles / 2);
+  a.join_heads = pieces <= 64;
   by_format(a.pool, [&](auto f, auto d) {
-    hipLaunchKernelGGL((paged_attention_kernel<decltype(f)::value, decltype(d)::value>),
-                       dim3(a.heads, a.table.sequences), dim3(kThreads), 0, stream, a);
+    constexpr int F = decltype(f)::value, D = decltype(d)::value;
+    if (s.waves_per_group == 8) {
+      hipLaunchKernelGGL((paged_attention_kernel<F, D, 8, 8>), dim3(groups), dim3(8 * kWave), 0,
+                         stream, a);
+    } else {
+      hipLaunchKernelGGL((paged_attention_kernel<F, D, 4, 16>), dim3(groups), dim3(4 * kWave), 0,
+                         stream, a);
+    }
   });
+  if (a.whole) return;
+  const int per_kv = a.heads / a.pool.kv_heads;
+  const int hb = per_kv < kHeadBlock ? per_kv : kHeadBlock;
+  const dim3 grid(a.join_heads ? s.units * hb : s.units, a.table.sequences);
+  auto join = [&](auto d, auto w) {
+    hipLaunchKernelGGL((paged_attention_join_kernel<decltype(d)::value, decltype(w)::value>), grid,
+                       dim3(kJoinThreads), 0, stream, a);
+  };
+  auto by_waves = [&](auto d) {
+    if (s.waves_per_group == 8) {
+      join(d, std::integral_constant<int, 8>{});
+    } else {
+      join(d, std::integral_constant<int, 4>{});
+    }
+  };
+  if (a.pool.head_dim == 64) {
+    by_waves(std::integral_constant<int, 64>{});
+  } else {
+    by_waves(std::integral_constant<int, 128>{});
+  }
 }
 
 }  // namespace qlin

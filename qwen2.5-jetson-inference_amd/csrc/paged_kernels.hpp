@@ -61,12 +61,20 @@ struct PagedAttnArgs {
   long long q_stride;
   int heads;
   uint16_t* out;
-  float* workspace;
+  float* records;   // [workgroups][2][heads of a unit][D + 4]: O, maximum, sum
+  // set by the launch
+  int head_blocks;  // of a KV head: its query heads / 16, rounded up
+  int units;        // KV heads x head blocks
+  int waves;        // of the grid
+  int whole;        // units are not cut
+  int join_heads;   // a workgroup of the join per query head
 };
 
 void launch_kv_store(const KvStoreArgs& a, hipStream_t stream);
 void launch_kv_load(const KvLoadArgs& a, hipStream_t stream);
-void launch_paged_attention(const PagedAttnArgs& a, hipStream_t stream);
+// Whether the tiles of the largest possible lengths can be counted in 32 bits.
+bool paged_attention_supported(const PagedAttnArgs& a);
+void launch_paged_attention(PagedAttnArgs a, hipStream_t stream);
 size_t paged_attention_workspace_bytes(int sequences, int heads, int kv_heads, int head_dim);
 
 }  // namespace qlin

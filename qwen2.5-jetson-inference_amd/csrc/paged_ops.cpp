@@ -209,7 +209,12 @@ extern "C" int infer_hip_attention_paged_decode(const infer_hip_kv_pages* pages,
   a.q_stride = query_stride;
   a.heads = num_heads;
   a.out = output;
-  a.workspace = static_cast<float*>(workspace);
+  a.records = static_cast<float*>(workspace);
+  if (!paged_attention_supported(a)) {
+    return fail(INFER_HIP_INVALID_ARGUMENT,
+                "%s: %d sequences of up to %d pages of %d are too many for one call", what,
+                a.table.sequences, a.table.max_pages, 1 << a.pool.page_shift);
+  }
   launch_paged_attention(a, stream);
   return check_launch(what);
 }

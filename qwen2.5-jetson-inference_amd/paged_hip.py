@@ -11,6 +11,8 @@ from __future__ import annotations
 
 import ctypes
 
+import torch
+
 import linear_hip
 from linear_hip import INVALID_ARGUMENT, InferError, _check, _stream
 
@@ -41,6 +43,7 @@ class _Table(ctypes.Structure):
 
 
 _lib = None
+_BF16, _I32, _F32, _U8 = torch.bfloat16, torch.int32, torch.float32, torch.uint8
 
 
 def load():
@@ -76,7 +79,6 @@ class KvPages:
     8-bit types (None for bfloat16)."""
 
     def __init__(self, key, value, key_scales=None, value_scales=None):
-        import torch
         formats = {torch.bfloat16: "bf16", torch.int8: "int8", torch.float8_e4m3fn: "fp8"}
         if key.dtype not in formats or key.dim() != 4:
             _bad(f"KvPages: key must be [pages, heads, page size, head_dim] of bfloat16, int8 or "
@@ -96,7 +98,7 @@ class KvPages:
         self.num_pages, self.num_kv_heads, self.page_size, self.head_dim = key.shape
         self.key, self.value, self.key_scales, self.value_scales = (
             key, value, key_scales, value_scales)
-        self.device = key.device
+        self.device, self.index = key.device, key.get_device()
         self._struct = _Pages(FORMATS[self.format], self.num_pages, self.page_size,
                               self.num_kv_heads, self.head_dim, key.data_ptr(), value.data_ptr(),
                               key_scales.data_ptr() if scaled else None,
@@ -107,7 +109,6 @@ class KvPages:
     def allocate(cls, num_pages: int, page_size: int, num_kv_heads: int, head_dim: int,
                  format: str = "bf16", device="cuda"):
         """A pool of its own, zeroed."""
-        import torch
         if format not in FORMATS:
             _bad(f"KvPages: format {format!r} (bf16, int8 or fp8)")
         dtype = {"bf16": torch.bfloat16, "int8": torch.int8, "fp8": torch.float8_e4m3fn}[format]
@@ -122,9 +123,13 @@ class KvPages:
         return cls(pages(), pages(), scales(), scales())
 
 
+# The checks below run on every call: they read each tensor as few times as
+# they can (an attribute costs 40-110 ns, a launch 2-3 us).
+
+
 def _at(t, dtype, pages, name):
     """Pointer of a contiguous tensor of a type on the pool's GPU."""
-    if t.dtype != dtype or t.device != pages.device or not t.is_contiguous():
+    if t.dtype is not dtype or t.get_device() != pages.index or not t.is_contiguous():
         _bad(f"{name} must be contiguous {dtype} on {pages.device} (got {t.dtype} on {t.device})")
     return t.data_ptr()
 
@@ -132,34 +137,35 @@ def _at(t, dtype, pages, name):
 def _table(table, pages):
     """infer_hip_kv_table of an int32 tensor [sequences, pages] whose rows may be
     longer (a slice of a wider table)."""
-    import torch
-    if table.dtype != torch.int32 or table.dim() != 2 or table.device != pages.device:
+    shape = table.shape
+    if table.dtype is not _I32 or len(shape) != 2 or table.get_device() != pages.index:
         _bad("block table must be int32 [sequences, pages] on the pool's GPU")
-    rows, width = table.shape
-    stride = table.stride(0) if rows > 1 else width
-    if table.stride(1) != 1 and width > 1:
+    rows, width = shape
+    stride, inner = table.stride()
+    if inner != 1 and width > 1:
         _bad("block table rows must be contiguous")
-    return _Table(table.data_ptr(), rows, width, stride)
+    return _Table(table.data_ptr(), rows, width, stride if rows > 1 else width)
 
 
-def _rows(t, heads, pages, name):
+def _rows(t, tokens, heads, pages, name):
     """Pointer and token stride of BF16 [tokens, heads, head_dim] with
     contiguous tokens."""
-    import torch
-    if t.dtype != torch.bfloat16 or t.dim() != 3 or t.device != pages.device:
-        _bad(f"{name} must be bfloat16 [tokens, heads, head_dim] on the pool's GPU")
-    n, h, d = t.shape
-    if d != pages.head_dim or (heads is not None and h != heads):
-        _bad(f"{name} of {h} heads of {d}: the pool has {pages.num_kv_heads} of {pages.head_dim}")
-    if t.stride(2) != 1 or (h > 1 and t.stride(1) != d):
+    if t.dtype is not _BF16 or t.get_device() != pages.index:
+        _bad(f"{name} must be bfloat16 on the pool's GPU")
+    shape, d = t.shape, pages.head_dim
+    if shape != (tokens, heads, d):
+        _bad(f"{name} must be [{tokens}, {heads}, {d}] (got {tuple(shape)})")
+    stride, between, inner = t.stride()
+    if inner != 1 or (heads > 1 and between != d):
         _bad(f"{name}: a token's heads must be contiguous")
-    return t.data_ptr(), t.stride(0) if n > 1 else h * d
+    return t.data_ptr(), stride if tokens > 1 else heads * d
 
 
-def _on(pages):
-    import torch
-    if torch.cuda.current_device() != pages.device.index:
+def _on(pages, stream):
+    """The stream, of the pool's GPU, which must be the current one."""
+    if torch.cuda.current_device() != pages.index:
         _bad(f"the pool is on {pages.device}, the current device is {torch.cuda.current_device()}")
+    return _stream(stream)
 
 
 def kv_pages_store(pages, table, positions, query, key, value, query_out=None, rope=None,
@@ -169,43 +175,39 @@ def kv_pages_store(pages, table, positions, query, key, value, query_out=None, r
     positions int32 [tokens], rope float32 [positions, head_dim / 2, 2],
     sequences int32 [tokens] or None (token t belongs to sequence t).  query
     None: only the cache is written."""
-    import torch
-    _on(pages)
-    tokens = positions.numel()
+    on = _on(pages, stream)
+    tokens, kv = positions.numel(), pages.num_kv_heads
     tab = _table(table, pages)
-    qp = qo = None
-    qs = os_ = heads = 0
+    qp = qo = rp = sp = None
+    qs = os_ = heads = rn = 0
     if query is not None:
-        if query_out is None or query.shape != query_out.shape or query.shape[0] != tokens:
+        heads = query.shape[1] if query.dim() == 3 else 0
+        if query_out is None or not heads:
             _bad("query and query_out must be [tokens, heads, head_dim]")
-        heads = query.shape[1]
-        qp, qs = _rows(query, heads, pages, "query")
-        qo, os_ = _rows(query_out, heads, pages, "query_out")
-    kp, ks = _rows(key, pages.num_kv_heads, pages, "key")
-    vp, vs = _rows(value, pages.num_kv_heads, pages, "value")
-    if key.shape[0] != tokens or value.shape[0] != tokens:
-        _bad(f"key and value must hold {tokens} tokens")
-    rp, rn = None, 0
+        qp, qs = _rows(query, tokens, heads, pages, "query")
+        qo, os_ = (qp, qs) if query_out is query else _rows(query_out, tokens, heads, pages,
+                                                            "query_out")
+    kp, ks = _rows(key, tokens, kv, pages, "key")
+    vp, vs = _rows(value, tokens, kv, pages, "value")
     if rope is not None:
-        if rope.dim() != 3 or rope.shape[1] != pages.head_dim // 2 or rope.shape[2] != 2:
+        shape = rope.shape
+        if shape[1:] != (pages.head_dim // 2, 2):
             _bad("rope must be float32 [positions, head_dim / 2, 2]")
-        rp, rn = _at(rope, torch.float32, pages, "rope"), rope.shape[0]
-    sp = None
+        rp, rn = _at(rope, _F32, pages, "rope"), shape[0]
     if sequences is not None:
         if sequences.numel() != tokens:
             _bad(f"sequences must hold {tokens} tokens")
-        sp = _at(sequences, torch.int32, pages, "sequences")
+        sp = _at(sequences, _I32, pages, "sequences")
     _check(load().infer_hip_kv_pages_store(
-        pages._ref, tab, sp, _at(positions, torch.int32, pages, "positions"), tokens, qp, qs,
-        heads, kp, ks, vp, vs, rp, rn, qo, os_, _stream(stream)))
+        pages._ref, tab, sp, _at(positions, _I32, pages, "positions"), tokens, qp, qs, heads, kp,
+        ks, vp, vs, rp, rn, qo, os_, on))
 
 
 def kv_pages_load(pages, table, lengths, key_cache, value_cache, stream=None) -> None:
     """The first lengths[s] positions of every sequence as BF16 into
     key_cache / value_cache [sequences, KV heads, capacity, head_dim]
     (infer_hip_kv_pages_load)."""
-    import torch
-    _on(pages)
+    on = _on(pages, stream)
     tab = _table(table, pages)
     shape = key_cache.shape
     if (len(shape) != 4 or value_cache.shape != shape or shape[0] != tab.num_sequences
@@ -214,9 +216,9 @@ def kv_pages_load(pages, table, lengths, key_cache, value_cache, stream=None) ->
     if lengths.numel() != tab.num_sequences:
         _bad(f"lengths must hold {tab.num_sequences} sequences")
     _check(load().infer_hip_kv_pages_load(
-        pages._ref, tab, _at(lengths, torch.int32, pages, "lengths"),
-        _at(key_cache, torch.bfloat16, pages, "key_cache"),
-        _at(value_cache, torch.bfloat16, pages, "value_cache"), shape[2], _stream(stream)))
+        pages._ref, tab, _at(lengths, _I32, pages, "lengths"),
+        _at(key_cache, _BF16, pages, "key_cache"), _at(value_cache, _BF16, pages, "value_cache"),
+        shape[2], on))
 
 
 def attention_paged_decode_workspace_bytes(num_sequences: int, num_heads: int,
@@ -227,17 +229,17 @@ def attention_paged_decode_workspace_bytes(num_sequences: int, num_heads: int,
 
 def attention_paged_decode(pages, table, lengths, query, output, workspace, stream=None) -> None:
     """Attention of one new token a sequence: query and output
-    [sequences, heads, head_dim], workspace a zeroed uint8 tensor of
+    [sequences, heads, head_dim], workspace a uint8 tensor of
     attention_paged_decode_workspace_bytes (infer_hip_attention_paged_decode)."""
-    import torch
-    _on(pages)
+    on = _on(pages, stream)
     tab = _table(table, pages)
-    qp, qs = _rows(query, None, pages, "query")
-    if output.shape != query.shape or query.shape[0] != tab.num_sequences:
+    shape = query.shape
+    if len(shape) != 3 or output.shape != shape:
         _bad("query and output must be [sequences, heads, head_dim]")
+    qp, qs = _rows(query, tab.num_sequences, shape[1], pages, "query")
     if lengths.numel() != tab.num_sequences:
         _bad(f"lengths must hold {tab.num_sequences} sequences")
     _check(load().infer_hip_attention_paged_decode(
-        pages._ref, tab, _at(lengths, torch.int32, pages, "lengths"), qp, qs, query.shape[1],
-        _at(output, torch.bfloat16, pages, "output"),
-        _at(workspace, torch.uint8, pages, "workspace"), workspace.numel(), _stream(stream)))
+        pages._ref, tab, _at(lengths, _I32, pages, "lengths"), qp, qs, shape[1],
+        _at(output, _BF16, pages, "output"), _at(workspace, _U8, pages, "workspace"),
+        workspace.numel(), on))
