@@ -23,16 +23,16 @@ def pack(q, scales):
 
 def product(q, scales, group, bias, x):
     """(Y in 64 bits, the bound on its FP32 sums): a group's sum is taken of
-    products as large as 143 |x| (the elements are held as 128 + u, the 136 too
-    much taken off the group's sum of x), in `group` roundings of 2^-24, and
-    the scaled sums of K / group groups added in as many."""
+    products as large as 31 |x| (the elements are held as 16 + u, u = q + 8, and
+    24 times the group's sum of x taken off), in 2 `group` roundings of 2^-24,
+    and the scaled sums of K / group groups added in as many."""
     n, k = q.shape
     s = scales.double()
     w = q.double() * s.repeat_interleave(group, dim=1)
     y = x.double() @ w.t()
     ax = x.double().abs()
     by_group = ax.view(x.shape[0], k // group, group).sum(dim=2) @ s.abs().t()
-    bound = by_group * 143 * 2 * group * 2.0 ** -24
+    bound = by_group * 31 * 2 * group * 2.0 ** -24
     bound += (ax @ w.abs().t()) * (k // group + 2) * 2.0 ** -24
     if bias is not None:
         y = y + bias.double()
