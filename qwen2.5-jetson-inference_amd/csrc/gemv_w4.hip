@@ -38,18 +38,19 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 // scale multiplies it into the FP32 total.  Terms are at most 31/16 |x| where
 // q x / 16 reaches 1/2 |x|, which costs two bits of FP32's 24.
 //
-// A workgroup has R row tiles (16 rows each); its waves split the 128-column
-// tiles, each a contiguous KiB of weights in one load, and meet in LDS in the
-// order of the waves.  Memory bounds it: per KiB of weights a SIMD issues about
-// 40 vector instructions and five MFMAs.
+// Two forms.  With many rows (w4a16_rows_kernel) a wave takes whole row tiles
+// over all of K, by itself, with the activations in LDS.  With fewer
+// (w4a16_split_kernel) the waves of a workgroup split one row tile's K and meet
+// in LDS, in the order of the waves.  Either keeps DP tiles of 128 columns, a
+// contiguous KiB of weights each, in flight per wave.  Memory bounds both: per
+// KiB a SIMD issues 45 to 70 vector instructions and eight MFMAs, 270 cycles at
+// most, and a CU's share of HBM is a KiB in 90 for its four SIMDs.
 //
 // Activations beyond FP32's reach (a sum that is not finite) are summed again
 // element by element, q s x in FP32.
-template <int G, int R>
 struct W4Piece {
-  uint4 w[R];
-  uint4 x[4];
-  uint2 s[R][kTileCols / G];  // four rows' scales
+  uint4 w;
+  uint2 s;  // four rows' scales, of the lane's group
 };
 
 __device__ __forceinline__ uint32_t word_of(const uint4& v, int i) {
@@ -85,124 +86,251 @@ __device__ float exact_dot(const W4Args& a, int row, int t) {
   return sum;
 }
 
-template <int G, int R>
-__global__ __launch_bounds__(R == 1 ? 1024 : 512) void w4a16_gemv_kernel(W4Args a) {
-  constexpr int kGroups = kTileCols / G, kSteps = G / 32;  // of a tile, of a group
-  constexpr int kRows = R * kTileRows, kPitch = kRows + 4;
-  extern __shared__ __align__(16) float partial[];  // [wave][token][kPitch]
-  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x / kWave;
-  const int tiles = (a.k + kTileCols - 1) / kTileCols;
-  const int row_tiles = (a.n + kTileRows - 1) / kTileRows;
-  const int first = blockIdx.x * R;
-  const int groups = a.k / G;
+// Column tile t of row tile rt.  Lane 16 g + r holds the scales of rows 4 g ..
+// + 3 for group r modulo the tile's groups: one load for all of them, and each
+// quad of lanes has every group.
+template <int G>
+__device__ __forceinline__ void load_piece(W4Piece& p, const W4Args& a, int rt, int t, int tiles,
+                                           int groups, int lane) {
+  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+  constexpr int kGroups = kTileCols / G;
+  p.w = load_stream16(a.w + (static_cast<size_t>(rt) * tiles + t) * kTileBytes + 16 * lane);
+  // past the last group the activations are 0
+  const int group = kGroups == 1 ? t : min(t * kGroups + (lane & (kGroups - 1)), groups - 1);
+  const u32x2 v = gload(reinterpret_cast<const u32x2*>(
+      a.s + (static_cast<size_t>(rt) * groups + group) * kTileRows + 4 * (lane >> 4)));
+  p.s = make_uint2(v.x, v.y);
+}
 
-  auto load = [&](W4Piece<G, R>& p, int t) {
+// v of lane J of the quad.
+template <int J>
+__device__ __forceinline__ float quad_lane(float v) {
+  return __int_as_float(
+      __builtin_amdgcn_update_dpp(0, __float_as_int(v), J * 0x55, 0xF, 0xF, true));
+}
+
+// total += the tile's products with x (four steps of 32 columns), over 16.
+template <int G>
+__device__ __forceinline__ void add_piece(f32x4_t& total, const W4Piece& p,
+                                          const bf16x8_t (&x)[4]) {
+  constexpr int kGroups = kTileCols / G, kSteps = G / 32;
+  const bf16x8_t minus_1_5 =
+      __builtin_bit_cast(bf16x8_t, make_uint4(0xBFC0BFC0u, 0xBFC0BFC0u, 0xBFC0BFC0u, 0xBFC0BFC0u));
+  const float s[4] = {bf16_lo(p.s.x), bf16_hi(p.s.x), bf16_lo(p.s.y), bf16_hi(p.s.y)};
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      const int rt = min(first + i, row_tiles - 1);  // past the last: read again, not stored
-      p.w[i] = load_stream16(a.w + (static_cast<size_t>(rt) * tiles + t) * kTileBytes + 16 * lane);
+  for (int j = 0; j < kGroups; ++j) {
+    f32x4_t d{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int j = 0; j < kGroups; ++j) {
-        const int group = min(t * kGroups + j, groups - 1);  // past the last: of columns x = 0
-        const uint16_t* s = a.s + (static_cast<size_t>(rt) * groups + group) * kTileRows + 4 * g;
-        p.s[i][j] = make_uint2(gload(reinterpret_cast<const uint32_t*>(s)),
-                               gload(reinterpret_cast<const uint32_t*>(s) + 1));
-      }
+    for (int i = j * kSteps; i < (j + 1) * kSteps; ++i) {
+      d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(minus_1_5, x[i], d, 0, 0, 0);
+      d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen_nibbles(word_of(p.w, i)), x[i], d, 0, 0, 0);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int col = t * kTileCols + 32 * i;
-      p.x[i] = make_uint4(0, 0, 0, 0);
-      if (col < a.k && r < a.tokens) {
-        p.x[i] = load_global16(a.x + static_cast<size_t>(r) * a.k + col + 8 * g);
-      }
+      const float f = kGroups == 1 ? s[i]
+                      : j == 0     ? quad_lane<0>(s[i])
+                      : j == 1     ? quad_lane<1>(s[i])
+                      : j == 2     ? quad_lane<2>(s[i])
+                                   : quad_lane<3>(s[i]);
+      total[i] = fmaf(f, d[i], total[i]);
     }
-  };
-  const bf16x8_t minus_1_5 =
-      __builtin_bit_cast(bf16x8_t, make_uint4(0xBFC0BFC0u, 0xBFC0BFC0u, 0xBFC0BFC0u, 0xBFC0BFC0u));
-  f32x4_t total[R];
-#pragma unroll
-  for (int i = 0; i < R; ++i) total[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  auto add = [&](const W4Piece<G, R>& p) {
-#pragma unroll
-    for (int j = 0; j < kGroups; ++j) {
-      f32x4_t base{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-      for (int i = 0; i < kSteps; ++i) {
-        base = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-            minus_1_5, __builtin_bit_cast(bf16x8_t, p.x[j * kSteps + i]), base, 0, 0, 0);
-      }
-#pragma unroll
-      for (int t = 0; t < R; ++t) {
-        f32x4_t d = base;
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-          d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-              widen_nibbles(word_of(p.w[t], j * kSteps + i)),
-              __builtin_bit_cast(bf16x8_t, p.x[j * kSteps + i]), d, 0, 0, 0);
-        }
-        const uint2 s = p.s[t][j];
-        total[t][0] = fmaf(bf16_lo(s.x), d[0], total[t][0]);
-        total[t][1] = fmaf(bf16_hi(s.x), d[1], total[t][1]);
-        total[t][2] = fmaf(bf16_lo(s.y), d[2], total[t][2]);
-        total[t][3] = fmaf(bf16_hi(s.y), d[3], total[t][3]);
-      }
-    }
-  };
-  for (int t = wave; t < tiles; t += 2 * waves) {  // two tiles' loads in flight
-    W4Piece<G, R> p0, p1;
-    load(p0, t);
-    const bool two = t + waves < tiles;
-    if (two) load(p1, t + waves);
-    add(p0);
-    if (two) add(p1);
   }
+}
 
-  if (r < a.tokens) {
-#pragma unroll
-    for (int i = 0; i < R; ++i) {
-      *reinterpret_cast<f32x4_t*>(partial + (wave * a.tokens + r) * kPitch + i * kTileRows + 4 * g) =
-          total[i];
+// The output from a sum over 16.
+__device__ __forceinline__ uint16_t finish(const W4Args& a, float v, int row) {
+  v *= 16.0f;
+  return f32_to_bf16(a.bias ? v + bf16_to_f32(a.bias[row]) : v);
+}
+
+// Whether a stored output may be that of a sum that overflowed.
+__device__ __forceinline__ bool not_finite(uint16_t y) { return (y & 0x7F80u) == 0x7F80u; }
+
+__device__ void finish_exactly(const W4Args& a, int row, int token) {
+  uint16_t* y = a.y + static_cast<size_t>(token) * a.n + row;
+  const float v = exact_dot(a, row, token);
+  *y = f32_to_bf16(a.bias ? v + bf16_to_f32(a.bias[row]) : v);
+}
+
+constexpr int kRowsWaves = 8, kRowsDepth = 4, kRowsGroups = 512;
+constexpr int kRowsX = 64 * 1024;  // the activations' room in LDS, twice a CU
+
+// Workgroup i takes the i-th of equal shares of the row tiles, its waves equal
+// shares of that.
+template <int G>
+__global__ __launch_bounds__(kRowsWaves * kWave, 4) void w4a16_rows_kernel(W4Args a) {
+  constexpr int DP = kRowsDepth;
+  extern __shared__ __align__(16) uint4 lds_x[];  // [8 columns][token], zero past K
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int tiles = (a.k + kTileCols - 1) / kTileCols, groups = a.k / G;
+  const int row_tiles = (a.n + kTileRows - 1) / kTileRows;
+  const long long share = static_cast<long long>(row_tiles) * blockIdx.x;
+  const int begin = share / gridDim.x, end = (share + row_tiles) / gridDim.x;
+  const int per_wave = (end - begin + kRowsWaves - 1) / kRowsWaves;
+  const int first = min(end, begin + wave * per_wave), last = min(end, first + per_wave);
+  const int count = (last - first) * tiles;
+
+  // Loads run DP tiles ahead, always: past the wave's last tile they read that
+  // one again, so that the compiler knows how many are in flight.
+  int rt_ahead = first, t_ahead = 0, ahead = 0;
+  auto load_next = [&](W4Piece& p) {
+    load_piece<G>(p, a, rt_ahead, t_ahead, tiles, groups, lane);
+    if (ahead + 1 < count) {
+      ++ahead;
+      if (++t_ahead == tiles) {
+        t_ahead = 0;
+        ++rt_ahead;
+      }
     }
+  };
+  W4Piece p[DP];
+  if (count > 0) {
+#pragma unroll
+    for (int i = 0; i < DP; ++i) load_next(p[i]);
+  }
+  // the activations, while those are on their way
+  const int chunks = a.k / 8;
+  for (int i = threadIdx.x; i < tiles * (kTileCols / 8) * a.tokens; i += kRowsWaves * kWave) {
+    const int chunk = i / a.tokens, token = i - chunk * a.tokens;
+    lds_x[i] = chunk < chunks ? load_global16(a.x + static_cast<size_t>(token) * a.k + 8 * chunk)
+                              : make_uint4(0, 0, 0, 0);
   }
   __syncthreads();
-  for (int e = threadIdx.x; e < kRows * a.tokens; e += blockDim.x) {
-    const int t = e / kRows, i = e % kRows, row = first * kTileRows + i;
-    if (row >= a.n) continue;
-    float v = 0.0f;
-    for (int w = 0; w < waves; ++w) v += partial[(w * a.tokens + t) * kPitch + i];
-    v *= 16.0f;
-    if (!__builtin_isfinite(v)) v = exact_dot(a, row, t);
-    a.y[static_cast<size_t>(t) * a.n + row] =
-        f32_to_bf16(a.bias ? v + bf16_to_f32(a.bias[row]) : v);
+  if (count <= 0) return;
+  // Lanes past the tokens take the last one's: their columns of Y^T are dropped.
+  const uint4* const mine = lds_x + g * a.tokens + min(r, a.tokens - 1);
+  const bool wide = (a.n & 3) == 0 && (reinterpret_cast<uintptr_t>(a.y) & 7u) == 0;
+
+  f32x4_t total{0.0f, 0.0f, 0.0f, 0.0f};
+  bool again = false;
+  int rt = first, t = 0;
+  for (int item = 0; item < count;) {
+#pragma unroll
+    for (int i = 0; i < DP; ++i) {
+      bf16x8_t x[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        x[j] = __builtin_bit_cast(bf16x8_t, mine[(t * 16 + 4 * j) * a.tokens]);
+      }
+      add_piece<G>(total, p[i], x);
+      load_next(p[i]);
+      if (++t == tiles) {
+        const int row = rt * kTileRows + 4 * g;
+        if (r < a.tokens) {
+          uint16_t* y = a.y + static_cast<size_t>(r) * a.n + row;
+          uint16_t v[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            v[j] = row + j < a.n ? finish(a, total[j], row + j) : 0;
+            again = again || not_finite(v[j]);
+          }
+          if (wide) {  // then the four rows are in the matrix or none is
+            if (row < a.n) {
+              store_global8(y, make_uint2(v[0] | static_cast<uint32_t>(v[1]) << 16,
+                                          v[2] | static_cast<uint32_t>(v[3]) << 16));
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if (row + j < a.n) y[j] = v[j];
+            }
+          }
+        }
+        total = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        t = 0;
+        ++rt;
+      }
+      if (++item == count) break;
+    }
+  }
+  if (again) {  // the lane's own outputs
+    for (int row = first * kTileRows; row < min(last * kTileRows, a.n); ++row) {
+      if ((row >> 2 & 3) == g && r < a.tokens &&
+          not_finite(a.y[static_cast<size_t>(r) * a.n + row])) {
+        finish_exactly(a, row, r);
+      }
+    }
   }
 }
 
-// Waves of a workgroup: as few tiles each as `most` waves allow, and no wave
-// without one.
-int waves_for(int tiles, int most) {
-  const int per = (tiles + most - 1) / most;
-  return (tiles + per - 1) / per;
+constexpr int kSplitWaves = 16;
+
+// Workgroup i: row tile i; wave w takes its column tiles w, w + waves, ...
+template <int G, int DP>
+__global__ __launch_bounds__(kSplitWaves * kWave) void w4a16_split_kernel(W4Args a) {
+  __shared__ float partial[kSplitWaves][kMaxTokens][kTileRows + 4];
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x / kWave;
+  const int tiles = (a.k + kTileCols - 1) / kTileCols, groups = a.k / G;
+  const int rt = blockIdx.x;
+  const uint16_t* x_row = a.x + static_cast<size_t>(min(r, a.tokens - 1)) * a.k + 8 * g;
+  f32x4_t total{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int t0 = wave; t0 < tiles; t0 += DP * waves) {
+    W4Piece p[DP];
+    uint4 x[DP][4];
+#pragma unroll
+    for (int i = 0; i < DP; ++i) {  // past the last tile: that one again
+      const int t = min(t0 + i * waves, tiles - 1);
+      load_piece<G>(p[i], a, rt, t, tiles, groups, lane);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        // columns past K count for nothing, from wherever they are read
+        const int col = t * kTileCols + 32 * j;
+        x[i][j] = load_global16(x_row + (col < a.k ? col : 0));
+        if (col >= a.k) x[i][j] = make_uint4(0, 0, 0, 0);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < DP; ++i) {
+      if (t0 + i * waves >= tiles) break;
+      bf16x8_t xb[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) xb[j] = __builtin_bit_cast(bf16x8_t, x[i][j]);
+      add_piece<G>(total, p[i], xb);
+    }
+  }
+  if (r < a.tokens) *reinterpret_cast<f32x4_t*>(&partial[wave][r][4 * g]) = total;
+  __syncthreads();
+  for (int e = threadIdx.x; e < kTileRows * a.tokens; e += blockDim.x) {
+    const int token = e / kTileRows, i = e % kTileRows, row = rt * kTileRows + i;
+    if (row >= a.n) continue;
+    float v = 0.0f;
+    for (int w = 0; w < waves; ++w) v += partial[w][token][i];
+    const uint16_t y = finish(a, v, row);
+    a.y[static_cast<size_t>(token) * a.n + row] = y;
+    if (not_finite(y)) finish_exactly(a, row, token);
+  }
 }
+
+constexpr int kCus = 256;
 
 template <int G>
 void launch_w4(const W4Args& a, hipStream_t stream) {
   const int row_tiles = (a.n + kTileRows - 1) / kTileRows;
   const int tiles = (a.k + kTileCols - 1) / kTileCols;
-  auto launch = [&](auto rows, int most) {
-    constexpr int R = decltype(rows)::value;
-    const int waves = waves_for(tiles, most);
-    const size_t lds = static_cast<size_t>(waves) * a.tokens * (R * kTileRows + 4) * sizeof(float);
-    hipLaunchKernelGGL((w4a16_gemv_kernel<G, R>), dim3((row_tiles + R - 1) / R),
-                       dim3(waves * kWave), lds, stream, a);
+  const size_t x_bytes = static_cast<size_t>(tiles) * kTileCols * 2 * a.tokens;
+  constexpr int kResident = kCus * 2 * kRowsWaves;  // waves of two workgroups a CU
+  if (row_tiles >= kResident / 2 && x_bytes <= kRowsX) {
+    hipLaunchKernelGGL((w4a16_rows_kernel<G>), dim3(kRowsGroups), dim3(kRowsWaves * kWave), x_bytes,
+                       stream, a);
+    return;
+  }
+  // Waves for the chip's room, at least two, of equal shares of the tiles.
+  const int room = kResident / row_tiles;
+  const int most = room < 2 ? 2 : room > kSplitWaves ? kSplitWaves : room;
+  const int per = (tiles + most - 1) / most;
+  const int waves = (tiles + per - 1) / per;
+  auto launch = [&](auto depth) {
+    hipLaunchKernelGGL((w4a16_split_kernel<G, decltype(depth)::value>), dim3(row_tiles),
+                       dim3(waves * kWave), 0, stream, a);
   };
-  if (row_tiles >= 2048) {
-    launch(std::integral_constant<int, 4>{}, 8);
-  } else if (row_tiles >= 1024) {
-    launch(std::integral_constant<int, 2>{}, 8);
+  if (per == 1) {
+    launch(std::integral_constant<int, 1>{});
+  } else if (per == 2) {
+    launch(std::integral_constant<int, 2>{});
   } else {
-    launch(std::integral_constant<int, 1>{}, 16);
+    launch(std::integral_constant<int, 3>{});
   }
 }
 
