@@ -109,20 +109,33 @@ __device__ __forceinline__ float quad_lane(float v) {
       __builtin_amdgcn_update_dpp(0, __float_as_int(v), J * 0x55, 0xF, 0xF, true));
 }
 
-// total += the tile's products with x (four steps of 32 columns), over 16.
+// -1.5 sum x over each group of a tile (four steps of 32 columns), for every row.
 template <int G>
-__device__ __forceinline__ void add_piece(f32x4_t& total, const W4Piece& p,
-                                          const bf16x8_t (&x)[4]) {
-  constexpr int kGroups = kTileCols / G, kSteps = G / 32;
+__device__ __forceinline__ void base_of(f32x4_t (&base)[kTileCols / G], const bf16x8_t (&x)[4]) {
+  constexpr int kSteps = G / 32;
   const bf16x8_t minus_1_5 =
       __builtin_bit_cast(bf16x8_t, make_uint4(0xBFC0BFC0u, 0xBFC0BFC0u, 0xBFC0BFC0u, 0xBFC0BFC0u));
+#pragma unroll
+  for (int j = 0; j < kTileCols / G; ++j) {
+    base[j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int i = j * kSteps; i < (j + 1) * kSteps; ++i) {
+      base[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(minus_1_5, x[i], base[j], 0, 0, 0);
+    }
+  }
+}
+
+// total += the tile's products with x, over 16.
+template <int G>
+__device__ __forceinline__ void add_piece(f32x4_t& total, const W4Piece& p, const bf16x8_t (&x)[4],
+                                          const f32x4_t (&base)[kTileCols / G]) {
+  constexpr int kGroups = kTileCols / G, kSteps = G / 32;
   const float s[4] = {bf16_lo(p.s.x), bf16_hi(p.s.x), bf16_lo(p.s.y), bf16_hi(p.s.y)};
 #pragma unroll
   for (int j = 0; j < kGroups; ++j) {
-    f32x4_t d{0.0f, 0.0f, 0.0f, 0.0f};
+    f32x4_t d = base[j];
 #pragma unroll
     for (int i = j * kSteps; i < (j + 1) * kSteps; ++i) {
-      d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(minus_1_5, x[i], d, 0, 0, 0);
       d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen_nibbles(word_of(p.w, i)), x[i], d, 0, 0, 0);
     }
 #pragma unroll
@@ -152,36 +165,62 @@ __device__ void finish_exactly(const W4Args& a, int row, int token) {
   *y = f32_to_bf16(a.bias ? v + bf16_to_f32(a.bias[row]) : v);
 }
 
-constexpr int kRowsWaves = 8, kRowsDepth = 4, kRowsGroups = 512;
-constexpr int kRowsX = 64 * 1024;  // the activations' room in LDS, twice a CU
+constexpr int kRowsDepth = 4, kRowsMaxWaves = 16;
+// Workgroups of the rows kernel a CU holds, and their waves, by their LDS.
+struct RowsShape {
+  int per_cu, waves;
+  size_t lds;  // at most
+};
+constexpr RowsShape kRowsShapes[] = {
+    {3, 8, 52 * 1024}, {2, 12, 78 * 1024}, {1, kRowsMaxWaves, 156 * 1024}};
+
+// LDS of the rows kernel: the activations [K / 8][TP tokens][8], zero past K and
+// past the tokens, then the groups' bases [K / G][TP][4].
+constexpr size_t rows_x_bytes(int tiles, int pitch) {
+  return static_cast<size_t>(tiles) * kTileCols * 2 * pitch;
+}
+constexpr size_t rows_lds_bytes(int tiles, int pitch, int group) {
+  return rows_x_bytes(tiles, pitch) + static_cast<size_t>(tiles) * (kTileCols / group) * pitch * 16;
+}
 
 // Workgroup i takes the i-th of equal shares of the row tiles, its waves equal
-// shares of that.
-template <int G>
-__global__ __launch_bounds__(kRowsWaves * kWave, 4) void w4a16_rows_kernel(W4Args a) {
-  constexpr int DP = kRowsDepth;
-  extern __shared__ __align__(16) uint4 lds_x[];  // [8 columns][token], zero past K
+// shares of that.  TP: room for that many tokens; lanes past it repeat others,
+// whose columns of Y^T are dropped.
+template <int G, int TP>
+__global__ __launch_bounds__(kRowsMaxWaves * kWave, 6) void w4a16_rows_kernel(W4Args a) {
+  constexpr int DP = kRowsDepth, kGroups = kTileCols / G;
+  extern __shared__ __align__(16) uint4 lds[];
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x / kWave;
   const int tiles = (a.k + kTileCols - 1) / kTileCols, groups = a.k / G;
   const int row_tiles = (a.n + kTileRows - 1) / kTileRows;
   const long long share = static_cast<long long>(row_tiles) * blockIdx.x;
   const int begin = share / gridDim.x, end = (share + row_tiles) / gridDim.x;
-  const int per_wave = (end - begin + kRowsWaves - 1) / kRowsWaves;
+  const int per_wave = (end - begin + waves - 1) / waves;
   const int first = min(end, begin + wave * per_wave), last = min(end, first + per_wave);
   const int count = (last - first) * tiles;
 
-  // Loads run DP tiles ahead, always: past the wave's last tile they read that
-  // one again, so that the compiler knows how many are in flight.
-  int rt_ahead = first, t_ahead = 0, ahead = 0;
+  // The wave's weights, and scales, follow each other in memory.  Loads run DP
+  // tiles ahead, always: past the wave's last tile they read that one again, so
+  // that the compiler knows how many are in flight.
+  typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+  const int in_last = groups - (tiles - 1) * kGroups;  // groups of a row's last tile
+  const uint32_t s_off = ((lane & (kGroups - 1)) * kTileRows + 4 * g) * 2;
+  const uint32_t s_off_last = (min(lane & (kGroups - 1), in_last - 1) * kTileRows + 4 * g) * 2;
+  const uint8_t* w_next = a.w + static_cast<size_t>(first) * tiles * kTileBytes;
+  const char* s_next =
+      reinterpret_cast<const char*>(a.s + static_cast<size_t>(first) * groups * kTileRows);
+  int t_ahead = 0, ahead = 0;
   auto load_next = [&](W4Piece& p) {
-    load_piece<G>(p, a, rt_ahead, t_ahead, tiles, groups, lane);
+    const bool ends = t_ahead + 1 == tiles;
+    p.w = load_stream16(w_next + 16 * lane);
+    const u32x2 v = gload(reinterpret_cast<const u32x2*>(s_next + (ends ? s_off_last : s_off)));
+    p.s = make_uint2(v.x, v.y);
     if (ahead + 1 < count) {
       ++ahead;
-      if (++t_ahead == tiles) {
-        t_ahead = 0;
-        ++rt_ahead;
-      }
+      w_next += kTileBytes;
+      s_next += (ends ? in_last : kGroups) * kTileRows * 2;
+      t_ahead = ends ? 0 : t_ahead + 1;
     }
   };
   W4Piece p[DP];
@@ -189,17 +228,30 @@ __global__ __launch_bounds__(kRowsWaves * kWave, 4) void w4a16_rows_kernel(W4Arg
 #pragma unroll
     for (int i = 0; i < DP; ++i) load_next(p[i]);
   }
-  // the activations, while those are on their way
+  // the activations, while those are on their way, and the bases of them
   const int chunks = a.k / 8;
-  for (int i = threadIdx.x; i < tiles * (kTileCols / 8) * a.tokens; i += kRowsWaves * kWave) {
-    const int chunk = i / a.tokens, token = i - chunk * a.tokens;
-    lds_x[i] = chunk < chunks ? load_global16(a.x + static_cast<size_t>(token) * a.k + 8 * chunk)
-                              : make_uint4(0, 0, 0, 0);
+  for (int i = threadIdx.x; i < tiles * (kTileCols / 8) * TP; i += blockDim.x) {
+    const int chunk = i / TP, token = i % TP;
+    lds[i] = chunk < chunks && token < a.tokens
+                 ? load_global16(a.x + static_cast<size_t>(token) * a.k + 8 * chunk)
+                 : make_uint4(0, 0, 0, 0);
+  }
+  __syncthreads();
+  const int lds_lane = g * TP + r % TP;  // of a step's 4 x TP pieces
+  f32x4_t* const bases = reinterpret_cast<f32x4_t*>(lds + tiles * (kTileCols / 8) * TP);
+  for (int t = wave; t < tiles; t += waves) {
+    bf16x8_t x[4];
+    f32x4_t base[kGroups];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = __builtin_bit_cast(bf16x8_t, lds[(t * 4 + j) * 4 * TP + lds_lane]);
+    base_of<G>(base, x);
+    if (lane < TP) {
+#pragma unroll
+      for (int j = 0; j < kGroups; ++j) bases[(t * kGroups + j) * TP + lane] = base[j];
+    }
   }
   __syncthreads();
   if (count <= 0) return;
-  // Lanes past the tokens take the last one's: their columns of Y^T are dropped.
-  const uint4* const mine = lds_x + g * a.tokens + min(r, a.tokens - 1);
   const bool wide = (a.n & 3) == 0 && (reinterpret_cast<uintptr_t>(a.y) & 7u) == 0;
 
   f32x4_t total{0.0f, 0.0f, 0.0f, 0.0f};
@@ -209,11 +261,14 @@ __global__ __launch_bounds__(kRowsWaves * kWave, 4) void w4a16_rows_kernel(W4Arg
 #pragma unroll
     for (int i = 0; i < DP; ++i) {
       bf16x8_t x[4];
+      f32x4_t base[kGroups];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        x[j] = __builtin_bit_cast(bf16x8_t, mine[(t * 16 + 4 * j) * a.tokens]);
+        x[j] = __builtin_bit_cast(bf16x8_t, lds[(t * 4 + j) * 4 * TP + lds_lane]);
       }
-      add_piece<G>(total, p[i], x);
+#pragma unroll
+      for (int j = 0; j < kGroups; ++j) base[j] = bases[(t * kGroups + j) * TP + r % TP];
+      add_piece<G>(total, p[i], x, base);
       load_next(p[i]);
       if (++t == tiles) {
         const int row = rt * kTileRows + 4 * g;
@@ -287,7 +342,9 @@ __global__ __launch_bounds__(kSplitWaves * kWave) void w4a16_split_kernel(W4Args
       bf16x8_t xb[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) xb[j] = __builtin_bit_cast(bf16x8_t, x[i][j]);
-      add_piece<G>(total, p[i], xb);
+      f32x4_t base[kTileCols / G];
+      base_of<G>(base, xb);
+      add_piece<G>(total, p[i], xb, base);
     }
   }
   if (r < a.tokens) *reinterpret_cast<f32x4_t*>(&partial[wave][r][4 * g]) = total;
@@ -304,21 +361,33 @@ __global__ __launch_bounds__(kSplitWaves * kWave) void w4a16_split_kernel(W4Args
 }
 
 constexpr int kCus = 256;
+constexpr int kRowsTiles = 2048;       // row tiles from which a wave takes whole ones
+constexpr int kSplitRoom = 16 * kCus;  // waves that the split kernel fills the chip with
 
 template <int G>
 void launch_w4(const W4Args& a, hipStream_t stream) {
   const int row_tiles = (a.n + kTileRows - 1) / kTileRows;
   const int tiles = (a.k + kTileCols - 1) / kTileCols;
-  const size_t x_bytes = static_cast<size_t>(tiles) * kTileCols * 2 * a.tokens;
-  constexpr int kResident = kCus * 2 * kRowsWaves;  // waves of two workgroups a CU
-  if (row_tiles >= kResident / 2 && x_bytes <= kRowsX) {
-    hipLaunchKernelGGL((w4a16_rows_kernel<G>), dim3(kRowsGroups), dim3(kRowsWaves * kWave), x_bytes,
-                       stream, a);
+  const int pitch = a.tokens == 1 ? 1 : a.tokens <= 4 ? 4 : 16;
+  for (const RowsShape& shape : kRowsShapes) {
+    const size_t lds = rows_lds_bytes(tiles, pitch, G);
+    if (row_tiles < kRowsTiles || lds > shape.lds) continue;
+    auto launch = [&](auto tp) {
+      hipLaunchKernelGGL((w4a16_rows_kernel<G, decltype(tp)::value>), dim3(shape.per_cu * kCus),
+                         dim3(shape.waves * kWave), lds, stream, a);
+    };
+    if (pitch == 1) {
+      launch(std::integral_constant<int, 1>{});
+    } else if (pitch == 4) {
+      launch(std::integral_constant<int, 4>{});
+    } else {
+      launch(std::integral_constant<int, 16>{});
+    }
     return;
   }
-  // Waves for the chip's room, at least two, of equal shares of the tiles.
-  const int room = kResident / row_tiles;
-  const int most = room < 2 ? 2 : room > kSplitWaves ? kSplitWaves : room;
+  // Waves for the chip's room, at least eight, of equal shares of the tiles.
+  const int room = kSplitRoom / row_tiles;
+  const int most = room < 8 ? 8 : room > kSplitWaves ? kSplitWaves : room;
   const int per = (tiles + most - 1) / most;
   const int waves = (tiles + per - 1) / per;
   auto launch = [&](auto depth) {
