@@ -311,23 +311,32 @@ __global__ __launch_bounds__(kRowsMaxWaves * kWave, 6) void w4a16_rows_kernel(W4
 
 constexpr int kSplitWaves = 16;
 
-// Workgroup i: row tile i; wave w takes its column tiles w, w + waves, ...
-template <int G, int DP>
+// Workgroup i: row tiles [i R, (i + 1) R); wave w takes their column tiles w, w +
+// waves, ..., DP of them in flight.  With R > 1 the activations, four KiB a tile
+// at 16 tokens, are read for R KiB of weights.
+template <int G, int DP, int R>
 __global__ __launch_bounds__(kSplitWaves * kWave) void w4a16_split_kernel(W4Args a) {
-  __shared__ float partial[kSplitWaves][kMaxTokens][kTileRows + 4];
+  constexpr int kPitch = R * kTileRows + 4;
+  extern __shared__ __align__(16) float partial[];  // [wave][token][kPitch]
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x / kWave;
   const int tiles = (a.k + kTileCols - 1) / kTileCols, groups = a.k / G;
-  const int rt = blockIdx.x;
+  const int row_tiles = (a.n + kTileRows - 1) / kTileRows;
+  const int first = blockIdx.x * R;
   const uint16_t* x_row = a.x + static_cast<size_t>(min(r, a.tokens - 1)) * a.k + 8 * g;
-  f32x4_t total{0.0f, 0.0f, 0.0f, 0.0f};
+  f32x4_t total[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) total[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   for (int t0 = wave; t0 < tiles; t0 += DP * waves) {
-    W4Piece p[DP];
+    W4Piece p[DP][R];
     uint4 x[DP][4];
 #pragma unroll
-    for (int i = 0; i < DP; ++i) {  // past the last tile: that one again
+    for (int i = 0; i < DP; ++i) {  // past the last tile, or row tile: that one again
       const int t = min(t0 + i * waves, tiles - 1);
-      load_piece<G>(p[i], a, rt, t, tiles, groups, lane);
+#pragma unroll
+      for (int j = 0; j < R; ++j) {
+        load_piece<G>(p[i][j], a, min(first + j, row_tiles - 1), t, tiles, groups, lane);
+      }
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         // columns past K count for nothing, from wherever they are read
@@ -344,16 +353,24 @@ __global__ __launch_bounds__(kSplitWaves * kWave) void w4a16_split_kernel(W4Args
       for (int j = 0; j < 4; ++j) xb[j] = __builtin_bit_cast(bf16x8_t, x[i][j]);
       f32x4_t base[kTileCols / G];
       base_of<G>(base, xb);
-      add_piece<G>(total, p[i], xb, base);
+#pragma unroll
+      for (int j = 0; j < R; ++j) add_piece<G>(total[j], p[i][j], xb, base);
     }
   }
-  if (r < a.tokens) *reinterpret_cast<f32x4_t*>(&partial[wave][r][4 * g]) = total;
+  if (r < a.tokens) {
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      *reinterpret_cast<f32x4_t*>(partial + (wave * a.tokens + r) * kPitch + j * kTileRows + 4 * g) =
+          total[j];
+    }
+  }
   __syncthreads();
-  for (int e = threadIdx.x; e < kTileRows * a.tokens; e += blockDim.x) {
-    const int token = e / kTileRows, i = e % kTileRows, row = rt * kTileRows + i;
+  for (int e = threadIdx.x; e < R * kTileRows * a.tokens; e += blockDim.x) {
+    const int token = e / (R * kTileRows), i = e % (R * kTileRows);
+    const int row = first * kTileRows + i;
     if (row >= a.n) continue;
     float v = 0.0f;
-    for (int w = 0; w < waves; ++w) v += partial[w][token][i];
+    for (int w = 0; w < waves; ++w) v += partial[(w * a.tokens + token) * kPitch + i];
     const uint16_t y = finish(a, v, row);
     a.y[static_cast<size_t>(token) * a.n + row] = y;
     if (not_finite(y)) finish_exactly(a, row, token);
@@ -362,6 +379,7 @@ __global__ __launch_bounds__(kSplitWaves * kWave) void w4a16_split_kernel(W4Args
 
 constexpr int kCus = 256;
 constexpr int kRowsTiles = 2048;       // row tiles from which a wave takes whole ones
+constexpr int kPairTiles = 1024;       // row tiles from which the split kernel takes two, of 9 tokens up
 constexpr int kSplitRoom = 16 * kCus;  // waves that the split kernel fills the chip with
 
 template <int G>
@@ -390,16 +408,26 @@ void launch_w4(const W4Args& a, hipStream_t stream) {
   const int most = room < 8 ? 8 : room > kSplitWaves ? kSplitWaves : room;
   const int per = (tiles + most - 1) / most;
   const int waves = (tiles + per - 1) / per;
-  auto launch = [&](auto depth) {
-    hipLaunchKernelGGL((w4a16_split_kernel<G, decltype(depth)::value>), dim3(row_tiles),
-                       dim3(waves * kWave), 0, stream, a);
+  auto launch = [&](auto depth, auto rows) {
+    constexpr int R = decltype(rows)::value;
+    const size_t lds = static_cast<size_t>(waves) * a.tokens * (R * kTileRows + 4) * sizeof(float);
+    hipLaunchKernelGGL((w4a16_split_kernel<G, decltype(depth)::value, R>),
+                       dim3((row_tiles + R - 1) / R), dim3(waves * kWave), lds, stream, a);
   };
-  if (per == 1) {
-    launch(std::integral_constant<int, 1>{});
+  using One = std::integral_constant<int, 1>;
+  using Two = std::integral_constant<int, 2>;
+  if (row_tiles >= kPairTiles && a.tokens > 8) {
+    if (per == 1) {
+      launch(One{}, Two{});
+    } else {
+      launch(Two{}, Two{});
+    }
+  } else if (per == 1) {
+    launch(One{}, One{});
   } else if (per == 2) {
-    launch(std::integral_constant<int, 2>{});
+    launch(Two{}, One{});
   } else {
-    launch(std::integral_constant<int, 3>{});
+    launch(std::integral_constant<int, 3>{}, One{});
   }
 }
 

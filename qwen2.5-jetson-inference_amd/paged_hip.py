@@ -129,42 +129,44 @@ class KvPages:
 
 def _at(t, dtype, pages, name):
     """Pointer of a contiguous tensor of a type on the pool's GPU."""
-    if t.dtype is not dtype or t.get_device() != pages.index or not t.is_contiguous():
-        _bad(f"{name} must be contiguous {dtype} on {pages.device} (got {t.dtype} on {t.device})")
-    return t.data_ptr()
+    if t.dtype is dtype and t.get_device() == pages.index and t.is_contiguous():
+        return t.data_ptr()
+    _bad(f"{name} must be contiguous {dtype} on {pages.device} (got {t.dtype} on {t.device})")
 
 
 def _table(table, pages):
     """infer_hip_kv_table of an int32 tensor [sequences, pages] whose rows may be
     longer (a slice of a wider table)."""
-    shape = table.shape
-    if table.dtype is not _I32 or len(shape) != 2 or table.get_device() != pages.index:
+    if table.dtype is not _I32 or table.dim() != 2 or table.get_device() != pages.index:
         _bad("block table must be int32 [sequences, pages] on the pool's GPU")
-    rows, width = shape
+    rows, width = table.shape
     stride, inner = table.stride()
     if inner != 1 and width > 1:
         _bad("block table rows must be contiguous")
     return _Table(table.data_ptr(), rows, width, stride if rows > 1 else width)
 
 
-def _rows(t, tokens, heads, pages, name):
+def _rows(t, shape, pages, name):
     """Pointer and token stride of BF16 [tokens, heads, head_dim] with
     contiguous tokens."""
-    if t.dtype is not _BF16 or t.get_device() != pages.index:
-        _bad(f"{name} must be bfloat16 on the pool's GPU")
-    shape, d = t.shape, pages.head_dim
-    if shape != (tokens, heads, d):
-        _bad(f"{name} must be [{tokens}, {heads}, {d}] (got {tuple(shape)})")
+    if t.dtype is not _BF16 or t.get_device() != pages.index or t.shape != shape:
+        _bad(f"{name} must be bfloat16 {list(shape)} on {pages.device} (got {t.dtype} "
+             f"{list(t.shape)} on {t.device})")
     stride, between, inner = t.stride()
-    if inner != 1 or (heads > 1 and between != d):
+    if inner != 1 or (between != shape[2] and shape[1] > 1):
         _bad(f"{name}: a token's heads must be contiguous")
-    return t.data_ptr(), stride if tokens > 1 else heads * d
+    return t.data_ptr(), stride if shape[0] > 1 else shape[1] * shape[2]
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _on(pages, stream):
     """The stream, of the pool's GPU, which must be the current one."""
     if torch.cuda.current_device() != pages.index:
         _bad(f"the pool is on {pages.device}, the current device is {torch.cuda.current_device()}")
+    if stream is None and _raw_stream is not None:
+        return _raw_stream(pages.index)
     return _stream(stream)
 
 
@@ -176,24 +178,25 @@ def kv_pages_store(pages, table, positions, query, key, value, query_out=None, r
     sequences int32 [tokens] or None (token t belongs to sequence t).  query
     None: only the cache is written."""
     on = _on(pages, stream)
-    tokens, kv = positions.numel(), pages.num_kv_heads
+    tokens, d = positions.numel(), pages.head_dim
     tab = _table(table, pages)
     qp = qo = rp = sp = None
     qs = os_ = heads = rn = 0
     if query is not None:
-        heads = query.shape[1] if query.dim() == 3 else 0
-        if query_out is None or not heads:
+        if query_out is None or query.dim() != 3:
             _bad("query and query_out must be [tokens, heads, head_dim]")
-        qp, qs = _rows(query, tokens, heads, pages, "query")
-        qo, os_ = (qp, qs) if query_out is query else _rows(query_out, tokens, heads, pages,
-                                                            "query_out")
-    kp, ks = _rows(key, tokens, kv, pages, "key")
-    vp, vs = _rows(value, tokens, kv, pages, "value")
+        heads = query.shape[1]
+        shape = (tokens, heads, d)
+        qp, qs = _rows(query, shape, pages, "query")
+        qo, os_ = (qp, qs) if query_out is query else _rows(query_out, shape, pages, "query_out")
+    shape = (tokens, pages.num_kv_heads, d)
+    kp, ks = _rows(key, shape, pages, "key")
+    vp, vs = _rows(value, shape, pages, "value")
     if rope is not None:
-        shape = rope.shape
-        if shape[1:] != (pages.head_dim // 2, 2):
+        rn = rope.shape[0]
+        if rope.shape != (rn, d // 2, 2):
             _bad("rope must be float32 [positions, head_dim / 2, 2]")
-        rp, rn = _at(rope, _F32, pages, "rope"), shape[0]
+        rp = _at(rope, _F32, pages, "rope")
     if sequences is not None:
         if sequences.numel() != tokens:
             _bad(f"sequences must hold {tokens} tokens")
@@ -236,7 +239,10 @@ def attention_paged_decode(pages, table, lengths, query, output, workspace, stre
     shape = query.shape
     if len(shape) != 3 or output.shape != shape:
         _bad("query and output must be [sequences, heads, head_dim]")
-    qp, qs = _rows(query, tab.num_sequences, shape[1], pages, "query")
+    if shape[0] != tab.num_sequences or shape[2] != pages.head_dim:
+        _bad(f"query of {shape[0]} sequences and head_dim {shape[2]}: the table has "
+             f"{tab.num_sequences}, the pool {pages.head_dim}")
+    qp, qs = _rows(query, shape, pages, "query")
     if lengths.numel() != tab.num_sequences:
         _bad(f"lengths must hold {tab.num_sequences} sequences")
     _check(load().infer_hip_attention_paged_decode(
