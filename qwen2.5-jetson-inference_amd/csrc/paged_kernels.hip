@@ -3,6 +3,8 @@
 #include <float.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "device_common.hpp"
 #include "paged_kernels.hpp"
 
@@ -587,8 +589,11 @@ __global__ __launch_bounds__(W * kWave, 2) void paged_attention_kernel(PagedAttn
       look_up(next);
     }
 
-    for (int idx = start; idx < end; ++idx) {
-      const bool more = idx + 1 < end;
+    // One tile; MORE (a constant): another follows, whose loads are issued on the
+    // way.  The last tile is apart from the loop, so that every pass of the loop
+    // has the same loads in flight and waits for those it needs alone.
+    auto step = [&](int idx, auto more_tiles) {
+      constexpr bool more = decltype(more_tiles)::value;
       // S of both halves, times the keys' scales
       float s[8];
 #pragma unroll
@@ -725,7 +730,9 @@ __global__ __launch_bounds__(W * kWave, 2) void paged_attention_kernel(PagedAttn
           look_up(next);
         }
       }
-    }
+    };
+    for (int idx = start; idx < end - 1; ++idx) step(idx, std::true_type{});
+    step(end - 1, std::false_type{});
   }
 
   // ---- empty sequences
