@@ -238,8 +238,7 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kTileKeys = 32;
 constexpr int kHeadBlock = 16;       // query heads of a unit at most
-constexpr int kJoinThreads = 512;    // of the join, and the parts a thread has in flight
-constexpr int kJoinBatch = 8;
+constexpr int kJoinBatch = 8;          // parts a thread of the join has in flight
 constexpr float kRescaleSlack = 6.0f;  // p <= 2^6 before the maximum is moved
 
 // A uniform 32-bit word that nothing writes while the kernel runs, through the
@@ -797,11 +796,12 @@ __global__ __launch_bounds__(W * kWave, 2) void paged_attention_kernel(PagedAttn
   }
 }
 
-// Joins the units that lie over several workgroups of the launch before: one
-// workgroup per (unit, sequence), or (a.join_heads 1) per query head of one.
-template <int D, int W>
-__global__ __launch_bounds__(kJoinThreads) void paged_attention_join_kernel(PagedAttnArgs a) {
-  __shared__ __align__(16) float smem[kJoinThreads * 6];
+// Joins the units that lie over several workgroups of the launch before, of W
+// waves: a workgroup of T threads per (unit, sequence), or (a.join_heads 1) per
+// query head of one.
+template <int D, int W, int T>
+__global__ __launch_bounds__(T) void paged_attention_join_kernel(PagedAttnArgs a) {
+  __shared__ __align__(16) float smem[T * 6];
   const int lane = threadIdx.x & 63;
   const int seq = blockIdx.y;
   const int cap = a.table.max_pages << a.pool.page_shift;
@@ -830,8 +830,8 @@ __global__ __launch_bounds__(kJoinThreads) void paged_attention_join_kernel(Page
 
   // The threads are as many rows of `items` as fit, row i taking parts i, i +
   // rows, ...; what the rows found is joined through LDS.
-  const int rows = max(1, kJoinThreads / items), row = rows > 1 ? threadIdx.x / items : 0;
-  for (int e0 = 0; e0 < items; e0 += kJoinThreads) {
+  const int rows = max(1, T / items), row = rows > 1 ? threadIdx.x / items : 0;
+  for (int e0 = 0; e0 < items; e0 += T) {
     const int e = rows > 1 ? static_cast<int>(threadIdx.x) - row * items
                            : e0 + static_cast<int>(threadIdx.x);
     const bool busy = e < items && row < rows;
@@ -940,7 +940,17 @@ void launch_kv_load(const KvLoadArgs& a, hipStream_t stream) {
 // 128, in workgroups of 8 (of 4 where a unit has more than 8 query heads, whose
 // states fill the LDS).
 constexpr int kCus = 256;
-constexpr int kWholeTiles = 32;  // a unit of more is cut
+// Units of more tiles are cut.  The join's launch takes about 3.7 us; a unit left
+// whole is read by one CU, 1.2 us a tile of each wave (one sequence of 14 / 2 / 64
+// heads in BF16: 500 keys 7.4 whole against 9.9 cut, 1000 keys 9.9 against 9.8;
+// 28 / 4 / 128 in INT8: 500 keys 9.2 against 10.3, 1000 keys 12.3 against 10.4).
+// With more than two units a workgroup the pieces' sizes differ by up to a unit,
+// 0.3 us a tile (100 sequences of 500 keys, 28 / 4 / 128 in BF16: 15.7 against
+// 17.6; beyond, only small ones stay whole).
+constexpr int kWholeTiles = 24, kWholeTilesMany = 8;
+// Parts of a unit from which a workgroup of the join has 512 threads (1 x 131001
+// keys, 128 parts: 34.6 us, 38.0 with 256; 16 x 1000 keys: 11.2 and 10.1).
+constexpr int kJoinParts = 96;
 
 struct PagedAttnShape {
   int head_blocks, units, waves_per_group, groups, record_floats;
@@ -983,7 +993,7 @@ void launch_paged_attention(PagedAttnArgs a, hipStream_t stream) {
   const unsigned groups = static_cast<unsigned>(wanted < s.groups ? wanted : s.groups);
   a.waves = groups * s.waves_per_group;
   const long long pieces = static_cast<long long>(a.table.sequences) * s.units;
-  a.whole = most_tiles(a) <= (pieces <= s.groups ? kWholeTiles : kWholeTiles / 2);
+  a.whole = most_tiles(a) <= (pieces <= 2 * s.groups ? kWholeTiles : kWholeTilesMany);
   a.join_heads = pieces <= 64;
   by_format(a.pool, [&](auto f, auto d) {
     constexpr int F = decltype(f)::value, D = decltype(d)::value;
@@ -999,9 +1009,14 @@ void launch_paged_attention(PagedAttnArgs a, hipStream_t stream) {
   const int per_kv = a.heads / a.pool.kv_heads;
   const int hb = per_kv < kHeadBlock ? per_kv : kHeadBlock;
   const dim3 grid(a.join_heads ? s.units * hb : s.units, a.table.sequences);
+  const long long parts = s.groups / pieces < wanted / pieces ? s.groups / pieces : wanted / pieces;
   auto join = [&](auto d, auto w) {
-    hipLaunchKernelGGL((paged_attention_join_kernel<decltype(d)::value, decltype(w)::value>), grid,
-                       dim3(kJoinThreads), 0, stream, a);
+    constexpr int D = decltype(d)::value, W = decltype(w)::value;
+    if (parts >= kJoinParts) {
+      hipLaunchKernelGGL((paged_attention_join_kernel<D, W, 512>), grid, dim3(512), 0, stream, a);
+    } else {
+      hipLaunchKernelGGL((paged_attention_join_kernel<D, W, 256>), grid, dim3(256), 0, stream, a);
+    }
   };
   auto by_waves = [&](auto d) {
     if (s.waves_per_group == 8) {
