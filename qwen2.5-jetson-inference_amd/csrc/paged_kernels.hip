@@ -796,10 +796,10 @@ __global__ __launch_bounds__(W * kWave, 2) void paged_attention_kernel(PagedAttn
   }
 }
 
-// Joins the units that lie over several workgroups of the launch before, of W
-// waves: a workgroup of T threads per (unit, sequence), or (a.join_heads 1) per
-// query head of one.
-template <int D, int W, int T>
+// Joins the units that lie over several workgroups of the launch before: a
+// workgroup of T threads per (unit, sequence), or (a.join_heads 1) per query head
+// of one.
+template <int D, int T>
 __global__ __launch_bounds__(T) void paged_attention_join_kernel(PagedAttnArgs a) {
   __shared__ __align__(16) float smem[T * 6];
   const int lane = threadIdx.x & 63;
@@ -817,7 +817,7 @@ __global__ __launch_bounds__(T) void paged_attention_join_kernel(PagedAttnArgs a
   before = __builtin_amdgcn_readlane(wave_scan(before), kWave - 1);
   all = __builtin_amdgcn_readlane(wave_scan(all), kWave - 1);
   tiles = __builtin_amdgcn_readlane(wave_scan(tiles), kWave - 1);
-  const int piece = piece_of(all * a.units, a.waves) * W;
+  const int piece = piece_of(all * a.units, a.waves) * a.piece_waves;
   const int unit = a.join_heads ? blockIdx.x / hb : blockIdx.x;
   const int first = before * a.units + unit * tiles;
   const int from = first / piece, to = (first + tiles - 1) / piece;
@@ -952,8 +952,18 @@ constexpr int kWholeTiles = 24, kWholeTilesMany = 8;
 // keys, 128 parts: 34.6 us, 38.0 with 256; 16 x 1000 keys: 11.2 and 10.1).
 constexpr int kJoinParts = 96;
 
+// Workgroups of 4 waves instead of 8 start and meet sooner, and spread cut units
+// over more CUs: where all units are whole and small or few (1 x 101 keys 5.5 ->
+// 4.8 us, 100 x 250 of 14 / 2 / 64 heads 7.4 -> 6.5, but 100 x 500 8.7 -> 9.9), and
+// for cut ones of calls with at most kSmallTiles tiles (16 x 2000 keys 10.7 -> 10.0;
+// 1 x 100000, as many waves and twice the parts, 16.0 -> 19.1).
+constexpr int kSmallWholeTiles = 8, kSmallWholeUnits = 64, kSmallTiles = 4096;
+
 struct PagedAttnShape {
-  int head_blocks, units, waves_per_group, groups, record_floats;
+  int head_blocks, units;
+  int block_heads;  // query heads of a full unit
+  int max_groups;   // workgroups at most
+  int record_floats;
 };
 
 static PagedAttnShape paged_attention_shape(int heads, int kv_heads, int head_dim) {
@@ -961,15 +971,15 @@ static PagedAttnShape paged_attention_shape(int heads, int kv_heads, int head_di
   const int per_kv = heads / kv_heads;
   s.head_blocks = (per_kv + kHeadBlock - 1) / kHeadBlock;
   s.units = kv_heads * s.head_blocks;
-  s.waves_per_group = per_kv <= 8 ? 8 : 4;
-  s.groups = 8 / s.waves_per_group * kCus;
-  s.record_floats = (per_kv < kHeadBlock ? per_kv : kHeadBlock) * (head_dim + 4);
+  s.block_heads = per_kv < kHeadBlock ? per_kv : kHeadBlock;
+  s.max_groups = 2 * kCus;
+  s.record_floats = s.block_heads * (head_dim + 4);
   return s;
 }
 
-size_t paged_attention_workspace_bytes(int, int heads, int kv_heads, int head_dim) {
+size_t paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim) {
   const PagedAttnShape s = paged_attention_shape(heads, kv_heads, head_dim);
-  return static_cast<size_t>(s.groups) * 2 * s.record_floats * sizeof(float);
+  return static_cast<size_t>(s.max_groups) * 2 * s.record_floats * sizeof(float);
 }
 
 // Tiles of a sequence that fills its table.
@@ -980,55 +990,55 @@ static long long most_tiles(const PagedAttnArgs& a) {
 
 bool paged_attention_supported(const PagedAttnArgs& a) {
   const PagedAttnShape s = paged_attention_shape(a.heads, a.pool.kv_heads, a.pool.head_dim);
-  return static_cast<double>(most_tiles(a)) * a.table.sequences * s.units < 2147000000.0;
+  return most_tiles(a) * a.table.sequences * s.units < 2147000000LL;
 }
 
 void launch_paged_attention(PagedAttnArgs a, hipStream_t stream) {
   const PagedAttnShape s = paged_attention_shape(a.heads, a.pool.kv_heads, a.pool.head_dim);
   a.head_blocks = s.head_blocks;
   a.units = s.units;
+  const long long tiles = most_tiles(a), units = static_cast<long long>(a.table.sequences) * s.units;
+  a.whole = tiles <= (units <= 2 * kCus ? kWholeTiles : kWholeTilesMany);
+  const bool small =
+      s.block_heads > 8 || (a.whole ? tiles <= kSmallWholeTiles || units <= kSmallWholeUnits
+                                    : tiles * units <= kSmallTiles);
   // no more workgroups than the tables have tiles for, one a wave
-  const long long most = most_tiles(a) * a.table.sequences * s.units;
-  const long long wanted = (most + s.waves_per_group - 1) / s.waves_per_group;
-  const unsigned groups = static_cast<unsigned>(wanted < s.groups ? wanted : s.groups);
-  a.waves = groups * s.waves_per_group;
-  const long long pieces = static_cast<long long>(a.table.sequences) * s.units;
-  a.whole = most_tiles(a) <= (pieces <= 2 * s.groups ? kWholeTiles : kWholeTilesMany);
-  a.join_heads = pieces <= 64;
+  const int waves = small ? 4 : 8, room = small ? 2 * kCus : kCus;
+  const long long wanted = (tiles * units + waves - 1) / waves;
+  const int groups = static_cast<int>(wanted < room ? wanted : room);
+  a.waves = groups * waves;
   by_format(a.pool, [&](auto f, auto d) {
     constexpr int F = decltype(f)::value, D = decltype(d)::value;
-    if (s.waves_per_group == 8) {
-      hipLaunchKernelGGL((paged_attention_kernel<F, D, 8, 8>), dim3(groups), dim3(8 * kWave), 0,
+    if (s.block_heads > 8) {
+      hipLaunchKernelGGL((paged_attention_kernel<F, D, 4, 16>), dim3(groups), dim3(4 * kWave), 0,
+                         stream, a);
+    } else if (small) {
+      hipLaunchKernelGGL((paged_attention_kernel<F, D, 4, 8>), dim3(groups), dim3(4 * kWave), 0,
                          stream, a);
     } else {
-      hipLaunchKernelGGL((paged_attention_kernel<F, D, 4, 16>), dim3(groups), dim3(4 * kWave), 0,
+      hipLaunchKernelGGL((paged_attention_kernel<F, D, 8, 8>), dim3(groups), dim3(8 * kWave), 0,
                          stream, a);
     }
   });
   if (a.whole) return;
-  const int per_kv = a.heads / a.pool.kv_heads;
-  const int hb = per_kv < kHeadBlock ? per_kv : kHeadBlock;
-  const dim3 grid(a.join_heads ? s.units * hb : s.units, a.table.sequences);
-  const long long parts = s.groups / pieces < wanted / pieces ? s.groups / pieces : wanted / pieces;
-  auto join = [&](auto d, auto w) {
-    constexpr int D = decltype(d)::value, W = decltype(w)::value;
-    if (parts >= kJoinParts) {
-      hipLaunchKernelGGL((paged_attention_join_kernel<D, W, 512>), grid, dim3(512), 0, stream, a);
+  a.join_heads = units <= 64;
+  a.piece_waves = waves;
+  const dim3 grid(a.join_heads ? s.units * s.block_heads : s.units, a.table.sequences);
+  auto join = [&](auto d, auto threads) {
+    constexpr int D = decltype(d)::value, T = decltype(threads)::value;
+    hipLaunchKernelGGL((paged_attention_join_kernel<D, T>), grid, dim3(T), 0, stream, a);
+  };
+  auto by_dim = [&](auto threads) {
+    if (a.pool.head_dim == 64) {
+      join(std::integral_constant<int, 64>{}, threads);
     } else {
-      hipLaunchKernelGGL((paged_attention_join_kernel<D, W, 256>), grid, dim3(256), 0, stream, a);
+      join(std::integral_constant<int, 128>{}, threads);
     }
   };
-  auto by_waves = [&](auto d) {
-    if (s.waves_per_group == 8) {
-      join(d, std::integral_constant<int, 8>{});
-    } else {
-      join(d, std::integral_constant<int, 4>{});
-    }
-  };
-  if (a.pool.head_dim == 64) {
-    by_waves(std::integral_constant<int, 64>{});
+  if (groups / units >= kJoinParts) {
+    by_dim(std::integral_constant<int, 512>{});
   } else {
-    by_waves(std::integral_constant<int, 128>{});
+    by_dim(std::integral_constant<int, 256>{});
   }
 }
 

@@ -68,6 +68,7 @@ struct PagedAttnArgs {
   int waves;        // of the grid
   int whole;        // units are not cut
   int join_heads;   // a workgroup of the join per query head
+  int piece_waves;  // of a workgroup that the join's parts come from
 };
 
 void launch_kv_store(const KvStoreArgs& a, hipStream_t stream);
@@ -75,6 +76,6 @@ void launch_kv_load(const KvLoadArgs& a, hipStream_t stream);
 // Whether the tiles of the largest possible lengths can be counted in 32 bits.
 bool paged_attention_supported(const PagedAttnArgs& a);
 void launch_paged_attention(PagedAttnArgs a, hipStream_t stream);
-size_t paged_attention_workspace_bytes(int sequences, int heads, int kv_heads, int head_dim);
+size_t paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim);
 
 }  // namespace qlin

@@ -174,7 +174,7 @@ extern "C" size_t infer_hip_attention_paged_decode_workspace_bytes(int num_seque
       (head_dim != 64 && head_dim != 128)) {
     return 0;
   }
-  return paged_attention_workspace_bytes(num_sequences, num_heads, num_kv_heads, head_dim);
+  return paged_attention_workspace_bytes(num_heads, num_kv_heads, head_dim);
 }
 
 extern "C" int infer_hip_attention_paged_decode(const infer_hip_kv_pages* pages,
@@ -197,8 +197,7 @@ extern "C" int infer_hip_attention_paged_decode(const infer_hip_kv_pages* pages,
   if (rc == INFER_HIP_OK) rc = check_rows(output, row, row, "output", what);
   if (rc != INFER_HIP_OK) return rc;
   if (!lengths) return fail(INFER_HIP_INVALID_ARGUMENT, "%s: null lengths", what);
-  const size_t need = paged_attention_workspace_bytes(a.table.sequences, num_heads,
-                                                      a.pool.kv_heads, a.pool.head_dim);
+  const size_t need = paged_attention_workspace_bytes(num_heads, a.pool.kv_heads, a.pool.head_dim);
   if (!workspace || !aligned16(workspace) || workspace_bytes < need) {
     return fail(INFER_HIP_INVALID_ARGUMENT,
                 "%s: workspace of %zu bytes, 16-byte aligned, needed (%zu given)", what, need,
