@@ -131,8 +131,11 @@ int infer_hip_gemm_w8a16(const int8_t* weight, const uint16_t* scales,
  *   Y[t,n] = bf16(sum_g s[n,g] (sum_{k in group g} q[n,k] X[t,k]) + bias[n])
  * with q in [-8, 7], group_size 32, 64 or 128 dividing in_features, BF16
  * scales, FP32 sums and 1 to 16 tokens ([tokens, in_features] in,
- * [tokens, out_features] out).  weight, scales and input are 16-byte
- * aligned.
+ * [tokens, out_features] out, which overlaps no input).  weight, scales and
+ * input are 16-byte aligned; out_features <= 2^28, in_features <= 2^24.
+ * Terms of a group's sum are taken of (q + 24) / 16 and 24 / 16, so its
+ * rounding goes by 31 |X|; where a sum overflows it is taken again of q s X,
+ * so infinities and NaN come out as that sum's.
  *
  * The weights are laid out once, in tiles of 16 rows by 128 columns that a
  * wave reads as one contiguous KiB: weight holds

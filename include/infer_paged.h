@@ -70,8 +70,8 @@ typedef struct infer_hip_kv_pages {
 typedef struct infer_hip_kv_table {
   const int* pages;
   int num_sequences; /* at most 65535 */
-  int max_pages;
-  int stride; /* entries between rows, >= max_pages */
+  int max_pages;     /* at most 2^30 positions */
+  int stride;        /* entries between rows, >= max_pages */
 } infer_hip_kv_table;
 
 /* For each of `tokens` tokens t at positions[t] of sequence sequences[t]
@@ -117,7 +117,8 @@ int infer_hip_kv_pages_load(const infer_hip_kv_pages* pages, const infer_hip_kv_
  * between sequences (a multiple of 8), already rotated; output is contiguous;
  * both 16-byte aligned.  FP32 softmax statistics and sums.  A length of zero or
  * less (an empty slot of the batch) gives zeros; a length past the table's
- * pages ends there.  A sequence whose pages within its length are not all in
+ * pages ends there.  Scores that are all -infinity give NaN, as the quotient
+ * does.  A sequence whose pages within its length are not all in
  * the pool gives NaN.  Rows behind a sequence's length never count, whatever
  * they hold.
  *

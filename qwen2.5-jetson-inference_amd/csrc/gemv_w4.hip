@@ -431,6 +431,9 @@ void launch_w4(const W4Args& a, hipStream_t stream) {
   }
 }
 
+// Sizes whose padded forms can be counted in 32 bits.
+constexpr int kMaxRows = 1 << 28, kMaxCols = 1 << 24;
+
 bool group_ok(int group, int k) {
   return (group == 32 || group == 64 || group == 128) && k > 0 && k % group == 0;
 }
@@ -503,6 +506,10 @@ extern "C" int infer_hip_gemv_w4a16(const uint8_t* weight, const uint16_t* scale
     return fail(INFER_HIP_INVALID_ARGUMENT,
                 "gemv_w4a16: N=%d K=%d group %d (32, 64 or 128, dividing K)", out_features,
                 in_features, group_size);
+  }
+  if (out_features > kMaxRows || in_features > kMaxCols) {
+    return fail(INFER_HIP_INVALID_ARGUMENT, "gemv_w4a16: N=%d K=%d are over %d x %d", out_features,
+                in_features, kMaxRows, kMaxCols);
   }
   if (tokens < 1 || tokens > kMaxTokens) {
     return fail(INFER_HIP_INVALID_ARGUMENT, "gemv_w4a16: %d tokens (1 to %d)", tokens, kMaxTokens);

@@ -377,9 +377,9 @@ __device__ __forceinline__ int piece_of(int total, int waves) {
   return max(1, (total + waves - 1) / waves);
 }
 
-// Four dimensions of the output from O and the sum of the weights (0: no keys).
+// Four dimensions of the output from O and the sum of the weights.
 __device__ __forceinline__ void store_out(uint16_t* out, f32x4_t o, float sum) {
-  const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+  const float inv = 1.0f / sum;
   store_global8(out, make_uint2(pack2_bf16(o[0] * inv, o[1] * inv),
                                 pack2_bf16(o[2] * inv, o[3] * inv)));
 }
@@ -677,7 +677,7 @@ __global__ __launch_bounds__(W * kWave, 2) void paged_attention_kernel(PagedAttn
         const int h = t.block * kHeadBlock + r;
         if (begin == 0 && t.tile + 1 == t.tiles) {
           if (h < heads_per_kv) {
-            const float inv = sum_l == 0.0f ? 0.0f : 1.0f / sum_l;
+            const float inv = 1.0f / sum_l;
             uint16_t* out = a.out + (static_cast<size_t>(t.seq) * a.heads + t.kvh * heads_per_kv + h) * D +
                             4 * g * NO;
 #pragma unroll

@@ -14,6 +14,7 @@ using namespace qlin;
 namespace {
 
 constexpr int kMaxSequences = 65535;  // a grid dimension
+constexpr int kMaxPositions = 1 << 30;  // of a sequence
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
@@ -54,10 +55,11 @@ int check_table(const infer_hip_kv_table* t, const KvPool& pool, KvTable* out,
                 const char* what) {
   if (!t || !t->pages) return fail(INFER_HIP_INVALID_ARGUMENT, "%s: null block table", what);
   if (t->num_sequences < 1 || t->num_sequences > kMaxSequences || t->max_pages < 1 ||
-      t->stride < t->max_pages || t->max_pages > (INT_MAX >> pool.page_shift)) {
+      t->stride < t->max_pages || t->max_pages > (kMaxPositions >> pool.page_shift)) {
     return fail(INFER_HIP_INVALID_ARGUMENT,
-                "%s: bad block table (%d sequences of at most %d, %d pages, stride %d)", what,
-                t->num_sequences, kMaxSequences, t->max_pages, t->stride);
+                "%s: bad block table (%d sequences of at most %d, %d pages of at most %d "
+                "positions, stride %d)",
+                what, t->num_sequences, kMaxSequences, t->max_pages, kMaxPositions, t->stride);
   }
   *out = KvTable{t->pages, t->num_sequences, t->max_pages, t->stride};
   return INFER_HIP_OK;

@@ -62,6 +62,37 @@ def test_many_rows(hip, dev, group):
     check(run(hip, dev, q, s, group, b, x), *ref.product(q, s, group, b, x))
 
 
+# Whole row tiles a wave (32768 rows up): one token, a few, sixteen; groups that end
+# inside a column tile; rows that end inside a tile or a 4-row piece; LDS for three,
+# two and one workgroup a CU, and too little.  Pairs of row tiles (16384 rows up and
+# 9 tokens up) with one and several column tiles a wave.
+@pytest.mark.parametrize("n,k,group,tokens", [
+    (33001, 160, 32, 16), (32773, 1088, 64, 1), (40008, 4096, 128, 16), (33000, 96, 32, 2),
+    (34567, 2432, 64, 9), (50001, 1536, 64, 4), (32768, 32, 32, 1), (33000, 8960, 64, 16),
+    (20001, 384, 64, 12), (18000, 4864, 128, 16), (17001, 3168, 32, 9), (20003, 2048, 32, 8)])
+def test_product_of_many_rows(hip, dev, n, k, group, tokens):
+    q, s, x, b = make(n, k, group, tokens, n + k, bias=tokens % 2 == 0)
+    got = run(hip, dev, q, s, group, b, x)
+    y, bound = ref.product(q.to(dev), s.to(dev), group, None if b is None else b.to(dev), x.to(dev))
+    check(got, y.cpu(), bound.cpu())
+
+
+@pytest.mark.parametrize("tokens", [1, 3, 16])
+def test_infinities_in_many_rows(hip, dev, tokens):
+    """The form for many rows: the last token has an infinity and a NaN apart."""
+    n, k, group = 32805, 256, 64
+    q, s, x, b = make(n, k, group, tokens, 77, bias=True)
+    x[-1, 200] = math.inf
+    got = run(hip, dev, q, s, group, b, x).double()
+    if tokens > 1:
+        check(got[:-1], *ref.product(q, s, group, b, x[:-1]))
+    want = math.inf * (q[:, 200].double() * s[:, 200 // group].double())
+    assert torch.equal(got[-1].isnan(), want.isnan())
+    assert torch.equal(got[-1][~want.isnan()], want[~want.isnan()])
+    x[-1, 3] = math.nan
+    assert run(hip, dev, q, s, group, b, x)[-1].isnan().all()
+
+
 @pytest.mark.parametrize("group", [32, 64, 128])
 def test_every_value_at_every_column(hip, dev, group):
     """One-hot activations read single weights back: exact."""

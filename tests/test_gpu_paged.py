@@ -376,6 +376,26 @@ def test_attention_bad_pages_give_nan_and_lengths_end_with_the_table(paged, dev)
         check_attention(out[s:s + 1], [exact], [n], d)
 
 
+def test_attention_infinite_scores(paged, dev):
+    """Scores of -inf have no weight; of all -inf, or one +inf, the result is NaN."""
+    d, page = 64, 16
+    g = gen(8)
+    table, total = ref.tables([40, 40, 40], page, g)
+    pool = ref.Pool("bf16", total, page, 1, d, g)
+    for s, rows, value in ((0, (3, 17, 39), -math.inf), (1, range(40), -math.inf),
+                           (2, (20,), math.inf)):
+        for p in rows:
+            pool.parts[0][int(table[s, p // page]), 0, p % page, 5] = value
+    q = bf16((3, 2, d), g)
+    q[..., 5] = 1.0
+    pages, out = pool.to_device(paged, dev), torch.empty((3, 2, d), dtype=torch.bfloat16, device=dev)
+    run_attention(paged, dev, pages, table.to(dev), [40, 40, 40], q.to(dev), out)
+    keep = [p for p in range(40) if p not in (3, 17, 39)]
+    exact = ref.attend(q[0], pool.rows(0, table[0], 40)[:, keep], pool.rows(1, table[0], 40)[:, keep])
+    check_attention(out[:1], [exact], [37], d)
+    assert out[1:].isnan().all()
+
+
 @pytest.mark.parametrize("where", ["query", "key", "value"])
 def test_attention_nan_stays_in_its_sequence(paged, dev, where):
     lengths = [100, 700, 64]

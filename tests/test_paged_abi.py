@@ -224,6 +224,7 @@ W4 = dict(weight=A, scales=A, group=64, bias=None, input=A, output=A, tokens=1, 
     (dict(weight=None), "null"), (dict(scales=None), "null"), (dict(input=None), "null"),
     (dict(output=None), "null"), (dict(group=16), "group"), (dict(group=128), "group"),
     (dict(k=0), "group"), (dict(k=-64), "group"), (dict(n=0), "N=0"), (dict(tokens=0), "tokens"),
+    (dict(n=(1 << 28) + 1), "over"), (dict(k=(1 << 24) + 64), "over"),
     (dict(tokens=17), "tokens"), (dict(weight=A + 8), "aligned"), (dict(input=A + 2), "aligned"),
     (dict(scales=A + 8), "aligned")])
 def test_w4_refusals(hip, change, why):
