@@ -217,7 +217,7 @@ __global__ __launch_bounds__(kThreads) void kv_load_kernel(KvLoadArgs a) {
 // written by it, one inside a workgroup is joined there through LDS, and one
 // over several by a second launch, in the order of its tiles.  (Joined inside
 // the launch by the last workgroup to arrive, in two levels of 16, 131001 keys
-// of two KV heads took 42 us against 35: coherent stores, an atomic and the loads
+// of two KV heads took 42 us against 35 at that time: coherent stores, an atomic and the loads
 // of what other XCDs wrote cost 4 us a level under load.)  Where the tables
 // leave room for short sequences only, the cuts move to the units' ends
 // instead and the second launch is left out.
@@ -238,7 +238,6 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kTileKeys = 32;
 constexpr int kHeadBlock = 16;       // query heads of a unit at most
-constexpr int kJoinBatch = 8;          // parts a thread of the join has in flight
 constexpr float kRescaleSlack = 6.0f;  // p <= 2^6 before the maximum is moved
 
 // A uniform 32-bit word that nothing writes while the kernel runs, through the
@@ -247,19 +246,31 @@ __device__ __forceinline__ int scalar_word(const int* p) {
   return *(const __attribute__((address_space(4))) int*)(reinterpret_cast<uintptr_t>(p));
 }
 
+// N bytes of a lane; NT: marked as not to be kept in the caches.
+template <bool NT, typename T>
+__device__ __forceinline__ T load_as(const void* p) {
+  const QLIN_GLOBAL T* const at = (const QLIN_GLOBAL T*)(p);
+  return NT ? __builtin_nontemporal_load(at) : *at;
+}
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
 template <int N>
 struct Words;
 template <>
 struct Words<4> {
   uint32_t w[1];
-  __device__ __forceinline__ void load(const uint8_t* p) { w[0] = gload(reinterpret_cast<const uint32_t*>(p)); }
+  template <bool NT>
+  __device__ __forceinline__ void load(const uint8_t* p) {
+    w[0] = load_as<NT, uint32_t>(p);
+  }
 };
 template <>
 struct Words<8> {
   uint32_t w[2];
+  template <bool NT>
   __device__ __forceinline__ void load(const uint8_t* p) {
-    typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-    const u32x2 v = gload(reinterpret_cast<const u32x2*>(p));
+    const u32x2 v = load_as<NT, u32x2>(p);
     w[0] = v.x;
     w[1] = v.y;
   }
@@ -267,8 +278,9 @@ struct Words<8> {
 template <>
 struct Words<16> {
   uint32_t w[4];
+  template <bool NT>
   __device__ __forceinline__ void load(const uint8_t* p) {
-    const uint4 v = load_global16(p);
+    const u32x4 v = load_as<NT, u32x4>(p);
     w[0] = v.x;
     w[1] = v.y;
     w[2] = v.z;
@@ -403,8 +415,9 @@ struct PartTag {
   int begin, end;  // the part's tiles; end 0: no part
 };
 
-// W waves a workgroup; HB: room for that many query heads of a unit in LDS.
-template <int F, int D, int W, int HB>
+// W waves a workgroup; HB: room for that many query heads of a unit in LDS; NT:
+// keys and values are not to be kept in the caches.
+template <int F, int D, int W, int HB, bool NT>
 __global__ __launch_bounds__(W * kWave, 2) void paged_attention_kernel(PagedAttnArgs a) {
   constexpr int ES = F == kBf16 ? 2 : 1;
   constexpr int RB = D * ES;       // bytes of a row
@@ -541,7 +554,7 @@ __global__ __launch_bounds__(W * kWave, 2) void paged_attention_kernel(PagedAttn
       }
     };
 
-    uint4 k[2][KC];
+    u32x4 k[2][KC];
     Words<VB> v[8];
     f32x4_t ks[2], vs[2];
     const uint32_t k_off = r * RB + 16 * g, v_off = 4 * g * RB + r * VB;
@@ -550,7 +563,7 @@ __global__ __launch_bounds__(W * kWave, 2) void paged_attention_kernel(PagedAttn
       for (int h = 0; h < 2; ++h) {
         const uint8_t* base = static_cast<const uint8_t*>(a.pool.key) + row[h] * RB;
 #pragma unroll
-        for (int c = 0; c < KC; ++c) k[h][c] = load_global16(base + k_off + 64 * c);
+        for (int c = 0; c < KC; ++c) k[h][c] = load_as<NT, u32x4>(base + k_off + 64 * c);
         if (F != kBf16) {
           ks[h] = gload(reinterpret_cast<const f32x4_t*>(a.pool.key_scales + row[h]) + g);
         }
@@ -561,7 +574,7 @@ __global__ __launch_bounds__(W * kWave, 2) void paged_attention_kernel(PagedAttn
       for (int h = 0; h < 2; ++h) {
         const uint8_t* base = static_cast<const uint8_t*>(a.pool.value) + row[h] * RB;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[4 * h + i].load(base + v_off + i * RB);
+        for (int i = 0; i < 4; ++i) v[4 * h + i].template load<NT>(base + v_off + i * RB);
         if (F != kBf16) {
           vs[h] = gload(reinterpret_cast<const f32x4_t*>(a.pool.value_scales + row[h]) + g);
         }
@@ -801,7 +814,9 @@ __global__ __launch_bounds__(W * kWave, 2) void paged_attention_kernel(PagedAttn
 // of one.
 template <int D, int T>
 __global__ __launch_bounds__(T) void paged_attention_join_kernel(PagedAttnArgs a) {
-  __shared__ __align__(16) float smem[T * 6];
+  constexpr int kJoinBatch = T == 512 ? 8 : 4;  // parts that a thread has in flight
+  __shared__ f32x4_t part_o[T];
+  __shared__ float2 part_ml[T];
   const int lane = threadIdx.x & 63;
   const int seq = blockIdx.y;
   const int cap = a.table.max_pages << a.pool.page_shift;
@@ -866,24 +881,32 @@ __global__ __launch_bounds__(T) void paged_attention_join_kernel(PagedAttnArgs a
       }
     }
     if (rows > 1) {
-      float* mine = smem + (row * items + e) * 6;
       if (busy) {
-        mine[0] = o[0];
-        mine[1] = o[1];
-        mine[2] = o[2];
-        mine[3] = o[3];
-        mine[4] = top;
-        mine[5] = sum_l;
+        part_o[row * items + e] = o;
+        part_ml[row * items + e] = make_float2(top, sum_l);
       }
       __syncthreads();
-      for (int i = 1; i < rows && row == 0; ++i) {
-        const float* other = smem + (i * items + e) * 6;
-        const float next = fmaxf(top, other[4]);
+      for (int i = 1; i < rows && row == 0; i += kJoinBatch) {
+        f32x4_t x[kJoinBatch];
+        float2 ml[kJoinBatch];
+        float next = top;
+#pragma unroll
+        for (int b = 0; b < kJoinBatch; ++b) {
+          const int at = min(i + b, rows - 1) * items + e;
+          x[b] = part_o[at];
+          ml[b] = part_ml[at];
+          next = fmaxf(next, ml[b].x);
+        }
         const float old = __builtin_amdgcn_exp2f(top - next);
-        const float w = __builtin_amdgcn_exp2f(other[4] - next);
         top = next;
-        sum_l = sum_l * old + w * other[5];
-        o = o * old + w * f32x4_t{other[0], other[1], other[2], other[3]};
+        sum_l *= old;
+        o *= old;
+#pragma unroll
+        for (int b = 0; b < kJoinBatch; ++b) {
+          const float w = i + b < rows ? __builtin_amdgcn_exp2f(ml[b].x - next) : 0.0f;
+          sum_l += w * ml[b].y;
+          o += w * x[b];
+        }
       }
     }
     if (busy && row == 0) {
@@ -959,6 +982,14 @@ constexpr int kJoinParts = 96;
 // 1 x 100000, as many waves and twice the parts, 16.0 -> 19.1).
 constexpr int kSmallWholeTiles = 8, kSmallWholeUnits = 64, kSmallTiles = 4096;
 
+// A call whose tables have room for more keys and values than this finds little of
+// them in the 256 MB memory-side cache, next to what else a model's layers read, and
+// does better not to fill the caches, unless several head blocks read the same keys.
+// 134 MB: 34.5 -> 30.6 us, 350 MB: 67 -> 60.6.  Where the lengths fall far short of
+// the tables' room it costs nothing with cold caches (39 MB 13.9 -> 14.0 us, 123 MB
+// 29.4 -> 27.2), and up to a fifth where earlier calls left all of it in the cache.
+constexpr long long kStreamBytes = 96ll << 20;
+
 struct PagedAttnShape {
   int head_blocks, units;
   int block_heads;  // query heads of a full unit
@@ -1002,6 +1033,9 @@ void launch_paged_attention(PagedAttnArgs a, hipStream_t stream) {
   const bool small =
       s.block_heads > 8 || (a.whole ? tiles <= kSmallWholeTiles || units <= kSmallWholeUnits
                                     : tiles * units <= kSmallTiles);
+  const long long bytes = tiles * a.table.sequences * kTileKeys * 2 * a.pool.kv_heads *
+                          a.pool.head_dim * (a.pool.format == kBf16 ? 2 : 1);
+  const bool streams = bytes > kStreamBytes && s.head_blocks == 1;
   // no more workgroups than the tables have tiles for, one a wave
   const int waves = small ? 4 : 8, room = small ? 2 * kCus : kCus;
   const long long wanted = (tiles * units + waves - 1) / waves;
@@ -1009,15 +1043,26 @@ void launch_paged_attention(PagedAttnArgs a, hipStream_t stream) {
   a.waves = groups * waves;
   by_format(a.pool, [&](auto f, auto d) {
     constexpr int F = decltype(f)::value, D = decltype(d)::value;
+    auto launch = [&](auto w, auto hb, auto nt) {
+      constexpr int W = decltype(w)::value, HB = decltype(hb)::value;
+      hipLaunchKernelGGL((paged_attention_kernel<F, D, W, HB, decltype(nt)::value>), dim3(groups),
+                         dim3(W * kWave), 0, stream, a);
+    };
+    using Four = std::integral_constant<int, 4>;
+    using Eight = std::integral_constant<int, 8>;
+    using Sixteen = std::integral_constant<int, 16>;
     if (s.block_heads > 8) {
-      hipLaunchKernelGGL((paged_attention_kernel<F, D, 4, 16>), dim3(groups), dim3(4 * kWave), 0,
-                         stream, a);
+      if (streams) {
+        launch(Four{}, Sixteen{}, std::true_type{});
+      } else {
+        launch(Four{}, Sixteen{}, std::false_type{});
+      }
     } else if (small) {
-      hipLaunchKernelGGL((paged_attention_kernel<F, D, 4, 8>), dim3(groups), dim3(4 * kWave), 0,
-                         stream, a);
+      launch(Four{}, Eight{}, std::false_type{});
+    } else if (streams) {
+      launch(Eight{}, Eight{}, std::true_type{});
     } else {
-      hipLaunchKernelGGL((paged_attention_kernel<F, D, 8, 8>), dim3(groups), dim3(8 * kWave), 0,
-                         stream, a);
+      launch(Eight{}, Eight{}, std::false_type{});
     }
   });
   if (a.whole) return;

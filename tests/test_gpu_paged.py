@@ -254,9 +254,9 @@ def test_load_ends_with_the_table_and_marks_bad_pages(paged, dev):
 # -------------------------------------------------------------- attention --
 
 def attention_case(paged, dev, fmt, heads, kv, d, page, lengths, seed, std=1.0, qstd=1.0,
-                   poison=True):
+                   poison=True, width=None):
     g = gen(seed)
-    table, total = ref.tables(lengths, page, g)
+    table, total = ref.tables(lengths, page, g, width=width)
     pool = ref.Pool(fmt, total, page, kv, d, g, std)
     q = bf16((len(lengths), heads, d), g, qstd)
     out64 = [ref.attend(q[s], pool.rows(0, table[s], n), pool.rows(1, table[s], n))
@@ -319,6 +319,18 @@ def test_attention_of_ragged_sequences(paged, dev, fmt, heads, kv, d, page):
 def test_attention_split_over_long_sequences(paged, dev, fmt, heads, kv, d, page, lengths):
     _, pages, table, q, out, out64 = attention_case(paged, dev, fmt, heads, kv, d, page, lengths,
                                                     len(lengths) + page)
+    run_attention(paged, dev, pages, table, lengths, q, out)
+    check_attention(out, out64, lengths, d)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("heads,kv,d,page", [(7, 1, 64, 16), (28, 4, 128, 32), (16, 1, 64, 64),
+                                             (24, 2, 128, 16), (40, 2, 64, 128)])
+def test_attention_of_tables_with_much_room(paged, dev, fmt, heads, kv, d, page):
+    """Short and long sequences under tables for 400000 positions each."""
+    lengths = [1, 5000, 0, 33, 1200]
+    _, pages, table, q, out, out64 = attention_case(paged, dev, fmt, heads, kv, d, page, lengths,
+                                                    heads + d, width=400000 // page)
     run_attention(paged, dev, pages, table, lengths, q, out)
     check_attention(out, out64, lengths, d)
 
