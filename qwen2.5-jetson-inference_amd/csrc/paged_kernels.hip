@@ -168,8 +168,18 @@ __global__ __launch_bounds__(kThreads) void kv_store_kernel(KvStoreArgs a) {
 // ------------------------------------------------------------------- load --
 
 // One lane per 8 elements of a row; blockIdx.x over rows, y the KV head, z the
-// sequence.
-template <int F, int D>
+// sequence.  NT: what is written is not to be kept in the caches.
+template <bool NT>
+__device__ __forceinline__ void store_as(void* p, uint4 v) {
+  const u32x4 w = {v.x, v.y, v.z, v.w};
+  if (NT) {
+    __builtin_nontemporal_store(w, (QLIN_GLOBAL u32x4*)(p));
+  } else {
+    *(QLIN_GLOBAL u32x4*)(p) = w;
+  }
+}
+
+template <int F, int D, bool NT>
 __global__ __launch_bounds__(kThreads) void kv_load_kernel(KvLoadArgs a) {
   constexpr int L = D / 8;
   const int seq = blockIdx.z, head = blockIdx.y, c = threadIdx.x % L;
@@ -183,25 +193,25 @@ __global__ __launch_bounds__(kThreads) void kv_load_kernel(KvLoadArgs a) {
       ((static_cast<size_t>(seq) * a.pool.kv_heads + head) * a.capacity + pos) * D + 8 * c;
   if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.pool.num_pages)) {
     const uint4 nan = make_uint4(0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u, 0x7FC07FC0u);
-    store_global16(a.key_cache + to, nan);
-    store_global16(a.value_cache + to, nan);
+    store_as<NT>(a.key_cache + to, nan);
+    store_as<NT>(a.value_cache + to, nan);
     return;
   }
   const size_t at = pool_row(a.pool, page, head, pos & ((1 << a.pool.page_shift) - 1));
   if (F == kBf16) {
     const uint4 k = load_global16(static_cast<const uint16_t*>(a.pool.key) + at * D + 8 * c);
     const uint4 v = load_global16(static_cast<const uint16_t*>(a.pool.value) + at * D + 8 * c);
-    store_global16(a.key_cache + to, k);
-    store_global16(a.value_cache + to, v);
+    store_as<NT>(a.key_cache + to, k);
+    store_as<NT>(a.value_cache + to, v);
     return;
   }
   const uint2 k = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.pool.key) + at * D + 8 * c);
   const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.pool.value) + at * D + 8 * c);
   float x[8];
   dequantise8<F>(k, a.pool.key_scales[at], x);
-  store_global16(a.key_cache + to, pack8(x));
+  store_as<NT>(a.key_cache + to, pack8(x));
   dequantise8<F>(v, a.pool.value_scales[at], x);
-  store_global16(a.value_cache + to, pack8(x));
+  store_as<NT>(a.value_cache + to, pack8(x));
 }
 
 // -------------------------------------------------------------- attention --
@@ -947,6 +957,16 @@ void launch_kv_store(const KvStoreArgs& a, hipStream_t stream) {
   });
 }
 
+// Bytes that little is left of in the 256 MB memory-side cache when they are read
+// again, next to what else a model's layers read.
+constexpr long long kStreamBytes = 96ll << 20;
+
+// A load that writes more than kStreamBytes does not leave it in the caches: 12 x
+// 9000 rows of 4 x 128 INT8 36 -> 25.5 us, 64 x 1000 of 8 x 64 FP8 32 -> 18.  A
+// kernel that reads all of it next, and does nothing else, is slower by as much
+// (both together 111 us either way; after a store of the same rows 287 -> 284); a
+// smaller load's reader finds it in the cache (8 x 8000 of 2 x 64: 18.9 us for both,
+// 20.8 without).
 void launch_kv_load(const KvLoadArgs& a, hipStream_t stream) {
   const long long most = static_cast<long long>(a.table.max_pages) << a.pool.page_shift;
   const long long rows = a.capacity < most ? a.capacity : most;
@@ -954,8 +974,13 @@ void launch_kv_load(const KvLoadArgs& a, hipStream_t stream) {
     constexpr int per = kThreads / (decltype(d)::value / 8);
     const dim3 grid(static_cast<unsigned>((rows + per - 1) / per), a.pool.kv_heads,
                     a.table.sequences);
-    hipLaunchKernelGGL((kv_load_kernel<decltype(f)::value, decltype(d)::value>), grid,
-                       dim3(kThreads), 0, stream, a);
+    constexpr int F = decltype(f)::value, D = decltype(d)::value;
+    const long long bytes = 4ll * a.table.sequences * a.pool.kv_heads * rows * D;
+    if (bytes > kStreamBytes) {
+      hipLaunchKernelGGL((kv_load_kernel<F, D, true>), grid, dim3(kThreads), 0, stream, a);
+    } else {
+      hipLaunchKernelGGL((kv_load_kernel<F, D, false>), grid, dim3(kThreads), 0, stream, a);
+    }
   });
 }
 
@@ -981,14 +1006,6 @@ constexpr int kJoinParts = 96;
 // for cut ones of calls with at most kSmallTiles tiles (16 x 2000 keys 10.7 -> 10.0;
 // 1 x 100000, as many waves and twice the parts, 16.0 -> 19.1).
 constexpr int kSmallWholeTiles = 8, kSmallWholeUnits = 64, kSmallTiles = 4096;
-
-// A call whose tables have room for more keys and values than this finds little of
-// them in the 256 MB memory-side cache, next to what else a model's layers read, and
-// does better not to fill the caches, unless several head blocks read the same keys.
-// 134 MB: 34.5 -> 30.6 us, 350 MB: 67 -> 60.6.  Where the lengths fall far short of
-// the tables' room it costs nothing with cold caches (39 MB 13.9 -> 14.0 us, 123 MB
-// 29.4 -> 27.2), and up to a fifth where earlier calls left all of it in the cache.
-constexpr long long kStreamBytes = 96ll << 20;
 
 struct PagedAttnShape {
   int head_blocks, units;
@@ -1024,6 +1041,11 @@ bool paged_attention_supported(const PagedAttnArgs& a) {
   return most_tiles(a) * a.table.sequences * s.units < 2147000000LL;
 }
 
+// A call whose tables have room for more keys and values than kStreamBytes reads
+// them past the caches, unless several head blocks read the same keys.  134 MB: 34.5
+// -> 30.6 us, 350 MB: 67 -> 60.6.  Where the lengths fall far short of the tables'
+// room it costs nothing with cold caches (39 MB 13.9 -> 14.0 us, 123 MB 29.4 ->
+// 27.2), and up to a fifth where earlier calls left all of it in the cache.
 void launch_paged_attention(PagedAttnArgs a, hipStream_t stream) {
   const PagedAttnShape s = paged_attention_shape(a.heads, a.pool.kv_heads, a.pool.head_dim);
   a.head_blocks = s.head_blocks;

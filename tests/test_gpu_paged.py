@@ -235,6 +235,24 @@ def test_load_reads_back(paged, dev, fmt, kv, d, page, capacity):
             assert (got[:, n:] == fill).all()
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("kv,d,capacity", [(1, 64, 400003), (2, 128, 100001)])
+def test_load_of_much(paged, dev, fmt, kv, d, capacity):
+    """Outputs past 96 MiB, of which little is live."""
+    page, g, lengths = 64, gen(d), [1, 700, 0, 65]
+    table, total = ref.tables(lengths, page, g, width=-(-capacity // page))
+    pool = ref.Pool(fmt, total, page, kv, d, g)
+    kc = torch.full((len(lengths), kv, capacity, d), 3.0, dtype=torch.bfloat16, device=dev)
+    vc = kc.clone()
+    paged.kv_pages_load(pool.to_device(paged, dev), table.to(dev),
+                        torch.tensor(lengths, dtype=torch.int32, device=dev), kc, vc)
+    for i, cache in enumerate((kc, vc)):
+        for s, n in enumerate(lengths):
+            exact = pool.rows(i, table[s], n)
+            assert ((cache[s, :, :n].cpu().double() - exact).abs() <= exact.abs() * 2.0 ** -8).all()
+            assert bool((cache[s, :, n:] == 3.0).all())
+
+
 def test_load_ends_with_the_table_and_marks_bad_pages(paged, dev):
     g = gen(5)
     pool = ref.Pool("int8", 4, 16, 1, 64, g)
