@@ -39,12 +39,19 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 // q x / 16 reaches 1/2 |x|, which costs two bits of FP32's 24.
 //
 // Two forms.  With many rows (w4a16_rows_kernel) a wave takes whole row tiles
-// over all of K, by itself, with the activations in LDS.  With fewer
-// (w4a16_split_kernel) the waves of a workgroup split one row tile's K and meet
-// in LDS, in the order of the waves.  Either keeps DP tiles of 128 columns, a
-// contiguous KiB of weights each, in flight per wave.  Memory bounds both: per
-// KiB a SIMD issues 45 to 70 vector instructions and eight MFMAs, 270 cycles at
-// most, and a CU's share of HBM is a KiB in 90 for its four SIMDs.
+// over all of K, by itself, with the activations and the groups' starts in LDS.
+// With fewer (w4a16_split_kernel) the waves of a workgroup split one or two row
+// tiles' K and meet in LDS, in the order of the waves; the activations come from
+// L2 for every row tile, 128 bytes a token and KiB of weights.  Either keeps DP
+// tiles of 128 columns, a contiguous KiB of weights each, in flight per wave.
+//
+// Bound.  The weights' bytes and the waits at a call's start and end: 16 tokens by
+// 151936 x 896 in groups of 32 takes 22 us for 81 MB (3.7 TB/s; a read alone runs at
+// 7.0), 1 by 152064 x 3584 in groups of 128 52 us (5.3 TB/s), 1 by 40000 x 4096
+// 19.7 us (4.4 TB/s), 1 by 896 x 896 3.1 us, of which 1.7 are an empty launch.  The
+// vector instructions (about 60 a tile) would allow a KiB in 65 cycles of a CU, whose
+// share of HBM is a KiB in 90.  Where K is long and row tiles are few (16 x 1536 x
+// 8960, 12.8 us) it is the activations, all of them read by each CU at 64 bytes a ns.
 //
 // Activations beyond FP32's reach (a sum that is not finite) are summed again
 // element by element, q s x in FP32.
@@ -95,7 +102,7 @@ __device__ __forceinline__ void load_piece(W4Piece& p, const W4Args& a, int rt, 
   typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
   constexpr int kGroups = kTileCols / G;
   p.w = load_stream16(a.w + (static_cast<size_t>(rt) * tiles + t) * kTileBytes + 16 * lane);
-  // past the last group the activations are 0
+  // past the last group: that one again
   const int group = kGroups == 1 ? t : min(t * kGroups + (lane & (kGroups - 1)), groups - 1);
   const u32x2 v = gload(reinterpret_cast<const u32x2*>(
       a.s + (static_cast<size_t>(rt) * groups + group) * kTileRows + 4 * (lane >> 4)));
@@ -311,25 +318,40 @@ __global__ __launch_bounds__(kRowsMaxWaves * kWave, 6) void w4a16_rows_kernel(W4
 
 constexpr int kSplitWaves = 16;
 
+// v of lane `from` (0 .. S - 1) of the S lanes next to each other that v's lane is of.
+template <int S, int FROM>
+__device__ __forceinline__ uint4 share_lane(const uint4& v) {
+  if (S == 1) return v;
+  auto one = [](uint32_t w) {
+    constexpr int kPerm = S == 4 ? FROM * 0x55 : FROM ? 0xF5 : 0xA0;  // quad lanes
+    return static_cast<uint32_t>(
+        __builtin_amdgcn_update_dpp(0, static_cast<int>(w), kPerm, 0xF, 0xF, true));
+  };
+  return make_uint4(one(v.x), one(v.y), one(v.z), one(v.w));
+}
+
 // Workgroup i: row tiles [i R, (i + 1) R); wave w takes their column tiles w, w +
 // waves, ..., DP of them in flight.  With R > 1 the activations, four KiB a tile
-// at 16 tokens, are read for R KiB of weights.
-template <int G, int DP, int R>
+// at 16 tokens, are read for R KiB of weights.  With at most 16 / S tokens S columns
+// of Y^T are one token's, and each of their lanes reads one of S parts of the tile's
+// activations and hands it to the others: 4 / S KiB a tile.
+template <int G, int S, int DP, int R>
 __global__ __launch_bounds__(kSplitWaves * kWave) void w4a16_split_kernel(W4Args a) {
-  constexpr int kPitch = R * kTileRows + 4;
+  constexpr int kPitch = R * kTileRows + 4, kLoads = 4 / S;
   extern __shared__ __align__(16) float partial[];  // [wave][token][kPitch]
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x / kWave;
   const int tiles = (a.k + kTileCols - 1) / kTileCols, groups = a.k / G;
   const int row_tiles = (a.n + kTileRows - 1) / kTileRows;
   const int first = blockIdx.x * R;
-  const uint16_t* x_row = a.x + static_cast<size_t>(min(r, a.tokens - 1)) * a.k + 8 * g;
+  const int x_part = r % S * kLoads * 32;
+  const uint16_t* x_row = a.x + static_cast<size_t>(min(r / S, a.tokens - 1)) * a.k + 8 * g;
   f32x4_t total[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) total[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
   for (int t0 = wave; t0 < tiles; t0 += DP * waves) {
     W4Piece p[DP][R];
-    uint4 x[DP][4];
+    uint4 x[DP][kLoads];
 #pragma unroll
     for (int i = 0; i < DP; ++i) {  // past the last tile, or row tile: that one again
       const int t = min(t0 + i * waves, tiles - 1);
@@ -338,29 +360,47 @@ __global__ __launch_bounds__(kSplitWaves * kWave) void w4a16_split_kernel(W4Args
         load_piece<G>(p[i][j], a, min(first + j, row_tiles - 1), t, tiles, groups, lane);
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        // columns past K count for nothing, from wherever they are read
-        const int col = t * kTileCols + 32 * j;
+      for (int j = 0; j < kLoads; ++j) {
+        // columns past K have no scale, from wherever they are read
+        const int col = t * kTileCols + x_part + 32 * j;
         x[i][j] = load_global16(x_row + (col < a.k ? col : 0));
-        if (col >= a.k) x[i][j] = make_uint4(0, 0, 0, 0);
       }
     }
+    // The loads stay ahead of the products' branch, which else each would move
+    // behind (1 x 1536 x 8960 7.9 us so, 6.7 here).
+    asm volatile("" ::: "memory");
 #pragma unroll
     for (int i = 0; i < DP; ++i) {
       if (t0 + i * waves >= tiles) break;
       bf16x8_t xb[4];
+      auto put = [&](auto from) {
+        constexpr int kFrom = decltype(from)::value;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) xb[j] = __builtin_bit_cast(bf16x8_t, x[i][j]);
+        for (int j = 0; j < kLoads; ++j) {
+          xb[kFrom * kLoads + j] = __builtin_bit_cast(bf16x8_t, share_lane<S, kFrom>(x[i][j]));
+        }
+      };
+      put(std::integral_constant<int, 0>{});
+      if constexpr (S > 1) put(std::integral_constant<int, 1>{});
+      if constexpr (S > 2) {
+        put(std::integral_constant<int, 2>{});
+        put(std::integral_constant<int, 3>{});
+      }
       f32x4_t base[kTileCols / G];
       base_of<G>(base, xb);
 #pragma unroll
-      for (int j = 0; j < R; ++j) add_piece<G>(total[j], p[i][j], xb, base);
+      for (int j = 0; j < R; ++j) {
+        if (kTileCols / G > 1 && (t0 + i * waves) * (kTileCols / G) + (lane & (kTileCols / G - 1)) >= groups) {
+          p[i][j].s = make_uint2(0, 0);
+        }
+        add_piece<G>(total[j], p[i][j], xb, base);
+      }
     }
   }
-  if (r < a.tokens) {
+  if (r % S == 0 && r / S < a.tokens) {
 #pragma unroll
     for (int j = 0; j < R; ++j) {
-      *reinterpret_cast<f32x4_t*>(partial + (wave * a.tokens + r) * kPitch + j * kTileRows + 4 * g) =
+      *reinterpret_cast<f32x4_t*>(partial + (wave * a.tokens + r / S) * kPitch + j * kTileRows + 4 * g) =
           total[j];
     }
   }
@@ -378,8 +418,17 @@ __global__ __launch_bounds__(kSplitWaves * kWave) void w4a16_split_kernel(W4Args
 }
 
 constexpr int kCus = 256;
-constexpr int kRowsTiles = 2048;       // row tiles from which a wave takes whole ones
-constexpr int kPairTiles = 1024;       // row tiles from which the split kernel takes two, of 9 tokens up
+// Row tiles from which a wave takes whole ones.  Few tokens: as many as the chip
+// then has waves (1 x 100000 x 2048 24.8 us split, 25.0 in rows; 65536 17.1 and 18.0;
+// 128000 30.9 and 29.4).  More than 8, whose activations the split kernel reads at
+// the weights' own rate or faster: fewer, if K is long (16 x 40000 x 4096 28.0 us
+// split, 25.6 in rows; x 1536 13.4 and 13.3; 16 x 32768 x 1024 7.8 and 10.4).
+constexpr int kRowsTiles = 6144, kRowsTilesMany = 2048, kRowsLongTiles = 12;
+// Row tiles from which the split kernel takes two a workgroup: half the activations'
+// reads, half the workgroups (16 x 17920 x 1536 10.7 -> 9.5 us; 1 x 40000 x 4096 22.7
+// -> 19.7, 1 x 30000 x 1024 6.9 -> 6.5, but 1 x 17920 x 1536 6.3 -> 6.7).
+constexpr int kPairTiles = 1536, kPairTilesMany = 1024;
+constexpr int kManyTokens = 9;         // tokens from which the above say "many"
 constexpr int kSplitRoom = 16 * kCus;  // waves that the split kernel fills the chip with
 
 template <int G>
@@ -387,9 +436,13 @@ void launch_w4(const W4Args& a, hipStream_t stream) {
   const int row_tiles = (a.n + kTileRows - 1) / kTileRows;
   const int tiles = (a.k + kTileCols - 1) / kTileCols;
   const int pitch = a.tokens == 1 ? 1 : a.tokens <= 4 ? 4 : 16;
+  const bool many = a.tokens >= kManyTokens;
   for (const RowsShape& shape : kRowsShapes) {
     const size_t lds = rows_lds_bytes(tiles, pitch, G);
-    if (row_tiles < kRowsTiles || lds > shape.lds) continue;
+    if (row_tiles < (many && tiles > kRowsLongTiles ? kRowsTilesMany : kRowsTiles) ||
+        lds > shape.lds) {
+      continue;
+    }
     auto launch = [&](auto tp) {
       hipLaunchKernelGGL((w4a16_rows_kernel<G, decltype(tp)::value>), dim3(shape.per_cu * kCus),
                          dim3(shape.waves * kWave), lds, stream, a);
@@ -403,31 +456,42 @@ void launch_w4(const W4Args& a, hipStream_t stream) {
     }
     return;
   }
-  // Waves for the chip's room, at least eight, of equal shares of the tiles.
+  // Waves for the chip's room, at least eight, of equal shares of the tiles.  A wave's
+  // loads in flight are all of its tiles up to five with up to four tokens; with more,
+  // whose activations fill a CU's queue of loads, one (5 x 1536 x 8960 7.8 us, 9.1
+  // with four; 16 x 896 x 4864 7.9, 8.8 with two) or two where that is all of them (8 x
+  // 17920 x 1536 7.3, 7.5 with one) or the pairs halve the activations.
   const int room = kSplitRoom / row_tiles;
   const int most = room < 8 ? 8 : room > kSplitWaves ? kSplitWaves : room;
   const int per = (tiles + most - 1) / most;
   const int waves = (tiles + per - 1) / per;
-  auto launch = [&](auto depth, auto rows) {
+  auto launch = [&](auto share, auto depth, auto rows) {
     constexpr int R = decltype(rows)::value;
     const size_t lds = static_cast<size_t>(waves) * a.tokens * (R * kTileRows + 4) * sizeof(float);
-    hipLaunchKernelGGL((w4a16_split_kernel<G, decltype(depth)::value, R>),
+    hipLaunchKernelGGL((w4a16_split_kernel<G, decltype(share)::value, decltype(depth)::value, R>),
                        dim3((row_tiles + R - 1) / R), dim3(waves * kWave), lds, stream, a);
   };
   using One = std::integral_constant<int, 1>;
   using Two = std::integral_constant<int, 2>;
-  if (row_tiles >= kPairTiles && a.tokens > 8) {
-    if (per == 1) {
-      launch(One{}, Two{});
+  using Four = std::integral_constant<int, 4>;
+  using Five = std::integral_constant<int, 5>;
+  auto by_share = [&](auto depth, auto rows) {
+    if (many) {
+      launch(One{}, depth, rows);
     } else {
-      launch(Two{}, Two{});
+      a.tokens > 4 ? launch(Two{}, depth, rows) : launch(Four{}, depth, rows);
     }
+  };
+  if (row_tiles >= (many ? kPairTilesMany : kPairTiles)) {
+    per == 1 ? by_share(One{}, Two{}) : by_share(Two{}, Two{});
   } else if (per == 1) {
-    launch(One{}, One{});
+    by_share(One{}, One{});
   } else if (per == 2) {
-    launch(Two{}, One{});
+    by_share(Two{}, One{});
+  } else if (a.tokens > 4) {
+    by_share(One{}, One{});
   } else {
-    launch(std::integral_constant<int, 3>{}, One{});
+    per <= 4 ? launch(Four{}, Four{}, One{}) : launch(Four{}, Five{}, One{});
   }
 }
 

@@ -62,14 +62,18 @@ def test_many_rows(hip, dev, group):
     check(run(hip, dev, q, s, group, b, x), *ref.product(q, s, group, b, x))
 
 
-# Whole row tiles a wave (32768 rows up): one token, a few, sixteen; groups that end
-# inside a column tile; rows that end inside a tile or a 4-row piece; LDS for three,
-# two and one workgroup a CU, and too little.  Pairs of row tiles (16384 rows up and
-# 9 tokens up) with one and several column tiles a wave.
+# Whole row tiles a wave (98304 rows up; 32768 for 9 tokens up and long K): one token,
+# a few, sixteen; groups that end inside a column tile; rows that end inside a tile or
+# a 4-row piece; LDS for three, two and one workgroup a CU, and too little.  Pairs of
+# row tiles (24576 rows up; 16384 for 9 tokens up) with one and several column tiles a
+# wave, for up to 4, 8 and 16 tokens.
 @pytest.mark.parametrize("n,k,group,tokens", [
     (33001, 160, 32, 16), (32773, 1088, 64, 1), (40008, 4096, 128, 16), (33000, 96, 32, 2),
     (34567, 2432, 64, 9), (50001, 1536, 64, 4), (32768, 32, 32, 1), (33000, 8960, 64, 16),
-    (20001, 384, 64, 12), (18000, 4864, 128, 16), (17001, 3168, 32, 9), (20003, 2048, 32, 8)])
+    (20001, 384, 64, 12), (18000, 4864, 128, 16), (17001, 3168, 32, 9), (20003, 2048, 32, 8),
+    (98305, 160, 32, 1), (98319, 1088, 64, 4), (98306, 96, 32, 3), (99001, 416, 32, 8),
+    (100004, 128, 128, 16), (24577, 1088, 64, 5), (24580, 96, 32, 1), (30001, 2432, 32, 4),
+    (33001, 160, 32, 8), (33017, 1184, 32, 16), (26011, 192, 64, 7)])
 def test_product_of_many_rows(hip, dev, n, k, group, tokens):
     q, s, x, b = make(n, k, group, tokens, n + k, bias=tokens % 2 == 0)
     got = run(hip, dev, q, s, group, b, x)
@@ -78,9 +82,10 @@ def test_product_of_many_rows(hip, dev, n, k, group, tokens):
 
 
 @pytest.mark.parametrize("tokens", [1, 3, 16])
-def test_infinities_in_many_rows(hip, dev, tokens):
-    """The form for many rows: the last token has an infinity and a NaN apart."""
-    n, k, group = 32805, 256, 64
+@pytest.mark.parametrize("n", [32805, 98341])
+def test_infinities_in_many_rows(hip, dev, n, tokens):
+    """The forms for many rows: the last token has an infinity and a NaN apart."""
+    k, group = 256, 64
     q, s, x, b = make(n, k, group, tokens, 77, bias=True)
     x[-1, 200] = math.inf
     got = run(hip, dev, q, s, group, b, x).double()
@@ -136,6 +141,28 @@ def test_activations_at_the_ends_of_their_range(hip, dev, special, tokens):
     want = special * w  # 0 x inf is NaN
     assert torch.equal(got[-1].isnan(), want.isnan())
     assert torch.equal(got[-1][~want.isnan()], want[~want.isnan()])
+
+
+@pytest.mark.parametrize("n,k,group", [(50, 96, 32), (70, 1088, 64), (25000, 160, 32)])
+@pytest.mark.parametrize("tokens", [1, 5, 9])
+@pytest.mark.parametrize("special", [math.inf, 3.0e38])
+def test_column_tiles_that_end_before_their_last_group(hip, dev, n, k, group, tokens, special):
+    """Nothing of a token's first columns comes in for columns past K."""
+    q, s, x, b = make(n, k, group, tokens, 21, bias=True)
+    q[0, 0], q[1, 0] = 0, 5
+    x[0, 0] = special
+    got = run(hip, dev, q, s, group, b, x).double()
+    if tokens > 1:
+        check(got[1:], *ref.product(q, s, group, b, x[1:]))
+    w = q[:, 0].double() * s[:, 0].double()
+    if math.isfinite(special):
+        y, bound = ref.product(q, s, group, b, x[:1])
+        # q s x in FP32, of sums whose terms are as large as the first
+        check(got[:1], y, bound + (w * special).abs() * (k + 2) * 2.0 ** -24)
+    else:
+        want = special * w
+        assert torch.equal(got[0].isnan(), want.isnan())
+        assert torch.equal(got[0][~want.isnan()], want[~want.isnan()])
 
 
 @pytest.mark.parametrize("tokens", [1, 8])
