@@ -102,6 +102,28 @@ inline void gemm_w8a16(const int8_t* weight, const uint16_t* scales, int group_s
                              out_features, in_features, stream));
 }
 
+// 4-bit weights (infer_hip_gemv_w4a16), 1 to 16 tokens.  No reference counterpart.
+// pack_w4a16 lays row-major values in [-8, 7] and BF16 scales out on the host.
+struct W4A16Weights {
+  std::vector<uint8_t> weight;
+  std::vector<uint16_t> scales;
+};
+inline W4A16Weights pack_w4a16(const int8_t* values, const uint16_t* scales, int group_size,
+                               int out_features, int in_features) {
+  W4A16Weights w;
+  w.weight.resize(infer_hip_w4a16_weight_bytes(out_features, in_features));
+  w.scales.resize(infer_hip_w4a16_scale_count(out_features, in_features, group_size));
+  check(infer_hip_w4a16_pack(values, scales, group_size, out_features, in_features,
+                             w.weight.data(), w.scales.data()));
+  return w;
+}
+inline void gemv_w4a16(const uint8_t* weight, const uint16_t* scales, int group_size,
+                       const uint16_t* bias, const uint16_t* input, uint16_t* output, int tokens,
+                       int out_features, int in_features, hipStream_t stream) {
+  check(infer_hip_gemv_w4a16(weight, scales, group_size, bias, input, output, tokens,
+                             out_features, in_features, stream));
+}
+
 // gemm_w8a16 / gemm_bf16 with a caller workspace (infer_hip_gemm_*_ws): a
 // lone long-K call splits K over the idle CUs.  No reference counterpart.
 inline size_t gemm_workspace_bytes(int max_tokens, int out_features, int in_features) {

@@ -2,6 +2,8 @@
 do not fill a tile, columns that do not fill one, values at the ends of their
 range, activations that are huge, infinite or NaN, captured graphs."""
 import math
+import os
+import subprocess
 
 import pytest
 import torch
@@ -212,3 +214,10 @@ def test_captured(hip, dev):
         eager = torch.empty_like(out)
         hip.gemv_w4a16(packed, tiled, 64, db, dx, eager, 4, 896, 4864)
         assert torch.equal(out.view(torch.int16), eager.view(torch.int16))
+
+
+def test_cpp_face(dev):
+    binary = os.path.join(os.path.dirname(os.path.abspath(__file__)), "cpp", "test_w4a16")
+    assert os.path.exists(binary), "build() compiles tests/cpp/test_w4a16"
+    out = subprocess.run([binary], capture_output=True, text=True, timeout=120)
+    assert out.returncode == 0 and "PASSED" in out.stdout, out.stdout + out.stderr

@@ -3,6 +3,7 @@ refusals before any HIP call, and the host packer and quantiser."""
 import ctypes
 import os
 import re
+import subprocess
 
 import numpy as np
 import pytest
@@ -233,3 +234,12 @@ def test_w4_refusals(hip, change, why):
     rc = hip.load().infer_hip_gemv_w4a16(*args.values(), None)
     assert rc == hip.INVALID_ARGUMENT
     assert why in hip.load().infer_hip_last_error().decode()
+
+
+def test_cpp_packer():
+    # the parts of tests/cpp/test_w4a16.cpp that need no GPU
+    cpp = os.path.join(ROOT, "tests", "cpp")
+    subprocess.run(["make", "-C", cpp, "test_w4a16"], check=True, capture_output=True, timeout=300)
+    out = subprocess.run([os.path.join(cpp, "test_w4a16"), "host"], capture_output=True, text=True,
+                         timeout=60)
+    assert out.returncode == 0 and "PASSED" in out.stdout, out.stdout + out.stderr
