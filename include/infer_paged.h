@@ -115,12 +115,13 @@ int infer_hip_kv_pages_load(const infer_hip_kv_pages* pages, const infer_hip_kv_
  *   output[s][h] = bf16(softmax(query[s][h] K^T / sqrt(head_dim)) V).
  * query is BF16 [num_sequences][num_heads][head_dim] with query_stride elements
  * between sequences (a multiple of 8), already rotated; output is contiguous;
- * both 16-byte aligned.  FP32 softmax statistics and sums.  A length of zero or
- * less (an empty slot of the batch) gives zeros; a length past the table's
- * pages ends there.  Scores that are all -infinity give NaN, as the quotient
- * does.  A sequence whose pages within its length are not all in
- * the pool gives NaN.  Rows behind a sequence's length never count, whatever
- * they hold.
+ * both 16-byte aligned.  FP32 softmax statistics and sums; the sum of weights
+ * (up to 2^6 each) times values is divided at the end, so values near FP32's
+ * largest overflow.  A length of zero or less (an empty slot of the batch)
+ * gives zeros; a length past the table's pages ends there.  Scores that are
+ * all -infinity give NaN, as the quotient does.  A sequence whose pages within
+ * its length are not all in the pool gives NaN.  Rows behind a sequence's
+ * length never count, whatever they hold.
  *
  * The work of all sequences is cut into equal parts over the chip on the
  * device, from the lengths, and the parts of a head joined in a fixed order:

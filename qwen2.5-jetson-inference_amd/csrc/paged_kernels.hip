@@ -100,8 +100,17 @@ __device__ __forceinline__ void rotate8(float (&lo)[8], float (&hi)[8], const fl
 
 // ------------------------------------------------------------------ store --
 
-// A row (token, query head | key head | value head) takes D / 16 lanes; lane c
-// holds elements 8 c .. + 8 of both halves, i.e. whole RoPE pairs.
+// q' = q R(pos), k' = k R(pos), v' = v; q' to BF16; a row x of k' or v' to x / s in
+// the pool's format, s = max|x| / limit.  A row (token, query head | key head | value
+// head) takes D / 16 lanes; lane c holds elements 8 c .. + 8 of both halves, i.e.
+// whole RoPE pairs, so a row's maximum is three exchanges at most and nothing waits
+// for another row: any number of tokens, of any sequences, is one grid.
+//
+// Bound: bytes.  6 prompts of up to 5000 tokens of 32 + 2 x 8 heads of 128 in FP8 (396
+// MB) 79 us, 5.0 TB/s, as a copy.  A decode step (24 tokens of 14 + 2 x 2 heads of
+// 64) is 3.0 us, 1.7 of them the launch, the rest three dependent reads: position,
+// table, row.  Non-temporal loads or stores gained 2-3 % on some sizes and lost as
+// much on others.
 template <int F, int D>
 __global__ __launch_bounds__(kThreads) void kv_store_kernel(KvStoreArgs a) {
   constexpr int L = D / 16;
@@ -167,8 +176,10 @@ __global__ __launch_bounds__(kThreads) void kv_store_kernel(KvStoreArgs a) {
 
 // ------------------------------------------------------------------- load --
 
-// One lane per 8 elements of a row; blockIdx.x over rows, y the KV head, z the
-// sequence.  NT: what is written is not to be kept in the caches.
+// bf16(element * scale), one rounding.  One lane per 8 elements of a row; blockIdx.x
+// over rows, y the KV head, z the sequence; the grid covers the capacity, and rows
+// behind a length end after one load.  Bound: bytes (launch_kv_load has the figures).
+// NT: what is written is not to be kept in the caches.
 template <bool NT>
 __device__ __forceinline__ void store_as(void* p, uint4 v) {
   const u32x4 w = {v.x, v.y, v.z, v.w};
@@ -227,7 +238,7 @@ __global__ __launch_bounds__(kThreads) void kv_load_kernel(KvLoadArgs a) {
 // written by it, one inside a workgroup is joined there through LDS, and one
 // over several by a second launch, in the order of its tiles.  (Joined inside
 // the launch by the last workgroup to arrive, in two levels of 16, 131001 keys
-// of two KV heads took 42 us against 35 at that time: coherent stores, an atomic and the loads
+// of two KV heads took 42 us against 35 with a second launch, before other changes: coherent stores, an atomic and the loads
 // of what other XCDs wrote cost 4 us a level under load.)  Where the tables
 // leave room for short sequences only, the cuts move to the units' ends
 // instead and the second launch is left out.
@@ -242,6 +253,13 @@ __global__ __launch_bounds__(kThreads) void kv_load_kernel(KvLoadArgs a) {
 // scores and the weights.  A weight is the sum of two BF16 numbers (2^-17 of it
 // is lost): one alone rounds as coarsely as the output and made the error
 // 1.35 times the output rounding's own; maxima, sums and O are FP32.
+//
+// Bound.  Large calls: the cache's bytes, 1 x 131001 keys of 2 x 128 in BF16 (134 MB)
+// 30.6 us, 64 sequences of up to 4000 of 8 x 128 in FP8 (270 MB) 52 us, 5.2 TB/s;
+// a read alone runs at 7.0.  A tile in flight a wave and eight waves a CU are what
+// the registers hold (two tiles in flight, or more waves, gained nothing).  Small
+// calls: the launches and their chains of dependent reads, lengths, table, keys: 1 x
+// 101 keys 4.8 us, 16 x 2000 in INT8 9.4 us, 3.7 of them the second launch.
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
@@ -997,8 +1015,12 @@ constexpr int kCus = 256;
 // 17.6; beyond, only small ones stay whole).
 constexpr int kWholeTiles = 24, kWholeTilesMany = 8;
 // Parts of a unit from which a workgroup of the join has 512 threads (1 x 131001
-// keys, 128 parts: 34.6 us, 38.0 with 256; 16 x 1000 keys: 11.2 and 10.1).
+// keys, 128 parts: 30.5 us, 31.1 with 256; 16 x 2000 keys, 16 parts: 10.3 and 9.4).
 constexpr int kJoinParts = 96;
+// Units up to which the join has a workgroup for each of their query heads (1 x
+// 131001 keys 30.6 us, 46.0 with one a unit; 8 x 20000 keys of 14 / 2 / 64, 16 units,
+// 14.0 and 18.6; 64 x 4000 keys, 512 units, 55.0 and 52.7).
+constexpr int kJoinHeadUnits = 64;
 
 // Workgroups of 4 waves instead of 8 start and meet sooner, and spread cut units
 // over more CUs: where all units are whole and small or few (1 x 101 keys 5.5 ->
@@ -1088,7 +1110,7 @@ void launch_paged_attention(PagedAttnArgs a, hipStream_t stream) {
     }
   });
   if (a.whole) return;
-  a.join_heads = units <= 64;
+  a.join_heads = units <= kJoinHeadUnits;
   a.piece_waves = waves;
   const dim3 grid(a.join_heads ? s.units * s.block_heads : s.units, a.table.sequences);
   auto join = [&](auto d, auto threads) {
