@@ -46,12 +46,13 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 // tiles of 128 columns, a contiguous KiB of weights each, in flight per wave.
 //
 // Bound.  The weights' bytes and the waits at a call's start and end: 16 tokens by
-// 151936 x 896 in groups of 32 takes 22 us for 81 MB (3.7 TB/s; a read alone runs at
-// 7.0), 1 by 152064 x 3584 in groups of 128 52 us (5.3 TB/s), 1 by 40000 x 4096
-// 19.7 us (4.4 TB/s), 1 by 896 x 896 3.1 us, of which 1.7 are an empty launch.  The
-// vector instructions (about 60 a tile) would allow a KiB in 65 cycles of a CU, whose
-// share of HBM is a KiB in 90.  Where K is long and row tiles are few (16 x 1536 x
-// 8960, 12.8 us) it is the activations, all of them read by each CU at 64 bytes a ns.
+// 151936 x 896 in groups of 32 takes 20.4 us for 81 MB (4.0 TB/s; a read alone runs at
+// 7.0), 1 by 152064 x 3584 in groups of 128 50 us (5.6 TB/s), 1 by 40000 x 4096 18.4
+// us (4.7 TB/s), 1 by 896 x 896 3.1 us, of which 1.7 are an empty launch.  The vector
+// instructions (60 to 80 a tile, by the group) would allow a KiB in 65 to 85 cycles of
+// a CU, whose share of HBM is a KiB in 90.  Where K is long and row tiles are few (16 x
+// 1536 x 8960, 12.5 us) it is the activations, all of them read by each CU at 64 bytes
+// a ns.
 //
 // Activations beyond FP32's reach (a sum that is not finite) are summed again
 // element by element, q s x in FP32.
@@ -64,11 +65,17 @@ __device__ __forceinline__ uint32_t word_of(const uint4& v, int i) {
   return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
 }
 
+// The constants of widen_nibbles in registers: as literals they cost an instruction
+// more a pair (and, or) than the one that takes three operands.
+struct NibbleBits {
+  uint32_t mantissa = 0x00780078u, one = 0x3F803F80u;
+  __device__ __forceinline__ NibbleBits() { asm("" : "+s"(mantissa), "+v"(one)); }
+};
+
 // Eight nibbles as 1 + u / 16 in BF16.
-__device__ __forceinline__ bf16x8_t widen_nibbles(uint32_t w) {
-  constexpr uint32_t kMantissa = 0x00780078u, kOne = 0x3F803F80u;
-  const uint4 v = make_uint4(((w << 3) & kMantissa) | kOne, ((w >> 1) & kMantissa) | kOne,
-                             ((w >> 5) & kMantissa) | kOne, ((w >> 9) & kMantissa) | kOne);
+__device__ __forceinline__ bf16x8_t widen_nibbles(uint32_t w, const NibbleBits& c) {
+  const uint4 v = make_uint4(((w << 3) & c.mantissa) | c.one, ((w >> 1) & c.mantissa) | c.one,
+                             ((w >> 5) & c.mantissa) | c.one, ((w >> 9) & c.mantissa) | c.one);
   return __builtin_bit_cast(bf16x8_t, v);
 }
 
@@ -113,7 +120,7 @@ __device__ __forceinline__ void load_piece(W4Piece& p, const W4Args& a, int rt, 
 template <int J>
 __device__ __forceinline__ float quad_lane(float v) {
   return __int_as_float(
-      __builtin_amdgcn_update_dpp(0, __float_as_int(v), J * 0x55, 0xF, 0xF, true));
+      __builtin_amdgcn_mov_dpp(__float_as_int(v), J * 0x55, 0xF, 0xF, true));
 }
 
 // -1.5 sum x over each group of a tile (four steps of 32 columns), for every row.
@@ -135,7 +142,8 @@ __device__ __forceinline__ void base_of(f32x4_t (&base)[kTileCols / G], const bf
 // total += the tile's products with x, over 16.
 template <int G>
 __device__ __forceinline__ void add_piece(f32x4_t& total, const W4Piece& p, const bf16x8_t (&x)[4],
-                                          const f32x4_t (&base)[kTileCols / G]) {
+                                          const f32x4_t (&base)[kTileCols / G],
+                                          const NibbleBits& bits) {
   constexpr int kGroups = kTileCols / G, kSteps = G / 32;
   const float s[4] = {bf16_lo(p.s.x), bf16_hi(p.s.x), bf16_lo(p.s.y), bf16_hi(p.s.y)};
 #pragma unroll
@@ -143,7 +151,7 @@ __device__ __forceinline__ void add_piece(f32x4_t& total, const W4Piece& p, cons
     f32x4_t d = base[j];
 #pragma unroll
     for (int i = j * kSteps; i < (j + 1) * kSteps; ++i) {
-      d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen_nibbles(word_of(p.w, i)), x[i], d, 0, 0, 0);
+      d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen_nibbles(word_of(p.w, i), bits), x[i], d, 0, 0, 0);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -172,8 +180,11 @@ __device__ void finish_exactly(const W4Args& a, int row, int token) {
   *y = f32_to_bf16(a.bias ? v + bf16_to_f32(a.bias[row]) : v);
 }
 
-constexpr int kRowsDepth = 4, kRowsMaxWaves = 16;
-// Workgroups of the rows kernel a CU holds, and their waves, by their LDS.
+// Tiles in flight per wave of the rows kernel: 16 x 151936 x 896 20.1 us, 21.0 with 4
+// (whose first loads delay the activations), 19.8 with 2, which loses 4-8 % on long K.
+constexpr int kRowsDepth = 3, kRowsMaxWaves = 16;
+// Workgroups of the rows kernel a CU holds, and their waves, by their LDS: as many as
+// the registers allow (two of 8 waves: 16 x 151936 x 896 24.6 us, three: 21.4).
 struct RowsShape {
   int per_cu, waves;
   size_t lds;  // at most
@@ -196,6 +207,7 @@ constexpr size_t rows_lds_bytes(int tiles, int pitch, int group) {
 template <int G, int TP>
 __global__ __launch_bounds__(kRowsMaxWaves * kWave, 6) void w4a16_rows_kernel(W4Args a) {
   constexpr int DP = kRowsDepth, kGroups = kTileCols / G;
+  constexpr int kHead = TP == 16 ? 4 : TP == 4 ? 2 : 1;
   extern __shared__ __align__(16) uint4 lds[];
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x / kWave;
@@ -209,39 +221,54 @@ __global__ __launch_bounds__(kRowsMaxWaves * kWave, 6) void w4a16_rows_kernel(W4
 
   // The wave's weights, and scales, follow each other in memory.  Loads run DP
   // tiles ahead, always: past the wave's last tile they read that one again, so
-  // that the compiler knows how many are in flight.
+  // that the compiler knows how many are in flight; the addresses are kept from it,
+  // as it would copy such a tile instead of loading it, and then wait for all.
   typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
   const int in_last = groups - (tiles - 1) * kGroups;  // groups of a row's last tile
   const uint32_t s_off = ((lane & (kGroups - 1)) * kTileRows + 4 * g) * 2;
   const uint32_t s_off_last = (min(lane & (kGroups - 1), in_last - 1) * kTileRows + 4 * g) * 2;
-  const uint8_t* w_next = a.w + static_cast<size_t>(first) * tiles * kTileBytes;
+  const int from = min(first, row_tiles - 1);  // also of a wave with no tiles
+  const uint8_t* w_next = a.w + static_cast<size_t>(from) * tiles * kTileBytes;
   const char* s_next =
-      reinterpret_cast<const char*>(a.s + static_cast<size_t>(first) * groups * kTileRows);
+      reinterpret_cast<const char*>(a.s + static_cast<size_t>(from) * groups * kTileRows);
+  const int s_step = kGroups * kTileRows * 2, s_step_last = in_last * kTileRows * 2;
   int t_ahead = 0, ahead = 0;
   auto load_next = [&](W4Piece& p) {
     const bool ends = t_ahead + 1 == tiles;
     p.w = load_stream16(w_next + 16 * lane);
     const u32x2 v = gload(reinterpret_cast<const u32x2*>(s_next + (ends ? s_off_last : s_off)));
     p.s = make_uint2(v.x, v.y);
-    if (ahead + 1 < count) {
-      ++ahead;
-      w_next += kTileBytes;
-      s_next += (ends ? in_last : kGroups) * kTileRows * 2;
-      t_ahead = ends ? 0 : t_ahead + 1;
-    }
+    const int more = ahead + 1 < count ? -1 : 0;  // a mask: as branches the
+    ahead -= more;                                // advance would part the block
+    w_next += kTileBytes & more;
+    s_next += (ends ? s_step_last : s_step) & more;
+    t_ahead -= more;
+    t_ahead = t_ahead == tiles ? 0 : t_ahead;
+    asm("" : "+s"(w_next), "+s"(s_next));
   };
-  W4Piece p[DP];
-  if (count > 0) {
+  // The activations' first loads go ahead of the weights', whose return they would
+  // wait for, and reach LDS while those are on their way.
+  const int chunks = a.k / 8, pieces = tiles * (kTileCols / 8) * TP;
+  auto inside = [&](int i) { return i < pieces && i / TP < chunks && i % TP < a.tokens; };
+  auto x_at = [&](int i) { return a.x + static_cast<size_t>(i % TP) * a.k + 8 * (i / TP); };
+  uint4 head[kHead];
 #pragma unroll
-    for (int i = 0; i < DP; ++i) load_next(p[i]);
+  for (int b = 0; b < kHead; ++b) {
+    const int i = threadIdx.x + b * blockDim.x;
+    head[b] = load_global16(inside(i) ? x_at(i) : a.x);
   }
-  // the activations, while those are on their way, and the bases of them
-  const int chunks = a.k / 8;
-  for (int i = threadIdx.x; i < tiles * (kTileCols / 8) * TP; i += blockDim.x) {
-    const int chunk = i / TP, token = i % TP;
-    lds[i] = chunk < chunks && token < a.tokens
-                 ? load_global16(a.x + static_cast<size_t>(token) * a.k + 8 * chunk)
-                 : make_uint4(0, 0, 0, 0);
+  asm volatile("" ::: "memory");
+  W4Piece p[DP];
+#pragma unroll
+  for (int i = 0; i < DP; ++i) load_next(p[i]);
+  asm volatile("" ::: "memory");
+#pragma unroll
+  for (int b = 0; b < kHead; ++b) {
+    const int i = threadIdx.x + b * blockDim.x;
+    if (i < pieces) lds[i] = inside(i) ? head[b] : make_uint4(0, 0, 0, 0);
+  }
+  for (int i = threadIdx.x + kHead * blockDim.x; i < pieces; i += blockDim.x) {
+    lds[i] = inside(i) ? load_global16(x_at(i)) : make_uint4(0, 0, 0, 0);
   }
   __syncthreads();
   const int lds_lane = g * TP + r % TP;  // of a step's 4 x TP pieces
@@ -261,50 +288,64 @@ __global__ __launch_bounds__(kRowsMaxWaves * kWave, 6) void w4a16_rows_kernel(W4
   if (count <= 0) return;
   const bool wide = (a.n & 3) == 0 && (reinterpret_cast<uintptr_t>(a.y) & 7u) == 0;
 
+  const NibbleBits bits;
   f32x4_t total{0.0f, 0.0f, 0.0f, 0.0f};
   bool again = false;
   int rt = first, t = 0;
-  for (int item = 0; item < count;) {
+  auto piece = [&](int i, auto more) {
+    bf16x8_t x[4];
+    f32x4_t base[kGroups];
 #pragma unroll
-    for (int i = 0; i < DP; ++i) {
-      bf16x8_t x[4];
-      f32x4_t base[kGroups];
+    for (int j = 0; j < 4; ++j) {
+      x[j] = __builtin_bit_cast(bf16x8_t, lds[(t * 4 + j) * 4 * TP + lds_lane]);
+    }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        x[j] = __builtin_bit_cast(bf16x8_t, lds[(t * 4 + j) * 4 * TP + lds_lane]);
-      }
+    for (int j = 0; j < kGroups; ++j) base[j] = bases[(t * kGroups + j) * TP + r % TP];
+    add_piece<G>(total, p[i], x, base, bits);
+    if (decltype(more)::value) load_next(p[i]);
+    if (++t == tiles) {
+      const int row = rt * kTileRows + 4 * g;
+      if (r < a.tokens) {
+        uint16_t* y = a.y + static_cast<size_t>(r) * a.n + row;
+        uint16_t v[4];
+        f32x4_t b{0.0f, 0.0f, 0.0f, 0.0f};
+        if (a.bias) {
 #pragma unroll
-      for (int j = 0; j < kGroups; ++j) base[j] = bases[(t * kGroups + j) * TP + r % TP];
-      add_piece<G>(total, p[i], x, base);
-      load_next(p[i]);
-      if (++t == tiles) {
-        const int row = rt * kTileRows + 4 * g;
-        if (r < a.tokens) {
-          uint16_t* y = a.y + static_cast<size_t>(r) * a.n + row;
-          uint16_t v[4];
+          for (int j = 0; j < 4; ++j) b[j] = bf16_to_f32(a.bias[min(row + j, a.n - 1)]);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          v[j] = f32_to_bf16(fmaf(total[j], 16.0f, b[j]));
+          again = again || (row + j < a.n && not_finite(v[j]));
+        }
+        if (wide) {  // then the four rows are in the matrix or none is
+          if (row < a.n) {
+            store_global8(y, make_uint2(v[0] | static_cast<uint32_t>(v[1]) << 16,
+                                        v[2] | static_cast<uint32_t>(v[3]) << 16));
+          }
+        } else {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            v[j] = row + j < a.n ? finish(a, total[j], row + j) : 0;
-            again = again || not_finite(v[j]);
-          }
-          if (wide) {  // then the four rows are in the matrix or none is
-            if (row < a.n) {
-              store_global8(y, make_uint2(v[0] | static_cast<uint32_t>(v[1]) << 16,
-                                          v[2] | static_cast<uint32_t>(v[3]) << 16));
-            }
-          } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              if (row + j < a.n) y[j] = v[j];
-            }
+            if (row + j < a.n) y[j] = v[j];
           }
         }
-        total = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-        t = 0;
-        ++rt;
       }
-      if (++item == count) break;
+      total = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+      t = 0;
+      ++rt;
     }
+  };
+  // DP tiles a pass, left from a single place: with a way out behind each, the wait
+  // for the first piece's loads would be for the way from all of them.  The last pass
+  // loads nothing.
+  int item = 0;
+  for (; item + DP < count; item += DP) {
+#pragma unroll
+    for (int i = 0; i < DP; ++i) piece(i, std::true_type{});
+  }
+#pragma unroll
+  for (int i = 0; i < DP; ++i) {
+    if (item + i < count) piece(i, std::false_type{});
   }
   if (again) {  // the lane's own outputs
     for (int row = first * kTileRows; row < min(last * kTileRows, a.n); ++row) {
@@ -346,6 +387,7 @@ __global__ __launch_bounds__(kSplitWaves * kWave) void w4a16_split_kernel(W4Args
   const int first = blockIdx.x * R;
   const int x_part = r % S * kLoads * 32;
   const uint16_t* x_row = a.x + static_cast<size_t>(min(r / S, a.tokens - 1)) * a.k + 8 * g;
+  const NibbleBits bits;
   f32x4_t total[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) total[i] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
@@ -393,7 +435,7 @@ __global__ __launch_bounds__(kSplitWaves * kWave) void w4a16_split_kernel(W4Args
         if (kTileCols / G > 1 && (t0 + i * waves) * (kTileCols / G) + (lane & (kTileCols / G - 1)) >= groups) {
           p[i][j].s = make_uint2(0, 0);
         }
-        add_piece<G>(total[j], p[i][j], xb, base);
+        add_piece<G>(total[j], p[i][j], xb, base, bits);
       }
     }
   }
@@ -418,15 +460,15 @@ __global__ __launch_bounds__(kSplitWaves * kWave) void w4a16_split_kernel(W4Args
 }
 
 constexpr int kCus = 256;
-// Row tiles from which a wave takes whole ones.  Few tokens: as many as the chip
-// then has waves (1 x 100000 x 2048 24.8 us split, 25.0 in rows; 65536 17.1 and 18.0;
-// 128000 30.9 and 29.4).  More than 8, whose activations the split kernel reads at
-// the weights' own rate or faster: fewer, if K is long (16 x 40000 x 4096 28.0 us
-// split, 25.6 in rows; x 1536 13.4 and 13.3; 16 x 32768 x 1024 7.8 and 10.4).
-constexpr int kRowsTiles = 6144, kRowsTilesMany = 2048, kRowsLongTiles = 12;
+// Row tiles from which a wave takes whole ones (1 x 65536 x 1024 10.6 us split, 10.1 in
+// rows; 8 x 80000 x 2048 22.7 and 19.9; 1 x 40000 x 4096 18.4 and 20.7).  More than 8
+// tokens, whose activations the split kernel reads at the weights' own rate or faster:
+// fewer, if K is long (16 x 40000 x 4096 28.0 and 22.3; 16 x 32768 x 1024 7.8 and 9.3).
+constexpr int kRowsTiles = 4096, kRowsTilesMany = 2048, kRowsLongTiles = 12;
 // Row tiles from which the split kernel takes two a workgroup: half the activations'
 // reads, half the workgroups (16 x 17920 x 1536 10.7 -> 9.5 us; 1 x 40000 x 4096 22.7
-// -> 19.7, 1 x 30000 x 1024 6.9 -> 6.5, but 1 x 17920 x 1536 6.3 -> 6.7).
+// -> 19.7, 1 x 30000 x 1024 6.9 -> 6.5, but 1 x 17920 x 1536 6.3 -> 6.7; an instruction
+// a pair of nibbles less has since taken 2-7 % off each).
 constexpr int kPairTiles = 1536, kPairTilesMany = 1024;
 constexpr int kManyTokens = 9;         // tokens from which the above say "many"
 constexpr int kSplitRoom = 16 * kCus;  // waves that the split kernel fills the chip with

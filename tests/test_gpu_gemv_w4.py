@@ -64,7 +64,7 @@ def test_many_rows(hip, dev, group):
     check(run(hip, dev, q, s, group, b, x), *ref.product(q, s, group, b, x))
 
 
-# Whole row tiles a wave (98304 rows up; 32768 for 9 tokens up and long K): one token,
+# Whole row tiles a wave (65536 rows up; 32768 for 9 tokens up and long K): one token,
 # a few, sixteen; groups that end inside a column tile; rows that end inside a tile or
 # a 4-row piece; LDS for three, two and one workgroup a CU, and too little.  Pairs of
 # row tiles (24576 rows up; 16384 for 9 tokens up) with one and several column tiles a
@@ -75,7 +75,7 @@ def test_many_rows(hip, dev, group):
     (20001, 384, 64, 12), (18000, 4864, 128, 16), (17001, 3168, 32, 9), (20003, 2048, 32, 8),
     (98305, 160, 32, 1), (98319, 1088, 64, 4), (98306, 96, 32, 3), (99001, 416, 32, 8),
     (100004, 128, 128, 16), (24577, 1088, 64, 5), (24580, 96, 32, 1), (30001, 2432, 32, 4),
-    (33001, 160, 32, 8), (33017, 1184, 32, 16), (26011, 192, 64, 7)])
+    (33001, 160, 32, 8), (33017, 1184, 32, 16), (26011, 192, 64, 7), (65537, 1504, 32, 2), (65600, 64, 64, 1)])
 def test_product_of_many_rows(hip, dev, n, k, group, tokens):
     q, s, x, b = make(n, k, group, tokens, n + k, bias=tokens % 2 == 0)
     got = run(hip, dev, q, s, group, b, x)
