@@ -979,7 +979,7 @@ void launch_kv_store(const KvStoreArgs& a, hipStream_t stream) {
 // again, next to what else a model's layers read.
 constexpr long long kStreamBytes = 96ll << 20;
 
-// A load that writes more than kStreamBytes does not leave it in the caches: 12 x
+// A load into caches of more than kStreamBytes does not leave them there: 12 x
 // 9000 rows of 4 x 128 INT8 36 -> 25.5 us, 64 x 1000 of 8 x 64 FP8 32 -> 18.  A
 // kernel that reads all of it next, and does nothing else, is slower by as much
 // (both together 111 us either way; after a store of the same rows 287 -> 284); a

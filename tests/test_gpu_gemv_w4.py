@@ -83,6 +83,24 @@ def test_product_of_many_rows(hip, dev, n, k, group, tokens):
     check(got, y.cpu(), bound.cpu())
 
 
+@pytest.mark.parametrize("tokens", [1, 16])
+def test_weights_past_32_bits(hip, dev, tokens):
+    """The last rows of more than 2^32 bytes of weights."""
+    n, k, group, last = (1 << 18) + 4800, 32768, 64, 48
+    g = torch.Generator(device=dev).manual_seed(3)
+    packed = torch.randint(0, 256, (n * k // 2,), generator=g, dtype=torch.uint8, device=dev)
+    scales = (torch.rand(n * (k // group), generator=g, device=dev) * 0.02).to(torch.bfloat16)
+    assert packed.numel() > 1 << 32
+    x = torch.randn((tokens, k), generator=g, device=dev).to(torch.bfloat16)
+    out = torch.empty((tokens, n), dtype=torch.bfloat16, device=dev)
+    hip.gemv_w4a16(packed, scales, group, None, x, out, tokens, n, k)
+    for at in (0, n - last):
+        q = ref.unpack(packed[at * k // 2:(at + last) * k // 2].cpu(), last, k)
+        s = scales[at * (k // group):(at + last) * (k // group)].cpu().view(last // 16, -1, 16)
+        s = s.transpose(1, 2).reshape(last, -1)
+        check(out[:, at:at + last].cpu(), *ref.product(q, s, group, None, x.cpu()))
+
+
 @pytest.mark.parametrize("tokens", [1, 3, 16])
 @pytest.mark.parametrize("n", [32805, 98341])
 def test_infinities_in_many_rows(hip, dev, n, tokens):

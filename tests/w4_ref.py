@@ -21,6 +21,15 @@ def pack(q, scales):
     return packed.reshape(-1), s.view(rows // 16, 16, -1).transpose(1, 2).contiguous().view(-1)
 
 
+def unpack(packed, n, k):
+    """int8 q [n, k] of packed weight bytes (whole tiles of rows)."""
+    words = packed.view(n // 16, -(-k // 128), 4, 16, 4, 4).to(torch.int64)
+    dword = sum(words[..., i] << (8 * i) for i in range(4))  # [tile row, tile, b, r, i]
+    u = torch.stack([(dword >> (4 * COLUMN.index(c))) & 15 for c in range(8)], dim=-1)
+    # -> [tile row, r, tile, i, b, column]
+    return (u.permute(0, 3, 1, 4, 2, 5).reshape(n, -1)[:, :k] - 8).to(torch.int8)
+
+
 def product(q, scales, group, bias, x):
     """(Y in 64 bits, the bound on its FP32 sums): a group's sum is taken of
     products as large as 31 |x| (the elements are held as 16 + u, u = q + 8, and
