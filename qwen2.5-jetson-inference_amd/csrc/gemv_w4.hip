@@ -51,8 +51,7 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 // us (4.7 TB/s), 1 by 896 x 896 3.1 us, of which 1.7 are an empty launch.  The vector
 // instructions (60 to 80 a tile, by the group) would allow a KiB in 65 to 85 cycles of
 // a CU, whose share of HBM is a KiB in 90.  Where K is long and row tiles are few (16 x
-// 1536 x 8960, 12.5 us) it is the activations, all of them read by each CU at 64 bytes
-// a ns.
+// 1536 x 8960, 9.7 us) it is the activations, all of them read by each CU.
 //
 // Activations beyond FP32's reach (a sum that is not finite) are summed again
 // element by element, q s x in FP32.
@@ -192,13 +191,16 @@ struct RowsShape {
 constexpr RowsShape kRowsShapes[] = {
     {3, 8, 52 * 1024}, {2, 12, 78 * 1024}, {1, kRowsMaxWaves, 156 * 1024}};
 
-// LDS of the rows kernel: the activations [K / 8][TP tokens][8], zero past K and
-// past the tokens, then the groups' bases [K / G][TP][4].
-constexpr size_t rows_x_bytes(int tiles, int pitch) {
-  return static_cast<size_t>(tiles) * kTileCols * 2 * pitch;
+// LDS of the rows kernel: the activations [K / 8][pitch][8] for TP tokens, zero past K
+// and past the tokens, then the groups' bases [K / G][TP][4].  With 16 tokens a piece
+// of 16 bytes more for each 8 columns: a token's neighbouring pieces, which neighbouring
+// lanes load, then go to different banks.
+constexpr int x_pitch(int tp) { return tp == 16 ? 17 : tp; }
+constexpr size_t rows_x_bytes(int tiles, int tp) {
+  return static_cast<size_t>(tiles) * kTileCols * 2 * x_pitch(tp);
 }
-constexpr size_t rows_lds_bytes(int tiles, int pitch, int group) {
-  return rows_x_bytes(tiles, pitch) + static_cast<size_t>(tiles) * (kTileCols / group) * pitch * 16;
+constexpr size_t rows_lds_bytes(int tiles, int tp, int group) {
+  return rows_x_bytes(tiles, tp) + static_cast<size_t>(tiles) * (kTileCols / group) * tp * 16;
 }
 
 // Workgroup i takes the i-th of equal shares of the row tiles, its waves equal
@@ -208,6 +210,7 @@ template <int G, int TP>
 __global__ __launch_bounds__(kRowsMaxWaves * kWave, 6) void w4a16_rows_kernel(W4Args a) {
   constexpr int DP = kRowsDepth, kGroups = kTileCols / G;
   constexpr int kHead = TP == 16 ? 4 : TP == 4 ? 2 : 1;
+  constexpr int kPieces = kTileCols / 8, kPitch = x_pitch(TP);  // of a tile; in LDS
   extern __shared__ __align__(16) uint4 lds[];
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x / kWave;
@@ -248,36 +251,37 @@ __global__ __launch_bounds__(kRowsMaxWaves * kWave, 6) void w4a16_rows_kernel(W4
   };
   // The activations' first loads go ahead of the weights', whose return they would
   // wait for, and reach LDS while those are on their way.
-  const int chunks = a.k / 8, pieces = tiles * (kTileCols / 8) * TP;
-  auto inside = [&](int i) { return i < pieces && i / TP < chunks && i % TP < a.tokens; };
-  auto x_at = [&](int i) { return a.x + static_cast<size_t>(i % TP) * a.k + 8 * (i / TP); };
+  const int chunks = a.k / 8, pieces = tiles * kPieces * TP;
+  auto chunk_of = [&](int i) { return i / (kPieces * TP) * kPieces + i % kPieces; };
+  auto token_of = [&](int i) { return i / kPieces % TP; };
+  auto inside = [&](int i) { return chunk_of(i) < chunks && token_of(i) < a.tokens; };
+  auto load_x = [&](int i) {
+    return load_global16(i < pieces && inside(i)
+                             ? a.x + static_cast<size_t>(token_of(i)) * a.k + 8 * chunk_of(i)
+                             : a.x);
+  };
+  auto keep_x = [&](int i, const uint4& v) {
+    if (i < pieces) lds[chunk_of(i) * kPitch + token_of(i)] = inside(i) ? v : make_uint4(0, 0, 0, 0);
+  };
   uint4 head[kHead];
 #pragma unroll
-  for (int b = 0; b < kHead; ++b) {
-    const int i = threadIdx.x + b * blockDim.x;
-    head[b] = load_global16(inside(i) ? x_at(i) : a.x);
-  }
+  for (int b = 0; b < kHead; ++b) head[b] = load_x(threadIdx.x + b * blockDim.x);
   asm volatile("" ::: "memory");
   W4Piece p[DP];
 #pragma unroll
   for (int i = 0; i < DP; ++i) load_next(p[i]);
   asm volatile("" ::: "memory");
 #pragma unroll
-  for (int b = 0; b < kHead; ++b) {
-    const int i = threadIdx.x + b * blockDim.x;
-    if (i < pieces) lds[i] = inside(i) ? head[b] : make_uint4(0, 0, 0, 0);
-  }
-  for (int i = threadIdx.x + kHead * blockDim.x; i < pieces; i += blockDim.x) {
-    lds[i] = inside(i) ? load_global16(x_at(i)) : make_uint4(0, 0, 0, 0);
-  }
+  for (int b = 0; b < kHead; ++b) keep_x(threadIdx.x + b * blockDim.x, head[b]);
+  for (int i = threadIdx.x + kHead * blockDim.x; i < pieces; i += blockDim.x) keep_x(i, load_x(i));
   __syncthreads();
-  const int lds_lane = g * TP + r % TP;  // of a step's 4 x TP pieces
-  f32x4_t* const bases = reinterpret_cast<f32x4_t*>(lds + tiles * (kTileCols / 8) * TP);
+  const int lds_lane = g * kPitch + r % TP;  // of a step's 4 x kPitch pieces
+  f32x4_t* const bases = reinterpret_cast<f32x4_t*>(lds + tiles * kPieces * kPitch);
   for (int t = wave; t < tiles; t += waves) {
     bf16x8_t x[4];
     f32x4_t base[kGroups];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = __builtin_bit_cast(bf16x8_t, lds[(t * 4 + j) * 4 * TP + lds_lane]);
+    for (int j = 0; j < 4; ++j) x[j] = __builtin_bit_cast(bf16x8_t, lds[(t * 4 + j) * 4 * kPitch + lds_lane]);
     base_of<G>(base, x);
     if (lane < TP) {
 #pragma unroll
@@ -297,7 +301,7 @@ __global__ __launch_bounds__(kRowsMaxWaves * kWave, 6) void w4a16_rows_kernel(W4
     f32x4_t base[kGroups];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      x[j] = __builtin_bit_cast(bf16x8_t, lds[(t * 4 + j) * 4 * TP + lds_lane]);
+      x[j] = __builtin_bit_cast(bf16x8_t, lds[(t * 4 + j) * 4 * kPitch + lds_lane]);
     }
 #pragma unroll
     for (int j = 0; j < kGroups; ++j) base[j] = bases[(t * kGroups + j) * TP + r % TP];
@@ -371,6 +375,14 @@ __device__ __forceinline__ uint4 share_lane(const uint4& v) {
   return make_uint4(one(v.x), one(v.y), one(v.z), one(v.w));
 }
 
+// v of lane `from` / 4.
+__device__ __forceinline__ uint4 lane_of(const uint4& v, int from) {
+  auto one = [&](uint32_t w) {
+    return static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(from, static_cast<int>(w)));
+  };
+  return make_uint4(one(v.x), one(v.y), one(v.z), one(v.w));
+}
+
 // Workgroup i: row tiles [i R, (i + 1) R); wave w takes their column tiles w, w +
 // waves, ..., DP of them in flight.  With R > 1 the activations, four KiB a tile
 // at 16 tokens, are read for R KiB of weights.  With at most 16 / S tokens S columns
@@ -385,8 +397,13 @@ __global__ __launch_bounds__(kSplitWaves * kWave) void w4a16_split_kernel(W4Args
   const int tiles = (a.k + kTileCols - 1) / kTileCols, groups = a.k / G;
   const int row_tiles = (a.n + kTileRows - 1) / kTileRows;
   const int first = blockIdx.x * R;
-  const int x_part = r % S * kLoads * 32;
-  const uint16_t* x_row = a.x + static_cast<size_t>(min(r / S, a.tokens - 1)) * a.k + 8 * g;
+  // Lane 16 g + r multiplies token r / S's columns 8 g .. of each step of 32, but loads
+  // what the lane with g and r's low bits exchanged does: four lanes in a row then read
+  // 64 bytes in a row, not 16 of four tokens (16 x 8960 x 1536 7.4 -> 5.7 us, 16 x 1536 x
+  // 8960 12.5 -> 9.7, 5 x 17920 x 1536 in groups of 128 6.8 -> 6.2).
+  const int gl = lane & 3, rl = (lane & 12) | g, from = 4 * ((r & 3) << 4 | (r & 12) | g);
+  const int x_part = rl % S * kLoads * 32;
+  const uint16_t* x_row = a.x + static_cast<size_t>(min(rl / S, a.tokens - 1)) * a.k + 8 * gl;
   const NibbleBits bits;
   f32x4_t total[R];
 #pragma unroll
@@ -415,6 +432,8 @@ __global__ __launch_bounds__(kSplitWaves * kWave) void w4a16_split_kernel(W4Args
     for (int i = 0; i < DP; ++i) {
       if (t0 + i * waves >= tiles) break;
       bf16x8_t xb[4];
+#pragma unroll
+      for (int j = 0; j < kLoads; ++j) x[i][j] = lane_of(x[i][j], from);
       auto put = [&](auto from) {
         constexpr int kFrom = decltype(from)::value;
 #pragma unroll
@@ -463,12 +482,11 @@ constexpr int kCus = 256;
 // Row tiles from which a wave takes whole ones (1 x 65536 x 1024 10.6 us split, 10.1 in
 // rows; 8 x 80000 x 2048 22.7 and 19.9; 1 x 40000 x 4096 18.4 and 20.7).  More than 8
 // tokens, whose activations the split kernel reads at the weights' own rate or faster:
-// fewer, if K is long (16 x 40000 x 4096 28.0 and 22.3; 16 x 32768 x 1024 7.8 and 9.3).
+// fewer, if K is long (16 x 40000 x 4096 23.9 and 22.2; 16 x 32768 x 1024 6.9 and 9.3).
 constexpr int kRowsTiles = 4096, kRowsTilesMany = 2048, kRowsLongTiles = 12;
 // Row tiles from which the split kernel takes two a workgroup: half the activations'
-// reads, half the workgroups (16 x 17920 x 1536 10.7 -> 9.5 us; 1 x 40000 x 4096 22.7
-// -> 19.7, 1 x 30000 x 1024 6.9 -> 6.5, but 1 x 17920 x 1536 6.3 -> 6.7; an instruction
-// a pair of nibbles less has since taken 2-7 % off each).
+// reads, half the workgroups (16 x 17920 x 1536 8.1 -> 7.8 us, 16 x 30000 x 1024 8.9 -> 7.2, 1 x
+// 40000 x 4096 21.6 -> 18.1, 1 x 30000 x 1024 6.7 -> 6.5, but 1 x 17920 x 1536 5.8 -> 6.4).
 constexpr int kPairTiles = 1536, kPairTilesMany = 1024;
 constexpr int kManyTokens = 9;         // tokens from which the above say "many"
 constexpr int kSplitRoom = 16 * kCus;  // waves that the split kernel fills the chip with
@@ -477,10 +495,10 @@ template <int G>
 void launch_w4(const W4Args& a, hipStream_t stream) {
   const int row_tiles = (a.n + kTileRows - 1) / kTileRows;
   const int tiles = (a.k + kTileCols - 1) / kTileCols;
-  const int pitch = a.tokens == 1 ? 1 : a.tokens <= 4 ? 4 : 16;
+  const int room_for = a.tokens == 1 ? 1 : a.tokens <= 4 ? 4 : 16;
   const bool many = a.tokens >= kManyTokens;
   for (const RowsShape& shape : kRowsShapes) {
-    const size_t lds = rows_lds_bytes(tiles, pitch, G);
+    const size_t lds = rows_lds_bytes(tiles, room_for, G);
     if (row_tiles < (many && tiles > kRowsLongTiles ? kRowsTilesMany : kRowsTiles) ||
         lds > shape.lds) {
       continue;
@@ -489,20 +507,20 @@ void launch_w4(const W4Args& a, hipStream_t stream) {
       hipLaunchKernelGGL((w4a16_rows_kernel<G, decltype(tp)::value>), dim3(shape.per_cu * kCus),
                          dim3(shape.waves * kWave), lds, stream, a);
     };
-    if (pitch == 1) {
+    if (room_for == 1) {
       launch(std::integral_constant<int, 1>{});
-    } else if (pitch == 4) {
+    } else if (room_for == 4) {
       launch(std::integral_constant<int, 4>{});
     } else {
       launch(std::integral_constant<int, 16>{});
     }
     return;
   }
-  // Waves for the chip's room, at least eight, of equal shares of the tiles.  A wave's
-  // loads in flight are all of its tiles up to five with up to four tokens; with more,
-  // whose activations fill a CU's queue of loads, one (5 x 1536 x 8960 7.8 us, 9.1
-  // with four; 16 x 896 x 4864 7.9, 8.8 with two) or two where that is all of them (8 x
-  // 17920 x 1536 7.3, 7.5 with one) or the pairs halve the activations.
+  // Waves for the chip's room, at least eight, of equal shares of the tiles (12 or 16:
+  // 1 x 17920 x 1536 7.7 us for 6.3; 4 or 6: 9 x 30000 x 1024 7.0 for 6.5, though 1 x
+  // 30000 x 1024 6.2).  A wave's loads in flight are all of its tiles up to five with up
+  // to four tokens, two with more (16 x 3584 x 18944 20.0 us with one, 17.0 with two, 18.3
+  // with three; 9 x 1536 x 8960 7.8, 8.4, 8.4).
   const int room = kSplitRoom / row_tiles;
   const int most = room < 8 ? 8 : room > kSplitWaves ? kSplitWaves : room;
   const int per = (tiles + most - 1) / most;
@@ -528,10 +546,8 @@ void launch_w4(const W4Args& a, hipStream_t stream) {
     per == 1 ? by_share(One{}, Two{}) : by_share(Two{}, Two{});
   } else if (per == 1) {
     by_share(One{}, One{});
-  } else if (per == 2) {
+  } else if (per == 2 || a.tokens > 4) {
     by_share(Two{}, One{});
-  } else if (a.tokens > 4) {
-    by_share(One{}, One{});
   } else {
     per <= 4 ? launch(Four{}, Four{}, One{}) : launch(Four{}, Five{}, One{});
   }
