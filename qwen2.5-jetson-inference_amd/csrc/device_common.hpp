@@ -256,6 +256,14 @@ __device__ __forceinline__ void store_global8(void* p, uint2 v) {
   *(QLIN_GLOBAL u32x2*)(p) = u32x2{v.x, v.y};
 }
 
+// v of lane `from` / 4.
+__device__ __forceinline__ uint4 lane_of(const uint4& v, int from) {
+  auto one = [&](uint32_t w) {
+    return static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(from, static_cast<int>(w)));
+  };
+  return make_uint4(one(v.x), one(v.y), one(v.z), one(v.w));
+}
+
 // 16-byte global load marked as streaming (the weights are read once per
 // call, so they should not displace reused lines).
 __device__ __forceinline__ uint4 load_stream16(const void* p) {

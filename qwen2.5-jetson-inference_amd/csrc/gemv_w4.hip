@@ -375,14 +375,6 @@ __device__ __forceinline__ uint4 share_lane(const uint4& v) {
   return make_uint4(one(v.x), one(v.y), one(v.z), one(v.w));
 }
 
-// v of lane `from` / 4.
-__device__ __forceinline__ uint4 lane_of(const uint4& v, int from) {
-  auto one = [&](uint32_t w) {
-    return static_cast<uint32_t>(__builtin_amdgcn_ds_bpermute(from, static_cast<int>(w)));
-  };
-  return make_uint4(one(v.x), one(v.y), one(v.z), one(v.w));
-}
-
 // Workgroup i: row tiles [i R, (i + 1) R); wave w takes their column tiles w, w +
 // waves, ..., DP of them in flight.  With R > 1 the activations, four KiB a tile
 // at 16 tokens, are read for R KiB of weights.  With at most 16 / S tokens S columns

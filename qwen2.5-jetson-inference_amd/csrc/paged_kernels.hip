@@ -585,7 +585,15 @@ __global__ __launch_bounds__(W * kWave, 2) void paged_attention_kernel(PagedAttn
     u32x4 k[2][KC];
     Words<VB> v[8];
     f32x4_t ks[2], vs[2];
-    const uint32_t k_off = r * RB + 16 * g, v_off = 4 * g * RB + r * VB;
+    // In BF16 a lane loads of the keys what the lane with g and r's low bits exchanged
+    // multiplies: four lanes in a row then read 64 bytes in a row, not 16 of four keys (28
+    // / 4 / 128 heads: 1 x 500 keys 9.0 -> 8.1 us, 16 x 500 9.4 -> 8.5, 1 x 131001 30.7 ->
+    // 30.4).  8-bit keys, half the loads, lose by the exchange (in INT8 8.4 -> 9.1, 8.6 ->
+    // 9.2).
+    constexpr bool kTurned = F == kBf16;
+    const uint32_t k_off = kTurned ? ((lane & 12) | g) * RB + 16 * (lane & 3) : r * RB + 16 * g;
+    const uint32_t v_off = 4 * g * RB + r * VB;
+    const int from = 4 * ((r & 3) << 4 | (r & 12) | g);
     auto load_keys = [&] {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -642,8 +650,9 @@ __global__ __launch_bounds__(W * kWave, 2) void paged_attention_kernel(PagedAttn
 #pragma unroll
         for (int c = 0; c < KC; ++c) {
           if (F == kBf16) {
-            d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, k[h][c]), q[c],
-                                                        d, 0, 0, 0);
+            const uint4 mine = lane_of(__builtin_bit_cast(uint4, k[h][c]), from);
+            d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, mine), q[c], d,
+                                                        0, 0, 0);
           } else {
             d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen8<F>(k[h][c].x, k[h][c].y), q[2 * c],
                                                         d, 0, 0, 0);
