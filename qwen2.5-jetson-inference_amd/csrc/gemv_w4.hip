@@ -46,7 +46,7 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 // tiles of 128 columns, a contiguous KiB of weights each, in flight per wave.
 //
 // Bound.  The weights' bytes and the waits at a call's start and end: 16 tokens by
-// 151936 x 896 in groups of 32 takes 20.4 us for 81 MB (4.0 TB/s; a read alone runs at
+// 151936 x 896 in groups of 32 takes 20 us for 81 MB (4.1 TB/s; a read alone runs at
 // 7.0), 1 by 152064 x 3584 in groups of 128 50 us (5.6 TB/s), 1 by 40000 x 4096 18.4
 // us (4.7 TB/s), 1 by 896 x 896 3.1 us, of which 1.7 are an empty launch.  The vector
 // instructions (60 to 80 a tile, by the group) would allow a KiB in 65 to 85 cycles of

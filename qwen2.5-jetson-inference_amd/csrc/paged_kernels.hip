@@ -255,11 +255,11 @@ __global__ __launch_bounds__(kThreads) void kv_load_kernel(KvLoadArgs a) {
 // 1.35 times the output rounding's own; maxima, sums and O are FP32.
 //
 // Bound.  Large calls: the cache's bytes, 1 x 131001 keys of 2 x 128 in BF16 (134 MB)
-// 30.6 us, 64 sequences of up to 4000 of 8 x 128 in FP8 (270 MB) 52 us, 5.2 TB/s;
+// 30.4 us, 64 sequences of up to 4000 of 8 x 128 in FP8 (270 MB) 52 us, 5.2 TB/s;
 // a read alone runs at 7.0.  A tile in flight a wave and eight waves a CU are what
 // the registers hold (two tiles in flight, or more waves, gained nothing).  Small
 // calls: the launches and their chains of dependent reads, lengths, table, keys: 1 x
-// 101 keys 4.8 us, 16 x 2000 in INT8 9.4 us, 3.7 of them the second launch.
+// 101 keys 4.7 us, 16 x 2000 in INT8 9.4 us, 3.1 of them the second launch.
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
