@@ -120,18 +120,27 @@ __global__ __launch_bounds__(kThreads) void kv_store_kernel(KvStoreArgs a) {
   const unsigned t = item / rows;
   if (t >= static_cast<unsigned>(a.tokens)) return;  // whole groups of L lanes
   const int row = item % rows;
+  // Position, sequence and row are read together, then the page and the rotation.
   const int pos = a.positions[t];
-  if (pos < 0 || (a.rope && pos >= a.rope_positions)) return;
-
+  const int seq = a.sequence_ids ? a.sequence_ids[t] : static_cast<int>(t);
   const bool is_q = row < a.heads;
   const bool is_v = row >= a.heads + a.pool.kv_heads;
   const int head = is_q ? row : is_v ? row - a.heads - a.pool.kv_heads : row - a.heads;
   const uint16_t* src = (is_q ? a.q + t * a.q_stride : is_v ? a.v + t * a.v_stride
                                                             : a.k + t * a.k_stride) +
                         static_cast<size_t>(head) * D + 8 * c;
+  const uint4 row_lo = load_global16(src), row_hi = load_global16(src + D / 2);
+  asm volatile("" ::: "memory");  // not behind the ways out
+  if (pos < 0 || (a.rope && pos >= a.rope_positions)) return;
+  const int index = pos >> a.pool.page_shift;
+  const bool placed = !is_q &&
+                      static_cast<unsigned>(seq) < static_cast<unsigned>(a.table.sequences) &&
+                      index < a.table.max_pages;
+  const int page =
+      placed ? a.table.pages[static_cast<size_t>(seq) * a.table.stride + index] : -1;
   float lo[8], hi[8];
-  unpack8(load_global16(src), lo);
-  unpack8(load_global16(src + D / 2), hi);
+  unpack8(row_lo, lo);
+  unpack8(row_hi, hi);
   if (a.rope && !is_v) {
     rotate8(lo, hi, a.rope + static_cast<size_t>(pos) * D + 16 * c);
   }
@@ -141,13 +150,6 @@ __global__ __launch_bounds__(kThreads) void kv_store_kernel(KvStoreArgs a) {
     store_global16(dst + D / 2, pack8(hi));
     return;
   }
-  const int seq = a.sequence_ids ? a.sequence_ids[t] : static_cast<int>(t);
-  const int index = pos >> a.pool.page_shift;
-  if (static_cast<unsigned>(seq) >= static_cast<unsigned>(a.table.sequences) ||
-      index >= a.table.max_pages) {
-    return;
-  }
-  const int page = a.table.pages[static_cast<size_t>(seq) * a.table.stride + index];
   if (static_cast<unsigned>(page) >= static_cast<unsigned>(a.pool.num_pages)) return;
   const size_t at = pool_row(a.pool, page, head, pos & ((1 << a.pool.page_shift) - 1));
   void* pages = is_v ? a.pool.value : a.pool.key;
