@@ -107,9 +107,9 @@ __device__ __forceinline__ void rotate8(float (&lo)[8], float (&hi)[8], const fl
 // for another row: any number of tokens, of any sequences, is one grid.
 //
 // Bound: bytes.  6 prompts of up to 5000 tokens of 32 + 2 x 8 heads of 128 in FP8 (396
-// MB) 79 us, 5.0 TB/s, as a copy.  A decode step (24 tokens of 14 + 2 x 2 heads of
-// 64) is 3.0 us, 1.7 of them the launch, the rest three dependent reads: position,
-// table, row.  Non-temporal loads or stores gained 2-3 % on some sizes and lost as
+// MB) 76 us, 5.2 TB/s, a copy 5.0.  A decode step (24 tokens of 14 + 2 x 2 heads of
+// 64) is 2.9 us, 1.7 of them the launch, the rest two reads one behind the other:
+// position, sequence and row, then page and rotation.  Non-temporal loads or stores gained 2-3 % on some sizes and lost as
 // much on others.
 template <int F, int D>
 __global__ __launch_bounds__(kThreads) void kv_store_kernel(KvStoreArgs a) {
