@@ -150,7 +150,8 @@ __device__ __forceinline__ void add_piece(f32x4_t& total, const W4Piece& p, cons
     f32x4_t d = base[j];
 #pragma unroll
     for (int i = j * kSteps; i < (j + 1) * kSteps; ++i) {
-      d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen_nibbles(word_of(p.w, i), bits), x[i], d, 0, 0, 0);
+      d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen_nibbles(word_of(p.w, i), bits), x[i], d, 0,
+                                                  0, 0);
     }
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -261,7 +262,9 @@ __global__ __launch_bounds__(kRowsMaxWaves * kWave, 6) void w4a16_rows_kernel(W4
                              : a.x);
   };
   auto keep_x = [&](int i, const uint4& v) {
-    if (i < pieces) lds[chunk_of(i) * kPitch + token_of(i)] = inside(i) ? v : make_uint4(0, 0, 0, 0);
+    if (i < pieces) {
+      lds[chunk_of(i) * kPitch + token_of(i)] = inside(i) ? v : make_uint4(0, 0, 0, 0);
+    }
   };
   uint4 head[kHead];
 #pragma unroll
@@ -281,7 +284,9 @@ __global__ __launch_bounds__(kRowsMaxWaves * kWave, 6) void w4a16_rows_kernel(W4
     bf16x8_t x[4];
     f32x4_t base[kGroups];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = __builtin_bit_cast(bf16x8_t, lds[(t * 4 + j) * 4 * kPitch + lds_lane]);
+    for (int j = 0; j < 4; ++j) {
+      x[j] = __builtin_bit_cast(bf16x8_t, lds[(t * 4 + j) * 4 * kPitch + lds_lane]);
+    }
     base_of<G>(base, x);
     if (lane < TP) {
 #pragma unroll
@@ -382,7 +387,7 @@ __device__ __forceinline__ uint4 share_lane(const uint4& v) {
 // activations and hands it to the others: 4 / S KiB a tile.
 template <int G, int S, int DP, int R>
 __global__ __launch_bounds__(kSplitWaves * kWave) void w4a16_split_kernel(W4Args a) {
-  constexpr int kPitch = R * kTileRows + 4, kLoads = 4 / S;
+  constexpr int kPitch = R * kTileRows + 4, kLoads = 4 / S, kGroups = kTileCols / G;
   extern __shared__ __align__(16) float partial[];  // [wave][token][kPitch]
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x / kWave;
@@ -443,7 +448,7 @@ __global__ __launch_bounds__(kSplitWaves * kWave) void w4a16_split_kernel(W4Args
       base_of<G>(base, xb);
 #pragma unroll
       for (int j = 0; j < R; ++j) {
-        if (kTileCols / G > 1 && (t0 + i * waves) * (kTileCols / G) + (lane & (kTileCols / G - 1)) >= groups) {
+        if (kGroups > 1 && (t0 + i * waves) * kGroups + (lane & (kGroups - 1)) >= groups) {
           p[i][j].s = make_uint2(0, 0);
         }
         add_piece<G>(total[j], p[i][j], xb, base, bits);
@@ -453,8 +458,8 @@ __global__ __launch_bounds__(kSplitWaves * kWave) void w4a16_split_kernel(W4Args
   if (r % S == 0 && r / S < a.tokens) {
 #pragma unroll
     for (int j = 0; j < R; ++j) {
-      *reinterpret_cast<f32x4_t*>(partial + (wave * a.tokens + r / S) * kPitch + j * kTileRows + 4 * g) =
-          total[j];
+      float* const at = partial + (wave * a.tokens + r / S) * kPitch + j * kTileRows + 4 * g;
+      *reinterpret_cast<f32x4_t*>(at) = total[j];
     }
   }
   __syncthreads();
@@ -636,7 +641,8 @@ extern "C" int infer_hip_gemv_w4a16(const uint8_t* weight, const uint16_t* scale
     return fail(INFER_HIP_INVALID_ARGUMENT,
                 "gemv_w4a16: weight, scales and input must be 16-byte aligned");
   }
-  const W4Args a{weight, scales, bias, input, output, tokens, out_features, in_features, group_size};
+  const W4Args a{weight, scales,       bias,        input,     output,
+                 tokens, out_features, in_features, group_size};
   if (group_size == 32) {
     launch_w4<32>(a, stream);
   } else if (group_size == 64) {

@@ -109,8 +109,8 @@ __device__ __forceinline__ void rotate8(float (&lo)[8], float (&hi)[8], const fl
 // Bound: bytes.  6 prompts of up to 5000 tokens of 32 + 2 x 8 heads of 128 in FP8 (396
 // MB) 76 us, 5.2 TB/s, a copy 5.0.  A decode step (24 tokens of 14 + 2 x 2 heads of
 // 64) is 2.9 us, 1.7 of them the launch, the rest two reads one behind the other:
-// position, sequence and row, then page and rotation.  Non-temporal loads or stores gained 2-3 % on some sizes and lost as
-// much on others.
+// position, sequence and row, then page and rotation.  Non-temporal loads or stores
+// gained 2-3 % on some sizes and lost as much on others.
 template <int F, int D>
 __global__ __launch_bounds__(kThreads) void kv_store_kernel(KvStoreArgs a) {
   constexpr int L = D / 16;
@@ -167,7 +167,9 @@ __global__ __launch_bounds__(kThreads) void kv_store_kernel(KvStoreArgs a) {
     m = max(m, max(__float_as_uint(fabsf(lo[i])), __float_as_uint(fabsf(hi[i]))));
   }
 #pragma unroll
-  for (int o = 1; o < L; o <<= 1) m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), o)));
+  for (int o = 1; o < L; o <<= 1) {
+    m = max(m, static_cast<uint32_t>(__shfl_xor(static_cast<int>(m), o)));
+  }
   const float scale = m >= 0x7F800000u ? __uint_as_float(0x7FC00000u)
                                        : __uint_as_float(m) / kLimit<F>;
   uint8_t* dst = static_cast<uint8_t*>(pages) + at * D + 8 * c;
@@ -218,8 +220,10 @@ __global__ __launch_bounds__(kThreads) void kv_load_kernel(KvLoadArgs a) {
     store_as<NT>(a.value_cache + to, v);
     return;
   }
-  const uint2 k = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.pool.key) + at * D + 8 * c);
-  const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.pool.value) + at * D + 8 * c);
+  const uint2 k = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.pool.key) +
+                                                  at * D + 8 * c);
+  const uint2 v = *reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.pool.value) +
+                                                  at * D + 8 * c);
   float x[8];
   dequantise8<F>(k, a.pool.key_scales[at], x);
   store_as<NT>(a.key_cache + to, pack8(x));
@@ -240,10 +244,11 @@ __global__ __launch_bounds__(kThreads) void kv_load_kernel(KvLoadArgs a) {
 // written by it, one inside a workgroup is joined there through LDS, and one
 // over several by a second launch, in the order of its tiles.  (Joined inside
 // the launch by the last workgroup to arrive, in two levels of 16, 131001 keys
-// of two KV heads took 42 us against 35 with a second launch, before other changes: coherent stores, an atomic and the loads
-// of what other XCDs wrote cost 4 us a level under load.)  Where the tables
-// leave room for short sequences only, the cuts move to the units' ends
-// instead and the second launch is left out.
+// of two KV heads took 42 us against 35 with a second launch, before other
+// changes: coherent stores, an atomic and the loads of what other XCDs wrote
+// cost 4 us a level under load.)  Where the tables leave room for short
+// sequences only, the cuts move to the units' ends instead and the second
+// launch is left out.
 //
 // Tile.  S = K Q^T and O^T = V^T P^T on v_mfma_f32_16x16x32_bf16.  With lane =
 // 16 g + r: S's lanes hold head r's scores of keys 4 g .. + 3 of the tile's two
@@ -394,9 +399,11 @@ __device__ __forceinline__ void turn_values(const Words<N> (&v)[8], bf16x8_t (&f
 
 // Over the four lanes r, 16 + r, 32 + r, 48 + r.
 __device__ __forceinline__ float groups_max(float v) {
-  const auto a = __builtin_amdgcn_permlane16_swap(__float_as_int(v), __float_as_int(v), false, false);
+  int w = __float_as_int(v);
+  const auto a = __builtin_amdgcn_permlane16_swap(w, w, false, false);
   v = fmaxf(__int_as_float(a[0]), __int_as_float(a[1]));
-  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_int(v), __float_as_int(v), false, false);
+  w = __float_as_int(v);
+  const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
   return fmaxf(__int_as_float(b[0]), __int_as_float(b[1]));
 }
 __device__ __forceinline__ float groups_sum(float v) {
@@ -575,7 +582,8 @@ __global__ __launch_bounds__(W * kWave, 2) void paged_attention_kernel(PagedAttn
       const bool two = t.tile * kTileKeys + 16 < t.n;
       const uint32_t head_row = static_cast<uint32_t>(t.kvh) << a.pool.page_shift;
       bad = static_cast<uint32_t>(e0) >= pages;
-      row[0] = static_cast<size_t>(bad ? 0 : e0) * page_rows + head_row + (t.tile * kTileKeys & mask);
+      row[0] = static_cast<size_t>(bad ? 0 : e0) * page_rows + head_row +
+               (t.tile * kTileKeys & mask);
       row[1] = row[0] + (two ? 16 : 0);
       if (small_pages) {
         const bool bad1 = static_cast<uint32_t>(e1) >= pages;
@@ -730,13 +738,16 @@ __global__ __launch_bounds__(W * kWave, 2) void paged_attention_kernel(PagedAttn
         if (begin == 0 && t.tile + 1 == t.tiles) {
           if (h < heads_per_kv) {
             const float inv = 1.0f / sum_l;
-            uint16_t* out = a.out + (static_cast<size_t>(t.seq) * a.heads + t.kvh * heads_per_kv + h) * D +
-                            4 * g * NO;
+            const int head = t.kvh * heads_per_kv + h;
+            uint16_t* out =
+                a.out + (static_cast<size_t>(t.seq) * a.heads + head) * D + 4 * g * NO;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               uint32_t w[NO / 2];
 #pragma unroll
-              for (int j = 0; j < NO / 2; ++j) w[j] = pack2_bf16(acc[2 * j][i] * inv, acc[2 * j + 1][i] * inv);
+              for (int j = 0; j < NO / 2; ++j) {
+                w[j] = pack2_bf16(acc[2 * j][i] * inv, acc[2 * j + 1][i] * inv);
+              }
               if constexpr (NO == 8) {
                 store_global16(out + i * NO, make_uint4(w[0], w[1], w[2], w[3]));
               } else {
@@ -836,8 +847,8 @@ __global__ __launch_bounds__(W * kWave, 2) void paged_attention_kernel(PagedAttn
         o += f * *reinterpret_cast<const f32x4_t*>(smem + at * D + d);
       }
       if (whole) {
-        store_out(a.out + (static_cast<size_t>(tag.seq) * a.heads + kvh * heads_per_kv + head) * D + d,
-                  o, sum_l);
+        const size_t out_head = static_cast<size_t>(tag.seq) * a.heads + kvh * heads_per_kv + head;
+        store_out(a.out + out_head * D + d, o, sum_l);
       } else {
         const int side = tag.begin == 0 ? 1 : 0;  // 1: the unit's first workgroup
         float* rec = a.records + (static_cast<size_t>(blockIdx.x * 2 + side) * hb + h) * (D + 4);
@@ -1083,7 +1094,8 @@ void launch_paged_attention(PagedAttnArgs a, hipStream_t stream) {
   const PagedAttnShape s = paged_attention_shape(a.heads, a.pool.kv_heads, a.pool.head_dim);
   a.head_blocks = s.head_blocks;
   a.units = s.units;
-  const long long tiles = most_tiles(a), units = static_cast<long long>(a.table.sequences) * s.units;
+  const long long tiles = most_tiles(a);
+  const long long units = static_cast<long long>(a.table.sequences) * s.units;
   a.whole = tiles <= (units <= 2 * kCus ? kWholeTiles : kWholeTilesMany);
   const bool small =
       s.block_heads > 8 || (a.whole ? tiles <= kSmallWholeTiles || units <= kSmallWholeUnits
