@@ -233,7 +233,7 @@ __global__ __launch_bounds__(kThreads) void kv_load_kernel(KvLoadArgs a) {
 
 // -------------------------------------------------------------- attention --
 //
-// out[s][h] = sum_j p_j v_j / sum_j p_j, p_j = 2^(log2(e) q.k_j / sqrt(d) - m).
+// out[s][h] = sum_j p_j v_j / sum_j p_j, p_j = 2^((q.k_j - m) log2(e) / sqrt(d)).
 //
 // Work.  A unit is a (sequence, KV head, block of at most 16 query heads) and
 // has ceil(length / 32) tiles of 32 keys.  All tiles of a call, in the order
@@ -259,7 +259,11 @@ __global__ __launch_bounds__(kThreads) void kv_load_kernel(KvLoadArgs a) {
 // multiplied.  8-bit elements become BF16 exactly; their scales go onto the
 // scores and the weights.  A weight is the sum of two BF16 numbers (2^-17 of it
 // is lost): one alone rounds as coarsely as the output and made the error
-// 1.35 times the output rounding's own; maxima, sums and O are FP32.
+// 1.35 times the output rounding's own; maxima, sums and O are FP32.  The maximum m
+// is a sum q.k itself and comes off before the factor: the difference of two close
+// scores is exact, so the largest one's weight is 1 however large it is.  (Taken off
+// as a rounded product, an exponent keeps half of the product's last bit, 2^7 from
+// 2^31 up.)
 //
 // Bound.  Large calls: the cache's bytes, 1 x 131001 keys of 2 x 128 in BF16 (134 MB)
 // 30.4 us, 64 sequences of up to 4000 of 8 x 128 in FP8 (270 MB) 52 us, 5.2 TB/s;
@@ -274,6 +278,10 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 constexpr int kTileKeys = 32;
 constexpr int kHeadBlock = 16;       // query heads of a unit at most
 constexpr float kRescaleSlack = 6.0f;  // p <= 2^6 before the maximum is moved
+
+// log2(e) / sqrt(D): a weight's exponent per unit of q.k.
+template <int D>
+constexpr float kExponent = D == 64 ? 0.18033688011112042f : 0.12751743082459868f;
 
 // A uniform 32-bit word that nothing writes while the kernel runs, through the
 // scalar cache.
@@ -627,7 +635,6 @@ __global__ __launch_bounds__(W * kWave, 2) void paged_attention_kernel(PagedAttn
       }
     };
 
-    const float scale = 1.44269504088896340736f / sqrtf(static_cast<float>(D));
     f32x4_t acc[NO];
     float m = -FLT_MAX, l = 0.0f;
 #pragma unroll
@@ -688,9 +695,10 @@ __global__ __launch_bounds__(W * kWave, 2) void paged_attention_kernel(PagedAttn
       }
       float top = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])),
                         fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
-      top = groups_max(top) * scale;
-      if (__any(top > m + kRescaleSlack)) {
-        const float up = fmaxf(m, top), old = __builtin_amdgcn_exp2f(m - up);
+      top = groups_max(top);
+      if (__any(top - m > kRescaleSlack / kExponent<D>)) {
+        const float up = fmaxf(m, top);
+        const float old = __builtin_amdgcn_exp2f((m - up) * kExponent<D>);
         m = up;
         l *= old;
 #pragma unroll
@@ -699,7 +707,7 @@ __global__ __launch_bounds__(W * kWave, 2) void paged_attention_kernel(PagedAttn
       float p[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        p[e] = __builtin_amdgcn_exp2f(fmaf(s[e], scale, -m));
+        p[e] = __builtin_amdgcn_exp2f((s[e] - m) * kExponent<D>);
         l += p[e];
         if (F != kBf16) p[e] *= vs[e >> 2][e & 3];
       }
@@ -842,7 +850,7 @@ __global__ __launch_bounds__(W * kWave, 2) void paged_attention_kernel(PagedAttn
       f32x4_t o{0.0f, 0.0f, 0.0f, 0.0f};
       for (uint32_t w = in; w; w &= w - 1) {
         const int at = __builtin_ctz(w) * HB + h;
-        const float f = __builtin_amdgcn_exp2f(ml_at[at * 2] - top);
+        const float f = __builtin_amdgcn_exp2f((ml_at[at * 2] - top) * kExponent<D>);
         sum_l += f * ml_at[at * 2 + 1];
         o += f * *reinterpret_cast<const f32x4_t*>(smem + at * D + d);
       }
@@ -919,13 +927,13 @@ __global__ __launch_bounds__(T) void paged_attention_join_kernel(PagedAttnArgs a
       float next = top;
 #pragma unroll
       for (int b = 0; b < kJoinBatch; ++b) next = fmaxf(next, ml[b][0]);
-      const float old = __builtin_amdgcn_exp2f(top - next);
+      const float old = __builtin_amdgcn_exp2f((top - next) * kExponent<D>);
       top = next;
       sum_l *= old;
       o *= old;
 #pragma unroll
       for (int b = 0; b < kJoinBatch; ++b) {
-        const float w = __builtin_amdgcn_exp2f(ml[b][0] - next);
+        const float w = __builtin_amdgcn_exp2f((ml[b][0] - next) * kExponent<D>);
         sum_l += w * ml[b][1];
         o += w * x[b];
       }
@@ -947,13 +955,14 @@ __global__ __launch_bounds__(T) void paged_attention_join_kernel(PagedAttnArgs a
           ml[b] = part_ml[at];
           next = fmaxf(next, ml[b].x);
         }
-        const float old = __builtin_amdgcn_exp2f(top - next);
+        const float old = __builtin_amdgcn_exp2f((top - next) * kExponent<D>);
         top = next;
         sum_l *= old;
         o *= old;
 #pragma unroll
         for (int b = 0; b < kJoinBatch; ++b) {
-          const float w = i + b < rows ? __builtin_amdgcn_exp2f(ml[b].x - next) : 0.0f;
+          const float w =
+              i + b < rows ? __builtin_amdgcn_exp2f((ml[b].x - next) * kExponent<D>) : 0.0f;
           sum_l += w * ml[b].y;
           o += w * x[b];
         }
