@@ -117,11 +117,13 @@ int infer_hip_kv_pages_load(const infer_hip_kv_pages* pages, const infer_hip_kv_
  * between sequences (a multiple of 8), already rotated; output is contiguous;
  * both 16-byte aligned.  FP32 softmax statistics and sums; the sum of weights
  * (up to 2^6 each) times values is divided at the end, so values near FP32's
- * largest overflow.  A length of zero or less (an empty slot of the batch)
- * gives zeros; a length past the table's pages ends there.  Scores that are
- * all -infinity give NaN, as the quotient does.  A sequence whose pages within
- * its length are not all in the pool gives NaN.  Rows behind a sequence's
- * length never count, whatever they hold.
+ * largest overflow.  An infinite value of BF16 pages gives that infinity, or
+ * NaN where the other one meets it or its weight is 0 in FP32.  A length of
+ * zero or less (an empty slot of the batch) gives zeros; a length past the
+ * table's pages ends there.  Scores that are all -infinity give NaN, as the
+ * quotient does.  A sequence whose pages within its length are not all in the
+ * pool gives NaN.  Rows behind a sequence's length never count, whatever they
+ * hold.
  *
  * The work of all sequences is cut into equal parts over the chip on the
  * device, from the lengths, and the parts of a head joined in a fixed order:

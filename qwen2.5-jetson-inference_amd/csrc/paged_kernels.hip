@@ -257,9 +257,11 @@ __global__ __launch_bounds__(kThreads) void kv_load_kernel(KvLoadArgs a) {
 // eight keys' dimensions r D / 16 .. and pair them up in registers.  Keys and
 // values go from memory to registers once, the next tile's while this one is
 // multiplied.  8-bit elements become BF16 exactly; their scales go onto the
-// scores and the weights.  A weight is the sum of two BF16 numbers (2^-17 of it
-// is lost): one alone rounds as coarsely as the output and made the error
-// 1.35 times the output rounding's own; maxima, sums and O are FP32.  The maximum m
+// scores and the weights.  A weight is the sum of three BF16 numbers of eight bits
+// each, exactly, none of them negative, so that an infinite value gives that infinity
+// (rounded to one, the error was 1.35 times the output rounding's own; to two, a
+// remainder of 0 or below made NaN of infinities; the third costs 0-4 %).  Maxima,
+// sums and O are FP32.  The maximum m
 // is a sum q.k itself and comes off before the factor: the difference of two close
 // scores is exact, so the largest one's weight is 1 however large it is.  (Taken off
 // as a rounded product, an exponent keeps half of the product's last bit, 2^7 from
@@ -405,6 +407,29 @@ __device__ __forceinline__ void turn_values(const Words<N> (&v)[8], bf16x8_t (&f
   }
 }
 
+// The top eight bits of eight numbers of one sign, as BF16, and the rest left of them:
+// taken three times, all 24.
+__device__ __forceinline__ bf16x8_t take_top8(float (&p)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    w[i] = high_halves(__float_as_uint(p[2 * i]), __float_as_uint(p[2 * i + 1]));
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) p[i] -= __uint_as_float(__float_as_uint(p[i]) & 0xFFFF0000u);
+  return __builtin_bit_cast(bf16x8_t, make_uint4(w[0], w[1], w[2], w[3]));
+}
+
+// A lower part that is 0 as 2^-126: an infinite value times every part of a weight is
+// that infinity then, where 0 would make it NaN.  8-bit pages hold no infinities.
+template <int F>
+__device__ __forceinline__ bf16x8_t part_above_zero(bf16x8_t p) {
+  typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
+  if (F != kBf16) return p;
+  const u16x8 least = 0x0080, bits = __builtin_bit_cast(u16x8, p);
+  return __builtin_bit_cast(bf16x8_t, __builtin_elementwise_max(bits, least));
+}
+
 // Over the four lanes r, 16 + r, 32 + r, 48 + r.
 __device__ __forceinline__ float groups_max(float v) {
   int w = __float_as_int(v);
@@ -434,9 +459,15 @@ __device__ __forceinline__ int piece_of(int total, int waves) {
   return max(1, (total + waves - 1) / waves);
 }
 
+// What O is divided by, inverted: without any weight NaN (the 2^-126s of
+// part_above_zero leave O a little off 0).
+__device__ __forceinline__ float inverse(float sum) {
+  return sum == 0.0f ? __uint_as_float(0x7FC00000u) : 1.0f / sum;
+}
+
 // Four dimensions of the output from O and the sum of the weights.
 __device__ __forceinline__ void store_out(uint16_t* out, f32x4_t o, float sum) {
-  const float inv = 1.0f / sum;
+  const float inv = inverse(sum);
   store_global8(out, make_uint2(pack2_bf16(o[0] * inv, o[1] * inv),
                                 pack2_bf16(o[2] * inv, o[3] * inv)));
 }
@@ -721,18 +752,18 @@ __global__ __launch_bounds__(W * kWave, 2) void paged_attention_kernel(PagedAttn
           }
         }
       }
-      const uint4 hi = pack8(p);
-      float rest[8];
-      unpack8(hi, rest);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) rest[e] = p[e] - rest[e];
-      const bf16x8_t p_hi = __builtin_bit_cast(bf16x8_t, hi);
-      const bf16x8_t p_lo = __builtin_bit_cast(bf16x8_t, pack8(rest));
+      const bf16x8_t p_hi = take_top8(p);
+      const bf16x8_t p_mid = part_above_zero<F>(take_top8(p));
+      const bf16x8_t p_lo = part_above_zero<F>(take_top8(p));
       bf16x8_t vf[NO];
       turn_values<F, D, VB>(v, vf);
 #pragma unroll
       for (int j = 0; j < NO; ++j) {
         acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[j], p_hi, acc[j], 0, 0, 0);
+      }
+#pragma unroll
+      for (int j = 0; j < NO; ++j) {
+        acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf[j], p_mid, acc[j], 0, 0, 0);
       }
 #pragma unroll
       for (int j = 0; j < NO; ++j) {
@@ -745,7 +776,7 @@ __global__ __launch_bounds__(W * kWave, 2) void paged_attention_kernel(PagedAttn
         const int h = t.block * kHeadBlock + r;
         if (begin == 0 && t.tile + 1 == t.tiles) {
           if (h < heads_per_kv) {
-            const float inv = 1.0f / sum_l;
+            const float inv = inverse(sum_l);
             const int head = t.kvh * heads_per_kv + h;
             uint16_t* out =
                 a.out + (static_cast<size_t>(t.seq) * a.heads + head) * D + 4 * g * NO;
@@ -873,8 +904,8 @@ __global__ __launch_bounds__(W * kWave, 2) void paged_attention_kernel(PagedAttn
 template <int D, int T>
 __global__ __launch_bounds__(T) void paged_attention_join_kernel(PagedAttnArgs a) {
   constexpr int kJoinBatch = T == 512 ? 8 : 4;  // parts that a thread has in flight
-  __shared__ f32x4_t part_o[T];
-  __shared__ float2 part_ml[T];
+  __shared__ f32x4_t part_o[T + 1];  // the last: no part
+  __shared__ float2 part_ml[T + 1];
   const int lane = threadIdx.x & 63;
   const int seq = blockIdx.y;
   const int cap = a.table.max_pages << a.pool.page_shift;
@@ -943,6 +974,10 @@ __global__ __launch_bounds__(T) void paged_attention_join_kernel(PagedAttnArgs a
         part_o[row * items + e] = o;
         part_ml[row * items + e] = make_float2(top, sum_l);
       }
+      if (threadIdx.x == 0) {
+        part_o[T] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        part_ml[T] = make_float2(-FLT_MAX, 0.0f);
+      }
       __syncthreads();
       for (int i = 1; i < rows && row == 0; i += kJoinBatch) {
         f32x4_t x[kJoinBatch];
@@ -950,7 +985,7 @@ __global__ __launch_bounds__(T) void paged_attention_join_kernel(PagedAttnArgs a
         float next = top;
 #pragma unroll
         for (int b = 0; b < kJoinBatch; ++b) {
-          const int at = min(i + b, rows - 1) * items + e;
+          const int at = i + b < rows ? (i + b) * items + e : T;
           x[b] = part_o[at];
           ml[b] = part_ml[at];
           next = fmaxf(next, ml[b].x);
@@ -961,8 +996,7 @@ __global__ __launch_bounds__(T) void paged_attention_join_kernel(PagedAttnArgs a
         o *= old;
 #pragma unroll
         for (int b = 0; b < kJoinBatch; ++b) {
-          const float w =
-              i + b < rows ? __builtin_amdgcn_exp2f((ml[b].x - next) * kExponent<D>) : 0.0f;
+          const float w = __builtin_amdgcn_exp2f((ml[b].x - next) * kExponent<D>);
           sum_l += w * ml[b].y;
           o += w * x[b];
         }
