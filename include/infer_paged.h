@@ -90,7 +90,8 @@ typedef struct infer_hip_kv_table {
  * rope_positions, writes nothing.  One whose sequence is not in the table,
  * whose position is past the table's pages or whose page is not in the pool
  * stores nothing (its query is still rotated).  Two tokens of a call must not
- * share a slot: that slot then holds an unspecified row. */
+ * share a slot: that slot then holds an unspecified row.  A call takes at most
+ * 2^36 - 4096 elements: tokens x (num_heads + 2 num_kv_heads) x head_dim. */
 int infer_hip_kv_pages_store(const infer_hip_kv_pages* pages, const infer_hip_kv_table* table,
                              const int* sequences, const int* positions, int tokens,
                              const uint16_t* query, long long query_stride, int num_heads,
@@ -104,7 +105,8 @@ int infer_hip_kv_pages_store(const infer_hip_kv_pages* pages, const infer_hip_kv
  * [num_sequences][num_kv_heads][capacity][head_dim] — per sequence the layout
  * of infer_hip_attention_prefill_bf16.  Rows at or past a sequence's length
  * keep what they hold.  Lengths past the table's pages end there; rows on a
- * page that is not in the pool read as NaN. */
+ * page that is not in the pool read as NaN.  The smaller of capacity and the
+ * table's positions times head_dim is at most 2^35 - 2048. */
 int infer_hip_kv_pages_load(const infer_hip_kv_pages* pages, const infer_hip_kv_table* table,
                             const int* lengths, uint16_t* key_cache, uint16_t* value_cache,
                             int capacity, hipStream_t stream);

@@ -1030,8 +1030,21 @@ static void by_format(const KvPool& p, Fn&& f) {
   }
 }
 
+static long long store_rows(const KvStoreArgs& a) {
+  return a.tokens * (a.heads + 2ll * a.pool.kv_heads);
+}
+
+// Threads of a grid's x, whole workgroups of them, are under 2^32.
+static bool countable(long long rows, int lanes) {
+  return rows <= ((1ll << 32) - kThreads) / lanes;
+}
+
+bool kv_store_supported(const KvStoreArgs& a) {
+  return countable(store_rows(a), a.pool.head_dim / 16);
+}
+
 void launch_kv_store(const KvStoreArgs& a, hipStream_t stream) {
-  const long long items = static_cast<long long>(a.tokens) * (a.heads + 2 * a.pool.kv_heads);
+  const long long items = store_rows(a);
   by_format(a.pool, [&](auto f, auto d) {
     constexpr int per = kThreads / (decltype(d)::value / 16);
     const unsigned blocks = static_cast<unsigned>((items + per - 1) / per);
@@ -1044,6 +1057,16 @@ void launch_kv_store(const KvStoreArgs& a, hipStream_t stream) {
 // again, next to what else a model's layers read.
 constexpr long long kStreamBytes = 96ll << 20;
 
+// Positions of a sequence that a load's grid covers.
+static long long load_rows(const KvLoadArgs& a) {
+  const long long most = static_cast<long long>(a.table.max_pages) << a.pool.page_shift;
+  return a.capacity < most ? a.capacity : most;
+}
+
+bool kv_load_supported(const KvLoadArgs& a) {
+  return countable(load_rows(a), a.pool.head_dim / 8);
+}
+
 // A load into caches of more than kStreamBytes does not leave them there: 12 x
 // 9000 rows of 4 x 128 INT8 36 -> 25.5 us, 64 x 1000 of 8 x 64 FP8 32 -> 18.  A
 // kernel that reads all of it next, and does nothing else, is slower by as much
@@ -1051,8 +1074,7 @@ constexpr long long kStreamBytes = 96ll << 20;
 // smaller load's reader finds it in the cache (8 x 8000 of 2 x 64: 18.9 us for both,
 // 20.8 without).
 void launch_kv_load(const KvLoadArgs& a, hipStream_t stream) {
-  const long long most = static_cast<long long>(a.table.max_pages) << a.pool.page_shift;
-  const long long rows = a.capacity < most ? a.capacity : most;
+  const long long rows = load_rows(a);
   by_format(a.pool, [&](auto f, auto d) {
     constexpr int per = kThreads / (decltype(d)::value / 8);
     const dim3 grid(static_cast<unsigned>((rows + per - 1) / per), a.pool.kv_heads,

@@ -71,6 +71,9 @@ struct PagedAttnArgs {
   int piece_waves;  // of a workgroup that the join's parts come from
 };
 
+// Whether the launch's threads can be counted in 32 bits.
+bool kv_store_supported(const KvStoreArgs& a);
+bool kv_load_supported(const KvLoadArgs& a);
 void launch_kv_store(const KvStoreArgs& a, hipStream_t stream);
 void launch_kv_load(const KvLoadArgs& a, hipStream_t stream);
 // Whether the tiles of the largest possible lengths can be counted in 32 bits.

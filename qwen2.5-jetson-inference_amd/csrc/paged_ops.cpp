@@ -2,7 +2,6 @@
 // the launches of paged_kernels.hip.
 #include <hip/hip_runtime.h>
 
-#include <climits>
 #include <cstdint>
 
 #include "infer_paged.h"
@@ -120,10 +119,6 @@ extern "C" int infer_hip_kv_pages_store(
                 "%s: rope needs a position (%d given) and 16-byte alignment", what,
                 rope_positions);
   }
-  if ((num_heads + 2ll * a.pool.kv_heads) * tokens > INT_MAX) {
-    return fail(INFER_HIP_INVALID_ARGUMENT, "%s: %d tokens are too many for one call", what,
-                tokens);
-  }
   a.sequence_ids = sequences;
   a.positions = positions;
   a.tokens = tokens;
@@ -138,6 +133,10 @@ extern "C" int infer_hip_kv_pages_store(
   a.q_out_stride = query_out_stride;
   a.rope = rope;
   a.rope_positions = rope_positions;
+  if (!kv_store_supported(a)) {
+    return fail(INFER_HIP_INVALID_ARGUMENT, "%s: %d tokens are too many for one call", what,
+                tokens);
+  }
   launch_kv_store(a, stream);
   return check_launch(what);
 }
@@ -163,6 +162,10 @@ extern "C" int infer_hip_kv_pages_load(const infer_hip_kv_pages* pages,
   a.key_cache = key_cache;
   a.value_cache = value_cache;
   a.capacity = capacity;
+  if (!kv_load_supported(a)) {
+    return fail(INFER_HIP_INVALID_ARGUMENT,
+                "%s: %d positions of a sequence are too many for one call", what, capacity);
+  }
   launch_kv_load(a, stream);
   return check_launch(what);
 }
