@@ -13,6 +13,7 @@ There is no fallback: if the library is missing, :func:`load` raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -201,6 +202,12 @@ def _ptr(t):
 _raw_stream = _raw_device = None
 
 
+def _current_device():
+    """The current GPU's index; without one, an index that no tensor has."""
+    import torch
+    return torch.cuda.current_device() if torch.cuda.is_available() else -2
+
+
 def _stream(stream):
     global _raw_stream, _raw_device
     if stream is None:
@@ -322,12 +329,56 @@ def pack_w4a16(values, scales, group_size: int):
     return packed, tiled
 
 
+@functools.lru_cache(maxsize=1024)
+def _w4a16_bytes(group_size, tokens, n, k):
+    """Bytes of weight, scales, bias, input and output (0: a shape that the C ABI
+    refuses)."""
+    lib = load()
+    tiled = 2 * lib.infer_hip_w4a16_scale_count(n, k, group_size)
+    if tiled == 0 or tokens < 1:
+        return 0, 0, 0, 0, 0
+    return lib.infer_hip_w4a16_weight_bytes(n, k), tiled, 2 * n, 2 * tokens * k, 2 * tokens * n
+
+
+def _w4a16_ptr(t, types, least, device, name):
+    """Pointer of a contiguous tensor of at least `least` bytes on the current GPU;
+    addresses are taken as they are."""
+    if t is None or type(t) is int:
+        return t
+    if t.nbytes >= least and t.dtype in types and t.get_device() == device and t.is_contiguous():
+        return t.data_ptr()
+    if t.nbytes < least or t.dtype not in types:
+        raise InferError(INVALID_ARGUMENT,
+                         f"gemv_w4a16: {name} of {t.nbytes} bytes of {t.dtype}: {least} bytes of "
+                         f"{' or '.join(str(x) for x in types)} needed")
+    if t.is_cuda and t.get_device() != device:
+        raise InferError(INVALID_ARGUMENT, f"gemv_w4a16: {name} is not on the current GPU")
+    return _ptr(t)
+
+
+_words = _bytes = None  # types of 16-bit words and of bytes
+
+
 def gemv_w4a16(weight, scales, group_size, bias, input, output, tokens, out_features,
                in_features, stream=None):
-    """1 to 16 tokens by packed 4-bit weights (infer_hip_gemv_w4a16)."""
-    _check(load().infer_hip_gemv_w4a16(_ptr(weight), _ptr(scales), group_size, _ptr(bias),
-                                       _ptr(input), _ptr(output), tokens, out_features,
-                                       in_features, _stream(stream)))
+    """1 to 16 tokens by packed 4-bit weights (infer_hip_gemv_w4a16).  weight is uint8
+    and scales BF16 (or words) as pack_w4a16 lays them out, the rest BF16 (or words);
+    buffers may be longer than the shape needs."""
+    global _words, _bytes
+    if _words is None:
+        import torch
+        _bytes = torch.uint8, torch.int8
+        _words = torch.bfloat16, torch.int16, torch.uint16
+    w, s, b, x, y = _w4a16_bytes(group_size, tokens, out_features, in_features)
+    device = _current_device() if _raw_device is None else _raw_device()
+    status = (_lib or load()).infer_hip_gemv_w4a16(
+        _w4a16_ptr(weight, _bytes, w, device, "weight"),
+        _w4a16_ptr(scales, _words, s, device, "scales"), group_size,
+        _w4a16_ptr(bias, _words, b, device, "bias"), _w4a16_ptr(input, _words, x, device, "input"),
+        _w4a16_ptr(output, _words, y, device, "output"), tokens, out_features, in_features,
+        _stream(stream) if stream is not None or _raw_stream is None else _raw_stream(device))
+    if status:
+        _check(status)
 
 
 # MFMA workgroup tiles (rows x columns of Y) of the explicit-tile entries.
