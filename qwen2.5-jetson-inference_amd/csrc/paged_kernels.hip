@@ -1152,9 +1152,11 @@ bool paged_attention_supported(const PagedAttnArgs& a) {
 
 // A call whose tables have room for more keys and values than kStreamBytes reads
 // them past the caches, unless several head blocks read the same keys.  134 MB: 34.5
-// -> 30.6 us, 350 MB: 67 -> 60.6.  Where the lengths fall far short of the tables'
+// -> 30.6 us, 350 MB: 67 -> 60.6; of 256 short sequences, 268 MB of room and half of it
+// live, 32.5 -> 29.3.  Where the lengths fall far short of the tables'
 // room it costs nothing with cold caches (39 MB 13.9 -> 14.0 us, 123 MB 29.4 ->
-// 27.2), and up to a fifth where earlier calls left all of it in the cache.
+// 27.2), and up to a fifth where earlier calls left all of it in the cache (200
+// sequences, 131 MB of room and half of it live: 18.2 -> 19.9).
 void launch_paged_attention(PagedAttnArgs a, hipStream_t stream) {
   const PagedAttnShape s = paged_attention_shape(a.heads, a.pool.kv_heads, a.pool.head_dim);
   a.head_blocks = s.head_blocks;
@@ -1183,18 +1185,15 @@ void launch_paged_attention(PagedAttnArgs a, hipStream_t stream) {
     using Four = std::integral_constant<int, 4>;
     using Eight = std::integral_constant<int, 8>;
     using Sixteen = std::integral_constant<int, 16>;
+    auto by_caches = [&](auto w, auto hb) {
+      streams ? launch(w, hb, std::true_type{}) : launch(w, hb, std::false_type{});
+    };
     if (s.block_heads > 8) {
-      if (streams) {
-        launch(Four{}, Sixteen{}, std::true_type{});
-      } else {
-        launch(Four{}, Sixteen{}, std::false_type{});
-      }
+      by_caches(Four{}, Sixteen{});
     } else if (small) {
-      launch(Four{}, Eight{}, std::false_type{});
-    } else if (streams) {
-      launch(Eight{}, Eight{}, std::true_type{});
+      by_caches(Four{}, Eight{});
     } else {
-      launch(Eight{}, Eight{}, std::false_type{});
+      by_caches(Eight{}, Eight{});
     }
   });
   if (a.whole) return;

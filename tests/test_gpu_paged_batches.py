@@ -93,3 +93,12 @@ def test_captured_large_batch_follows_lengths(paged, dev):
         exact = [ref.attend(q[s].cpu(), pool.rows(0, host[s], n), pool.rows(1, host[s], n))
                  for s, n in enumerate(step)]
         check_attention(out, exact, step, d)
+
+
+@pytest.mark.parametrize("fmt,count", [("bf16", 200), ("int8", 400), ("fp8", 400)])
+def test_short_sequences_past_the_caches(paged, dev, fmt, count):
+    """Tables of 8 tiles with room for more than 96 MiB."""
+    lengths = ragged(count, 256, 6, AROUND_64)
+    _, pages, table, q, out, out64 = attention_case(paged, dev, fmt, 8, 4, 128, 64, lengths, count)
+    run_attention(paged, dev, pages, table, lengths, q, out)
+    check_attention(out, out64, lengths, 128)
