@@ -13,6 +13,7 @@ using namespace qlin;
 namespace {
 
 constexpr int kMaxSequences = 65535;  // a grid dimension
+constexpr int kMaxHeads = 65535;
 constexpr int kMaxPositions = 1 << 30;  // of a sequence
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -32,7 +33,7 @@ int check_pool(const infer_hip_kv_pages* p, KvPool* out, const char* what) {
   if (p->head_dim != 64 && p->head_dim != 128) {
     return fail(INFER_HIP_INVALID_ARGUMENT, "%s: head_dim %d (64 or 128)", what, p->head_dim);
   }
-  if (p->num_pages < 1 || p->num_kv_heads < 1 || p->num_kv_heads > 65535) {
+  if (p->num_pages < 1 || p->num_kv_heads < 1 || p->num_kv_heads > kMaxHeads) {
     return fail(INFER_HIP_INVALID_ARGUMENT, "%s: bad pool (%d pages, %d kv heads)", what,
                 p->num_pages, p->num_kv_heads);
   }
@@ -175,7 +176,7 @@ extern "C" size_t infer_hip_attention_paged_decode_workspace_bytes(int num_seque
                                                                    int num_kv_heads,
                                                                    int head_dim) {
   if (num_sequences < 1 || num_sequences > kMaxSequences || num_kv_heads < 1 ||
-      num_heads < num_kv_heads || num_heads % num_kv_heads != 0 ||
+      num_heads < num_kv_heads || num_heads > kMaxHeads || num_heads % num_kv_heads != 0 ||
       (head_dim != 64 && head_dim != 128)) {
     return 0;
   }
@@ -193,7 +194,7 @@ extern "C" int infer_hip_attention_paged_decode(const infer_hip_kv_pages* pages,
   int rc = check_pool(pages, &a.pool, what);
   if (rc == INFER_HIP_OK) rc = check_table(table, a.pool, &a.table, what);
   if (rc != INFER_HIP_OK) return rc;
-  if (num_heads < 1 || num_heads > 65535 || num_heads % a.pool.kv_heads != 0) {
+  if (num_heads < 1 || num_heads > kMaxHeads || num_heads % a.pool.kv_heads != 0) {
     return fail(INFER_HIP_INVALID_ARGUMENT, "%s: %d query heads on %d kv heads", what, num_heads,
                 a.pool.kv_heads);
   }
