@@ -134,8 +134,10 @@ int infer_hip_gemm_w8a16(const int8_t* weight, const uint16_t* scales,
  * [tokens, out_features] out, which overlaps no input).  weight, scales and
  * input are 16-byte aligned; out_features <= 2^28, in_features <= 2^24.
  * Terms of a group's sum are taken of (q + 24) / 16 and 24 / 16, so its
- * rounding goes by 31 |X|; where a sum overflows it is taken again of q s X,
- * so infinities and NaN come out as that sum's.
+ * rounding goes by 31 |X|: an activation leaves a few times 2^-20 |X| s in
+ * each row, also where its q is 0 (the size of BF16's rounding of the output
+ * once one activation is some 2^13 times the others).  Where a sum overflows it
+ * is taken again of q s X, so infinities and NaN come out as that sum's.
  *
  * The weights are laid out once, in tiles of 16 rows by 128 columns that a
  * wave reads as one contiguous KiB: weight holds
@@ -145,8 +147,10 @@ int infer_hip_gemm_w8a16(const int8_t* weight, const uint16_t* scales,
  * scales are [ceil(N/16)][K / group_size][16], zero past the matrix.
  * infer_hip_w4a16_pack makes both from row-major q [N][K] (one int8 each)
  * and BF16 scales [N][K / group_size], in host memory and without a GPU, into
- * infer_hip_w4a16_weight_bytes bytes and infer_hip_w4a16_scale_count words
- * (both 0 for shapes that are not supported). */
+ * infer_hip_w4a16_weight_bytes bytes and infer_hip_w4a16_scale_count words.
+ * Both are 0 for sizes under 1, the latter also for a group size that is not
+ * supported or does not divide in_features; neither looks at the product's own
+ * limits. */
 size_t infer_hip_w4a16_weight_bytes(int out_features, int in_features);
 size_t infer_hip_w4a16_scale_count(int out_features, int in_features, int group_size);
 int infer_hip_w4a16_pack(const int8_t* values, const uint16_t* scales, int group_size,
