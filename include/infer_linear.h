@@ -136,7 +136,7 @@ int infer_hip_gemm_w8a16(const int8_t* weight, const uint16_t* scales,
  * Terms of a group's sum are taken of (q + 24) / 16 and 24 / 16, so its
  * rounding goes by 31 |X|: an activation leaves a few times 2^-20 |X| s in
  * each row, also where its q is 0 (the size of BF16's rounding of the output
- * once one activation is some 2^13 times the others).  Where a sum overflows it
+ * once one activation is some 2^14 times the others).  Where a sum overflows it
  * is taken again of q s X, so infinities and NaN come out as that sum's.
  *
  * The weights are laid out once, in tiles of 16 rows by 128 columns that a

@@ -66,7 +66,10 @@ typedef struct infer_hip_kv_pages {
 
 /* Block table (device memory): position p of sequence s is slot p % page_size
  * of page pages[s * stride + p / page_size].  max_pages entries of a row may be
- * used; entries behind a sequence's last page are never read. */
+ * used; entries behind a sequence's last page are never read.  max_pages bounds
+ * the lengths, and the launches go by that bound, as they cannot see the
+ * lengths: where a table is wider than any sequence of the batch, pass the
+ * columns that are in use (max_pages smaller than stride). */
 typedef struct infer_hip_kv_table {
   const int* pages;
   int num_sequences; /* at most 65535 */
@@ -116,8 +119,8 @@ int infer_hip_kv_pages_load(const infer_hip_kv_pages* pages, const infer_hip_kv_
  * h / (num_heads / num_kv_heads)
  *   output[s][h] = bf16(softmax(query[s][h] K^T / sqrt(head_dim)) V).
  * query is BF16 [num_sequences][num_heads][head_dim] with query_stride elements
- * between sequences (a multiple of 8), already rotated; output is contiguous;
- * both 16-byte aligned.  FP32 softmax statistics and sums; the sum of weights
+ * between sequences (a multiple of 8), already rotated; output is contiguous
+ * and overlaps nothing; both 16-byte aligned.  FP32 softmax statistics and sums; the sum of weights
  * (up to 2^6 each) times values is divided at the end, so values near FP32's
  * largest overflow.  An infinite value of BF16 pages gives that infinity, or
  * NaN where the other one meets it or its weight is 0 in FP32.  A length of
@@ -132,7 +135,10 @@ int infer_hip_kv_pages_load(const infer_hip_kv_pages* pages, const infer_hip_kv_
  * results do not change from run to run.  lengths must not change while the
  * call runs.  workspace: device memory of
  * infer_hip_attention_paged_decode_workspace_bytes, 16-byte aligned, holding
- * nothing between calls; calls that share one must not overlap. */
+ * nothing between calls; calls that share one must not overlap.  It depends on
+ * the heads alone, and is 0 for shapes that a call refuses.  num_sequences x
+ * the table's positions x the KV heads (each counted once for 16 of its query
+ * heads) are at most 6.8e10. */
 size_t infer_hip_attention_paged_decode_workspace_bytes(int num_sequences, int num_heads,
                                                         int num_kv_heads, int head_dim);
 int infer_hip_attention_paged_decode(const infer_hip_kv_pages* pages,

@@ -180,9 +180,6 @@ __global__ __launch_bounds__(kThreads) void kv_store_kernel(KvStoreArgs a) {
 
 // ------------------------------------------------------------------- load --
 
-// bf16(element * scale), one rounding.  One lane per 8 elements of a row; blockIdx.x
-// over rows, y the KV head, z the sequence; the grid covers the capacity, and rows
-// behind a length end after one load.  Bound: bytes (launch_kv_load has the figures).
 // NT: what is written is not to be kept in the caches.
 template <bool NT>
 __device__ __forceinline__ void store_as(void* p, uint4 v) {
@@ -194,6 +191,9 @@ __device__ __forceinline__ void store_as(void* p, uint4 v) {
   }
 }
 
+// bf16(element * scale), one rounding.  One lane per 8 elements of a row; blockIdx.x
+// over rows, y the KV head, z the sequence; the grid covers the capacity, and rows
+// behind a length end after one load.  Bound: bytes (launch_kv_load has the figures).
 template <int F, int D, bool NT>
 __global__ __launch_bounds__(kThreads) void kv_load_kernel(KvLoadArgs a) {
   constexpr int L = D / 8;
@@ -261,18 +261,17 @@ __global__ __launch_bounds__(kThreads) void kv_load_kernel(KvLoadArgs a) {
 // each, exactly, none of them negative, so that an infinite value gives that infinity
 // (rounded to one, the error was 1.35 times the output rounding's own; to two, a
 // remainder of 0 or below made NaN of infinities; the third costs 0-4 %).  Maxima,
-// sums and O are FP32.  The maximum m
-// is a sum q.k itself and comes off before the factor: the difference of two close
-// scores is exact, so the largest one's weight is 1 however large it is.  (Taken off
-// as a rounded product, an exponent keeps half of the product's last bit, 2^7 from
-// 2^31 up.)
+// sums and O are FP32.  The maximum m is a sum q.k itself and comes off before the
+// factor: the difference of two close scores is exact, so the largest one's weight is 1
+// however large it is.  (Taken off as a rounded product, it leaves half of the product's
+// last bit in the exponent, 2^7 from 2^31 up.)
 //
 // Bound.  Large calls: the cache's bytes, 1 x 131001 keys of 2 x 128 in BF16 (134 MB)
-// 30.4 us, 64 sequences of up to 4000 of 8 x 128 in FP8 (270 MB) 52 us, 5.2 TB/s;
+// 30.5 us, 64 sequences of up to 4000 of 8 x 128 in FP8 (270 MB) 53 us, 5.1 TB/s;
 // a read alone runs at 7.0.  A tile in flight a wave and eight waves a CU are what
 // the registers hold (two tiles in flight, or more waves, gained nothing).  Small
 // calls: the launches and their chains of dependent reads, lengths, table, keys: 1 x
-// 101 keys 4.7 us, 16 x 2000 in INT8 9.4 us, 3.1 of them the second launch.
+// 101 keys 4.8 us, 16 x 2000 in INT8 9.6 us, 3.1 of them the second launch.
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
@@ -1072,7 +1071,8 @@ bool kv_load_supported(const KvLoadArgs& a) {
 // kernel that reads all of it next, and does nothing else, is slower by as much
 // (both together 111 us either way; after a store of the same rows 287 -> 284); a
 // smaller load's reader finds it in the cache (8 x 8000 of 2 x 64: 18.9 us for both,
-// 20.8 without).
+// 20.8 without).  So the gain is the load's own, and that of what runs between; the next
+// reader pays it back.
 void launch_kv_load(const KvLoadArgs& a, hipStream_t stream) {
   const long long rows = load_rows(a);
   by_format(a.pool, [&](auto f, auto d) {
@@ -1093,16 +1093,18 @@ void launch_kv_load(const KvLoadArgs& a, hipStream_t stream) {
 // 128, in workgroups of 8 (of 4 where a unit has more than 8 query heads, whose
 // states fill the LDS).
 constexpr int kCus = 256;
-// Units of more tiles are cut.  The join's launch takes about 3.7 us; a unit left
-// whole is read by one CU, 1.2 us a tile of each wave (one sequence of 14 / 2 / 64
-// heads in BF16: 500 keys 7.4 whole against 9.9 cut, 1000 keys 9.9 against 9.8;
-// 28 / 4 / 128 in INT8: 500 keys 9.2 against 10.3, 1000 keys 12.3 against 10.4).
+// Units of more tiles, by the tables' room, are cut.  The join's launch takes 3.1 to
+// 5.9 us; a unit left whole is read by one CU, 1.2 us a tile of each wave (one sequence
+// of 14 / 2 / 64 heads in BF16: 500 keys 7.4 whole against 9.9 cut, 1000 keys 9.9 against
+// 9.8; 28 / 4 / 128 in INT8: 500 keys 9.2 against 10.3, 1000 keys 12.3 against 10.4).
 // With more than two units a workgroup the pieces' sizes differ by up to a unit,
 // 0.3 us a tile (100 sequences of 500 keys, 28 / 4 / 128 in BF16: 15.7 against
 // 17.6; beyond, only small ones stay whole).
 constexpr int kWholeTiles = 24, kWholeTilesMany = 8;
-// Parts of a unit from which a workgroup of the join has 512 threads (1 x 131001
-// keys, 128 parts: 30.5 us, 31.1 with 256; 16 x 2000 keys, 16 parts: 10.3 and 9.4).
+// Parts of a unit from which a workgroup of the join has 512 threads (8 heads of 64 on
+// one KV head, 131001 keys, 256 parts: 19.1 us, 24.2 with 256; 14 / 2 / 64, 20000 keys,
+// 128 parts: 12.3 and 12.9; 12 / 2 / 128, 131001 keys, 128 parts: 30.5 and 31.1; 28 / 4 /
+// 128, 30000 keys, 128 parts: 19.7 and 19.8; 16 x 2000 keys, 16 parts: 10.3 and 9.4).
 constexpr int kJoinParts = 96;
 // Units up to which the join has a workgroup for each of their query heads (1 x
 // 131001 keys 30.6 us, 46.0 with one a unit; 8 x 20000 keys of 14 / 2 / 64, 16 units,
