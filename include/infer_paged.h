@@ -122,7 +122,8 @@ int infer_hip_kv_pages_load(const infer_hip_kv_pages* pages, const infer_hip_kv_
  * between sequences (a multiple of 8), already rotated; output is contiguous
  * and overlaps nothing; both 16-byte aligned.  FP32 softmax statistics and sums; the sum of weights
  * (up to 2^6 each) times values is divided at the end, so values near FP32's
- * largest overflow.  An infinite value of BF16 pages gives that infinity, or
+ * largest overflow, and values under some 2^-110 lose bits to FP32's smallest
+ * normal number.  An infinite value of BF16 pages gives that infinity, or
  * NaN where the other one meets it or its weight is 0 in FP32.  A length of
  * zero or less (an empty slot of the batch) gives zeros; a length past the
  * table's pages ends there.  Scores that are all -infinity give NaN, as the
