@@ -120,13 +120,13 @@ int infer_hip_kv_pages_load(const infer_hip_kv_pages* pages, const infer_hip_kv_
  *   output[s][h] = bf16(softmax(query[s][h] K^T / sqrt(head_dim)) V).
  * query is BF16 [num_sequences][num_heads][head_dim] with query_stride elements
  * between sequences (a multiple of 8), already rotated; output is contiguous
- * and overlaps nothing; both 16-byte aligned.  FP32 softmax statistics and sums; the sum of weights
- * (up to 2^6 each) times values is divided at the end, so values near FP32's
- * largest overflow, and values under some 2^-110 lose bits to FP32's smallest
- * normal number.  An infinite value of BF16 pages gives that infinity, or
- * NaN where the other one meets it or its weight is 0 in FP32.  A length of
- * zero or less (an empty slot of the batch) gives zeros; a length past the
- * table's pages ends there.  Scores that are all -infinity give NaN, as the
+ * and overlaps nothing; both 16-byte aligned.  FP32 softmax statistics and
+ * sums; the sum of weights (up to 2^6 each) times values is divided at the
+ * end, so values near FP32's largest overflow, and values under some 2^-110
+ * lose bits to its smallest normal number.  An infinite value of BF16 pages
+ * gives that infinity, or NaN where the other one meets it or its weight is 0
+ * in FP32.  A length of zero or less (an empty slot of the batch) gives zeros;
+ * a length past the table's pages ends there.  Scores that are all -infinity give NaN, as the
  * quotient does.  A sequence whose pages within its length are not all in the
  * pool gives NaN.  Rows behind a sequence's length never count, whatever they
  * hold.
@@ -136,10 +136,10 @@ int infer_hip_kv_pages_load(const infer_hip_kv_pages* pages, const infer_hip_kv_
  * results do not change from run to run.  lengths must not change while the
  * call runs.  workspace: device memory of
  * infer_hip_attention_paged_decode_workspace_bytes, 16-byte aligned, holding
- * nothing between calls; calls that share one must not overlap.  It depends on
- * the heads alone, and is 0 for shapes that a call refuses.  num_sequences x
- * the table's positions x the KV heads (each counted once for 16 of its query
- * heads) are at most 6.8e10. */
+ * nothing between calls; calls that share one must not overlap.  Its size goes
+ * by the heads and head_dim alone, and is 0 for shapes that a call refuses.
+ * num_sequences x the table's positions x the KV heads (each counted once for
+ * 16 of its query heads) are at most 6.8e10. */
 size_t infer_hip_attention_paged_decode_workspace_bytes(int num_sequences, int num_heads,
                                                         int num_kv_heads, int head_dim);
 int infer_hip_attention_paged_decode(const infer_hip_kv_pages* pages,
