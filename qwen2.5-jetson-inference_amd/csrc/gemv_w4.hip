@@ -36,7 +36,11 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 // group's accumulator starts from -1.5 sum x (one more MFMA, of the constant,
 // shared by the wave's row tiles) and holds sum q x / 16 in FP32; the group's
 // scale multiplies it into the FP32 total.  Terms are at most 31/16 |x| where
-// q x / 16 reaches 1/2 |x|, which costs two bits of FP32's 24.
+// q x / 16 reaches 1/2 |x|, which costs two bits of FP32's 24, and a large activation
+// leaves its rounding in rows whose q is 0 too.  With q itself (the nibbles as E4M3
+// bytes with a sign, converted to BF16 two at a time: 17 instructions a dword for 8, no
+// starts) neither is so, but 16 x 151936 x 896 takes 23.0 us for 20.4, 1 x 152064 x 3584
+// 65 for 53, 16 x 1536 x 8960 10.7 for 9.7 (1 x 896 x 896 without a bias 3.0 for 3.2).
 //
 // Two forms.  With many rows (w4a16_rows_kernel) a wave takes whole row tiles
 // over all of K, by itself, with the activations and the groups' starts in LDS.
