@@ -12,6 +12,9 @@
  *   infer_hip_kv_pages_load            pages read back as the contiguous BF16
  *                                      cache the other operators use
  *   infer_hip_attention_paged_decode   attention of one new token a sequence
+ *   infer_hip_kv_pages_assign          pages for a step's new tokens, and the
+ *                                      positions that kv_pages_store takes
+ *   infer_hip_kv_pages_release         the pages of sequences that have ended
  *
  * Conventions are infer_linear.h's: caller-owned device memory, BF16 as 16-bit
  * words, work enqueued on `stream` of the current device and never
@@ -147,6 +150,68 @@ int infer_hip_attention_paged_decode(const infer_hip_kv_pages* pages,
                                      const uint16_t* query, long long query_stride,
                                      int num_heads, uint16_t* output, void* workspace,
                                      size_t workspace_bytes, hipStream_t stream);
+
+/* ---- Pages of a step ------------------------------------------------------
+ * The pages that no sequence uses are the first *free_count entries of
+ * free_pages (int [num_pages], device memory), the last of them handed out
+ * first.  Layers whose pools have the same number of pages share one table and
+ * one such list.  Both operators are integers only, have one result whatever
+ * the launch, and read everything on the device when the work runs.
+ *
+ * infer_hip_kv_pages_assign: sequence s holds lengths[s] positions and gets
+ * added[s] more (negative: 0), over a block table [num_sequences][max_pages]
+ * with `stride` entries between rows, at most 65535 sequences and 2^30
+ * positions, page_size as a pool's.  It needs
+ *   need[s] = ceil((lengths[s] + added[s]) / page_size) - ceil(lengths[s] / page_size)
+ * pages; sequences are served in order while the unused pages last:
+ *   ends[s] = need[0] + ... + need[s],
+ *   served[s] = need[s] == 0 or ends[s] <= *free_count,
+ *   its j-th new page = free_pages[*free_count - 1 - (ends[s] - need[s]) - j].
+ * A sequence is also not served, and needs nothing, if lengths[s] + added[s]
+ * is past the table's positions or, where tokens are packed, if its tokens end
+ * past `tokens` (then nor is any later one that gets some; ends counts them).
+ * Written are the table's entries of new pages, lengths_out[s] (lengths[s] +
+ * added[s], or lengths[s] if not served) and *free_count_out.
+ *
+ * Tokens.  With sequences given they are packed, those of sequence 0 first:
+ * token starts[s] + i (starts[s] = added[0] + ... + added[s - 1], served or
+ * not; int [num_sequences + 1], may be NULL, saturating at 2^31 - 1) is
+ * position lengths[s] + i of sequence s: positions[t] and sequences[t].
+ * With sequences NULL token s belongs to sequence s (the decode step's form:
+ * tokens == num_sequences, starts NULL, and a sequence with added[s] > 1 is
+ * not served).  Tokens that are not served, idle or past the last one have
+ * position, sequence and slot -1, which kv_pages_store takes as padding.
+ * slots[t] (may be NULL) is page * page_size + position % page_size, the
+ * token's row of one KV head's pages laid end to end; -1 if the page is not in
+ * [0, num_pages).
+ *
+ * infer_hip_kv_pages_release: the pages of the sequences with finished[s] != 0
+ * go back, in order of sequence and position, onto free_pages: the i-th of
+ * `total` becomes entry *free_count + total - 1 - i, so that an assignment
+ * right after hands them out in that order, and releasing what was just
+ * assigned restores the list.  lengths_out[s] is 0 for them and lengths[s] for
+ * the others, *free_count_out = *free_count + total; the table keeps its
+ * entries, which nothing reads any more.  Entries past num_pages (the list of
+ * a pool whose pages were released twice) are dropped.
+ *
+ * lengths_out may be lengths, and free_count_out free_count; the buffers
+ * overlap in no other way.  A *free_count outside [0, num_pages] is taken as
+ * the nearer of the two, num_pages is at most 2^30.  workspace: device memory
+ * of infer_hip_kv_pages_plan_workspace_bytes(num_sequences) (0: refused
+ * shapes), 16-byte aligned, holding nothing between calls; calls that share
+ * one must not overlap. */
+size_t infer_hip_kv_pages_plan_workspace_bytes(int num_sequences);
+int infer_hip_kv_pages_assign(int* table, int num_sequences, int max_pages, int stride,
+                              int page_size, const int* free_pages, int num_pages,
+                              const int* free_count, int* free_count_out, const int* lengths,
+                              const int* added, int* lengths_out, int tokens, int* positions,
+                              int* sequences, long long* slots, int* starts, void* workspace,
+                              size_t workspace_bytes, hipStream_t stream);
+int infer_hip_kv_pages_release(const int* table, int num_sequences, int max_pages, int stride,
+                               int page_size, int* free_pages, int num_pages,
+                               const int* free_count, int* free_count_out, const int* lengths,
+                               const int* finished, int* lengths_out, void* workspace,
+                               size_t workspace_bytes, hipStream_t stream);
 
 #ifdef __cplusplus
 }

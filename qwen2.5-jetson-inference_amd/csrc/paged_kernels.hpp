@@ -81,4 +81,36 @@ bool paged_attention_supported(const PagedAttnArgs& a);
 void launch_paged_attention(PagedAttnArgs a, hipStream_t stream);
 size_t paged_attention_workspace_bytes(int heads, int kv_heads, int head_dim);
 
+// Pages of a step (page_plan.hip).
+struct PagePlan {
+  int* table;
+  int sequences, max_pages, stride, page_shift;
+  int num_pages;
+  const int* free_count;
+  int* free_count_out;
+  const int* lengths;
+  int* lengths_out;
+};
+
+struct AssignArgs {
+  PagePlan plan;
+  const int* free_pages;
+  const int* added;
+  int tokens;
+  int* positions;
+  int* ids;  // null: token s is sequence s's
+  long long* slots;  // null: not wanted
+  int* starts;       // null: not wanted
+};
+
+struct ReleaseArgs {
+  PagePlan plan;
+  int* free_pages;
+  const int* finished;
+};
+
+size_t page_plan_workspace_bytes(int sequences);
+void launch_pages_assign(const AssignArgs& a, void* workspace, hipStream_t stream);
+void launch_pages_release(const ReleaseArgs& a, void* workspace, hipStream_t stream);
+
 }  // namespace qlin

@@ -1,5 +1,5 @@
 // C ABI of the paged KV cache (include/infer_paged.h): argument checks, then
-// the launches of paged_kernels.hip.
+// the launches of paged_kernels.hip and page_plan.hip.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -221,5 +221,102 @@ extern "C" int infer_hip_attention_paged_decode(const infer_hip_kv_pages* pages,
                 a.table.sequences, a.table.max_pages, 1 << a.pool.page_shift);
   }
   launch_paged_attention(a, stream);
+  return check_launch(what);
+}
+
+namespace {
+
+constexpr int kMaxPoolPages = 1 << 30;
+
+int check_plan(const PagePlan& p, int page_size, const void* workspace, size_t workspace_bytes,
+               PagePlan* out, const char* what) {
+  int shift = 4;
+  while (shift < 8 && (1 << shift) != page_size) ++shift;
+  if ((1 << shift) != page_size) {
+    return fail(INFER_HIP_INVALID_ARGUMENT, "%s: page_size %d (16, 32, 64, 128 or 256)", what,
+                page_size);
+  }
+  if (p.sequences < 1 || p.sequences > kMaxSequences || p.max_pages < 1 ||
+      p.stride < p.max_pages || p.max_pages > (kMaxPositions >> shift)) {
+    return fail(INFER_HIP_INVALID_ARGUMENT,
+                "%s: bad block table (%d sequences of at most %d, %d pages of at most %d "
+                "positions, stride %d)",
+                what, p.sequences, kMaxSequences, p.max_pages, kMaxPositions, p.stride);
+  }
+  if (p.num_pages < 1 || p.num_pages > kMaxPoolPages) {
+    return fail(INFER_HIP_INVALID_ARGUMENT, "%s: %d pages (1 to %d)", what, p.num_pages,
+                kMaxPoolPages);
+  }
+  if (!p.table || !p.free_count || !p.free_count_out || !p.lengths || !p.lengths_out) {
+    return fail(INFER_HIP_INVALID_ARGUMENT, "%s: null pointer", what);
+  }
+  const size_t need = page_plan_workspace_bytes(p.sequences);
+  if (!workspace || !aligned16(workspace) || workspace_bytes < need) {
+    return fail(INFER_HIP_INVALID_ARGUMENT,
+                "%s: workspace of %zu bytes, 16-byte aligned, needed (%zu given)", what, need,
+                workspace_bytes);
+  }
+  *out = p;
+  out->page_shift = shift;
+  return INFER_HIP_OK;
+}
+
+}  // namespace
+
+extern "C" size_t infer_hip_kv_pages_plan_workspace_bytes(int num_sequences) {
+  if (num_sequences < 1 || num_sequences > kMaxSequences) return 0;
+  return page_plan_workspace_bytes(num_sequences);
+}
+
+extern "C" int infer_hip_kv_pages_assign(int* table, int num_sequences, int max_pages, int stride,
+                                         int page_size, const int* free_pages, int num_pages,
+                                         const int* free_count, int* free_count_out,
+                                         const int* lengths, const int* added, int* lengths_out,
+                                         int tokens, int* positions, int* sequences,
+                                         long long* slots, int* starts, void* workspace,
+                                         size_t workspace_bytes, hipStream_t stream) {
+  const char* what = "kv_pages_assign";
+  AssignArgs a{};
+  const PagePlan p{table, num_sequences, max_pages, stride, 0, num_pages, free_count,
+                   free_count_out, lengths, lengths_out};
+  const int rc = check_plan(p, page_size, workspace, workspace_bytes, &a.plan, what);
+  if (rc != INFER_HIP_OK) return rc;
+  if (!free_pages || !added || !positions) {
+    return fail(INFER_HIP_INVALID_ARGUMENT, "%s: null pointer", what);
+  }
+  if (tokens < 1 || (!sequences && (tokens != num_sequences || starts))) {
+    return fail(INFER_HIP_INVALID_ARGUMENT,
+                "%s: %d tokens of %d sequences, sequences%s given, starts%s", what, tokens,
+                num_sequences, sequences ? "" : " not", starts ? "" : " not");
+  }
+  a.free_pages = free_pages;
+  a.added = added;
+  a.tokens = tokens;
+  a.positions = positions;
+  a.ids = sequences;
+  a.slots = slots;
+  a.starts = starts;
+  launch_pages_assign(a, workspace, stream);
+  return check_launch(what);
+}
+
+extern "C" int infer_hip_kv_pages_release(const int* table, int num_sequences, int max_pages,
+                                          int stride, int page_size, int* free_pages,
+                                          int num_pages, const int* free_count,
+                                          int* free_count_out, const int* lengths,
+                                          const int* finished, int* lengths_out, void* workspace,
+                                          size_t workspace_bytes, hipStream_t stream) {
+  const char* what = "kv_pages_release";
+  ReleaseArgs a{};
+  const PagePlan p{const_cast<int*>(table), num_sequences, max_pages, stride, 0, num_pages,
+                   free_count, free_count_out, lengths, lengths_out};
+  const int rc = check_plan(p, page_size, workspace, workspace_bytes, &a.plan, what);
+  if (rc != INFER_HIP_OK) return rc;
+  if (!free_pages || !finished) {
+    return fail(INFER_HIP_INVALID_ARGUMENT, "%s: null pointer", what);
+  }
+  a.free_pages = free_pages;
+  a.finished = finished;
+  launch_pages_release(a, workspace, stream);
   return check_launch(what);
 }

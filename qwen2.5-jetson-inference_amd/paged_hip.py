@@ -22,6 +22,9 @@ EXPORTED_SYMBOLS = (
     "infer_hip_kv_pages_load",
     "infer_hip_attention_paged_decode_workspace_bytes",
     "infer_hip_attention_paged_decode",
+    "infer_hip_kv_pages_plan_workspace_bytes",
+    "infer_hip_kv_pages_assign",
+    "infer_hip_kv_pages_release",
 )
 
 FORMATS = {"bf16": 0, "int8": 1, "fp8": 2}
@@ -44,6 +47,7 @@ class _Table(ctypes.Structure):
 
 _lib = None
 _BF16, _I32, _F32, _U8 = torch.bfloat16, torch.int32, torch.float32, torch.uint8
+_I64 = torch.int64
 
 
 def load():
@@ -59,6 +63,10 @@ def load():
         "infer_hip_kv_pages_load": ([pages, table, p, p, p, i, p], i),
         "infer_hip_attention_paged_decode_workspace_bytes": ([i, i, i, i], z),
         "infer_hip_attention_paged_decode": ([pages, table, p, p, ll, i, p, p, z, p], i),
+        "infer_hip_kv_pages_plan_workspace_bytes": ([i], z),
+        "infer_hip_kv_pages_assign": ([p, i, i, i, i, p, i, p, p, p, p, p, i, p, p, p, p, p, z, p],
+                                      i),
+        "infer_hip_kv_pages_release": ([p, i, i, i, i, p, i, p, p, p, p, p, p, z, p], i),
     }
     for name, (args, res) in sigs.items():
         fn = getattr(lib, name)
@@ -247,3 +255,73 @@ def attention_paged_decode(pages, table, lengths, query, output, workspace, stre
         pages._ref, tab, _at(lengths, _I32, pages, "lengths"), qp, qs, shape[1],
         _at(output, _BF16, pages, "output"), _at(workspace, _U8, pages, "workspace"),
         workspace.numel(), on))
+
+
+def kv_pages_plan_workspace_bytes(num_sequences: int) -> int:
+    return load().infer_hip_kv_pages_plan_workspace_bytes(num_sequences)
+
+
+class _Device:
+    """What the checks above read of a pool, from a tensor."""
+
+    def __init__(self, t):
+        self.device, self.index = t.device, t.get_device()
+
+
+def _flat(t, dtype, count, on, name):
+    if t.numel() != count:
+        _bad(f"{name} must hold {count} (got {t.numel()})")
+    return _at(t, dtype, on, name)
+
+
+def _plan(table, free, free_count, lengths, lengths_out, free_count_out, workspace, stream):
+    """The checks that both operators share: (where, stream, table, pointers)."""
+    on = _Device(table)
+    if on.index < 0:
+        _bad("block table must be on a GPU")
+    handle = _on(on, stream)
+    tab = _table(table, on)
+    n = tab.num_sequences
+    return on, handle, tab, (
+        _at(free, _I32, on, "free"), free.numel(), _flat(free_count, _I32, 1, on, "free_count"),
+        _flat(free_count if free_count_out is None else free_count_out, _I32, 1, on,
+              "free_count_out"),
+        _flat(lengths, _I32, n, on, "lengths"),
+        _flat(lengths if lengths_out is None else lengths_out, _I32, n, on, "lengths_out"),
+        _at(workspace, _U8, on, "workspace"))
+
+
+def kv_pages_assign(table, page_size: int, free, free_count, lengths, added, workspace, positions,
+                    sequences=None, slots=None, starts=None, lengths_out=None,
+                    free_count_out=None, stream=None) -> None:
+    """Pages for added[s] new tokens of every sequence, and the tokens'
+    positions (infer_hip_kv_pages_assign): table int32 [sequences, pages], free
+    int32 [pages of the pool] with free_count int32 [1] of them unused, lengths
+    and added int32 [sequences].  Written: the table's new entries, positions
+    and sequences int32 [tokens], slots int64 [tokens], starts int32
+    [sequences + 1], lengths_out and free_count_out (None: in place).
+    sequences None: token s belongs to sequence s."""
+    on, handle, tab, (fp, pages, fc, fo, ln, lo, ws) = _plan(
+        table, free, free_count, lengths, lengths_out, free_count_out, workspace, stream)
+    n, tokens = tab.num_sequences, positions.numel()
+    ap = _flat(added, _I32, n, on, "added")
+    pp = _at(positions, _I32, on, "positions")
+    ids = None if sequences is None else _flat(sequences, _I32, tokens, on, "sequences")
+    sl = None if slots is None else _flat(slots, _I64, tokens, on, "slots")
+    st = None if starts is None else _flat(starts, _I32, n + 1, on, "starts")
+    _check(load().infer_hip_kv_pages_assign(
+        tab.pages, n, tab.max_pages, tab.stride, page_size, fp, pages, fc, fo, ln, ap, lo, tokens,
+        pp, ids, sl, st, ws, workspace.numel(), handle))
+
+
+def kv_pages_release(table, page_size: int, free, free_count, lengths, finished, workspace,
+                     lengths_out=None, free_count_out=None, stream=None) -> None:
+    """The pages of the sequences with finished[s] != 0 (int32 [sequences]) back
+    onto free (infer_hip_kv_pages_release); the other arguments are
+    kv_pages_assign's."""
+    on, handle, tab, (fp, pages, fc, fo, ln, lo, ws) = _plan(
+        table, free, free_count, lengths, lengths_out, free_count_out, workspace, stream)
+    _check(load().infer_hip_kv_pages_release(
+        tab.pages, tab.num_sequences, tab.max_pages, tab.stride, page_size, fp, pages, fc, fo, ln,
+        _flat(finished, _I32, tab.num_sequences, on, "finished"), lo, ws, workspace.numel(),
+        handle))
