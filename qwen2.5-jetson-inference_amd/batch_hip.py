@@ -1,0 +1,166 @@
+"""Python binding of the operators of a served batch (include/infer_batch.h):
+low-rank adapters of many requests, and each sequence's next token.
+
+Arguments are torch CUDA tensors on the current device.  A nonzero status raises
+:class:`linear_hip.InferError`; shapes, types and devices that the C ABI cannot
+see are checked here.  No reference counterpart: the reference runs one
+sequence of one model (src/qwen2.cpp:597-674,
+Greedy-cy/qwen2.5-jetson-inference).
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+import linear_hip
+from linear_hip import INVALID_ARGUMENT, InferError, _check, _stream
+
+# Every symbol include/infer_batch.h declares.
+EXPORTED_SYMBOLS = (
+    "infer_hip_lora_workspace_bytes",
+    "infer_hip_lora_bf16",
+    "infer_hip_sample_workspace_bytes",
+    "infer_hip_sample_bf16",
+)
+
+MAX_TARGETS = 3
+
+
+class _Target(ctypes.Structure):
+    """infer_hip_lora_target."""
+    _fields_ = [("a", ctypes.c_void_p), ("b", ctypes.c_void_p), ("base", ctypes.c_void_p),
+                ("output", ctypes.c_void_p), ("out_features", ctypes.c_int),
+                ("base_stride", ctypes.c_longlong), ("output_stride", ctypes.c_longlong)]
+
+
+_lib = None
+_BF16, _I32, _F32, _U8 = torch.bfloat16, torch.int32, torch.float32, torch.uint8
+_ARRAYS = [None] + [_Target * n for n in range(1, MAX_TARGETS + 1)]
+
+
+def load():
+    global _lib
+    if _lib is not None:
+        return _lib
+    lib = linear_hip.load()
+    p, i, ll, z = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong, ctypes.c_size_t
+    sigs = {
+        "infer_hip_lora_workspace_bytes": ([i, i, i], z),
+        "infer_hip_lora_bf16": ([p, ll, p, i, i, p, i, i, i, p, p, p, z, p], i),
+        "infer_hip_sample_workspace_bytes": ([i, i], z),
+        "infer_hip_sample_bf16": ([p, ll, i, i, p, p, p, p, p, p, p, p, z, p], i),
+    }
+    for name, (args, res) in sigs.items():
+        fn = getattr(lib, name)
+        fn.argtypes = args
+        fn.restype = res
+    _lib = lib
+    return lib
+
+
+def _bad(text: str):
+    raise InferError(INVALID_ARGUMENT, text)
+
+
+# The checks below run on every call: they read each tensor as few times as they can.
+
+
+def _on(first, name, stream):
+    """The GPU of a call's first tensor, which must be the current one, and the
+    stream."""
+    index = first.get_device()
+    if index < 0:
+        _bad(f"{name} must be on a GPU (it is on {first.device})")
+    # a tensor there exists, so torch's HIP state does
+    if (linear_hip._raw_device or torch.cuda.current_device)() != index:
+        _bad(f"{name} is on {first.device}, the current device is {torch.cuda.current_device()}")
+    if stream is None and linear_hip._raw_stream is not None:
+        return index, linear_hip._raw_stream(index)
+    return index, _stream(stream)
+
+
+def _flat(t, dtype, count, index, name):
+    """Pointer of a contiguous tensor of `count` elements (None: any number)."""
+    if (t.dtype is dtype and t.get_device() == index and t.is_contiguous()
+            and (count is None or t.numel() == count)):
+        return t.data_ptr()
+    _bad(f"{name} must be {'' if count is None else count} contiguous {dtype} on GPU {index} "
+         f"(got {list(t.shape)} {t.dtype} on {t.device})")
+
+
+def _rows(t, rows, columns, index, name):
+    """Pointer and row stride of BF16 [rows, columns] with contiguous rows."""
+    if t.dtype is not _BF16 or t.get_device() != index or t.shape != (rows, columns):
+        _bad(f"{name} must be bfloat16 [{rows}, {columns}] on GPU {index} (got {list(t.shape)} "
+             f"{t.dtype} on {t.device})")
+    stride, inner = t.stride()
+    if inner != 1 and columns > 1:
+        _bad(f"{name}: rows must be contiguous")
+    return t.data_ptr(), stride if rows > 1 else columns
+
+
+def lora_workspace_bytes(tokens: int, max_rank: int, targets: int) -> int:
+    return load().infer_hip_lora_workspace_bytes(tokens, max_rank, targets)
+
+
+def lora(x, ids, targets, workspace, ranks=None, scales=None, stream=None) -> None:
+    """output = base + scales[i] B[i] (A[i] x), with i = ids[t] of each token t
+    (infer_hip_lora_bf16): x [tokens, K], ids int32 [tokens], targets one to three
+    (a [adapters, max_rank, K], b [adapters, N, max_rank], base [tokens, N] or
+    None, output [tokens, N]), ranks int32 and scales float32 [adapters] or
+    None, workspace uint8 of lora_workspace_bytes.  output may be base."""
+    index, on = _on(x, "x", stream)
+    if x.dim() != 2 or not 1 <= len(targets) <= MAX_TARGETS:
+        _bad(f"lora: x [tokens, K] and 1 to {MAX_TARGETS} targets (got {list(x.shape)}, "
+             f"{len(targets)})")
+    tokens, k = x.shape
+    xp, xs = _rows(x, tokens, k, index, "x")
+    shape = targets[0][0].shape
+    if len(shape) != 3 or shape[2] != k:
+        _bad(f"a must be [adapters, max_rank, {k}] (got {list(shape)})")
+    adapters, rank = shape[0], shape[1]
+    made = _ARRAYS[len(targets)]()
+    for target, (a, b, base, output) in zip(made, targets):
+        n = output.shape[-1]
+        if a.shape != shape or b.shape != (adapters, n, rank):
+            _bad(f"a must be {list(shape)} and b {[adapters, n, rank]} (got {list(a.shape)}, "
+                 f"{list(b.shape)})")
+        target.a = _flat(a, _BF16, None, index, "a")
+        target.b = _flat(b, _BF16, None, index, "b")
+        target.output, target.output_stride = _rows(output, tokens, n, index, "output")
+        target.out_features = n
+        if base is not None:
+            target.base, target.base_stride = _rows(base, tokens, n, index, "base")
+    _check(load().infer_hip_lora_bf16(
+        xp, xs, _flat(ids, _I32, tokens, index, "ids"), tokens, k, made, len(targets), adapters,
+        rank, None if ranks is None else _flat(ranks, _I32, adapters, index, "ranks"),
+        None if scales is None else _flat(scales, _F32, adapters, index, "scales"),
+        _flat(workspace, _U8, None, index, "workspace"), workspace.numel(), on))
+
+
+def sample_workspace_bytes(rows: int, vocab: int) -> int:
+    return load().infer_hip_sample_workspace_bytes(rows, vocab)
+
+
+def sample(logits, uniform, tokens, workspace, temperature=None, top_k=None, top_p=None,
+           min_p=None, probabilities=None, stream=None) -> None:
+    """The next token of every row of logits [rows, vocab] (infer_hip_sample_bf16):
+    uniform float32 [rows] in [0, 1), tokens int32 [rows] written; temperature,
+    top_p and min_p float32 and top_k int32 [rows] or None (off), probabilities
+    float32 [rows] written or None, workspace uint8 of
+    sample_workspace_bytes."""
+    index, on = _on(logits, "logits", stream)
+    if logits.dim() != 2:
+        _bad(f"logits must be [rows, vocab] (got {list(logits.shape)})")
+    rows, vocab = logits.shape
+    lp, stride = _rows(logits, rows, vocab, index, "logits")
+
+    def setting(t, dtype, name):
+        return None if t is None else _flat(t, dtype, rows, index, name)
+    _check(load().infer_hip_sample_bf16(
+        lp, stride, rows, vocab, setting(temperature, _F32, "temperature"),
+        setting(top_k, _I32, "top_k"), setting(top_p, _F32, "top_p"),
+        setting(min_p, _F32, "min_p"), _flat(uniform, _F32, rows, index, "uniform"),
+        _flat(tokens, _I32, rows, index, "tokens"), setting(probabilities, _F32, "probabilities"),
+        _flat(workspace, _U8, None, index, "workspace"), workspace.numel(), on))
