@@ -17,7 +17,7 @@ constexpr int kMaxAdapters = 1 << 20;
 constexpr int kMaxFeatures = 1 << 22;
 constexpr int kMaxRank = 128;
 constexpr int kMaxRows = 1 << 20;
-constexpr int kMaxVocab = 1 << 24;
+constexpr int kMaxVocab = 1 << 20;
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 

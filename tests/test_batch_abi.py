@@ -162,7 +162,7 @@ SAMPLE = dict(logits=A, stride=100, rows=3, vocab=100, temperature=A, top_k=A, t
 @pytest.mark.parametrize("change,why", [
     (dict(logits=None), "null"), (dict(logits=A + 1), "aligned"), (dict(stride=99), "stride"),
     (dict(stride=-100), "stride"), (dict(rows=0), "rows"), (dict(rows=(1 << 20) + 1), "rows"),
-    (dict(vocab=0), "tokens"), (dict(vocab=(1 << 24) + 1, stride=1 << 25), "tokens"),
+    (dict(vocab=0), "tokens"), (dict(vocab=(1 << 20) + 1, stride=1 << 25), "tokens"),
     (dict(uniform=None), "null"), (dict(tokens=None), "null"),
     (dict(workspace=None), "workspace"), (dict(workspace=A + 8), "workspace"),
     (dict(workspace_bytes=0), "workspace")])
@@ -173,7 +173,7 @@ def test_sample_refusals(hip, batch, change, why):
 
 def test_sample_workspace(batch):
     size = batch.sample_workspace_bytes
-    assert size(0, 5) == size(5, 0) == size(1 << 21, 5) == size(5, 1 << 25) == 0
+    assert size(0, 5) == size(5, 0) == size(1 << 21, 5) == size(5, 1 << 21) == 0
     assert 0 < size(1, 1) <= size(1, 151936) <= size(64, 151936)
 
 
