@@ -30,8 +30,8 @@ struct LoraArgs {
   const float* scales;  // null: 1
   uint16_t* h;          // [targets][tokens][2][rank_pitch(max_rank)]
   // set by the launch
-  int chunk;     // tokens of a unit's chunk
-  int units;     // of a chunk
+  int* groups;   // of more tokens than a workgroup gathers by itself
+  int units;     // of the call, or of a chunk
   int by_token;  // a unit is a token that is the first with its adapter, not an adapter
 };
 
