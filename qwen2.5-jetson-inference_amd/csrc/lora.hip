@@ -33,19 +33,28 @@ constexpr int kTile = 16;       // tokens, and rows of A
 constexpr int kGather = 256;    // tokens
 constexpr int kChunk = 1024;    // tokens grouped together beyond
 constexpr int kSet = 64;        // tokens of a unit then, at most
-constexpr int kCols = 128;      // of B h a wave
 constexpr int kExpandWaves = 4;
 
 // Words of a token's high (and low) part in the workspace: whole steps of the MFMA's K.
 __host__ __device__ constexpr int rank_pitch(int max_rank) { return (max_rank + 31) / 32 * 32; }
 
-// A unit's tokens; `adapter` -1: none has one.
+// A unit's tokens; `adapter` -1: none has one (and its rank is 0).
 struct Unit {
-  int adapter, count;
+  int adapter, count, rank;
+  float scale;
 };
 
 __device__ __forceinline__ int adapter_of(const LoraArgs& a, int id) {
   return static_cast<unsigned>(id) < static_cast<unsigned>(a.adapters) ? id : -1;
+}
+
+__device__ __forceinline__ Unit unit_of(const LoraArgs& a, int adapter, int count) {
+  Unit u{adapter, count, 0, 1.0f};
+  if (adapter >= 0) {
+    u.rank = a.ranks ? min(max(a.ranks[adapter], 0), a.max_rank) : a.max_rank;
+    if (a.scales) u.scale = a.scales[adapter];
+  }
+  return u;
 }
 
 // Unit `unit`'s tokens in order, by all of the workgroup's waves; count 0: no such unit.
@@ -68,33 +77,33 @@ __device__ __forceinline__ Unit gather_tokens(const LoraArgs& a, int unit, int* 
     }
     count += __popcll(mask);
   }
-  if (a.by_token && first != unit) return {-1, 0};
+  if (a.by_token && first != unit) return unit_of(a, -1, 0);
+  const Unit u = unit_of(a, mine, count);
   __syncthreads();
-  return {mine, count};
+  return u;
 }
 
-// The groups that a launch ahead has made: of each chunk `sets[chunk]` units, each an
-// adapter, the place of its first token in `order`, and the number of them.
+// The groups that a launch ahead has made: units, each an adapter, the place of its first
+// token in `order`, and the number of them (0: none).
 struct Groups {
-  int* sets;    // [chunks]
   int* order;   // [tokens]
   int4* units;  // [chunks][units of a chunk]
 };
 
 __host__ __device__ inline Groups groups_of(const LoraArgs& a) {
-  const int chunks = (a.tokens + kChunk - 1) / kChunk;
-  return {a.groups, a.groups + (chunks + 3) / 4 * 4,
-          reinterpret_cast<int4*>(a.groups + (chunks + 3) / 4 * 4 + (a.tokens + 3) / 4 * 4)};
+  return {a.groups, reinterpret_cast<int4*>(a.groups + (a.tokens + 3) / 4 * 4)};
 }
 
 __device__ __forceinline__ Unit grouped_tokens(const LoraArgs& a, int unit, int* list) {
   const Groups g = groups_of(a);
-  const int chunk = unit / a.units;
-  if (unit % a.units >= g.sets[chunk]) return {-1, 0};
-  const int4 u = g.units[unit];
-  if (static_cast<int>(threadIdx.x) < u.z) list[threadIdx.x] = g.order[u.y + threadIdx.x];
+  const int4 v = g.units[unit];
+  const int t = threadIdx.x;
+  int token = 0;
+  if (t < v.z) token = g.order[v.y + t];
+  const Unit u = unit_of(a, v.x, v.z);
+  if (t < v.z) list[t] = token;
   __syncthreads();
-  return {u.x, u.z};
+  return u;
 }
 
 template <bool GROUPED>
@@ -159,7 +168,9 @@ __global__ __launch_bounds__(kChunk) void lora_group_kernel(LoraArgs a) {
   start[2 * threadIdx.x + 1] = tokens - n1;
   unit[2 * threadIdx.x] = units - u0 - u1;
   unit[2 * threadIdx.x + 1] = units - u1;
-  if (threadIdx.x == 0) out.sets[blockIdx.x] = all;
+  for (int i = all + threadIdx.x; i < a.units; i += kChunk) {
+    out.units[blockIdx.x * a.units + i] = make_int4(-1, 0, 0, 0);
+  }
   __syncthreads();
   if (t < a.tokens) {
     const int at = first + start[place] + nth;
@@ -169,10 +180,6 @@ __global__ __launch_bounds__(kChunk) void lora_group_kernel(LoraArgs a) {
           make_int4(key[place], at, min(kSet, size[place] - nth), 0);
     }
   }
-}
-
-__device__ __forceinline__ int rank_of(const LoraArgs& a, int adapter) {
-  return a.ranks ? min(max(a.ranks[adapter], 0), a.max_rank) : a.max_rank;
 }
 
 __device__ __forceinline__ bf16x8_t as_bf16(const uint4& v) {
@@ -244,11 +251,10 @@ __global__ __launch_bounds__(WAVES * kWave) void lora_shrink_kernel(LoraArgs a) 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int m = lane & 15, g = lane >> 4;
   const Unit u = tokens_of<GROUPED>(a, blockIdx.x, list);
-  if (u.count == 0 || u.adapter < 0) return;
+  if (u.count == 0 || u.rank == 0) return;
   const int blocks = (a.max_rank + RT * kTile - 1) / (RT * kTile);
   const int c = blockIdx.y / blocks, rows = blockIdx.y % blocks * RT * kTile;
-  const int rank = rank_of(a, u.adapter), pitch = rank_pitch(a.max_rank);
-  const float scale = a.scales ? a.scales[u.adapter] : 1.0f;
+  const int rank = u.rank, pitch = rank_pitch(a.max_rank);
   const uint16_t* w[RT];
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
@@ -274,7 +280,7 @@ __global__ __launch_bounds__(WAVES * kWave) void lora_shrink_kernel(LoraArgs a) 
       const int at = tile * kTile + in / 4 % 16;
       if (at < u.count && row < pitch) {
         uint16_t high, low;
-        split_word(row < rank ? h * scale : 0.0f, high, low);
+        split_word(row < rank ? h * u.scale : 0.0f, high, low);
         uint16_t* to =
             a.h + (static_cast<size_t>(c) * a.tokens + list[at]) * 2 * pitch + row;
         to[0] = high;
@@ -284,21 +290,32 @@ __global__ __launch_bounds__(WAVES * kWave) void lora_shrink_kernel(LoraArgs a) 
   }
 }
 
-// KS: steps of 32 of the rank.  A wave takes 128 columns, lane m of each 16 the eight from
-// 8 m on, one of each of eight products, so that a token's 128 outputs are loaded and
-// stored 16 bytes a lane in a row.
-template <int KS>
+// KS: steps of 32 of the rank.  A wave takes 16 J columns, lane m of each 16 the J from
+// J m on, one of each of J products, so that a token's outputs are loaded and stored 2 J
+// bytes a lane in a row.
+template <int J>
+struct Words;
+template <>
+struct Words<8> {
+  typedef u32x4 type;
+};
+template <>
+struct Words<4> {
+  typedef uint32_t type __attribute__((ext_vector_type(2)));
+};
+
+template <int KS, int J, bool ONCE>
 struct Columns {
+  typedef typename Words<J>::type words;
   const LoraTarget& t;
   int n0, rank;
   bool wide;  // whole, and aligned
-  bf16x8_t w[KS][8];
+  bf16x8_t w[KS][J];
 
   __device__ __forceinline__ Columns(const LoraArgs& a, const LoraTarget& target, int block,
-                                     int adapter, int lane)
-      : t(target), n0(block * kCols + 8 * (lane & 15)), rank(0) {
-    if (adapter >= 0) rank = rank_of(a, adapter);
-    wide = n0 + 8 <= t.n && (t.out_stride & 7) == 0 &&
+                                     const Unit& u, int lane)
+      : t(target), n0(block * J * 16 + J * (lane & 15)), rank(u.rank) {
+    wide = n0 + J <= t.n && (t.out_stride & 7) == 0 &&
            (reinterpret_cast<uintptr_t>(t.out) & 15) == 0 &&
            (!t.base ||
             ((t.base_stride & 7) == 0 && (reinterpret_cast<uintptr_t>(t.base) & 15) == 0));
@@ -306,39 +323,42 @@ struct Columns {
     for (int s = 0; s < KS; ++s) {
       const int k = 32 * s + 8 * (lane >> 4);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < J; ++j) {
         uint4 v = make_uint4(0, 0, 0, 0);
         if (k < rank) {
-          const size_t row = static_cast<size_t>(adapter) * t.n + min(n0 + j, t.n - 1);
+          const size_t row = static_cast<size_t>(u.adapter) * t.n + min(n0 + j, t.n - 1);
           v = load_global16(t.b + row * a.max_rank + k);
         }
         w[s][j] = as_bf16(v);
       }
     }
   }
+  // Columns of B from the adapter's rank on as zeros.
   __device__ __forceinline__ void cut(int lane) {
     if (rank % 8 == 0) return;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       const int k = 32 * s + 8 * (lane >> 4);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < J; ++j) {
         w[s][j] = as_bf16(cut_words(__builtin_bit_cast(uint4, w[s][j]), k, rank));
       }
     }
   }
-  __device__ __forceinline__ uint4 base_of(int token) const {
-    return wide && t.base ? load_global16(t.base + token * t.base_stride + n0)
-                          : make_uint4(0, 0, 0, 0);
+  __device__ __forceinline__ words base_of(int token) const {
+    if (!wide || !t.base) return words(0u);
+    const QLIN_GLOBAL words* p =
+        (const QLIN_GLOBAL words*)(t.base + token * t.base_stride + n0);
+    return ONCE ? __builtin_nontemporal_load(p) : *p;
   }
-  __device__ __forceinline__ void multiply(f32x4_t (&sum)[8], const uint4 (&high)[KS],
+  __device__ __forceinline__ void multiply(f32x4_t (&sum)[J], const uint4 (&high)[KS],
                                            const uint4 (&low)[KS]) const {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) sum[j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int j = 0; j < J; ++j) sum[j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
+      for (int j = 0; j < J; ++j) {
         sum[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16(low[s]), w[s][j], sum[j], 0, 0, 0);
         sum[j] =
             __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16(high[s]), w[s][j], sum[j], 0, 0, 0);
@@ -346,21 +366,26 @@ struct Columns {
     }
   }
   // Row i of the sums is the token's.
-  __device__ __forceinline__ void store(int token, const f32x4_t (&sum)[8], int i, uint4 b) const {
+  __device__ __forceinline__ void store(int token, const f32x4_t (&sum)[J], int i, words b) const {
     uint16_t* out = t.out + token * t.out_stride + n0;
     if (wide) {
       if (rank) {
-        b = make_uint4(pack2_bf16(bf16_lo(b.x) + sum[0][i], bf16_hi(b.x) + sum[1][i]),
-                       pack2_bf16(bf16_lo(b.y) + sum[2][i], bf16_hi(b.y) + sum[3][i]),
-                       pack2_bf16(bf16_lo(b.z) + sum[4][i], bf16_hi(b.z) + sum[5][i]),
-                       pack2_bf16(bf16_lo(b.w) + sum[6][i], bf16_hi(b.w) + sum[7][i]));
+#pragma unroll
+        for (int j = 0; j < J; j += 2) {
+          b[j / 2] = pack2_bf16(bf16_lo(b[j / 2]) + sum[j][i], bf16_hi(b[j / 2]) + sum[j + 1][i]);
+        }
       }
-      store_global16(out, b);
+      QLIN_GLOBAL words* p = (QLIN_GLOBAL words*)out;
+      if (ONCE) {
+        __builtin_nontemporal_store(b, p);
+      } else {
+        *p = b;
+      }
       return;
     }
     const uint16_t* base = t.base ? t.base + token * t.base_stride + n0 : nullptr;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < J; ++j) {
       if (n0 + j >= t.n) continue;
       const uint16_t v = base ? base[j] : 0;
       out[j] = rank ? f32_to_bf16(bf16_to_f32(v) + sum[j][i]) : v;
@@ -368,18 +393,18 @@ struct Columns {
   }
 };
 
-// Block `block` of 128 columns over all targets: the target and the block within it;
-// -1 past the last.
-__device__ __forceinline__ int target_of(const LoraArgs& a, int& block) {
+// Block `block` of `columns` over all targets: the target and the block within it; -1 past
+// the last.
+__device__ __forceinline__ int target_of(const LoraArgs& a, int columns, int& block) {
   for (int c = 0; c < a.targets; ++c) {
-    const int blocks = (a.target[c].n + kCols - 1) / kCols;
+    const int blocks = (a.target[c].n + columns - 1) / columns;
     if (block < blocks) return c;
     block -= blocks;
   }
   return -1;
 }
 
-template <int KS, bool GROUPED>
+template <int KS, int J, bool GROUPED, bool ONCE>
 __global__ __launch_bounds__(kExpandWaves * kWave) void lora_expand_kernel(LoraArgs a) {
   __shared__ int list[GROUPED ? kSet : kGather];
   const int lane = threadIdx.x & (kWave - 1);
@@ -388,15 +413,16 @@ __global__ __launch_bounds__(kExpandWaves * kWave) void lora_expand_kernel(LoraA
   const Unit u = tokens_of<GROUPED>(a, blockIdx.x, list);
   if (u.count == 0) return;
   int block = blockIdx.y * kExpandWaves + wave;
-  const int c = target_of(a, block);
+  const int c = target_of(a, J * 16, block);
   if (c < 0) return;
   const LoraTarget& t = a.target[c];
   if (u.adapter < 0 && t.base == t.out) return;
-  Columns<KS> columns(a, t, block, u.adapter, lane);
-  const int rank = columns.rank, pitch = rank_pitch(a.max_rank);
+  Columns<KS, J, ONCE> columns(a, t, block, u, lane);
+  const int rank = u.rank, pitch = rank_pitch(a.max_rank);
   // A tile's h and bases are loaded while the one before it is computed.
   struct Tile {
-    uint4 high[KS], low[KS], base[4];
+    uint4 high[KS], low[KS];
+    typename Words<J>::type base[4];
   };
   auto load = [&](Tile& v, int tile) {
     const int token = list[min(tile * kTile + m, u.count - 1)];
@@ -424,7 +450,7 @@ __global__ __launch_bounds__(kExpandWaves * kWave) void lora_expand_kernel(LoraA
   for (; tile * kTile < u.count; tile += step) {
     now = next;
     if ((tile + step) * kTile < u.count) load(next, tile + step);
-    f32x4_t sum[8];
+    f32x4_t sum[J];
     columns.multiply(sum, now.high, now.low);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -449,39 +475,56 @@ size_t lora_workspace_bytes(int tokens, int max_rank, int targets) {
   size_t bytes = h_bytes(tokens, max_rank, targets);
   if (tokens > kGather) {
     const size_t chunks = chunks_of(tokens);
-    bytes += 4 * ((chunks + 3) / 4 * 4 + (static_cast<size_t>(tokens) + 3) / 4 * 4) +
+    bytes += 4 * ((static_cast<size_t>(tokens) + 3) / 4 * 4) +
              16 * chunks * units_of(tokens, kChunk);
   }
   return bytes;
 }
 
+// Bytes of bases and outputs beyond which they are not left in the caches.
+constexpr long long kStreamBytes = 96ll << 20;
+
+template <bool GROUPED>
+static void launch_expand(const LoraArgs& a, int units, int slots, hipStream_t stream) {
+  const int steps = rank_pitch(a.max_rank) / 32;
+  long long bytes = 0;
+  for (int i = 0; i < a.targets; ++i) bytes += 4ll * a.tokens * a.target[i].n;
+  auto run = [&](auto* kernel, int columns) {
+    int blocks = 0;
+    for (int i = 0; i < a.targets; ++i) blocks += (a.target[i].n + columns - 1) / columns;
+    hipLaunchKernelGGL(kernel, dim3(units, (blocks + kExpandWaves - 1) / kExpandWaves, slots),
+                       dim3(kExpandWaves * kWave), 0, stream, a);
+  };
+  if (GROUPED && bytes > kStreamBytes) {
+    steps == 1   ? run(lora_expand_kernel<1, 8, GROUPED, true>, 128)
+    : steps == 2 ? run(lora_expand_kernel<2, 8, GROUPED, true>, 128)
+    : steps == 3 ? run(lora_expand_kernel<3, 4, GROUPED, true>, 64)
+                 : run(lora_expand_kernel<4, 4, GROUPED, true>, 64);
+  } else {
+    steps == 1   ? run(lora_expand_kernel<1, 8, GROUPED, false>, 128)
+    : steps == 2 ? run(lora_expand_kernel<2, 4, GROUPED, false>, 64)
+    : steps == 3 ? run(lora_expand_kernel<3, 4, GROUPED, false>, 64)
+                 : run(lora_expand_kernel<4, 4, GROUPED, false>, 64);
+  }
+}
+
 void launch_lora(LoraArgs a, hipStream_t stream) {
   const int rank_tiles = (a.max_rank + kTile - 1) / kTile;
-  const int steps = rank_pitch(a.max_rank) / 32;
-  int blocks = 0;
-  for (int i = 0; i < a.targets; ++i) blocks += (a.target[i].n + kCols - 1) / kCols;
-  blocks = (blocks + kExpandWaves - 1) / kExpandWaves;
   if (a.tokens > kGather) {
     a.groups = reinterpret_cast<int*>(reinterpret_cast<char*>(a.h) +
                                       h_bytes(a.tokens, a.max_rank, a.targets));
     a.units = units_of(a.tokens, a.adapters);
     const int chunks = chunks_of(a.tokens), units = chunks * a.units;
     hipLaunchKernelGGL(lora_group_kernel, dim3(chunks), dim3(kChunk), 0, stream, a);
-    auto shrink = [&](auto* kernel, int tiles) {
+    auto shrink = [&](auto* kernel, int tiles, int waves) {
       hipLaunchKernelGGL(kernel, dim3(units, a.targets * ((rank_tiles + tiles - 1) / tiles),
                                       kSet / kTile),
-                         dim3(8 * kWave), 0, stream, a);
+                         dim3(waves * kWave), 0, stream, a);
     };
-    rank_tiles == 1   ? shrink(lora_shrink_kernel<1, 8, true>, 1)
-    : rank_tiles == 2 ? shrink(lora_shrink_kernel<2, 8, true>, 2)
-                      : shrink(lora_shrink_kernel<4, 8, true>, 4);
-    auto expand = [&](auto* kernel) {
-      hipLaunchKernelGGL(kernel, dim3(units, blocks), dim3(kExpandWaves * kWave), 0, stream, a);
-    };
-    steps == 1   ? expand(lora_expand_kernel<1, true>)
-    : steps == 2 ? expand(lora_expand_kernel<2, true>)
-    : steps == 3 ? expand(lora_expand_kernel<3, true>)
-                 : expand(lora_expand_kernel<4, true>);
+    rank_tiles == 1   ? shrink(lora_shrink_kernel<1, 16, true>, 1, 16)
+    : rank_tiles == 2 ? shrink(lora_shrink_kernel<2, 16, true>, 2, 16)
+                      : shrink(lora_shrink_kernel<4, 8, true>, 4, 8);
+    launch_expand<true>(a, units, 1, stream);
     return;
   }
   a.by_token = a.adapters + 1 > a.tokens;
@@ -491,14 +534,7 @@ void launch_lora(LoraArgs a, hipStream_t stream) {
   const int slots = std::min(tiles, 1 + a.tokens / (kTile * a.units));
   hipLaunchKernelGGL((lora_shrink_kernel<1, 16, false>),
                      dim3(a.units, a.targets * rank_tiles, slots), dim3(16 * kWave), 0, stream, a);
-  auto expand = [&](auto* kernel) {
-    hipLaunchKernelGGL(kernel, dim3(a.units, blocks, slots), dim3(kExpandWaves * kWave), 0, stream,
-                       a);
-  };
-  steps == 1   ? expand(lora_expand_kernel<1, false>)
-  : steps == 2 ? expand(lora_expand_kernel<2, false>)
-  : steps == 3 ? expand(lora_expand_kernel<3, false>)
-               : expand(lora_expand_kernel<4, false>);
+  launch_expand<false>(a, a.units, slots, stream);
 }
 
 }  // namespace qlin
