@@ -64,12 +64,14 @@ __device__ __forceinline__ Unit gather_tokens(const LoraArgs& a, int unit, int* 
 #pragma unroll
   for (int i = 0; i < kGather / kWave; ++i) {
     const int t = i * kWave + lane;
-    id[i] = t < a.tokens ? adapter_of(a, a.ids[t]) : -2;
+    id[i] = -2;
+    if (i * kWave < a.tokens && t < a.tokens) id[i] = adapter_of(a, a.ids[t]);
   }
   const int mine = a.by_token ? adapter_of(a, a.ids[unit]) : unit - 1;
   int count = 0, first = -1;
 #pragma unroll
   for (int i = 0; i < kGather / kWave; ++i) {
+    if (i * kWave >= a.tokens) break;
     const unsigned long long mask = __ballot(id[i] == mine);
     if (first < 0 && mask) first = i * kWave + __builtin_ctzll(mask);
     if (id[i] == mine && wave == 0) {
@@ -460,6 +462,85 @@ __global__ __launch_bounds__(kExpandWaves * kWave) void lora_expand_kernel(LoraA
   }
 }
 
+// Both products in one launch, for calls so small that it is launches and round trips
+// they wait for: a workgroup takes 16 waves' columns of a unit's target and computes
+// the unit's h for itself, in LDS.  A is read once for each such workgroup, from L2 as
+// a rule.
+constexpr int kFusedWaves = 16;
+
+template <int RT, int J>
+__global__ __launch_bounds__(kFusedWaves * kWave) void lora_fused_kernel(LoraArgs a) {
+  constexpr int KS = (RT + 1) / 2, kPitch = RT * kTile + 8;  // words of a row of h
+  __shared__ int list[kGather];
+  __shared__ f32x4_t part[kFusedWaves][RT][kWave];
+  __shared__ __align__(16) uint16_t h[2][kTile][kPitch];
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int m = lane & 15, g = lane >> 4;
+  const Unit u = gather_tokens(a, blockIdx.x, list);
+  if (u.count == 0) return;
+  int block = blockIdx.y;
+  const int c = target_of(a, kFusedWaves * J * 16, block);
+  const LoraTarget& t = a.target[c];
+  if (u.adapter < 0 && t.base == t.out) return;
+  block = block * kFusedWaves + wave;
+  const bool has = block * J * 16 < t.n;
+  Columns<KS, J, false> columns(a, t, has ? block : 0, u, lane);
+  const uint16_t* w[RT];
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    w[r] = t.a + (static_cast<size_t>(max(u.adapter, 0)) * a.max_rank +
+                  min(r * kTile + m, a.max_rank - 1)) * a.k;
+  }
+  columns.cut(lane);
+  for (int tile = blockIdx.z; tile * kTile < u.count; tile += gridDim.z) {
+    typename Words<J>::type base[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      base[i] = columns.base_of(list[min(tile * kTile + 4 * g + i, u.count - 1)]);
+    }
+    uint4 high[KS], low[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) high[s] = low[s] = make_uint4(0, 0, 0, 0);
+    if (u.rank) {
+      f32x4_t sum[RT];
+      const int token = list[min(tile * kTile + m, u.count - 1)];
+      shrink_steps<RT>(sum, a, w, a.x + token * a.x_stride, wave, kFusedWaves, g);
+#pragma unroll
+      for (int r = 0; r < RT; ++r) part[wave][r][lane] = sum[r];
+      __syncthreads();
+      for (int e = threadIdx.x; e < RT * kTile * kTile; e += kFusedWaves * kWave) {
+        const float* p = reinterpret_cast<const float*>(part) + e;
+        float v = p[0];
+#pragma unroll
+        for (int i = 1; i < kFusedWaves; ++i) v += p[i * RT * kWave * 4];
+        const int in = e % (kTile * kTile);
+        const int row = e / (kTile * kTile) * kTile + in / 64 * 4 + in % 4;
+        uint16_t* to = &h[0][in / 4 % 16][row];
+        split_word(row < u.rank ? v * u.scale : 0.0f, to[0], to[kTile * kPitch]);
+      }
+      __syncthreads();
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const int k = 32 * s + 8 * g;
+        if (k < RT * kTile) {
+          high[s] = *reinterpret_cast<const uint4*>(&h[0][m][k]);
+          low[s] = *reinterpret_cast<const uint4*>(&h[1][m][k]);
+        }
+      }
+    }
+    f32x4_t sum[J];
+    columns.multiply(sum, high, low);
+    if (has) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int at = tile * kTile + 4 * g + i;
+        if (at < u.count) columns.store(list[at], sum, i, base[i]);
+      }
+    }
+  }
+}
+
 int chunks_of(int tokens) { return (tokens + kChunk - 1) / kChunk; }
 int units_of(int tokens, int adapters) {  // of a chunk
   return (kChunk + kSet - 1) / kSet + std::min(std::min(tokens, kChunk), adapters + 1);
@@ -508,6 +589,25 @@ static void launch_expand(const LoraArgs& a, int units, int slots, hipStream_t s
   }
 }
 
+// A's bytes that the one launch may read, over all its workgroups.
+constexpr long long kFusedBytes = 24ll << 20;
+
+static bool launch_fused(const LoraArgs& a, int slots, hipStream_t stream) {
+  constexpr int kColumns = kFusedWaves * 64;
+  int blocks = 0;
+  for (int i = 0; i < a.targets; ++i) blocks += (a.target[i].n + kColumns - 1) / kColumns;
+  const long long units = std::min(a.units, a.tokens);
+  if (a.max_rank > 64 || 2ll * units * blocks * a.max_rank * a.k > kFusedBytes) return false;
+  auto run = [&](auto* kernel) {
+    hipLaunchKernelGGL(kernel, dim3(a.units, blocks, slots), dim3(kFusedWaves * kWave), 0, stream,
+                       a);
+  };
+  a.max_rank <= 16   ? run(lora_fused_kernel<1, 4>)
+  : a.max_rank <= 32 ? run(lora_fused_kernel<2, 4>)
+                     : run(lora_fused_kernel<4, 4>);
+  return true;
+}
+
 void launch_lora(LoraArgs a, hipStream_t stream) {
   const int rank_tiles = (a.max_rank + kTile - 1) / kTile;
   if (a.tokens > kGather) {
@@ -532,6 +632,7 @@ void launch_lora(LoraArgs a, hipStream_t stream) {
   // workgroups side by side for a unit's tiles, as many as it has if units are alike
   const int tiles = (a.tokens + kTile - 1) / kTile;
   const int slots = std::min(tiles, 1 + a.tokens / (kTile * a.units));
+  if (launch_fused(a, slots, stream)) return;
   hipLaunchKernelGGL((lora_shrink_kernel<1, 16, false>),
                      dim3(a.units, a.targets * rank_tiles, slots), dim3(16 * kWave), 0, stream, a);
   launch_expand<false>(a, a.units, slots, stream);
