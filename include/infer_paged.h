@@ -196,10 +196,10 @@ int infer_hip_attention_paged_decode(const infer_hip_kv_pages* pages,
  *
  * lengths_out may be lengths, and free_count_out free_count; the buffers
  * overlap in no other way.  A *free_count outside [0, num_pages] is taken as
- * the nearer of the two, num_pages is at most 2^30.  workspace: device memory
- * of infer_hip_kv_pages_plan_workspace_bytes(num_sequences) (0: refused
- * shapes), 16-byte aligned, holding nothing between calls; calls that share
- * one must not overlap. */
+ * the nearer of the two, num_pages and tokens are at most 2^30.  workspace:
+ * device memory of infer_hip_kv_pages_plan_workspace_bytes(num_sequences) (0:
+ * refused shapes), 16-byte aligned, holding nothing between calls; calls that
+ * share one must not overlap. */
 size_t infer_hip_kv_pages_plan_workspace_bytes(int num_sequences);
 int infer_hip_kv_pages_assign(int* table, int num_sequences, int max_pages, int stride,
                               int page_size, const int* free_pages, int num_pages,

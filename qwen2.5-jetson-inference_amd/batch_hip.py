@@ -14,7 +14,7 @@ import ctypes
 import torch
 
 import linear_hip
-from linear_hip import INVALID_ARGUMENT, InferError, _check, _stream
+from linear_hip import INVALID_ARGUMENT, InferError, _check, _flat, _here
 
 # Every symbol include/infer_batch.h declares.
 EXPORTED_SYMBOLS = (
@@ -63,35 +63,12 @@ def _bad(text: str):
     raise InferError(INVALID_ARGUMENT, text)
 
 
-# The checks below run on every call: they read each tensor as few times as they can.
-
-
-def _on(first, name, stream):
-    """The GPU of a call's first tensor, which must be the current one, and the
-    stream."""
-    index = first.get_device()
-    if index < 0:
-        _bad(f"{name} must be on a GPU (it is on {first.device})")
-    # a tensor there exists, so torch's HIP state does
-    if (linear_hip._raw_device or torch.cuda.current_device)() != index:
-        _bad(f"{name} is on {first.device}, the current device is {torch.cuda.current_device()}")
-    if stream is None and linear_hip._raw_stream is not None:
-        return index, linear_hip._raw_stream(index)
-    return index, _stream(stream)
-
-
-def _flat(t, dtype, count, index, name):
-    """Pointer of a contiguous tensor of `count` elements (None: any number)."""
-    if (t.dtype is dtype and t.get_device() == index and t.is_contiguous()
-            and (count is None or t.numel() == count)):
-        return t.data_ptr()
-    _bad(f"{name} must be {'' if count is None else count} contiguous {dtype} on GPU {index} "
-         f"(got {list(t.shape)} {t.dtype} on {t.device})")
-
-
 def _rows(t, rows, columns, index, name):
     """Pointer and row stride of BF16 [rows, columns] with contiguous rows."""
-    if t.dtype is not _BF16 or t.get_device() != index or t.shape != (rows, columns):
+    if t.dtype is _BF16 and t.get_device() == index and t.shape == (rows, columns):
+        if t.is_contiguous():
+            return t.data_ptr(), columns
+    else:
         _bad(f"{name} must be bfloat16 [{rows}, {columns}] on GPU {index} (got {list(t.shape)} "
              f"{t.dtype} on {t.device})")
     stride, inner = t.stride()
@@ -110,7 +87,7 @@ def lora(x, ids, targets, workspace, ranks=None, scales=None, stream=None) -> No
     (a [adapters, max_rank, K], b [adapters, N, max_rank], base [tokens, N] or
     None, output [tokens, N]), ranks int32 and scales float32 [adapters] or
     None, workspace uint8 of lora_workspace_bytes.  output may be base."""
-    index, on = _on(x, "x", stream)
+    index, on = _here(x, "x", stream)
     if x.dim() != 2 or not 1 <= len(targets) <= MAX_TARGETS:
         _bad(f"lora: x [tokens, K] and 1 to {MAX_TARGETS} targets (got {list(x.shape)}, "
              f"{len(targets)})")
@@ -150,7 +127,7 @@ def sample(logits, uniform, tokens, workspace, temperature=None, top_k=None, top
     top_p and min_p float32 and top_k int32 [rows] or None (off), probabilities
     float32 [rows] written or None, workspace uint8 of
     sample_workspace_bytes."""
-    index, on = _on(logits, "logits", stream)
+    index, on = _here(logits, "logits", stream)
     if logits.dim() != 2:
         _bad(f"logits must be [rows, vocab] (got {list(logits.shape)})")
     rows, vocab = logits.shape

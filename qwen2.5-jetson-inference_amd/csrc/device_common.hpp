@@ -128,6 +128,36 @@ __device__ __forceinline__ float wave_max(float v) {
   return fmaxf(__int_as_float(r32[0]), __int_as_float(r32[1]));
 }
 
+// v of the lane that a DPP control names, 0 where that is none (and in rows that ROWS
+// leaves out).
+template <int CTRL, int ROWS = 0xF>
+__device__ __forceinline__ unsigned from_lane(unsigned v) {
+  return __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xF, false);
+}
+template <int CTRL, int ROWS = 0xF>
+__device__ __forceinline__ double from_lane(double v) {
+  const unsigned long long w = __builtin_bit_cast(unsigned long long, v);
+  const unsigned lo = from_lane<CTRL, ROWS>(static_cast<unsigned>(w));
+  const unsigned hi = from_lane<CTRL, ROWS>(static_cast<unsigned>(w >> 32));
+  return __builtin_bit_cast(double, static_cast<unsigned long long>(hi) << 32 | lo);
+}
+
+// Inclusive sums over the lanes, by an associative `add` of which 0 is the zero: shifts
+// within rows of 16, then the rows' ends.
+template <class T, class F>
+__device__ __forceinline__ T wave_scan(T v, F add) {
+  v = add(v, from_lane<0x111>(v));  // row_shr 1, 2, 4, 8
+  v = add(v, from_lane<0x112>(v));
+  v = add(v, from_lane<0x114>(v));
+  v = add(v, from_lane<0x118>(v));
+  v = add(v, from_lane<0x142, 0xA>(v));  // row_bcast 15 into rows 1 and 3
+  return add(v, from_lane<0x143, 0xC>(v));  // row_bcast 31 into rows 2 and 3
+}
+template <class T>
+__device__ __forceinline__ T wave_scan(T v) {
+  return wave_scan(v, [](T a, T b) { return a + b; });
+}
+
 // Sum within each row of 16 lanes; every lane of the row receives it.
 __device__ __forceinline__ float row16_sum(float v) {
   v += dpp_from<kDppQuadSwap1>(v);

@@ -17,14 +17,7 @@ __device__ __forceinline__ unsigned add_sat(unsigned a, unsigned b) {
   return min(a + b, 0x7FFFFFFFu);
 }
 
-__device__ __forceinline__ unsigned wave_scan(unsigned v, int lane) {
-#pragma unroll
-  for (int d = 1; d < kWave; d *= 2) {
-    const unsigned o = __shfl_up(v, d);
-    if (lane >= d) v = add_sat(v, o);
-  }
-  return v;
-}
+__device__ __forceinline__ unsigned scan_sat(unsigned v) { return wave_scan(v, add_sat); }
 
 // What a token needs of its sequence: the first free entry of its new pages
 // (the j-th is entry first - j), and the positions it held, -1 if not served.
@@ -69,7 +62,7 @@ __device__ int scan_sequences(const AssignArgs& a, const Share& share, ScanLds& 
         need = ((length + add + round) >> p.page_shift) - ((length + round) >> p.page_shift);
       }
     }
-    const unsigned add_in = wave_scan(add, lane), need_in = wave_scan(need, lane);
+    const unsigned add_in = scan_sat(add), need_in = scan_sat(need);
     if (lane == kWave - 1) {
       lds.add[wave] = add_in;
       lds.need[wave] = need_in;
@@ -113,66 +106,84 @@ __device__ int scan_sequences(const AssignArgs& a, const Share& share, ScanLds& 
   return lds.used;
 }
 
-// Position, sequence and slot of tokens [t, t + 4), and the table's entry where a
-// token is the first of a new page, which every new page has.
-__device__ __forceinline__ void place_tokens(const AssignArgs& a, const Share& share, int t) {
+// Position, sequence and slot of N tokens, `apart` from t on, and the table's entry where a
+// token is the first of a new page, which every new page has.  Step by step for all of
+// them, without branches, so that their reads are on their way together.
+template <int N>
+__device__ __forceinline__ void place_tokens(const AssignArgs& a, const Share& share, int t,
+                                             int apart) {
   const PagePlan& p = a.plan;
-  const int page_mask = (1 << p.page_shift) - 1;
-  // The first sequence from `from` whose tokens end past `token`.
-  auto sequence_of = [&](int from, int token) {
-    int hi = p.sequences;
-    while (from < hi) {
-      const int mid = (from + hi) / 2;
-      if (share.starts[mid + 1] > token) {
-        hi = mid;
-      } else {
-        from = mid + 1;
+  const int page_mask = (1 << p.page_shift) - 1, last = p.sequences - 1;
+  int s[N], at[N], held[N], first[N], page[N];
+  bool live[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int token = t + i * apart;
+    live[i] = token < a.tokens;
+    s[i] = live[i] ? token : 0;
+    at[i] = 0;  // of the sequence's new tokens
+  }
+  if (a.ids) {  // the first sequence whose tokens end past each
+    int hi[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      s[i] = 0;
+      hi[i] = p.sequences;
+    }
+    for (int n = p.sequences; n > 0; n >>= 1) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int mid = (s[i] + hi[i]) / 2;
+        const bool past = share.starts[min(mid, last) + 1] > t + i * apart;
+        if (s[i] < hi[i]) {
+          if (past) {
+            hi[i] = mid;
+          } else {
+            s[i] = mid + 1;
+          }
+        }
       }
     }
-    return from;
-  };
-  int s = a.ids ? sequence_of(0, t) : t;
-  int position[4], id[4];
-  long long slot[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    position[i] = id[i] = -1;
-    slot[i] = -1;
-    int at = 0;  // of the sequence's new tokens
-    bool live = t + i < a.tokens;
-    if (a.ids) {
-      if (s < p.sequences && share.starts[s + 1] <= t + i) s = sequence_of(s + 1, t + i);
-      live = live && s < p.sequences;
-      if (live) at = t + i - share.starts[s];
-    } else {
-      s = t + i;
-      live = live && a.added[s] > 0;
+    for (int i = 0; i < N; ++i) {
+      live[i] = live[i] && s[i] <= last;
+      s[i] = min(s[i], last);
+      at[i] = t + i * apart - share.starts[s[i]];
     }
-    if (!live) continue;
-    const int held = share.held[s];
-    if (held < 0) continue;
-    const int pos = held + at, index = pos >> p.page_shift;
-    const int old_pages = (held + page_mask) >> p.page_shift;
-    int* entry = p.table + static_cast<size_t>(s) * p.stride + index;
-    int page;
-    if (index < old_pages) {
-      page = *entry;
-    } else {
-      page = a.free_pages[share.first[s] - (index - old_pages)];
-      if ((pos & page_mask) == 0) *entry = page;
-    }
-    position[i] = pos;
-    id[i] = s;
-    if (static_cast<unsigned>(page) < static_cast<unsigned>(p.num_pages)) {
-      slot[i] = (static_cast<long long>(page) << p.page_shift) + (pos & page_mask);
-    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) live[i] = live[i] && a.added[s[i]] > 0;
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (t + i < a.tokens) {
-      a.positions[t + i] = position[i];
-      if (a.ids) a.ids[t + i] = id[i];
-      if (a.slots) a.slots[t + i] = slot[i];
+  for (int i = 0; i < N; ++i) {
+    held[i] = share.held[s[i]];
+    first[i] = share.first[s[i]];
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    live[i] = live[i] && held[i] >= 0;
+    const int pos = held[i] + at[i], index = pos >> p.page_shift;
+    const int old_pages = (held[i] + page_mask) >> p.page_shift;
+    const int* from = index < old_pages
+                          ? p.table + static_cast<size_t>(s[i]) * p.stride + index
+                          : a.free_pages + (first[i] - (index - old_pages));
+    page[i] = live[i] ? *from : -1;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int token = t + i * apart, pos = held[i] + at[i];
+    if (live[i] && (pos & page_mask) == 0) {  // of no page that was there
+      p.table[static_cast<size_t>(s[i]) * p.stride + (pos >> p.page_shift)] = page[i];
+    }
+    const bool placed = static_cast<unsigned>(page[i]) < static_cast<unsigned>(p.num_pages);
+    if (token < a.tokens) {
+      a.positions[token] = live[i] ? pos : -1;
+      if (a.ids) a.ids[token] = live[i] ? s[i] : -1;
+      if (a.slots) {
+        a.slots[token] = live[i] && placed ? (static_cast<long long>(page[i]) << p.page_shift) +
+                                                 (pos & page_mask)
+                                           : -1;
+      }
     }
   }
 }
@@ -181,16 +192,48 @@ __device__ __forceinline__ Share share_of(int* workspace, int sequences) {
   return {workspace, workspace + sequences + 1, workspace + 2 * sequences + 1};
 }
 
+// Up to kHere sequences and one workgroup's tokens, or where nothing is written in place:
+// every workgroup plans all sequences for itself, in LDS, and the first writes the plan's
+// outputs.  Otherwise a launch of one workgroup writes the plan into the workspace and a
+// second one places the tokens.
+//
+// Bound: a step's launch and its chain of reads: lengths, then free entries or pages.  24
+// sequences XX us (1.7 an empty launch), 25 000 tokens of 8 prompts XX, 620 000 of 2000
+// sequences XX for 10 MB, mostly written.
+constexpr int kHere = 1024, kHereTokens = 1 << 17;
+
+template <int NT>
+__global__ __launch_bounds__(NT) void assign_kernel(AssignArgs a) {
+  __shared__ ScanLds lds;
+  __shared__ int starts[kHere + 1], held[kHere], first[kHere];
+  const Share share{starts, held, first};
+  const int used = scan_sequences(a, share, lds, blockIdx.x == 0);
+  // every thread of the workgroup has read the count by now
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.plan.free_count_out = unused_pages(a.plan) - used;
+  const int t = blockIdx.x * NT + threadIdx.x;
+  if (t < a.tokens) place_tokens<1>(a, share, t, 0);
+}
+
 __global__ __launch_bounds__(kWide) void assign_scan_kernel(AssignArgs a, int* workspace) {
   __shared__ ScanLds lds;
   const int used = scan_sequences(a, share_of(workspace, a.plan.sequences), lds, true);
-  // every thread has read the count by now
   if (threadIdx.x == 0) *a.plan.free_count_out = unused_pages(a.plan) - used;
 }
 
+// The starts are searched in LDS while they fit.
+constexpr int kStarts = 8192, kFillTokens = 1024;
+
+template <bool FITS>
 __global__ __launch_bounds__(256) void assign_fill_kernel(AssignArgs a, int* workspace) {
-  const int t = 4 * (blockIdx.x * blockDim.x + threadIdx.x);
-  if (t < a.tokens) place_tokens(a, share_of(workspace, a.plan.sequences), t);
+  __shared__ int starts[FITS ? kStarts : 1];
+  Share share = share_of(workspace, a.plan.sequences);
+  if (FITS && a.ids) {
+    for (int i = threadIdx.x; i <= a.plan.sequences; i += blockDim.x) starts[i] = share.starts[i];
+    __syncthreads();
+  }
+  if (FITS) share.starts = starts;
+  const int t = blockIdx.x * kFillTokens + threadIdx.x;
+  if (t < a.tokens) place_tokens<kFillTokens / 256>(a, share, t, 256);
 }
 
 }  // namespace
@@ -201,21 +244,98 @@ size_t page_plan_workspace_bytes(int sequences) {
 
 void launch_pages_assign(const AssignArgs& a, void* workspace, hipStream_t stream) {
   int* ws = static_cast<int*>(workspace);
+  const PagePlan& p = a.plan;
+  const int threads = p.sequences <= 256 && a.tokens <= kHereTokens ? 256 : kWide;
+  auto blocks = [&](int each) { return static_cast<unsigned>((a.tokens - 1) / each + 1); };
+  const bool in_place = p.lengths_out == p.lengths || p.free_count_out == p.free_count;
+  if (p.sequences <= kHere && a.tokens <= kHereTokens &&
+      (a.tokens <= threads || !in_place)) {
+    if (threads == 256) {
+      hipLaunchKernelGGL(assign_kernel<256>, dim3(blocks(256)), dim3(256), 0, stream, a);
+    } else {
+      hipLaunchKernelGGL(assign_kernel<kWide>, dim3(blocks(kWide)), dim3(kWide), 0, stream, a);
+    }
+    return;
+  }
   hipLaunchKernelGGL(assign_scan_kernel, dim3(1), dim3(kWide), 0, stream, a, ws);
-  const unsigned blocks = static_cast<unsigned>((a.tokens + 1023ll) / 1024);
-  hipLaunchKernelGGL(assign_fill_kernel, dim3(blocks), dim3(256), 0, stream, a, ws);
+  if (p.sequences < kStarts) {
+    hipLaunchKernelGGL(assign_fill_kernel<true>, dim3(blocks(kFillTokens)), dim3(256), 0, stream, a, ws);
+  } else {
+    hipLaunchKernelGGL(assign_fill_kernel<false>, dim3(blocks(kFillTokens)), dim3(256), 0, stream, a, ws);
+  }
 }
 
 namespace {
 
-// Where the pages of each ended sequence go: share.first[s] is its first page's entry,
-// share.held[s] how many there are.
+// Pages that go back, of sequence s.
+__device__ __forceinline__ unsigned ended_pages(const ReleaseArgs& a, int s, int length) {
+  const PagePlan& p = a.plan;
+  if (a.finished[s] == 0) return 0;
+  const unsigned round = (1u << p.page_shift) - 1;
+  return min((static_cast<unsigned>(max(length, 0)) + round) >> p.page_shift,
+             static_cast<unsigned>(p.max_pages));
+}
+
+// Sequence s's pages to the entries down from `top`.
+__device__ __forceinline__ void give_back(const ReleaseArgs& a, int s, int pages, int top) {
+  const PagePlan& p = a.plan;
+  const int* row = p.table + static_cast<size_t>(s) * p.stride;
+  for (int i = threadIdx.x; i < pages; i += blockDim.x) {
+    const int place = top - i;
+    if (place >= 0 && place < p.num_pages) a.free_pages[place] = row[i];
+  }
+}
+
+// Up to kReleaseHere sequences, nothing in place: a workgroup of each adds up the pages
+// that go back before its own, and all of them.  Otherwise one workgroup writes each
+// sequence's place into the workspace, and a second launch copies.
+//
+// Bound: as above; 750 000 pages of 1350 sequences XX us for 6 MB.
+constexpr int kReleaseHere = 4096;
+
+__global__ __launch_bounds__(256) void release_kernel(ReleaseArgs a) {
+  constexpr int kWaves = 256 / kWave;
+  __shared__ unsigned before_wave[kWaves], all_wave[kWaves];
+  const PagePlan& p = a.plan;
+  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, s = blockIdx.x;
+  const int length = p.lengths[s];
+  const unsigned mine = ended_pages(a, s, length);
+  unsigned before = 0, all = 0;
+  if (mine || s == 0) {
+    for (int i = threadIdx.x; i < p.sequences; i += 256) {
+      const unsigned pages = ended_pages(a, i, p.lengths[i]);
+      all = add_sat(all, pages);
+      if (i < s) before = add_sat(before, pages);
+    }
+    before = scan_sat(before);
+    all = scan_sat(all);
+    if (lane == kWave - 1) {
+      before_wave[wave] = before;
+      all_wave[wave] = all;
+    }
+  }
+  if (threadIdx.x == 0) p.lengths_out[s] = a.finished[s] ? 0 : length;
+  if (!mine && s) return;  // the same in all threads
+  __syncthreads();
+  before = all = 0;
+  for (int i = 0; i < kWaves; ++i) {
+    before = add_sat(before, before_wave[i]);
+    all = add_sat(all, all_wave[i]);
+  }
+  const unsigned end = add_sat(unused_pages(p), all);
+  if (s == 0 && threadIdx.x == 0) {
+    *p.free_count_out = min(end, static_cast<unsigned>(p.num_pages));
+  }
+  give_back(a, s, mine, static_cast<int>(end) - 1 - static_cast<int>(before));
+}
+
+// Where the pages of each ended sequence go: share.first[s] pages lie before its first one,
+// share.held[s] how many there are, share.starts[0] where the places end.
 __global__ __launch_bounds__(kWide) void release_scan_kernel(ReleaseArgs a, int* workspace) {
   __shared__ ScanLds lds;
   const PagePlan& p = a.plan;
   const Share share = share_of(workspace, p.sequences);
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  const unsigned round = (1u << p.page_shift) - 1;
   const int count = unused_pages(p);
   unsigned before = 0;
   for (int base = 0; base < p.sequences; base += kWide) {
@@ -223,14 +343,10 @@ __global__ __launch_bounds__(kWide) void release_scan_kernel(ReleaseArgs a, int*
     unsigned pages = 0;
     if (s < p.sequences) {
       const int length = p.lengths[s];
-      const bool ended = a.finished[s] != 0;
-      if (ended) {
-        pages = min((static_cast<unsigned>(max(length, 0)) + round) >> p.page_shift,
-                    static_cast<unsigned>(p.max_pages));
-      }
-      p.lengths_out[s] = ended ? 0 : length;
+      pages = ended_pages(a, s, length);
+      p.lengths_out[s] = a.finished[s] ? 0 : length;
     }
-    const unsigned in = wave_scan(pages, lane);
+    const unsigned in = scan_sat(pages);
     if (lane == kWave - 1) lds.need[wave] = in;
     __syncthreads();
     unsigned sum = before, mine = 0;
@@ -248,32 +364,30 @@ __global__ __launch_bounds__(kWide) void release_scan_kernel(ReleaseArgs a, int*
     __syncthreads();
   }
   if (threadIdx.x == 0) {
-    share.starts[0] = add_sat(count, before);  // where the last released page's place ends
-    *p.free_count_out = min(add_sat(count, before), static_cast<unsigned>(p.num_pages));
+    const unsigned end = add_sat(count, before);
+    share.starts[0] = end;
+    *p.free_count_out = min(end, static_cast<unsigned>(p.num_pages));
   }
 }
 
 __global__ __launch_bounds__(256) void release_copy_kernel(ReleaseArgs a, int* workspace) {
-  const PagePlan& p = a.plan;
-  const Share share = share_of(workspace, p.sequences);
-  for (int s = blockIdx.x; s < p.sequences; s += gridDim.x) {
-    const int pages = share.held[s];
-    const int top = share.starts[0] - 1 - share.first[s];
-    for (int i = threadIdx.x; i < pages; i += blockDim.x) {
-      const int place = top - i;
-      if (place >= 0 && place < p.num_pages) {
-        a.free_pages[place] = p.table[static_cast<size_t>(s) * p.stride + i];
-      }
-    }
-  }
+  const Share share = share_of(workspace, a.plan.sequences);
+  const int s = blockIdx.x;
+  give_back(a, s, share.held[s], share.starts[0] - 1 - share.first[s]);
 }
 
 }  // namespace
 
 void launch_pages_release(const ReleaseArgs& a, void* workspace, hipStream_t stream) {
   int* ws = static_cast<int*>(workspace);
+  const PagePlan& p = a.plan;
+  const bool in_place = p.lengths_out == p.lengths || p.free_count_out == p.free_count;
+  if (p.sequences <= kReleaseHere && !in_place) {
+    hipLaunchKernelGGL(release_kernel, dim3(p.sequences), dim3(256), 0, stream, a);
+    return;
+  }
   hipLaunchKernelGGL(release_scan_kernel, dim3(1), dim3(kWide), 0, stream, a, ws);
-  hipLaunchKernelGGL(release_copy_kernel, dim3(a.plan.sequences), dim3(256), 0, stream, a, ws);
+  hipLaunchKernelGGL(release_copy_kernel, dim3(p.sequences), dim3(256), 0, stream, a, ws);
 }
 
 }  // namespace qlin

@@ -227,6 +227,7 @@ extern "C" int infer_hip_attention_paged_decode(const infer_hip_kv_pages* pages,
 namespace {
 
 constexpr int kMaxPoolPages = 1 << 30;
+constexpr int kMaxPlanTokens = 1 << 30;
 
 int check_plan(const PagePlan& p, int page_size, const void* workspace, size_t workspace_bytes,
                PagePlan* out, const char* what) {
@@ -284,7 +285,8 @@ extern "C" int infer_hip_kv_pages_assign(int* table, int num_sequences, int max_
   if (!free_pages || !added || !positions) {
     return fail(INFER_HIP_INVALID_ARGUMENT, "%s: null pointer", what);
   }
-  if (tokens < 1 || (!sequences && (tokens != num_sequences || starts))) {
+  if (tokens < 1 || tokens > kMaxPlanTokens ||
+      (!sequences && (tokens != num_sequences || starts))) {
     return fail(INFER_HIP_INVALID_ARGUMENT,
                 "%s: %d tokens of %d sequences, sequences%s given, starts%s", what, tokens,
                 num_sequences, sequences ? "" : " not", starts ? "" : " not");

@@ -190,30 +190,6 @@ __device__ __forceinline__ Pick choose(Row& row, const Setting& s, const Weight&
 
 // ------------------------------------------------- sums over a wave's lanes --
 
-template <int CTRL, int ROWS = 0xF>
-__device__ __forceinline__ unsigned from_lane(unsigned v) {
-  return __builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xF, false);
-}
-template <int CTRL, int ROWS = 0xF>
-__device__ __forceinline__ double from_lane(double v) {
-  const unsigned long long w = __builtin_bit_cast(unsigned long long, v);
-  const unsigned lo = from_lane<CTRL, ROWS>(static_cast<unsigned>(w));
-  const unsigned hi = from_lane<CTRL, ROWS>(static_cast<unsigned>(w >> 32));
-  return __builtin_bit_cast(double, static_cast<unsigned long long>(hi) << 32 | lo);
-}
-
-// Inclusive sums over the lanes: shifts within rows of 16, then the rows' ends.
-template <class T>
-__device__ __forceinline__ T wave_scan(T v) {
-  v += from_lane<0x111>(v);  // row_shr 1, 2, 4, 8: 0 from outside the row
-  v += from_lane<0x112>(v);
-  v += from_lane<0x114>(v);
-  v += from_lane<0x118>(v);
-  v += from_lane<0x142, 0xA>(v);  // row_bcast 15 into rows 1 and 3
-  v += from_lane<0x143, 0xC>(v);  // row_bcast 31 into rows 2 and 3
-  return v;
-}
-
 __device__ __forceinline__ unsigned at_lane(unsigned v, int lane) {
   return __builtin_amdgcn_readlane(static_cast<int>(v), lane);
 }

@@ -223,6 +223,34 @@ def _stream(stream):
     return stream.cuda_stream
 
 
+def _flat(t, dtype, count, index, name):
+    """Pointer of a contiguous tensor of a type on GPU `index`, with `count`
+    elements (None: any number).  It runs for every tensor of a call and reads
+    each as few times as it can (an attribute costs 40-110 ns)."""
+    if (t.dtype is dtype and t.get_device() == index and t.is_contiguous()
+            and (count is None or t.numel() == count)):
+        return t.data_ptr()
+    raise InferError(INVALID_ARGUMENT,
+                     f"{name} must be {'' if count is None else str(count) + ' '}contiguous {dtype} "
+                     f"on GPU {index} (got {list(t.shape)} {t.dtype} on {t.device})")
+
+
+def _here(t, name, stream):
+    """(the GPU of a call's first tensor, which must be the current one; the
+    stream's handle)."""
+    index = t.get_device()
+    if index < 0:
+        raise InferError(INVALID_ARGUMENT, f"{name} must be on a GPU (it is on {t.device})")
+    # a tensor there exists, so torch's HIP state does
+    current = _raw_device() if _raw_device is not None else _current_device()
+    if current != index:
+        raise InferError(INVALID_ARGUMENT,
+                         f"{name} is on GPU {index}, the current device is {current}")
+    if stream is None and _raw_stream is not None:
+        return index, _raw_stream(index)
+    return index, _stream(stream)
+
+
 def _check(status: int) -> None:
     if status != OK:
         msg = load().infer_hip_last_error().decode("utf-8", "replace")

@@ -14,7 +14,7 @@ import ctypes
 import torch
 
 import linear_hip
-from linear_hip import INVALID_ARGUMENT, InferError, _check, _stream
+from linear_hip import INVALID_ARGUMENT, InferError, _check, _flat, _here, _stream
 
 # Every symbol include/infer_paged.h declares.
 EXPORTED_SYMBOLS = (
@@ -261,34 +261,23 @@ def kv_pages_plan_workspace_bytes(num_sequences: int) -> int:
     return load().infer_hip_kv_pages_plan_workspace_bytes(num_sequences)
 
 
-class _Device:
-    """What the checks above read of a pool, from a tensor."""
-
-    def __init__(self, t):
-        self.device, self.index = t.device, t.get_device()
-
-
-def _flat(t, dtype, count, on, name):
-    if t.numel() != count:
-        _bad(f"{name} must hold {count} (got {t.numel()})")
-    return _at(t, dtype, on, name)
-
-
 def _plan(table, free, free_count, lengths, lengths_out, free_count_out, workspace, stream):
-    """The checks that both operators share: (where, stream, table, pointers)."""
-    on = _Device(table)
-    if on.index < 0:
-        _bad("block table must be on a GPU")
-    handle = _on(on, stream)
-    tab = _table(table, on)
-    n = tab.num_sequences
-    return on, handle, tab, (
-        _at(free, _I32, on, "free"), free.numel(), _flat(free_count, _I32, 1, on, "free_count"),
-        _flat(free_count if free_count_out is None else free_count_out, _I32, 1, on,
-              "free_count_out"),
-        _flat(lengths, _I32, n, on, "lengths"),
-        _flat(lengths if lengths_out is None else lengths_out, _I32, n, on, "lengths_out"),
-        _at(workspace, _U8, on, "workspace"))
+    """What both operators take: (GPU, stream, their first pointers and sizes)."""
+    index, handle = _here(table, "block table", stream)
+    if table.dtype is not _I32 or table.dim() != 2:
+        _bad("block table must be int32 [sequences, pages]")
+    rows, width = table.shape
+    stride, inner = table.stride()
+    if inner != 1 and width > 1:
+        _bad("block table rows must be contiguous")
+    fc = _flat(free_count, _I32, 1, index, "free_count")
+    ln = _flat(lengths, _I32, rows, index, "lengths")
+    return (index, handle, rows, (table.data_ptr(), rows, width, stride if rows > 1 else width),
+            (_flat(free, _I32, None, index, "free"), free.numel(), fc,
+             fc if free_count_out is None else _flat(free_count_out, _I32, 1, index,
+                                                     "free_count_out"), ln),
+            ln if lengths_out is None else _flat(lengths_out, _I32, rows, index, "lengths_out"),
+            _flat(workspace, _U8, None, index, "workspace"))
 
 
 def kv_pages_assign(table, page_size: int, free, free_count, lengths, added, workspace, positions,
@@ -301,17 +290,16 @@ def kv_pages_assign(table, page_size: int, free, free_count, lengths, added, wor
     and sequences int32 [tokens], slots int64 [tokens], starts int32
     [sequences + 1], lengths_out and free_count_out (None: in place).
     sequences None: token s belongs to sequence s."""
-    on, handle, tab, (fp, pages, fc, fo, ln, lo, ws) = _plan(
-        table, free, free_count, lengths, lengths_out, free_count_out, workspace, stream)
-    n, tokens = tab.num_sequences, positions.numel()
-    ap = _flat(added, _I32, n, on, "added")
-    pp = _at(positions, _I32, on, "positions")
-    ids = None if sequences is None else _flat(sequences, _I32, tokens, on, "sequences")
-    sl = None if slots is None else _flat(slots, _I64, tokens, on, "slots")
-    st = None if starts is None else _flat(starts, _I32, n + 1, on, "starts")
+    index, handle, n, tab, pool, lo, ws = _plan(table, free, free_count, lengths, lengths_out,
+                                                free_count_out, workspace, stream)
+    tokens = positions.numel()
     _check(load().infer_hip_kv_pages_assign(
-        tab.pages, n, tab.max_pages, tab.stride, page_size, fp, pages, fc, fo, ln, ap, lo, tokens,
-        pp, ids, sl, st, ws, workspace.numel(), handle))
+        *tab, page_size, *pool, _flat(added, _I32, n, index, "added"), lo, tokens,
+        _flat(positions, _I32, None, index, "positions"),
+        None if sequences is None else _flat(sequences, _I32, tokens, index, "sequences"),
+        None if slots is None else _flat(slots, _I64, tokens, index, "slots"),
+        None if starts is None else _flat(starts, _I32, n + 1, index, "starts"), ws,
+        workspace.numel(), handle))
 
 
 def kv_pages_release(table, page_size: int, free, free_count, lengths, finished, workspace,
@@ -319,9 +307,8 @@ def kv_pages_release(table, page_size: int, free, free_count, lengths, finished,
     """The pages of the sequences with finished[s] != 0 (int32 [sequences]) back
     onto free (infer_hip_kv_pages_release); the other arguments are
     kv_pages_assign's."""
-    on, handle, tab, (fp, pages, fc, fo, ln, lo, ws) = _plan(
-        table, free, free_count, lengths, lengths_out, free_count_out, workspace, stream)
+    index, handle, n, tab, pool, lo, ws = _plan(table, free, free_count, lengths, lengths_out,
+                                                free_count_out, workspace, stream)
     _check(load().infer_hip_kv_pages_release(
-        tab.pages, tab.num_sequences, tab.max_pages, tab.stride, page_size, fp, pages, fc, fo, ln,
-        _flat(finished, _I32, tab.num_sequences, on, "finished"), lo, ws, workspace.numel(),
-        handle))
+        *tab, page_size, *pool, _flat(finished, _I32, n, index, "finished"), lo, ws,
+        workspace.numel(), handle))

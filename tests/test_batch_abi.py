@@ -70,7 +70,7 @@ def test_plan_refusals(hip, paged, change, why):
 
 @pytest.mark.parametrize("change,why", [
     (dict(added=None), "null"), (dict(positions=None), "null"), (dict(tokens=0), "tokens"),
-    (dict(sequences=None, starts=None), "tokens"), (dict(sequences=None, tokens=3), "starts")])
+    (dict(tokens=(1 << 30) + 1), "tokens"), (dict(sequences=None, starts=None), "tokens"), (dict(sequences=None, tokens=3), "starts")])
 def test_assign_refusals(hip, paged, change, why):
     lib = paged.load()
     refused(hip, lib, lib.infer_hip_kv_pages_assign, {**ASSIGN, **change}, why)
