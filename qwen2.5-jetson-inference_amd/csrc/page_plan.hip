@@ -32,6 +32,21 @@ struct ScanLds {
   unsigned used;
 };
 
+// Of the sums that each of `waves` waves left in LDS, and what came before them: those
+// before the wave, and all.
+struct SumPair {
+  unsigned before, all;
+};
+
+__device__ __forceinline__ SumPair sums_before(const unsigned* of_wave, int wave, int waves,
+                                               unsigned before) {
+  const int lane = threadIdx.x & (kWave - 1);
+  const unsigned in = add_sat(before, scan_sat(lane < waves ? of_wave[lane] : 0u));
+  const unsigned mine = __builtin_amdgcn_readlane(static_cast<int>(in), max(wave - 1, 0));
+  return {wave ? mine : before,
+          static_cast<unsigned>(__builtin_amdgcn_readlane(static_cast<int>(in), kWave - 1))};
+}
+
 __device__ __forceinline__ int unused_pages(const PagePlan& p) {
   return min(max(*p.free_count, 0), p.num_pages);
 }
@@ -41,7 +56,8 @@ __device__ __forceinline__ int unused_pages(const PagePlan& p) {
 // starts (all of lengths is read before; the caller writes free_count_out).
 __device__ int scan_sequences(const AssignArgs& a, const Share& share, ScanLds& lds, bool out) {
   const PagePlan& p = a.plan;
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int waves = blockDim.x / kWave;
   const unsigned positions = static_cast<unsigned>(p.max_pages) << p.page_shift;
   const unsigned round = (1u << p.page_shift) - 1;
@@ -68,15 +84,9 @@ __device__ int scan_sequences(const AssignArgs& a, const Share& share, ScanLds& 
       lds.need[wave] = need_in;
     }
     __syncthreads();
-    unsigned add_sum = add_before, need_sum = need_before, add_wave = 0, need_wave = 0;
-    for (int w = 0; w < waves; ++w) {
-      if (w == wave) {
-        add_wave = add_sum;
-        need_wave = need_sum;
-      }
-      add_sum = add_sat(add_sum, lds.add[w]);
-      need_sum = add_sat(need_sum, lds.need[w]);
-    }
+    const SumPair adds = sums_before(lds.add, wave, waves, add_before);
+    const SumPair needs = sums_before(lds.need, wave, waves, need_before);
+    const unsigned add_wave = adds.before, need_wave = needs.before;
     const unsigned add_end = add_sat(add_wave, add_in), need_end = add_sat(need_wave, need_in);
     // An exclusive sum as the inclusive one of the lane before: a saturated sum
     // cannot be taken back.
@@ -99,8 +109,8 @@ __device__ int scan_sequences(const AssignArgs& a, const Share& share, ScanLds& 
         }
       }
     }
-    add_before = add_sum;
-    need_before = need_sum;
+    add_before = adds.all;
+    need_before = needs.all;
     __syncthreads();
   }
   return lds.used;
@@ -123,25 +133,17 @@ __device__ __forceinline__ void place_tokens(const AssignArgs& a, const Share& s
     s[i] = live[i] ? token : 0;
     at[i] = 0;  // of the sequence's new tokens
   }
-  if (a.ids) {  // the first sequence whose tokens end past each
-    int hi[N];
+  if (a.ids) {  // how many sequences end at or before each: the first that does not
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      s[i] = 0;
-      hi[i] = p.sequences;
-    }
-    for (int n = p.sequences; n > 0; n >>= 1) {
+    for (int i = 0; i < N; ++i) s[i] = 0;
+    for (int step = 1 << (31 - __builtin_clz(p.sequences)); step > 0; step >>= 1) {
+      int start[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) start[i] = share.starts[min(s[i] + step, p.sequences)];
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const int mid = (s[i] + hi[i]) / 2;
-        const bool past = share.starts[min(mid, last) + 1] > t + i * apart;
-        if (s[i] < hi[i]) {
-          if (past) {
-            hi[i] = mid;
-          } else {
-            s[i] = mid + 1;
-          }
-        }
+        const int next = s[i] + step;
+        s[i] = next <= p.sequences && start[i] <= t + i * apart ? next : s[i];
       }
     }
 #pragma unroll
@@ -200,9 +202,11 @@ __device__ __forceinline__ Share share_of(int* workspace, int sequences) {
 // Bound: a step's launch and its chain of reads: lengths, then free entries or pages.  24
 // sequences XX us (1.7 an empty launch), 25 000 tokens of 8 prompts XX, 620 000 of 2000
 // sequences XX for 10 MB, mostly written.
-constexpr int kHere = 1024, kHereTokens = 1 << 17;
+constexpr int kHere = 2048;
+// Tokens from which a thread takes four.
+constexpr int kManyTokens = 1 << 16;
 
-template <int NT>
+template <int NT, int N>
 __global__ __launch_bounds__(NT) void assign_kernel(AssignArgs a) {
   __shared__ ScanLds lds;
   __shared__ int starts[kHere + 1], held[kHere], first[kHere];
@@ -210,8 +214,8 @@ __global__ __launch_bounds__(NT) void assign_kernel(AssignArgs a) {
   const int used = scan_sequences(a, share, lds, blockIdx.x == 0);
   // every thread of the workgroup has read the count by now
   if (blockIdx.x == 0 && threadIdx.x == 0) *a.plan.free_count_out = unused_pages(a.plan) - used;
-  const int t = blockIdx.x * NT + threadIdx.x;
-  if (t < a.tokens) place_tokens<1>(a, share, t, 0);
+  const int t = blockIdx.x * NT * N + threadIdx.x;
+  if (t < a.tokens) place_tokens<N>(a, share, t, NT);
 }
 
 __global__ __launch_bounds__(kWide) void assign_scan_kernel(AssignArgs a, int* workspace) {
@@ -228,7 +232,8 @@ __global__ __launch_bounds__(256) void assign_fill_kernel(AssignArgs a, int* wor
   __shared__ int starts[FITS ? kStarts : 1];
   Share share = share_of(workspace, a.plan.sequences);
   if (FITS && a.ids) {
-    for (int i = threadIdx.x; i <= a.plan.sequences; i += blockDim.x) starts[i] = share.starts[i];
+#pragma unroll 8
+    for (int i = threadIdx.x; i <= a.plan.sequences; i += 256) starts[i] = share.starts[i];
     __syncthreads();
   }
   if (FITS) share.starts = starts;
@@ -245,15 +250,18 @@ size_t page_plan_workspace_bytes(int sequences) {
 void launch_pages_assign(const AssignArgs& a, void* workspace, hipStream_t stream) {
   int* ws = static_cast<int*>(workspace);
   const PagePlan& p = a.plan;
-  const int threads = p.sequences <= 256 && a.tokens <= kHereTokens ? 256 : kWide;
   auto blocks = [&](int each) { return static_cast<unsigned>((a.tokens - 1) / each + 1); };
+  const int threads = p.sequences <= 256 && a.tokens <= kManyTokens ? 256 : kWide;
   const bool in_place = p.lengths_out == p.lengths || p.free_count_out == p.free_count;
-  if (p.sequences <= kHere && a.tokens <= kHereTokens &&
-      (a.tokens <= threads || !in_place)) {
+  if (p.sequences <= (in_place ? threads : kHere) && (a.tokens <= threads || !in_place)) {
     if (threads == 256) {
-      hipLaunchKernelGGL(assign_kernel<256>, dim3(blocks(256)), dim3(256), 0, stream, a);
+      hipLaunchKernelGGL((assign_kernel<256, 1>), dim3(blocks(256)), dim3(256), 0, stream, a);
+    } else if (a.tokens <= kManyTokens) {
+      hipLaunchKernelGGL((assign_kernel<kWide, 1>), dim3(blocks(kWide)), dim3(kWide), 0, stream,
+                         a);
     } else {
-      hipLaunchKernelGGL(assign_kernel<kWide>, dim3(blocks(kWide)), dim3(kWide), 0, stream, a);
+      hipLaunchKernelGGL((assign_kernel<kWide, 4>), dim3(blocks(4 * kWide)), dim3(kWide), 0,
+                         stream, a);
     }
     return;
   }
@@ -335,7 +343,8 @@ __global__ __launch_bounds__(kWide) void release_scan_kernel(ReleaseArgs a, int*
   __shared__ ScanLds lds;
   const PagePlan& p = a.plan;
   const Share share = share_of(workspace, p.sequences);
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int count = unused_pages(p);
   unsigned before = 0;
   for (int base = 0; base < p.sequences; base += kWide) {
@@ -349,18 +358,15 @@ __global__ __launch_bounds__(kWide) void release_scan_kernel(ReleaseArgs a, int*
     const unsigned in = scan_sat(pages);
     if (lane == kWave - 1) lds.need[wave] = in;
     __syncthreads();
-    unsigned sum = before, mine = 0;
-    for (int w = 0; w < kWide / kWave; ++w) {
-      if (w == wave) mine = sum;
-      sum = add_sat(sum, lds.need[w]);
-    }
+    const SumPair sums = sums_before(lds.need, wave, kWide / kWave, before);
+    const unsigned mine = sums.before;
     unsigned first = __shfl_up(in, 1);
     first = lane ? add_sat(mine, first) : mine;
     if (s < p.sequences) {
       share.held[s] = pages;
       share.first[s] = first;
     }
-    before = sum;
+    before = sums.all;
     __syncthreads();
   }
   if (threadIdx.x == 0) {
