@@ -286,6 +286,11 @@ __device__ __forceinline__ void store_global8(void* p, uint2 v) {
   *(QLIN_GLOBAL u32x2*)(p) = u32x2{v.x, v.y};
 }
 
+// A barrier for what lies in LDS; loads from memory stay on their way.
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
 // v of lane `from` / 4.
 __device__ __forceinline__ uint4 lane_of(const uint4& v, int from) {
   auto one = [&](uint32_t w) {

@@ -25,7 +25,7 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 // launch ahead groups each chunk of 1024 by a table in LDS.  Nothing is sorted, and a
 // captured graph follows ids that change.
 //
-// h = s A x: 16 rows of A by 16 tokens a tile, K split over a workgroup's waves and
+// h = s A x: 16 rows of A by 16 tokens a tile, K split over a workgroup's 16 waves and
 // joined in LDS in the order of the waves.  h is kept as high + low BF16 (2^-16 of it;
 // one BF16 number alone would add as much error as the output's rounding), and B h takes
 // two products.
@@ -203,39 +203,105 @@ __device__ __forceinline__ uint4 cut_words(uint4 v, int k, int rank) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// A wave's share of RT tiles of rows of A by the tile's tokens: steps of 32 columns,
-// each wave neighbouring ones, whose loads are on their way together.
+// h of RT tiles of rows of A by a tile's tokens, by 16 waves.  Each wave loads whole rows, a
+// KB in a row (as operands, 16 rows side by side, they would cost the CU's address unit
+// four times as much), into LDS, a chunk of columns at a time with kDepth of them on their
+// way; there it takes its steps of the chunk for all rows.
+constexpr int kShrinkWaves = 16;
+
 template <int RT>
-__device__ __forceinline__ void shrink_steps(f32x4_t (&sum)[RT], const LoraArgs& a,
-                                             const uint16_t* const (&w)[RT], const uint16_t* x,
-                                             int wave, int waves, int g) {
-  constexpr int kDepth = RT >= 4 ? 2 : RT == 2 ? 4 : 8;
-  const int steps = (a.k + 31) / 32, each = (steps + waves - 1) / waves;
-  const int end = min(steps, (wave + 1) * each);
+struct Stage {
+  static constexpr int kLoads = RT <= 2 ? 2 : 1;  // of a row's chunk
+  static constexpr int kColumns = 512 * kLoads;
+  static constexpr int kDepth = RT == 1 ? 4 : 3;
+  static constexpr int kSteps = kColumns / 32 / kShrinkWaves;  // of a wave
+  static constexpr int kPitch = kColumns + 8;
+  union {
+    __align__(16) uint16_t rows[(RT + 1) * kTile][kPitch];
+    f32x4_t part[kShrinkWaves][RT][kWave];
+  };
+};
+
+// rows: those of A that the wave loads, row `wave` of each tile, and its token's x.
+template <int RT>
+__device__ __forceinline__ void shrink_tile(f32x4_t (&sum)[RT], const LoraArgs& a,
+                                            const uint16_t* const (&rows)[RT + 1],
+                                            Stage<RT>& stage, int wave, int lane) {
+  typedef Stage<RT> S;
+  const int chunks = (a.k + S::kColumns - 1) / S::kColumns;
+  uint4 v[S::kDepth][RT + 1][S::kLoads];
+  auto load = [&](uint4 (&to)[RT + 1][S::kLoads], int chunk) {
+#pragma unroll
+    for (int i = 0; i <= RT; ++i) {
+#pragma unroll
+      for (int j = 0; j < S::kLoads; ++j) {
+        const int k = chunk * S::kColumns + 512 * j + 8 * lane;
+        to[i][j] = make_uint4(0, 0, 0, 0);
+        if (k < a.k) to[i][j] = load_global16(rows[i] + k);
+      }
+    }
+  };
+#pragma unroll
+  for (int d = 0; d < S::kDepth; ++d) {
+    if (d < chunks) load(v[d], d);
+  }
 #pragma unroll
   for (int r = 0; r < RT; ++r) sum[r] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  for (int base = wave * each; base < end; base += kDepth) {
-    uint4 p[kDepth][RT], q[kDepth];
+  for (int base = 0; base < chunks; base += S::kDepth) {
 #pragma unroll
-    for (int i = 0; i < kDepth; ++i) {
-      const int k = 32 * (base + i) + 8 * g;
-      const bool in = base + i < end && k < a.k;
-      q[i] = make_uint4(0, 0, 0, 0);
-      if (in) q[i] = load_global16(x + k);
+    for (int d = 0; d < S::kDepth; ++d) {
+      if (base + d >= chunks) break;
+      lds_barrier();
 #pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        p[i][r] = make_uint4(0, 0, 0, 0);
-        if (in) p[i][r] = load_global16(w[r] + k);
+      for (int i = 0; i <= RT; ++i) {
+#pragma unroll
+        for (int j = 0; j < S::kLoads; ++j) {
+          *reinterpret_cast<uint4*>(&stage.rows[i * kTile + wave][512 * j + 8 * lane]) = v[d][i][j];
+        }
+      }
+      lds_barrier();
+      if (base + d + S::kDepth < chunks) load(v[d], base + d + S::kDepth);
+#pragma unroll
+      for (int s = 0; s < S::kSteps; ++s) {
+        const int k = 32 * (wave * S::kSteps + s) + 8 * (lane >> 4);
+        auto piece = [&](int i) {
+          return as_bf16(
+              *reinterpret_cast<const uint4*>(&stage.rows[i * kTile + (lane & 15)][k]));
+        };
+        const bf16x8_t x = piece(RT);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          sum[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(piece(r), x, sum[r], 0, 0, 0);
+        }
       }
     }
+  }
+  lds_barrier();
 #pragma unroll
-    for (int i = 0; i < kDepth; ++i) {
+  for (int r = 0; r < RT; ++r) stage.part[wave][r][lane] = sum[r];
+  lds_barrier();
+}
+
+// Element e of the tile's h, row 16 (e / 256) + 4 (e / 64 % 4) + e % 4 of token e / 4 % 16:
+// the waves' sums in order.
+template <int RT>
+__device__ __forceinline__ float joined(const Stage<RT>& stage, int e) {
+  const float* p = reinterpret_cast<const float*>(stage.part) + e;
+  float h = p[0];
 #pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        sum[r] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16(p[i][r]), as_bf16(q[i]), sum[r],
-                                                         0, 0, 0);
-      }
-    }
+  for (int i = 1; i < kShrinkWaves; ++i) h += p[i * RT * kWave * 4];
+  return h;
+}
+__device__ __forceinline__ int row_of(int e) { return e / 256 * kTile + e / 64 % 4 * 4 + e % 4; }
+__device__ __forceinline__ int token_of(int e) { return e / 4 % 16; }
+
+template <int RT>
+__device__ __forceinline__ void stage_rows(const uint16_t* (&rows)[RT + 1], const LoraArgs& a,
+                                           const LoraTarget& t, int adapter, int first, int wave) {
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    rows[r] = t.a + (static_cast<size_t>(max(adapter, 0)) * a.max_rank +
+                     min(first + r * kTile + wave, a.max_rank - 1)) * a.k;
   }
 }
 
@@ -245,46 +311,32 @@ __device__ __forceinline__ void split_word(float h, uint16_t& high, uint16_t& lo
   low = (high & 0x7F80u) == 0x7F80u ? 0 : f32_to_bf16(h - bf16_to_f32(high));
 }
 
-template <int RT, int WAVES, bool GROUPED>
-__global__ __launch_bounds__(WAVES * kWave) void lora_shrink_kernel(LoraArgs a) {
-  __shared__ int list[GROUPED ? kSet : kGather];
-  __shared__ f32x4_t part[WAVES][RT][kWave];
+template <int RT, bool GROUPED>
+__global__ __launch_bounds__(kShrinkWaves * kWave) void lora_shrink_kernel(LoraArgs a) {
+  extern __shared__ __align__(16) char shared[];
+  Stage<RT>& stage = *reinterpret_cast<Stage<RT>*>(shared);
+  int* const list = reinterpret_cast<int*>(shared + sizeof(Stage<RT>));
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int m = lane & 15, g = lane >> 4;
   const Unit u = tokens_of<GROUPED>(a, blockIdx.x, list);
   if (u.count == 0 || u.rank == 0) return;
   const int blocks = (a.max_rank + RT * kTile - 1) / (RT * kTile);
-  const int c = blockIdx.y / blocks, rows = blockIdx.y % blocks * RT * kTile;
-  const int rank = u.rank, pitch = rank_pitch(a.max_rank);
-  const uint16_t* w[RT];
-#pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    w[r] = a.target[c].a + (static_cast<size_t>(u.adapter) * a.max_rank +
-                            min(rows + r * kTile + m, a.max_rank - 1)) * a.k;
-  }
+  const int c = blockIdx.y / blocks, first = blockIdx.y % blocks * RT * kTile;
+  const int pitch = rank_pitch(a.max_rank);
+  const uint16_t* rows[RT + 1];
+  stage_rows<RT>(rows, a, a.target[c], u.adapter, first, wave);
   for (int tile = blockIdx.z; tile * kTile < u.count; tile += gridDim.z) {
+    const int token = list[min(tile * kTile + wave, u.count - 1)];
+    rows[RT] = a.x + token * a.x_stride;
     f32x4_t sum[RT];
-    shrink_steps<RT>(sum, a, w, a.x + list[min(tile * kTile + m, u.count - 1)] * a.x_stride, wave,
-                     WAVES, g);
-    __syncthreads();
-#pragma unroll
-    for (int r = 0; r < RT; ++r) part[wave][r][lane] = sum[r];
-    __syncthreads();
-    // element e of a tile: row 4 (e / 64) + e % 4 of token e / 4 % 16
-    for (int e = threadIdx.x; e < RT * kTile * kTile; e += WAVES * kWave) {
-      const float* p = reinterpret_cast<const float*>(part) + e;
-      float h = p[0];
-#pragma unroll
-      for (int i = 1; i < WAVES; ++i) h += p[i * RT * kWave * 4];
-      const int in = e % (kTile * kTile);
-      const int row = rows + e / (kTile * kTile) * kTile + in / 64 * 4 + in % 4;
-      const int at = tile * kTile + in / 4 % 16;
+    shrink_tile<RT>(sum, a, rows, stage, wave, lane);
+    for (int e = threadIdx.x; e < RT * kTile * kTile; e += kShrinkWaves * kWave) {
+      const float h = joined<RT>(stage, e);
+      const int row = first + row_of(e), at = tile * kTile + token_of(e);
       if (at < u.count && row < pitch) {
         uint16_t high, low;
-        split_word(row < rank ? h * u.scale : 0.0f, high, low);
-        uint16_t* to =
-            a.h + (static_cast<size_t>(c) * a.tokens + list[at]) * 2 * pitch + row;
+        split_word(row < u.rank ? h * u.scale : 0.0f, high, low);
+        uint16_t* to = a.h + (static_cast<size_t>(c) * a.tokens + list[at]) * 2 * pitch + row;
         to[0] = high;
         to[pitch] = low;
       }
@@ -466,13 +518,12 @@ __global__ __launch_bounds__(kExpandWaves * kWave) void lora_expand_kernel(LoraA
 // they wait for: a workgroup takes 16 waves' columns of a unit's target and computes
 // the unit's h for itself, in LDS.  A is read once for each such workgroup, from L2 as
 // a rule.
-constexpr int kFusedWaves = 16;
-
 template <int RT, int J>
-__global__ __launch_bounds__(kFusedWaves * kWave) void lora_fused_kernel(LoraArgs a) {
+__global__ __launch_bounds__(kShrinkWaves * kWave) void lora_fused_kernel(LoraArgs a) {
   constexpr int KS = (RT + 1) / 2, kPitch = RT * kTile + 8;  // words of a row of h
-  __shared__ int list[kGather];
-  __shared__ f32x4_t part[kFusedWaves][RT][kWave];
+  extern __shared__ __align__(16) char shared[];
+  Stage<RT>& stage = *reinterpret_cast<Stage<RT>*>(shared);
+  int* const list = reinterpret_cast<int*>(shared + sizeof(Stage<RT>));
   __shared__ __align__(16) uint16_t h[2][kTile][kPitch];
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -480,19 +531,14 @@ __global__ __launch_bounds__(kFusedWaves * kWave) void lora_fused_kernel(LoraArg
   const Unit u = gather_tokens(a, blockIdx.x, list);
   if (u.count == 0) return;
   int block = blockIdx.y;
-  const int c = target_of(a, kFusedWaves * J * 16, block);
+  const int c = target_of(a, kShrinkWaves * J * 16, block);
   const LoraTarget& t = a.target[c];
   if (u.adapter < 0 && t.base == t.out) return;
-  block = block * kFusedWaves + wave;
+  block = block * kShrinkWaves + wave;
   const bool has = block * J * 16 < t.n;
   Columns<KS, J, false> columns(a, t, has ? block : 0, u, lane);
-  const uint16_t* w[RT];
-#pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    w[r] = t.a + (static_cast<size_t>(max(u.adapter, 0)) * a.max_rank +
-                  min(r * kTile + m, a.max_rank - 1)) * a.k;
-  }
-  columns.cut(lane);
+  const uint16_t* rows[RT + 1];
+  stage_rows<RT>(rows, a, t, u.adapter, 0, wave);
   for (int tile = blockIdx.z; tile * kTile < u.count; tile += gridDim.z) {
     typename Words<J>::type base[4];
 #pragma unroll
@@ -504,22 +550,15 @@ __global__ __launch_bounds__(kFusedWaves * kWave) void lora_fused_kernel(LoraArg
     for (int s = 0; s < KS; ++s) high[s] = low[s] = make_uint4(0, 0, 0, 0);
     if (u.rank) {
       f32x4_t sum[RT];
-      const int token = list[min(tile * kTile + m, u.count - 1)];
-      shrink_steps<RT>(sum, a, w, a.x + token * a.x_stride, wave, kFusedWaves, g);
-#pragma unroll
-      for (int r = 0; r < RT; ++r) part[wave][r][lane] = sum[r];
-      __syncthreads();
-      for (int e = threadIdx.x; e < RT * kTile * kTile; e += kFusedWaves * kWave) {
-        const float* p = reinterpret_cast<const float*>(part) + e;
-        float v = p[0];
-#pragma unroll
-        for (int i = 1; i < kFusedWaves; ++i) v += p[i * RT * kWave * 4];
-        const int in = e % (kTile * kTile);
-        const int row = e / (kTile * kTile) * kTile + in / 64 * 4 + in % 4;
-        uint16_t* to = &h[0][in / 4 % 16][row];
-        split_word(row < u.rank ? v * u.scale : 0.0f, to[0], to[kTile * kPitch]);
+      rows[RT] = a.x + list[min(tile * kTile + wave, u.count - 1)] * a.x_stride;
+      shrink_tile<RT>(sum, a, rows, stage, wave, lane);
+      for (int e = threadIdx.x; e < RT * kTile * kTile; e += kShrinkWaves * kWave) {
+        const int row = row_of(e);
+        uint16_t* to = &h[0][token_of(e)][row];
+        split_word(row < u.rank ? joined<RT>(stage, e) * u.scale : 0.0f, to[0],
+                   to[kTile * kPitch]);
       }
-      __syncthreads();
+      lds_barrier();
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
         const int k = 32 * s + 8 * g;
@@ -529,6 +568,7 @@ __global__ __launch_bounds__(kFusedWaves * kWave) void lora_fused_kernel(LoraArg
         }
       }
     }
+    if (tile == static_cast<int>(blockIdx.z)) columns.cut(lane);
     f32x4_t sum[J];
     columns.multiply(sum, high, low);
     if (has) {
@@ -593,18 +633,18 @@ static void launch_expand(const LoraArgs& a, int units, int slots, hipStream_t s
 constexpr long long kFusedBytes = 24ll << 20;
 
 static bool launch_fused(const LoraArgs& a, int slots, hipStream_t stream) {
-  constexpr int kColumns = kFusedWaves * 64;
+  constexpr int kColumns = kShrinkWaves * 64;
   int blocks = 0;
   for (int i = 0; i < a.targets; ++i) blocks += (a.target[i].n + kColumns - 1) / kColumns;
   const long long units = std::min(a.units, a.tokens);
   if (a.max_rank > 64 || 2ll * units * blocks * a.max_rank * a.k > kFusedBytes) return false;
-  auto run = [&](auto* kernel) {
-    hipLaunchKernelGGL(kernel, dim3(a.units, blocks, slots), dim3(kFusedWaves * kWave), 0, stream,
-                       a);
+  auto run = [&](auto* kernel, size_t lds) {
+    hipLaunchKernelGGL(kernel, dim3(a.units, blocks, slots), dim3(kShrinkWaves * kWave),
+                       lds + kGather * sizeof(int), stream, a);
   };
-  a.max_rank <= 16   ? run(lora_fused_kernel<1, 4>)
-  : a.max_rank <= 32 ? run(lora_fused_kernel<2, 4>)
-                     : run(lora_fused_kernel<4, 4>);
+  a.max_rank <= 16   ? run(lora_fused_kernel<1, 4>, sizeof(Stage<1>))
+  : a.max_rank <= 32 ? run(lora_fused_kernel<2, 4>, sizeof(Stage<2>))
+                     : run(lora_fused_kernel<4, 4>, sizeof(Stage<4>));
   return true;
 }
 
@@ -616,14 +656,14 @@ void launch_lora(LoraArgs a, hipStream_t stream) {
     a.units = units_of(a.tokens, a.adapters);
     const int chunks = chunks_of(a.tokens), units = chunks * a.units;
     hipLaunchKernelGGL(lora_group_kernel, dim3(chunks), dim3(kChunk), 0, stream, a);
-    auto shrink = [&](auto* kernel, int tiles, int waves) {
+    auto shrink = [&](auto* kernel, int tiles, size_t lds) {
       hipLaunchKernelGGL(kernel, dim3(units, a.targets * ((rank_tiles + tiles - 1) / tiles),
                                       kSet / kTile),
-                         dim3(waves * kWave), 0, stream, a);
+                         dim3(kShrinkWaves * kWave), lds + kSet * sizeof(int), stream, a);
     };
-    rank_tiles == 1   ? shrink(lora_shrink_kernel<1, 16, true>, 1, 16)
-    : rank_tiles == 2 ? shrink(lora_shrink_kernel<2, 16, true>, 2, 16)
-                      : shrink(lora_shrink_kernel<4, 8, true>, 4, 8);
+    rank_tiles == 1   ? shrink(lora_shrink_kernel<1, true>, 1, sizeof(Stage<1>))
+    : rank_tiles == 2 ? shrink(lora_shrink_kernel<2, true>, 2, sizeof(Stage<2>))
+                      : shrink(lora_shrink_kernel<4, true>, 4, sizeof(Stage<4>));
     launch_expand<true>(a, units, 1, stream);
     return;
   }
@@ -633,8 +673,9 @@ void launch_lora(LoraArgs a, hipStream_t stream) {
   const int tiles = (a.tokens + kTile - 1) / kTile;
   const int slots = std::min(tiles, 1 + a.tokens / (kTile * a.units));
   if (launch_fused(a, slots, stream)) return;
-  hipLaunchKernelGGL((lora_shrink_kernel<1, 16, false>),
-                     dim3(a.units, a.targets * rank_tiles, slots), dim3(16 * kWave), 0, stream, a);
+  hipLaunchKernelGGL((lora_shrink_kernel<1, false>),
+                     dim3(a.units, a.targets * rank_tiles, slots), dim3(kShrinkWaves * kWave),
+                     sizeof(Stage<1>) + kGather * sizeof(int), stream, a);
   launch_expand<false>(a, a.units, slots, stream);
 }
 

@@ -205,11 +205,6 @@ __device__ __forceinline__ T wave_total(T v) {
   return at_lane(wave_scan(v), kWave - 1);
 }
 
-// A barrier for what lies in LDS; loads from memory stay on their way.
-__device__ __forceinline__ void lds_barrier() {
-  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-}
-
 // ------------------------------------------------------- bisecting kernel --
 
 struct Lds {
