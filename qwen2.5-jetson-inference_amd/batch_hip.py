@@ -10,6 +10,7 @@ Greedy-cy/qwen2.5-jetson-inference).
 from __future__ import annotations
 
 import ctypes
+import struct
 
 import torch
 
@@ -36,7 +37,8 @@ class _Target(ctypes.Structure):
 
 _lib = None
 _BF16, _I32, _F32, _U8 = torch.bfloat16, torch.int32, torch.float32, torch.uint8
-_ARRAYS = [None] + [_Target * n for n in range(1, MAX_TARGETS + 1)]
+# One to three of _Target as bytes: a third of the time that setting its fields takes.
+_PACK = [struct.Struct("@" + "PPPPi4xqq" * n).pack for n in range(MAX_TARGETS + 1)]
 
 
 def load():
@@ -97,23 +99,25 @@ def lora(x, ids, targets, workspace, ranks=None, scales=None, stream=None) -> No
     if len(shape) != 3 or shape[2] != k:
         _bad(f"a must be [adapters, max_rank, {k}] (got {list(shape)})")
     adapters, rank = shape[0], shape[1]
-    made = _ARRAYS[len(targets)]()
-    for target, (a, b, base, output) in zip(made, targets):
+    made = []
+    for a, b, base, output in targets:
         n = output.shape[-1]
         if a.shape != shape or b.shape != (adapters, n, rank):
             _bad(f"a must be {list(shape)} and b {[adapters, n, rank]} (got {list(a.shape)}, "
                  f"{list(b.shape)})")
-        target.a = _flat(a, _BF16, None, index, "a")
-        target.b = _flat(b, _BF16, None, index, "b")
-        target.output, target.output_stride = _rows(output, tokens, n, index, "output")
-        target.out_features = n
-        if base is not None:
-            target.base, target.base_stride = _rows(base, tokens, n, index, "base")
-    _check(load().infer_hip_lora_bf16(
-        xp, xs, _flat(ids, _I32, tokens, index, "ids"), tokens, k, made, len(targets), adapters,
-        rank, None if ranks is None else _flat(ranks, _I32, adapters, index, "ranks"),
+        op, os_ = _rows(output, tokens, n, index, "output")
+        bp, bs = (0, 0) if base is None else (op, os_) if base is output else _rows(
+            base, tokens, n, index, "base")
+        made += (_flat(a, _BF16, None, index, "a"), _flat(b, _BF16, None, index, "b"), bp, op, n,
+                 bs, os_)
+    status = load().infer_hip_lora_bf16(
+        xp, xs, _flat(ids, _I32, tokens, index, "ids"), tokens, k, _PACK[len(targets)](*made),
+        len(targets), adapters, rank,
+        None if ranks is None else _flat(ranks, _I32, adapters, index, "ranks"),
         None if scales is None else _flat(scales, _F32, adapters, index, "scales"),
-        _flat(workspace, _U8, None, index, "workspace"), workspace.numel(), on))
+        _flat(workspace, _U8, None, index, "workspace"), workspace.numel(), on)
+    if status:
+        _check(status)
 
 
 def sample_workspace_bytes(rows: int, vocab: int) -> int:

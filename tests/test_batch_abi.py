@@ -103,7 +103,7 @@ LORA = dict(x=A, x_stride=64, ids=A, tokens=5, in_features=64, targets=None, num
 
 
 def lora_args(batch, target=(), **change):
-    t = batch._ARRAYS[3](*[batch._Target(*{**TARGET, **dict(target)}.values())] * 3)
+    t = (batch._Target * 3)(*[batch._Target(*{**TARGET, **dict(target)}.values())] * 3)
     return {**LORA, "targets": ctypes.cast(t, ctypes.c_void_p).value, **change}, t
 
 
@@ -137,6 +137,13 @@ def test_lora_target_refusals(hip, batch, target, why):
         args, keep = lora_args(batch, target, num_targets=n)
         refused(hip, lib, lib.infer_hip_lora_bf16, args, why)
         del keep
+
+
+def test_lora_targets_are_packed_as_the_structure(batch):
+    fields = [1 << 40, 2, 3, 4, 5, 6, 1 << 41]
+    for n in (1, 2, 3):
+        want = bytes((batch._Target * n)(*[batch._Target(*fields)] * n))
+        assert batch._PACK[n](*fields * n) == want
 
 
 def test_lora_workspace(batch):
