@@ -134,12 +134,22 @@ __global__ __launch_bounds__(kChunk) void lora_group_kernel(LoraArgs a) {
   if (t < a.tokens) {
     const int id = adapter_of(a, a.ids[t]);
     place = (static_cast<unsigned>(id) * 2654435761u >> 16) % kPlaces;
-    for (;;) {  // at most kChunk adapters in kPlaces places
-      const int was = atomicCAS(&key[place], -2, id);
-      if (was == -2 || was == id) break;
-      place = (place + 1) % kPlaces;
+    // a wave of one adapter, as in a prompt, asks once: 64 lanes at one address would wait
+    // for each other
+    const bool alike = !__ballot(id != __builtin_amdgcn_readfirstlane(id));
+    const int lanes = __popcll(__ballot(true));
+    if (!alike || lane == 0) {
+      for (;;) {  // at most kChunk adapters in kPlaces places
+        const int was = atomicCAS(&key[place], -2, id);
+        if (was == -2 || was == id) break;
+        place = (place + 1) % kPlaces;
+      }
+      nth = atomicAdd(&size[place], alike ? lanes : 1);
     }
-    nth = atomicAdd(&size[place], 1);
+    if (alike) {
+      place = __builtin_amdgcn_readfirstlane(place);
+      nth = __builtin_amdgcn_readfirstlane(nth) + lane;
+    }
   }
   __syncthreads();
   const int n0 = size[2 * threadIdx.x], n1 = size[2 * threadIdx.x + 1];
@@ -211,9 +221,10 @@ constexpr int kShrinkWaves = 16;
 
 template <int RT>
 struct Stage {
-  static constexpr int kLoads = RT <= 2 ? 2 : 1;  // of a row's chunk
+  // of a row's chunk: room for two workgroups a CU (one at RT 4)
+  static constexpr int kLoads = RT == 1 ? 2 : 1;
   static constexpr int kColumns = 512 * kLoads;
-  static constexpr int kDepth = RT == 1 ? 4 : 3;
+  static constexpr int kDepth = RT == 1 ? 4 : RT == 2 ? 3 : 2;
   static constexpr int kSteps = kColumns / 32 / kShrinkWaves;  // of a wave
   static constexpr int kPitch = kColumns + 8;
   union {
@@ -295,20 +306,25 @@ __device__ __forceinline__ float joined(const Stage<RT>& stage, int e) {
 __device__ __forceinline__ int row_of(int e) { return e / 256 * kTile + e / 64 % 4 * 4 + e % 4; }
 __device__ __forceinline__ int token_of(int e) { return e / 4 % 16; }
 
-template <int RT>
-__device__ __forceinline__ void stage_rows(const uint16_t* (&rows)[RT + 1], const LoraArgs& a,
-                                           const LoraTarget& t, int adapter, int first, int wave) {
-#pragma unroll
-  for (int r = 0; r < RT; ++r) {
-    rows[r] = t.a + (static_cast<size_t>(max(adapter, 0)) * a.max_rank +
-                     min(first + r * kTile + wave, a.max_rank - 1)) * a.k;
-  }
-}
-
 // h as high + low BF16; an infinity has no remainder.
 __device__ __forceinline__ void split_word(float h, uint16_t& high, uint16_t& low) {
   high = f32_to_bf16(h);
   low = (high & 0x7F80u) == 0x7F80u ? 0 : f32_to_bf16(h - bf16_to_f32(high));
+}
+
+// The rows of A that a wave loads of RT tiles from tile `first` on, of all targets' one
+// after the other (past the last: that one again).
+template <int RT>
+__device__ __forceinline__ void stage_rows(const uint16_t* (&rows)[RT + 1], const LoraArgs& a,
+                                           int adapter, int first, int wave) {
+  const int tiles = (a.max_rank + kTile - 1) / kTile;
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    const int q = min(first + r, a.targets * tiles - 1);
+    rows[r] = a.target[q / tiles].a +
+              (static_cast<size_t>(max(adapter, 0)) * a.max_rank +
+               min(q % tiles * kTile + wave, a.max_rank - 1)) * a.k;
+  }
 }
 
 template <int RT, bool GROUPED>
@@ -320,11 +336,10 @@ __global__ __launch_bounds__(kShrinkWaves * kWave) void lora_shrink_kernel(LoraA
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const Unit u = tokens_of<GROUPED>(a, blockIdx.x, list);
   if (u.count == 0 || u.rank == 0) return;
-  const int blocks = (a.max_rank + RT * kTile - 1) / (RT * kTile);
-  const int c = blockIdx.y / blocks, first = blockIdx.y % blocks * RT * kTile;
+  const int tiles = (a.max_rank + kTile - 1) / kTile, first = blockIdx.y * RT;
   const int pitch = rank_pitch(a.max_rank);
   const uint16_t* rows[RT + 1];
-  stage_rows<RT>(rows, a, a.target[c], u.adapter, first, wave);
+  stage_rows<RT>(rows, a, u.adapter, first, wave);
   for (int tile = blockIdx.z; tile * kTile < u.count; tile += gridDim.z) {
     const int token = list[min(tile * kTile + wave, u.count - 1)];
     rows[RT] = a.x + token * a.x_stride;
@@ -332,8 +347,9 @@ __global__ __launch_bounds__(kShrinkWaves * kWave) void lora_shrink_kernel(LoraA
     shrink_tile<RT>(sum, a, rows, stage, wave, lane);
     for (int e = threadIdx.x; e < RT * kTile * kTile; e += kShrinkWaves * kWave) {
       const float h = joined<RT>(stage, e);
-      const int row = first + row_of(e), at = tile * kTile + token_of(e);
-      if (at < u.count && row < pitch) {
+      const int q = first + row_of(e) / kTile, c = q / tiles;
+      const int row = q % tiles * kTile + row_of(e) % kTile, at = tile * kTile + token_of(e);
+      if (at < u.count && c < a.targets) {
         uint16_t high, low;
         split_word(row < u.rank ? h * u.scale : 0.0f, high, low);
         uint16_t* to = a.h + (static_cast<size_t>(c) * a.tokens + list[at]) * 2 * pitch + row;
@@ -538,7 +554,7 @@ __global__ __launch_bounds__(kShrinkWaves * kWave) void lora_fused_kernel(LoraAr
   const bool has = block * J * 16 < t.n;
   Columns<KS, J, false> columns(a, t, has ? block : 0, u, lane);
   const uint16_t* rows[RT + 1];
-  stage_rows<RT>(rows, a, t, u.adapter, 0, wave);
+  stage_rows<RT>(rows, a, u.adapter, c * ((a.max_rank + kTile - 1) / kTile), wave);
   for (int tile = blockIdx.z; tile * kTile < u.count; tile += gridDim.z) {
     typename Words<J>::type base[4];
 #pragma unroll
@@ -613,8 +629,11 @@ static void launch_expand(const LoraArgs& a, int units, int slots, hipStream_t s
   auto run = [&](auto* kernel, int columns) {
     int blocks = 0;
     for (int i = 0; i < a.targets; ++i) blocks += (a.target[i].n + columns - 1) / columns;
-    hipLaunchKernelGGL(kernel, dim3(units, (blocks + kExpandWaves - 1) / kExpandWaves, slots),
-                       dim3(kExpandWaves * kWave), 0, stream, a);
+    blocks = (blocks + kExpandWaves - 1) / kExpandWaves;
+    // a unit's four tiles side by side where there would be few workgroups
+    const long long few = static_cast<long long>((a.tokens + kSet - 1) / kSet) * blocks;
+    const int z = !GROUPED ? slots : few >= 1024 ? 1 : few >= 512 ? 2 : kSet / kTile;
+    hipLaunchKernelGGL(kernel, dim3(units, blocks, z), dim3(kExpandWaves * kWave), 0, stream, a);
   };
   if (GROUPED && bytes > kStreamBytes) {
     steps == 1   ? run(lora_expand_kernel<1, 8, GROUPED, true>, 128)
@@ -629,7 +648,10 @@ static void launch_expand(const LoraArgs& a, int units, int slots, hipStream_t s
   }
 }
 
-// A's bytes that the one launch may read, over all its workgroups.
+// The largest rank of the one launch (64 spills registers: 64 x 896 x 896 16.3 us, in two
+// launches 8.5; 32 33 tokens' q, k and v of 1536 9.5, 9.6), and A's bytes that it may read
+// over all its workgroups (64 x 3584 x 3584 at rank 16, 22 MB, 10.9 us, 12.2).
+constexpr int kFusedRank = 32;
 constexpr long long kFusedBytes = 24ll << 20;
 
 static bool launch_fused(const LoraArgs& a, int slots, hipStream_t stream) {
@@ -637,14 +659,13 @@ static bool launch_fused(const LoraArgs& a, int slots, hipStream_t stream) {
   int blocks = 0;
   for (int i = 0; i < a.targets; ++i) blocks += (a.target[i].n + kColumns - 1) / kColumns;
   const long long units = std::min(a.units, a.tokens);
-  if (a.max_rank > 64 || 2ll * units * blocks * a.max_rank * a.k > kFusedBytes) return false;
+  if (a.max_rank > kFusedRank || 2ll * units * blocks * a.max_rank * a.k > kFusedBytes) return false;
   auto run = [&](auto* kernel, size_t lds) {
     hipLaunchKernelGGL(kernel, dim3(a.units, blocks, slots), dim3(kShrinkWaves * kWave),
                        lds + kGather * sizeof(int), stream, a);
   };
-  a.max_rank <= 16   ? run(lora_fused_kernel<1, 4>, sizeof(Stage<1>))
-  : a.max_rank <= 32 ? run(lora_fused_kernel<2, 4>, sizeof(Stage<2>))
-                     : run(lora_fused_kernel<4, 4>, sizeof(Stage<4>));
+  a.max_rank <= 16 ? run(lora_fused_kernel<1, 4>, sizeof(Stage<1>))
+                   : run(lora_fused_kernel<2, 4>, sizeof(Stage<2>));
   return true;
 }
 
@@ -656,15 +677,17 @@ void launch_lora(LoraArgs a, hipStream_t stream) {
     a.units = units_of(a.tokens, a.adapters);
     const int chunks = chunks_of(a.tokens), units = chunks * a.units;
     hipLaunchKernelGGL(lora_group_kernel, dim3(chunks), dim3(kChunk), 0, stream, a);
+    // x once for all rows of A, up to four tiles of them (6001 x 1536 at rank 64: in twos
+    // 21.2 us, in fours 15.4)
+    const int all = a.targets * rank_tiles;
     auto shrink = [&](auto* kernel, int tiles, size_t lds) {
-      hipLaunchKernelGGL(kernel, dim3(units, a.targets * ((rank_tiles + tiles - 1) / tiles),
-                                      kSet / kTile),
+      hipLaunchKernelGGL(kernel, dim3(units, (all + tiles - 1) / tiles, kSet / kTile),
                          dim3(kShrinkWaves * kWave), lds + kSet * sizeof(int), stream, a);
     };
-    rank_tiles == 1   ? shrink(lora_shrink_kernel<1, true>, 1, sizeof(Stage<1>))
-    : rank_tiles == 2 ? shrink(lora_shrink_kernel<2, true>, 2, sizeof(Stage<2>))
-                      : shrink(lora_shrink_kernel<4, true>, 4, sizeof(Stage<4>));
-    launch_expand<true>(a, units, 1, stream);
+    all == 1   ? shrink(lora_shrink_kernel<1, true>, 1, sizeof(Stage<1>))
+    : all == 2 ? shrink(lora_shrink_kernel<2, true>, 2, sizeof(Stage<2>))
+               : shrink(lora_shrink_kernel<4, true>, 4, sizeof(Stage<4>));
+    launch_expand<true>(a, units, 0, stream);
     return;
   }
   a.by_token = a.adapters + 1 > a.tokens;
