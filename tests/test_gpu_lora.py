@@ -68,7 +68,13 @@ CASES = [
     (16, 256, [128, 64], 32, 5), (17, 1000, [1000, 24, 24], 40, 3), (33, 1536, [1536, 256, 256], 16, 40),
     (64, 520, [513], 64, 1), (65, 136, [127, 129], 96, 7), (128, 896, [4864, 4864], 128, 6),
     (200, 72, [300], 104, 300), (257, 4864, [896], 48, 9), (1024, 64, [200], 8, 5),
-    (1025, 64, [200], 72, 2000), (1100, 328, [136], 16, 33)]
+    (1025, 64, [200], 72, 2000), (1100, 328, [136], 16, 33),
+    # one launch and two, around ranks of 16, 32 and 64; rows of A beyond four tiles, of
+    # several targets in one; K around a chunk's columns
+    (3, 1024, [1025], 16, 2), (3, 1032, [1023], 32, 2), (7, 512, [65], 40, 2),
+    (256, 520, [70], 32, 1), (256, 2056, [40, 50, 60], 24, 255), (300, 64, [40, 41, 42], 24, 5),
+    (700, 1544, [24, 300], 56, 3), (513, 504, [33, 8, 9], 128, 2), (290, 4096, [128], 32, 1),
+    (2050, 8, [16], 8, 700)]
 
 
 @pytest.mark.parametrize("runs", [False, True])
@@ -199,6 +205,20 @@ def test_thousands_of_tokens(batch, dev):
     batch.lora(d["x"], d["ids"], [(d["a"][0], d["b"][0], d["base"][0], out)],
                workspace(batch, 5003, 32, 1, dev), ranks=d["ranks"], scales=d["scales"])
     check(out, s, 0)
+
+
+@pytest.mark.parametrize("n,rank", [(9000, 8), (9001, 64), (8999, 72), (9008, 128)])
+def test_outputs_too_large_for_the_caches(batch, dev, n, rank):
+    """Beyond 96 MiB of bases and outputs; every 37th token is looked at."""
+    tokens = 3001
+    s = make(tokens, 72, [n], rank, 5, n, runs=True)
+    d, out = on(s, dev), torch.empty((tokens, n), dtype=torch.bfloat16, device=dev)
+    batch.lora(d["x"], d["ids"], [(d["a"][0], d["b"][0], d["base"][0], out)],
+               workspace(batch, tokens, rank, 1, dev), ranks=d["ranks"], scales=d["scales"])
+    some = slice(0, tokens, 37)
+    part = dict(s, x=s["x"][some], ids=s["ids"][some], base=[s["base"][0][some]])
+    check(out[some], part, 0)
+    assert not out.isnan().any()
 
 
 def test_offsets_past_32_bits(batch, dev):

@@ -102,7 +102,7 @@ def test_decode_form(paged, dev, n, longest, page, in_place):
 @pytest.mark.parametrize("in_place", [False, True])
 @pytest.mark.parametrize("n,longest,page,pad", [
     (1, 1, 16, 0), (1, 5000, 16, 3), (3, 17, 16, 0), (8, 3000, 32, 13), (64, 70, 64, 1),
-    (300, 40, 16, 5), (1023, 9, 256, 0), (2048, 12, 128, 7), (2049, 12, 16, 2), (5000, 6, 16, 0)])
+    (300, 40, 16, 5), (300, 900, 16, 5), (200, 2000, 32, 0), (257, 3, 16, 1), (1023, 9, 256, 0), (2048, 12, 128, 7), (2049, 12, 16, 2), (5000, 6, 16, 0)])
 def test_packed_form(paged, dev, n, longest, page, pad, in_place):
     table, free, count, lengths, added = case(n, longest, page, "packed", n + longest)
     check_assign(paged, dev, page, table, free, count, lengths, added, max(1, sum(added)) + pad,
@@ -181,7 +181,8 @@ def test_a_slice_of_a_wider_table(paged, dev):
 
 @pytest.mark.parametrize("in_place", [False, True])
 @pytest.mark.parametrize("n,longest,page", [(1, 0, 16), (1, 1, 16), (3, 50, 16), (64, 4000, 16),
-                                            (1024, 200, 128), (2100, 90, 32), (5, 100000, 16)])
+                                            (1024, 200, 128), (2100, 90, 32), (5, 100000, 16), (4096, 30, 16),
+                                            (4097, 30, 16)])
 def test_release(paged, dev, n, longest, page, in_place):
     g = gen(n)
     lengths = torch.randint(0, longest + 1, (n,), generator=g).tolist()

@@ -77,7 +77,8 @@ def settings(rows, seed):
 @pytest.mark.parametrize("rows,vocab", [
     (1, 1), (3, 2), (5, 7), (4, 8), (9, 63), (33, 257), (40, 1000), (64, 4095), (20, 8192),
     (20, 8193), (12, 32003), (7, 65536), (7, 65537), (6, 100000), (24, 151936), (3, 155649),
-    (2, 262147), (300, 901)])
+    (2, 262147), (300, 901),
+    (5, 16384), (5, 16385), (5, 32768), (5, 32769), (3, 106497), (3, 155648), (2, 1048576)])
 def test_settings_together(batch, dev, rows, vocab):
     logits, uniform = rows_of(rows, vocab, vocab)
     check(batch, dev, logits, uniform, **settings(rows, vocab))
@@ -144,6 +145,25 @@ def test_masked_tokens_are_never_taken(batch, dev, vocab):
     check(batch, dev, logits, uniform, **settings(12, 6))
     check(batch, dev, logits, uniform, temperature=[1e-30] * 4 + [INF] * 4 + [3e38] * 4)
     check(batch, dev, logits, uniform, top_k=[vocab] * 12, top_p=[0.9] * 12)
+
+
+@pytest.mark.parametrize("vocab", [9000, 40000, 151936, 300007])
+@pytest.mark.parametrize("mask", [-INF, torch.finfo(torch.bfloat16).min, -1e4, -100.0])
+def test_masks_by_region(batch, dev, vocab, mask):
+    """Masks of half of the row, of its first piece alone, of all but that, of every second
+    run, and thin ones that few lanes of a wave see."""
+    logits, uniform = rows_of(7, vocab, 13)
+    at = torch.arange(vocab)
+    logits[0, vocab // 2:] = mask
+    logits[1, :4096] = mask
+    logits[2, 4096:] = mask
+    logits[3, at // 512 % 2 == 0] = mask
+    logits[4, at % 512 < 33] = mask
+    logits[5, at % 16 == 3] = mask
+    logits[6, at % 8 < 7] = mask
+    check(batch, dev, logits, uniform)
+    check(batch, dev, logits, uniform, **settings(7, vocab))
+    check(batch, dev, logits, uniform, temperature=[1e3] * 7)
 
 
 def test_infinities_and_nan(batch, dev):
