@@ -111,11 +111,11 @@ def test_in_place_without_base_and_without_settings(batch, dev, tokens, k, n, ra
     assert (out.cpu()[s["ids"] < 0] == 0).all()
 
 
-def test_the_result_is_the_same_every_time_and_for_any_batch(batch, dev):
-    """Run to run, and a token's result with others beside it or not."""
-    s = make(300, 1536, [1000], 32, 5, 7)
+@pytest.mark.parametrize("tokens,rank", [(20, 16), (200, 64), (1500, 32)])
+def test_the_result_is_the_same_every_time(batch, dev, tokens, rank):
+    s = make(tokens, 1536, [1000], rank, 5, 7)
     d = on(s, dev)
-    ws = workspace(batch, 300, 32, 1, dev)
+    ws = workspace(batch, tokens, rank, 1, dev)
     outs = []
     for _ in range(3):
         out = torch.empty_like(d["base"][0])
@@ -254,10 +254,11 @@ def test_an_adapter_past_2_32_elements(batch, dev):
     assert ((out.cpu().double() - want).abs() <= tol).all()
 
 
-def test_captured_calls_follow_the_ids(batch, dev):
-    s = make(30, 256, [300, 40], 16, 6, 16)
+@pytest.mark.parametrize("tokens,rank", [(30, 16), (100, 64), (400, 16)])
+def test_captured_calls_follow_the_ids(batch, dev, tokens, rank):
+    s = make(tokens, 256, [300, 40], rank, 6, 16)
     d = on(s, dev)
-    ws = workspace(batch, 30, 16, 2, dev)
+    ws = workspace(batch, tokens, rank, 2, dev)
     out = [torch.empty_like(y) for y in d["base"]]
     targets = list(zip(d["a"], d["b"], d["base"], out))
     torch.cuda.synchronize()
@@ -266,8 +267,8 @@ def test_captured_calls_follow_the_ids(batch, dev):
         with torch.cuda.graph(graph, stream=side):
             batch.lora(d["x"], d["ids"], targets, ws, ranks=d["ranks"], scales=d["scales"])
     for step in range(4):
-        s["ids"] = torch.randint(-1, 6, (30,), generator=gen(step), dtype=torch.int32)
-        s["x"] = bf16((30, 256), gen(step + 50))
+        s["ids"] = torch.randint(-1, 6, (tokens,), generator=gen(step), dtype=torch.int32)
+        s["x"] = bf16((tokens, 256), gen(step + 50))
         d["ids"].copy_(s["ids"])
         d["x"].copy_(s["x"])
         graph.replay()
