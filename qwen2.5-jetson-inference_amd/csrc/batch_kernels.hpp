@@ -33,6 +33,7 @@ struct LoraArgs {
   int* groups;   // of more tokens than a workgroup gathers by itself
   int units;     // of the call, or of a chunk
   int by_token;  // a unit is a token that is the first with its adapter, not an adapter
+  int blocks;    // of columns, where a launch counts units and blocks together
 };
 
 struct SampleArgs {

@@ -123,7 +123,8 @@ __global__ __launch_bounds__(kChunk) void lora_group_kernel(LoraArgs a) {
   __shared__ int start[kPlaces], unit[kPlaces];
   __shared__ int wave_tokens[kWaves], wave_units[kWaves];
   const Groups out = groups_of(a);
-  const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int first = blockIdx.x * kChunk, t = first + threadIdx.x;
   for (int i = threadIdx.x; i < kPlaces; i += kChunk) {
     key[i] = -2;
@@ -154,27 +155,19 @@ __global__ __launch_bounds__(kChunk) void lora_group_kernel(LoraArgs a) {
   __syncthreads();
   const int n0 = size[2 * threadIdx.x], n1 = size[2 * threadIdx.x + 1];
   const int u0 = (n0 + kSet - 1) / kSet, u1 = (n1 + kSet - 1) / kSet;
-  int tokens = n0 + n1, units = u0 + u1;
-#pragma unroll
-  for (int d = 1; d < kWave; d *= 2) {
-    const int x = __shfl_up(tokens, d), y = __shfl_up(units, d);
-    if (lane >= d) {
-      tokens += x;
-      units += y;
-    }
-  }
+  int tokens = wave_scan(static_cast<unsigned>(n0 + n1));
+  int units = wave_scan(static_cast<unsigned>(u0 + u1));
   if (lane == kWave - 1) {
     wave_tokens[wave] = tokens;
     wave_units[wave] = units;
   }
   __syncthreads();
-  int all = 0;
-  for (int w = 0; w < kWaves; ++w) {
-    if (w < wave) {
-      tokens += wave_tokens[w];
-      units += wave_units[w];
-    }
-    all += wave_units[w];
+  const unsigned tokens_in = wave_scan(lane < kWaves ? unsigned(wave_tokens[lane]) : 0u);
+  const unsigned units_in = wave_scan(lane < kWaves ? unsigned(wave_units[lane]) : 0u);
+  const int all = __builtin_amdgcn_readlane(static_cast<int>(units_in), kWave - 1);
+  if (wave) {
+    tokens += __builtin_amdgcn_readlane(static_cast<int>(tokens_in), wave - 1);
+    units += __builtin_amdgcn_readlane(static_cast<int>(units_in), wave - 1);
   }
   start[2 * threadIdx.x] = tokens - n0 - n1;
   start[2 * threadIdx.x + 1] = tokens - n1;
@@ -480,9 +473,10 @@ __global__ __launch_bounds__(kExpandWaves * kWave) void lora_expand_kernel(LoraA
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int m = lane & 15, g = lane >> 4;
-  const Unit u = tokens_of<GROUPED>(a, blockIdx.x, list);
+  // neighbouring workgroups have neighbouring columns, where they can be counted so
+  const Unit u = tokens_of<GROUPED>(a, a.blocks ? blockIdx.x / a.blocks : blockIdx.x, list);
   if (u.count == 0) return;
-  int block = blockIdx.y * kExpandWaves + wave;
+  int block = (a.blocks ? blockIdx.x % a.blocks : blockIdx.y) * kExpandWaves + wave;
   const int c = target_of(a, J * 16, block);
   if (c < 0) return;
   const LoraTarget& t = a.target[c];
@@ -618,11 +612,14 @@ size_t lora_workspace_bytes(int tokens, int max_rank, int targets) {
   return bytes;
 }
 
-// Bytes of bases and outputs beyond which they are not left in the caches.
-constexpr long long kStreamBytes = 96ll << 20;
+// Bytes of bases and outputs beyond which they are not left in the caches (6001 tokens by
+// 8960, 215 MB, 67.1 -> 64.1 us; 3000 by 2 x 4864, 117 MB, whose bases still are there, 31.6 ->
+// 36.7).
+constexpr long long kStreamBytes = 192ll << 20;
+constexpr long long kMostWorkgroups = (1ll << 32) / (kExpandWaves * kWave) - 1;
 
 template <bool GROUPED>
-static void launch_expand(const LoraArgs& a, int units, int slots, hipStream_t stream) {
+static void launch_expand(LoraArgs a, int units, int slots, hipStream_t stream) {
   const int steps = rank_pitch(a.max_rank) / 32;
   long long bytes = 0;
   for (int i = 0; i < a.targets; ++i) bytes += 4ll * a.tokens * a.target[i].n;
@@ -633,19 +630,24 @@ static void launch_expand(const LoraArgs& a, int units, int slots, hipStream_t s
     // a unit's four tiles side by side where there would be few workgroups
     const long long few = static_cast<long long>((a.tokens + kSet - 1) / kSet) * blocks;
     const int z = !GROUPED ? slots : few >= 1024 ? 1 : few >= 512 ? 2 : kSet / kTile;
-    hipLaunchKernelGGL(kernel, dim3(units, blocks, z), dim3(kExpandWaves * kWave), 0, stream, a);
+    const bool flat = static_cast<long long>(units) * blocks <= kMostWorkgroups;
+    a.blocks = flat ? blocks : 0;
+    hipLaunchKernelGGL(kernel, flat ? dim3(units * blocks, 1, z) : dim3(units, blocks, z),
+                       dim3(kExpandWaves * kWave), 0, stream, a);
   };
-  if (GROUPED && bytes > kStreamBytes) {
-    steps == 1   ? run(lora_expand_kernel<1, 8, GROUPED, true>, 128)
-    : steps == 2 ? run(lora_expand_kernel<2, 8, GROUPED, true>, 128)
-    : steps == 3 ? run(lora_expand_kernel<3, 4, GROUPED, true>, 64)
-                 : run(lora_expand_kernel<4, 4, GROUPED, true>, 64);
-  } else {
-    steps == 1   ? run(lora_expand_kernel<1, 8, GROUPED, false>, 128)
-    : steps == 2 ? run(lora_expand_kernel<2, 4, GROUPED, false>, 64)
-    : steps == 3 ? run(lora_expand_kernel<3, 4, GROUPED, false>, 64)
-                 : run(lora_expand_kernel<4, 4, GROUPED, false>, 64);
+  if constexpr (GROUPED) {
+    if (bytes > kStreamBytes) {
+      steps == 1   ? run(lora_expand_kernel<1, 8, true, true>, 128)
+      : steps == 2 ? run(lora_expand_kernel<2, 8, true, true>, 128)
+      : steps == 3 ? run(lora_expand_kernel<3, 4, true, true>, 64)
+                   : run(lora_expand_kernel<4, 4, true, true>, 64);
+      return;
+    }
   }
+  steps == 1   ? run(lora_expand_kernel<1, 8, GROUPED, false>, 128)
+  : steps == 2 ? run(lora_expand_kernel<2, 4, GROUPED, false>, 64)
+  : steps == 3 ? run(lora_expand_kernel<3, 4, GROUPED, false>, 64)
+               : run(lora_expand_kernel<4, 4, GROUPED, false>, 64);
 }
 
 // The largest rank of the one launch (64 spills registers: 64 x 896 x 896 16.3 us, in two
