@@ -102,12 +102,21 @@ def lora(x, ids, targets, workspace, ranks=None, scales=None, stream=None) -> No
     made = []
     for a, b, base, output in targets:
         n = output.shape[-1]
+        # contiguous, as a rule: looked at without a call for each
+        if (base is not None and a.dtype is _BF16 and a.get_device() == index and a.shape == shape
+                and a.is_contiguous() and b.dtype is _BF16 and b.get_device() == index
+                and b.shape == (adapters, n, rank) and b.is_contiguous()
+                and base.dtype is _BF16 and base.get_device() == index
+                and base.shape == (tokens, n) and base.is_contiguous()
+                and output.dtype is _BF16 and output.get_device() == index
+                and output.dim() == 2 and output.shape[0] == tokens and output.is_contiguous()):
+            made += (a.data_ptr(), b.data_ptr(), base.data_ptr(), output.data_ptr(), n, n, n)
+            continue
         if a.shape != shape or b.shape != (adapters, n, rank):
             _bad(f"a must be {list(shape)} and b {[adapters, n, rank]} (got {list(a.shape)}, "
                  f"{list(b.shape)})")
         op, os_ = _rows(output, tokens, n, index, "output")
-        bp, bs = (0, 0) if base is None else (op, os_) if base is output else _rows(
-            base, tokens, n, index, "base")
+        bp, bs = (0, 0) if base is None else _rows(base, tokens, n, index, "base")
         made += (_flat(a, _BF16, None, index, "a"), _flat(b, _BF16, None, index, "b"), bp, op, n,
                  bs, os_)
     status = load().infer_hip_lora_bf16(

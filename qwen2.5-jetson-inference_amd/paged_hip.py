@@ -261,8 +261,9 @@ def kv_pages_plan_workspace_bytes(num_sequences: int) -> int:
     return load().infer_hip_kv_pages_plan_workspace_bytes(num_sequences)
 
 
-def _plan(table, free, free_count, lengths, lengths_out, free_count_out, workspace, stream):
-    """What both operators take: (GPU, stream, their first pointers and sizes)."""
+def _plan_table(table, stream):
+    """(GPU, stream, pointer, rows, columns, distance of rows) of a plan's table,
+    which may be a slice of a wider one."""
     index, handle = _here(table, "block table", stream)
     if table.dtype is not _I32 or table.dim() != 2:
         _bad("block table must be int32 [sequences, pages]")
@@ -270,14 +271,7 @@ def _plan(table, free, free_count, lengths, lengths_out, free_count_out, workspa
     stride, inner = table.stride()
     if inner != 1 and width > 1:
         _bad("block table rows must be contiguous")
-    fc = _flat(free_count, _I32, 1, index, "free_count")
-    ln = _flat(lengths, _I32, rows, index, "lengths")
-    return (index, handle, rows, (table.data_ptr(), rows, width, stride if rows > 1 else width),
-            (_flat(free, _I32, None, index, "free"), free.numel(), fc,
-             fc if free_count_out is None else _flat(free_count_out, _I32, 1, index,
-                                                     "free_count_out"), ln),
-            ln if lengths_out is None else _flat(lengths_out, _I32, rows, index, "lengths_out"),
-            _flat(workspace, _U8, None, index, "workspace"))
+    return index, handle, table.data_ptr(), rows, width, stride if rows > 1 else width
 
 
 def kv_pages_assign(table, page_size: int, free, free_count, lengths, added, workspace, positions,
@@ -290,16 +284,35 @@ def kv_pages_assign(table, page_size: int, free, free_count, lengths, added, wor
     and sequences int32 [tokens], slots int64 [tokens], starts int32
     [sequences + 1], lengths_out and free_count_out (None: in place).
     sequences None: token s belongs to sequence s."""
-    index, handle, n, tab, pool, lo, ws = _plan(table, free, free_count, lengths, lengths_out,
-                                                free_count_out, workspace, stream)
+    index, on, tp, n, width, stride = _plan_table(table, stream)
+    if lengths_out is None:
+        lengths_out = lengths
+    if free_count_out is None:
+        free_count_out = free_count
     tokens = positions.numel()
-    _check(load().infer_hip_kv_pages_assign(
-        *tab, page_size, *pool, _flat(added, _I32, n, index, "added"), lo, tokens,
-        _flat(positions, _I32, None, index, "positions"),
+    # what every call has, looked at without a call for each
+    if not (lengths.dtype is _I32 and lengths.get_device() == index and lengths.numel() == n
+            and lengths.is_contiguous() and added.dtype is _I32 and added.get_device() == index
+            and added.numel() == n and added.is_contiguous() and lengths_out.dtype is _I32
+            and lengths_out.get_device() == index and lengths_out.numel() == n
+            and lengths_out.is_contiguous() and positions.dtype is _I32
+            and positions.get_device() == index and positions.is_contiguous()
+            and free.dtype is _I32 and free.get_device() == index and free.is_contiguous()):
+        for t, count, name in ((lengths, n, "lengths"), (added, n, "added"),
+                               (lengths_out, n, "lengths_out"), (positions, None, "positions"),
+                               (free, None, "free")):
+            _flat(t, _I32, count, index, name)
+    status = load().infer_hip_kv_pages_assign(
+        tp, n, width, stride, page_size, free.data_ptr(), free.numel(),
+        _flat(free_count, _I32, 1, index, "free_count"),
+        _flat(free_count_out, _I32, 1, index, "free_count_out"), lengths.data_ptr(),
+        added.data_ptr(), lengths_out.data_ptr(), tokens, positions.data_ptr(),
         None if sequences is None else _flat(sequences, _I32, tokens, index, "sequences"),
         None if slots is None else _flat(slots, _I64, tokens, index, "slots"),
-        None if starts is None else _flat(starts, _I32, n + 1, index, "starts"), ws,
-        workspace.numel(), handle))
+        None if starts is None else _flat(starts, _I32, n + 1, index, "starts"),
+        _flat(workspace, _U8, None, index, "workspace"), workspace.numel(), on)
+    if status:
+        _check(status)
 
 
 def kv_pages_release(table, page_size: int, free, free_count, lengths, finished, workspace,
@@ -307,8 +320,14 @@ def kv_pages_release(table, page_size: int, free, free_count, lengths, finished,
     """The pages of the sequences with finished[s] != 0 (int32 [sequences]) back
     onto free (infer_hip_kv_pages_release); the other arguments are
     kv_pages_assign's."""
-    index, handle, n, tab, pool, lo, ws = _plan(table, free, free_count, lengths, lengths_out,
-                                                free_count_out, workspace, stream)
-    _check(load().infer_hip_kv_pages_release(
-        *tab, page_size, *pool, _flat(finished, _I32, n, index, "finished"), lo, ws,
-        workspace.numel(), handle))
+    index, on, tp, n, width, stride = _plan_table(table, stream)
+    fc, ln = (_flat(free_count, _I32, 1, index, "free_count"),
+              _flat(lengths, _I32, n, index, "lengths"))
+    status = load().infer_hip_kv_pages_release(
+        tp, n, width, stride, page_size, _flat(free, _I32, None, index, "free"), free.numel(), fc,
+        fc if free_count_out is None else _flat(free_count_out, _I32, 1, index, "free_count_out"),
+        ln, _flat(finished, _I32, n, index, "finished"),
+        ln if lengths_out is None else _flat(lengths_out, _I32, n, index, "lengths_out"),
+        _flat(workspace, _U8, None, index, "workspace"), workspace.numel(), on)
+    if status:
+        _check(status)

@@ -188,3 +188,85 @@ def test_sample_binding_refuses_cpu_tensors(hip, batch):
     x = torch.zeros((2, 64), dtype=torch.bfloat16)
     with pytest.raises(hip.InferError, match="GPU"):
         batch.sample(x, torch.zeros(2), torch.zeros(2, dtype=torch.int32), x)
+
+
+# ------------------------------------------------------------------ bindings --
+
+class Accepts:
+    """In the library's place: every call is taken."""
+    def __getattr__(self, name):
+        return lambda *args: 0
+
+
+def bound_calls(batch, paged, dev):
+    """(binding, arguments) of sound calls whose tensors are on `dev`."""
+    def i(*shape):
+        return torch.zeros(shape, dtype=torch.int32, device=dev)
+
+    def f(*shape):
+        return torch.zeros(shape, dtype=torch.float32, device=dev)
+
+    def w(*shape):
+        return torch.zeros(shape, dtype=torch.bfloat16, device=dev)
+
+    u8 = torch.zeros(1 << 20, dtype=torch.uint8, device=dev)
+    yield paged.kv_pages_assign, dict(
+        table=i(3, 4), page_size=16, free=i(9), free_count=i(1), lengths=i(3), added=i(3),
+        workspace=u8, positions=i(7), sequences=i(7), slots=i(7).long(), starts=i(4),
+        lengths_out=i(3), free_count_out=i(1))
+    yield paged.kv_pages_release, dict(
+        table=i(3, 4), page_size=16, free=i(9), free_count=i(1), lengths=i(3), finished=i(3),
+        workspace=u8, lengths_out=i(3), free_count_out=i(1))
+    yield batch.sample, dict(
+        logits=w(3, 50), uniform=f(3), tokens=i(3), workspace=u8, temperature=f(3), top_k=i(3),
+        top_p=f(3), min_p=f(3), probabilities=f(3))
+
+    def lora(x, ids, a, b, base, output, workspace, ranks, scales):
+        batch.lora(x, ids, [(a, b, base, output)], workspace, ranks=ranks, scales=scales)
+    yield lora, dict(x=w(5, 64), ids=i(5), a=w(2, 8, 64), b=w(2, 40, 8), base=w(5, 40),
+                     output=w(5, 40), workspace=u8, ranks=i(2), scales=f(2))
+
+
+def test_bindings_refuse_other_types_counts_and_strides(hip, batch, paged, monkeypatch):
+    for module in (batch, paged):
+        monkeypatch.setattr(module, "load", Accepts)
+        monkeypatch.setattr(module, "_here", lambda t, name, stream: (t.get_device(), 0))
+    for call, args in bound_calls(batch, paged, "cpu"):
+        call(**args)
+        for name, t in args.items():
+            if not isinstance(t, torch.Tensor):
+                continue
+            bad = [t.short(), t.double()]
+            if name not in ("free", "positions", "workspace"):  # their size is the call's
+                bad.append(torch.cat([t, t]))
+            if t.numel() > 1:  # every second element
+                bad.append(torch.cat([t, t], dim=-1)[..., ::2])
+            if name == "table":  # any shape of two dimensions
+                bad = [t.short(), t.double(), t[0], torch.cat([t, t], dim=-1)[..., ::2]]
+            for k, other in enumerate(bad):
+                with pytest.raises(hip.InferError):
+                    call(**{**args, name: other})
+                    pytest.fail(f"{call.__name__}: {name}, {k}")
+
+
+def test_bindings_refuse_numbers_of_targets(hip, batch, monkeypatch):
+    monkeypatch.setattr(batch, "load", Accepts)
+    monkeypatch.setattr(batch, "_here", lambda t, name, stream: (t.get_device(), 0))
+
+    def w(*shape):
+        return torch.zeros(shape, dtype=torch.bfloat16)
+    target = (w(2, 8, 64), w(2, 40, 8), w(5, 40), w(5, 40))
+    args = (w(5, 64), torch.zeros(5, dtype=torch.int32))
+    for targets in ([], [target] * 4, [target, (w(2, 16, 64), w(2, 40, 16)) + target[2:]]):
+        with pytest.raises(hip.InferError):
+            batch.lora(*args, targets, torch.zeros(64, dtype=torch.uint8))
+
+
+@pytest.mark.gpu
+def test_bindings_refuse_tensors_of_the_host(hip, batch, paged, dev):
+    """After every other check of theirs has passed without a GPU."""
+    for call, args in bound_calls(batch, paged, dev):
+        for name, t in args.items():
+            if isinstance(t, torch.Tensor):
+                with pytest.raises(hip.InferError):
+                    call(**{**args, name: t.cpu()})
