@@ -483,6 +483,10 @@ __device__ __forceinline__ uint32_t larger_words(uint32_t a, uint32_t b) {
   return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a),
                                                                  __builtin_bit_cast(u16x2, b)));
 }
+__device__ __forceinline__ uint32_t add_words(uint32_t a, uint32_t b) {
+  return __builtin_bit_cast(uint32_t,
+                            __builtin_bit_cast(u16x2, a) + __builtin_bit_cast(u16x2, b));
+}
 __device__ __forceinline__ uint32_t smaller_words(uint32_t a, uint32_t b) {
   return __builtin_bit_cast(uint32_t, __builtin_elementwise_min(__builtin_bit_cast(u16x2, a),
                                                                  __builtin_bit_cast(u16x2, b)));
@@ -530,6 +534,17 @@ struct Pieces {
     u32x4 y = x[i];
     asm volatile("" : "+v"(y)::"memory");
     return y;
+  }
+  // Piece i, a number that the wave shares: by halves, as a jump over each piece's copy
+  // would fetch the code of all.
+  template <int from = 0, int to = NR>
+  __device__ __forceinline__ u32x4 pick(int i) const {
+    if constexpr (to - from == 1) {
+      return get(from);
+    } else {
+      constexpr int middle = (from + to) / 2;
+      return i < middle ? pick<from, middle>(i) : pick<middle, to>(i);
+    }
   }
 };
 
@@ -825,16 +840,19 @@ __device__ __forceinline__ bool locate(const SampleArgs& a, int row, const RowSp
                                        const Pick& pick, unsigned& nth, CountLds& lds) {
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  // Which of the eight words of piece i have it.
+  auto live = [&](int i) {
+    return first + i * kThreads + static_cast<int>(threadIdx.x) < last;
+  };
+  // Which of the eight words of piece i, any number that the wave shares, have it.
   auto words = [&](int i) {
     unsigned m = 0;
-    const u32x4 x = p.get(i);
+    const u32x4 x = p.pick(i);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const uint32_t d = v.differs(x[j]);
       m |= (d & 0xFFFFu ? 0u : 1u << 2 * j) | (d >> 16 ? 0u : 2u << 2 * j);
     }
-    return first + i * kThreads + static_cast<int>(threadIdx.x) < last ? m : 0u;
+    return live(i) ? m : 0u;
   };
   auto take = [&](int i, unsigned m, unsigned skip) {
     for (; skip; --skip) m &= m - 1;
@@ -843,26 +861,38 @@ __device__ __forceinline__ bool locate(const SampleArgs& a, int row, const RowSp
            pick.probability);
   };
   constexpr int kPart = 4;  // pieces looked at together
+  int hit = -1;
 #pragma unroll
   for (int k = 0; k < NR; k += kPart) {
     uint32_t least = 0xFFFFFFFFu;
 #pragma unroll
     for (int i = k; i < NR && i < k + kPart; ++i) {
-      const u32x4 x = p.get(i);
-      const uint32_t here =
-          smaller_words(smaller_words(v.differs(x[0]), v.differs(x[1])),
-                        smaller_words(v.differs(x[2]), v.differs(x[3])));
-      least = smaller_words(least, here);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) least = smaller_words(least, v.differs(p.x[i][j]));
     }
     if (!__ballot(min(least & 0xFFFFu, least >> 16) == 0)) continue;
 #pragma unroll
     for (int i = k; i < NR && i < k + kPart; ++i) {
-      const unsigned m = words(i);
-      if (m && pick.count == 1) take(i, m, 0);  // no other
-      if (m) atomicAdd(&lds.found[i], static_cast<unsigned>(__popc(m)));
+      const u32x4 x = p.get(i);
+      uint32_t others = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) others = add_words(others, smaller_words(v.differs(x[j]), 0x10001u));
+      const unsigned n = 8 - (others & 0xFFFFu) - (others >> 16);
+      if (n && live(i)) {
+        atomicAdd(&lds.found[i], n);
+        hit = i;
+      }
     }
   }
-  if (pick.count == 1) return false;
+  if (pick.count == 1) {  // no other
+    const unsigned long long has = __ballot(hit >= 0);
+    if (has) {
+      const int at = __builtin_amdgcn_readlane(hit, __builtin_ctzll(has));
+      const unsigned m = words(at);
+      if (m) take(at, m, 0);
+    }
+    return false;
+  }
   lds_barrier();
   const unsigned n = lane < NR ? lds.found[lane] : 0u, in = wave_scan(n);
   const unsigned long long past = __ballot(in > nth);
@@ -872,11 +902,7 @@ __device__ __forceinline__ bool locate(const SampleArgs& a, int row, const RowSp
   }
   const int at = __builtin_ctzll(past);
   nth -= at_lane(in, at) - at_lane(n, at);
-  unsigned m = 0;
-#pragma unroll
-  for (int i = 0; i < NR; ++i) {
-    if (i == at) m = words(i);
-  }
+  const unsigned m = words(at);
   const unsigned mine_in = wave_scan(static_cast<unsigned>(__popc(m)));
   if (lane == kWave - 1) lds.wave_count[wave] = mine_in;
   lds_barrier();
