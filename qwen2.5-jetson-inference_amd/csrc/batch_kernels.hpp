@@ -34,6 +34,7 @@ struct LoraArgs {
   int units;     // of the call, or of a chunk
   int by_token;  // a unit is a token that is the first with its adapter, not an adapter
   int blocks;    // of columns, where a launch counts units and blocks together
+  int parts;     // of K, each with sums in 32 bits: float [parts][targets][tokens][rank_pitch]
 };
 
 struct SampleArgs {

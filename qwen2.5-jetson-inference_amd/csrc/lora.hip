@@ -34,6 +34,8 @@ constexpr int kGather = 256;    // tokens
 constexpr int kChunk = 1024;    // tokens grouped together beyond
 constexpr int kSet = 64;        // tokens of a unit then, at most
 constexpr int kExpandWaves = 4;
+constexpr int kMostParts = 4;     // of K
+constexpr int kPartColumns = 768;
 
 // Words of a token's high (and low) part in the workspace: whole steps of the MFMA's K.
 __host__ __device__ constexpr int rank_pitch(int max_rank) { return (max_rank + 31) / 32 * 32; }
@@ -106,11 +108,6 @@ __device__ __forceinline__ Unit grouped_tokens(const LoraArgs& a, int unit, int*
   if (t < v.z) list[t] = token;
   __syncthreads();
   return u;
-}
-
-template <bool GROUPED>
-__device__ __forceinline__ Unit tokens_of(const LoraArgs& a, int unit, int* list) {
-  return GROUPED ? grouped_tokens(a, unit, list) : gather_tokens(a, unit, list);
 }
 
 // A chunk's tokens by adapter: a table of the chunk's adapters in LDS (twice as many
@@ -226,13 +223,14 @@ struct Stage {
   };
 };
 
-// rows: those of A that the wave loads, row `wave` of each tile, and its token's x.
+// rows: those of A that the wave loads, row `wave` of each tile, and its token's x, from
+// the first of `columns` on.
 template <int RT>
-__device__ __forceinline__ void shrink_tile(f32x4_t (&sum)[RT], const LoraArgs& a,
+__device__ __forceinline__ void shrink_tile(f32x4_t (&sum)[RT], int columns,
                                             const uint16_t* const (&rows)[RT + 1],
                                             Stage<RT>& stage, int wave, int lane) {
   typedef Stage<RT> S;
-  const int chunks = (a.k + S::kColumns - 1) / S::kColumns;
+  const int chunks = (columns + S::kColumns - 1) / S::kColumns;
   uint4 v[S::kDepth][RT + 1][S::kLoads];
   auto load = [&](uint4 (&to)[RT + 1][S::kLoads], int chunk) {
 #pragma unroll
@@ -241,7 +239,7 @@ __device__ __forceinline__ void shrink_tile(f32x4_t (&sum)[RT], const LoraArgs& 
       for (int j = 0; j < S::kLoads; ++j) {
         const int k = chunk * S::kColumns + 512 * j + 8 * lane;
         to[i][j] = make_uint4(0, 0, 0, 0);
-        if (k < a.k) to[i][j] = load_global16(rows[i] + k);
+        if (k < columns) to[i][j] = load_global16(rows[i] + k);
       }
     }
   };
@@ -320,14 +318,14 @@ __device__ __forceinline__ void stage_rows(const uint16_t* (&rows)[RT + 1], cons
   }
 }
 
-template <int RT, bool GROUPED>
+template <int RT>
 __global__ __launch_bounds__(kShrinkWaves * kWave) void lora_shrink_kernel(LoraArgs a) {
   extern __shared__ __align__(16) char shared[];
   Stage<RT>& stage = *reinterpret_cast<Stage<RT>*>(shared);
   int* const list = reinterpret_cast<int*>(shared + sizeof(Stage<RT>));
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const Unit u = tokens_of<GROUPED>(a, blockIdx.x, list);
+  const Unit u = grouped_tokens(a, blockIdx.x, list);
   if (u.count == 0 || u.rank == 0) return;
   const int tiles = (a.max_rank + kTile - 1) / kTile, first = blockIdx.y * RT;
   const int pitch = rank_pitch(a.max_rank);
@@ -337,7 +335,7 @@ __global__ __launch_bounds__(kShrinkWaves * kWave) void lora_shrink_kernel(LoraA
     const int token = list[min(tile * kTile + wave, u.count - 1)];
     rows[RT] = a.x + token * a.x_stride;
     f32x4_t sum[RT];
-    shrink_tile<RT>(sum, a, rows, stage, wave, lane);
+    shrink_tile<RT>(sum, a.k, rows, stage, wave, lane);
     for (int e = threadIdx.x; e < RT * kTile * kTile; e += kShrinkWaves * kWave) {
       const float h = joined<RT>(stage, e);
       const int q = first + row_of(e) / kTile, c = q / tiles;
@@ -349,6 +347,40 @@ __global__ __launch_bounds__(kShrinkWaves * kWave) void lora_shrink_kernel(LoraA
         to[0] = high;
         to[pitch] = low;
       }
+    }
+  }
+}
+
+// Of up to kGather tokens, where units are few: A x in a.parts of K, one to a workgroup, each
+// written in 32 bits; B h adds them up.
+__host__ __device__ inline int part_columns(const LoraArgs& a) {
+  return ((a.k + a.parts - 1) / a.parts + 63) / 64 * 64;
+}
+
+__global__ __launch_bounds__(kShrinkWaves * kWave) void lora_shrink_part_kernel(LoraArgs a) {
+  extern __shared__ __align__(16) char shared[];
+  Stage<1>& stage = *reinterpret_cast<Stage<1>*>(shared);
+  int* const list = reinterpret_cast<int*>(shared + sizeof(Stage<1>));
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const Unit u = gather_tokens(a, blockIdx.x, list);
+  if (u.count == 0 || u.rank == 0) return;
+  const int tiles = (a.max_rank + kTile - 1) / kTile;
+  const int part = blockIdx.y % a.parts, q = blockIdx.y / a.parts;
+  const int from = part * part_columns(a), columns = min(part_columns(a), a.k - from);
+  const int pitch = rank_pitch(a.max_rank);
+  const uint16_t* rows[2];
+  stage_rows<1>(rows, a, u.adapter, q, wave);
+  rows[0] += from;
+  float* const h = reinterpret_cast<float*>(a.h) +
+                   (static_cast<size_t>(part) * a.targets + q / tiles) * a.tokens * pitch;
+  for (int tile = blockIdx.z; tile * kTile < u.count; tile += gridDim.z) {
+    rows[1] = a.x + list[min(tile * kTile + wave, u.count - 1)] * a.x_stride + from;
+    f32x4_t sum[1];
+    shrink_tile<1>(sum, columns, rows, stage, wave, lane);
+    const int e = threadIdx.x, at = tile * kTile + token_of(e);
+    if (e < kTile * kTile && at < u.count) {
+      h[static_cast<size_t>(list[at]) * pitch + q % tiles * kTile + row_of(e)] = joined<1>(stage, e);
     }
   }
 }
@@ -467,14 +499,14 @@ __device__ __forceinline__ int target_of(const LoraArgs& a, int columns, int& bl
   return -1;
 }
 
-template <int KS, int J, bool GROUPED, bool ONCE>
+template <int KS, int J, bool ONCE>
 __global__ __launch_bounds__(kExpandWaves * kWave) void lora_expand_kernel(LoraArgs a) {
-  __shared__ int list[GROUPED ? kSet : kGather];
+  __shared__ int list[kSet];
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int m = lane & 15, g = lane >> 4;
   // neighbouring workgroups have neighbouring columns, where they can be counted so
-  const Unit u = tokens_of<GROUPED>(a, a.blocks ? blockIdx.x / a.blocks : blockIdx.x, list);
+  const Unit u = grouped_tokens(a, a.blocks ? blockIdx.x / a.blocks : blockIdx.x, list);
   if (u.count == 0) return;
   int block = (a.blocks ? blockIdx.x % a.blocks : blockIdx.y) * kExpandWaves + wave;
   const int c = target_of(a, J * 16, block);
@@ -524,6 +556,106 @@ __global__ __launch_bounds__(kExpandWaves * kWave) void lora_expand_kernel(LoraA
   }
 }
 
+// B h from the parts of h: a workgroup's waves add them up in the order of the parts, once
+// for all, into LDS.
+template <int KS, int J>
+__global__ __launch_bounds__(kExpandWaves * kWave) void lora_expand_parts_kernel(LoraArgs a) {
+  constexpr int kPitch = 32 * KS, kThreads = kExpandWaves * kWave;
+  constexpr int kFours = kTile * kPitch / 4, kMine = (kFours + kThreads - 1) / kThreads;
+  __shared__ int list[kGather];
+  __shared__ __align__(16) uint16_t h[2][2][kTile][kPitch + 8];
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int m = lane & 15, g = lane >> 4;
+  const Unit u = gather_tokens(a, blockIdx.x / a.blocks, list);
+  if (u.count == 0) return;
+  int block = blockIdx.x % a.blocks;
+  const int c = target_of(a, kExpandWaves * J * 16, block);
+  const LoraTarget& t = a.target[c];
+  if (u.adapter < 0 && t.base == t.out) return;
+  block = block * kExpandWaves + wave;
+  const bool has = block * J * 16 < t.n;
+  // A tile's parts and bases are loaded while the one before it is computed.
+  struct Tile {
+    f32x4_t part[kMine][kMostParts];
+    typename Words<J>::type base[4];
+  };
+  auto load_parts = [&](Tile& v, int tile) {
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int e = i * kThreads + threadIdx.x, row = e % (kPitch / 4) * 4;
+      const int token = list[min(tile * kTile + e / (kPitch / 4) % kTile, u.count - 1)];
+      const float* from = reinterpret_cast<const float*>(a.h) +
+                          (static_cast<size_t>(c) * a.tokens + token) * kPitch + row;
+#pragma unroll
+      for (int p = 0; p < kMostParts; ++p) {
+        v.part[i][p] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+        if (p < a.parts && row < u.rank) {
+          v.part[i][p] = *(const QLIN_GLOBAL f32x4_t*)(
+              from + static_cast<size_t>(p) * a.targets * a.tokens * kPitch);
+        }
+      }
+    }
+  };
+  auto load_base = [&](Tile& v, const auto& columns, int tile) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v.base[i] = columns.base_of(list[min(tile * kTile + 4 * g + i, u.count - 1)]);
+    }
+  };
+  const int step = gridDim.z;
+  int tile = blockIdx.z;
+  if (tile * kTile >= u.count) return;
+  Tile now, next;
+  load_parts(next, tile);
+  Columns<KS, J, false> columns(a, t, has ? block : 0, u, lane);
+  load_base(next, columns, tile);
+  columns.cut(lane);
+  for (int turn = 0; tile * kTile < u.count; tile += step, turn ^= 1) {
+    now = next;
+    if ((tile + step) * kTile < u.count) {
+      load_parts(next, tile + step);
+      load_base(next, columns, tile + step);
+    }
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int e = i * kThreads + threadIdx.x, row = e % (kPitch / 4) * 4;
+      uint16_t high[4], low[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        float sum = now.part[i][0][k];
+#pragma unroll
+        for (int p = 1; p < kMostParts; ++p) {
+          if (p < a.parts) sum += now.part[i][p][k];
+        }
+        split_word(row + k < u.rank ? sum * u.scale : 0.0f, high[k], low[k]);
+      }
+      if (kFours % kThreads == 0 || e < kFours) {
+        uint16_t* to = &h[turn][0][e / (kPitch / 4)][row];
+        *reinterpret_cast<uint2*>(to) = make_uint2(high[0] | high[1] << 16, high[2] | high[3] << 16);
+        *reinterpret_cast<uint2*>(to + kTile * (kPitch + 8)) =
+            make_uint2(low[0] | low[1] << 16, low[2] | low[3] << 16);
+      }
+    }
+    lds_barrier();
+    uint4 high[KS], low[KS];
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      high[s] = *reinterpret_cast<const uint4*>(&h[turn][0][m][32 * s + 8 * g]);
+      low[s] = *reinterpret_cast<const uint4*>(&h[turn][1][m][32 * s + 8 * g]);
+    }
+    f32x4_t sum[J];
+    columns.multiply(sum, high, low);
+    if (has) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int at = tile * kTile + 4 * g + i;
+        if (at < u.count) columns.store(list[at], sum, i, now.base[i]);
+      }
+    }
+  }
+}
+
 // Both products in one launch, for calls so small that it is launches and round trips
 // they wait for: a workgroup takes 16 waves' columns of a unit's target and computes
 // the unit's h for itself, in LDS.  A is read once for each such workgroup, from L2 as
@@ -561,7 +693,7 @@ __global__ __launch_bounds__(kShrinkWaves * kWave) void lora_fused_kernel(LoraAr
     if (u.rank) {
       f32x4_t sum[RT];
       rows[RT] = a.x + list[min(tile * kTile + wave, u.count - 1)] * a.x_stride;
-      shrink_tile<RT>(sum, a, rows, stage, wave, lane);
+      shrink_tile<RT>(sum, a.k, rows, stage, wave, lane);
       for (int e = threadIdx.x; e < RT * kTile * kTile; e += kShrinkWaves * kWave) {
         const int row = row_of(e);
         uint16_t* to = &h[0][token_of(e)][row];
@@ -596,6 +728,7 @@ int units_of(int tokens, int adapters) {  // of a chunk
   return (kChunk + kSet - 1) / kSet + std::min(std::min(tokens, kChunk), adapters + 1);
 }
 
+// Of h as two BF16 numbers, or as one part in 32 bits.
 size_t h_bytes(int tokens, int max_rank, int targets) {
   return static_cast<size_t>(targets) * tokens * 4 * rank_pitch(max_rank);
 }
@@ -603,13 +736,12 @@ size_t h_bytes(int tokens, int max_rank, int targets) {
 }  // namespace
 
 size_t lora_workspace_bytes(int tokens, int max_rank, int targets) {
-  size_t bytes = h_bytes(tokens, max_rank, targets);
-  if (tokens > kGather) {
-    const size_t chunks = chunks_of(tokens);
-    bytes += 4 * ((static_cast<size_t>(tokens) + 3) / 4 * 4) +
-             16 * chunks * units_of(tokens, kChunk);
-  }
-  return bytes;
+  const size_t parts = kMostParts * h_bytes(std::min(tokens, kGather), max_rank, targets);
+  if (tokens <= kGather) return parts;
+  const size_t chunks = chunks_of(tokens);
+  return std::max(parts, h_bytes(tokens, max_rank, targets) +
+                             4 * ((static_cast<size_t>(tokens) + 3) / 4 * 4) +
+                             16 * chunks * units_of(tokens, kChunk));
 }
 
 // Bytes of bases and outputs beyond which they are not left in the caches (6001 tokens by
@@ -618,8 +750,7 @@ size_t lora_workspace_bytes(int tokens, int max_rank, int targets) {
 constexpr long long kStreamBytes = 192ll << 20;
 constexpr long long kMostWorkgroups = (1ll << 32) / (kExpandWaves * kWave) - 1;
 
-template <bool GROUPED>
-static void launch_expand(LoraArgs a, int units, int slots, hipStream_t stream) {
+static void launch_expand(LoraArgs a, int units, hipStream_t stream) {
   const int steps = rank_pitch(a.max_rank) / 32;
   long long bytes = 0;
   for (int i = 0; i < a.targets; ++i) bytes += 4ll * a.tokens * a.target[i].n;
@@ -629,25 +760,48 @@ static void launch_expand(LoraArgs a, int units, int slots, hipStream_t stream) 
     blocks = (blocks + kExpandWaves - 1) / kExpandWaves;
     // a unit's four tiles side by side where there would be few workgroups
     const long long few = static_cast<long long>((a.tokens + kSet - 1) / kSet) * blocks;
-    const int z = !GROUPED ? slots : few >= 1024 ? 1 : few >= 512 ? 2 : kSet / kTile;
+    const int z = few >= 1024 ? 1 : few >= 512 ? 2 : kSet / kTile;
     const bool flat = static_cast<long long>(units) * blocks <= kMostWorkgroups;
     a.blocks = flat ? blocks : 0;
     hipLaunchKernelGGL(kernel, flat ? dim3(units * blocks, 1, z) : dim3(units, blocks, z),
                        dim3(kExpandWaves * kWave), 0, stream, a);
   };
-  if constexpr (GROUPED) {
-    if (bytes > kStreamBytes) {
-      steps == 1   ? run(lora_expand_kernel<1, 8, true, true>, 128)
-      : steps == 2 ? run(lora_expand_kernel<2, 8, true, true>, 128)
-      : steps == 3 ? run(lora_expand_kernel<3, 4, true, true>, 64)
-                   : run(lora_expand_kernel<4, 4, true, true>, 64);
-      return;
-    }
+  if (bytes > kStreamBytes) {
+    steps == 1   ? run(lora_expand_kernel<1, 8, true>, 128)
+    : steps == 2 ? run(lora_expand_kernel<2, 8, true>, 128)
+    : steps == 3 ? run(lora_expand_kernel<3, 4, true>, 64)
+                 : run(lora_expand_kernel<4, 4, true>, 64);
+    return;
   }
-  steps == 1   ? run(lora_expand_kernel<1, 8, GROUPED, false>, 128)
-  : steps == 2 ? run(lora_expand_kernel<2, 4, GROUPED, false>, 64)
-  : steps == 3 ? run(lora_expand_kernel<3, 4, GROUPED, false>, 64)
-               : run(lora_expand_kernel<4, 4, GROUPED, false>, 64);
+  steps == 1   ? run(lora_expand_kernel<1, 8, false>, 128)
+  : steps == 2 ? run(lora_expand_kernel<2, 4, false>, 64)
+  : steps == 3 ? run(lora_expand_kernel<3, 4, false>, 64)
+               : run(lora_expand_kernel<4, 4, false>, 64);
+}
+
+static void launch_parts(LoraArgs a, int slots, hipStream_t stream) {
+  const int rows = a.targets * ((a.max_rank + kTile - 1) / kTile);
+  // as long as a part has kPartColumns and the workgroups all run at once
+  const long long units = std::min(a.units, a.tokens);
+  a.parts = 1;
+  while (a.parts < kMostParts && a.k >= 2 * a.parts * kPartColumns &&
+         2 * a.parts * units * rows * slots <= 256) {
+    a.parts *= 2;
+  }
+  hipLaunchKernelGGL(lora_shrink_part_kernel, dim3(a.units, rows * a.parts, slots),
+                     dim3(kShrinkWaves * kWave), sizeof(Stage<1>) + kGather * sizeof(int), stream,
+                     a);
+  auto run = [&](auto* kernel, int columns) {
+    a.blocks = 0;
+    for (int i = 0; i < a.targets; ++i) a.blocks += (a.target[i].n + columns - 1) / columns;
+    hipLaunchKernelGGL(kernel, dim3(a.units * a.blocks, 1, slots), dim3(kExpandWaves * kWave), 0,
+                       stream, a);
+  };
+  const int steps = rank_pitch(a.max_rank) / 32;
+  steps == 1   ? run(lora_expand_parts_kernel<1, 8>, 128 * kExpandWaves)
+  : steps == 2 ? run(lora_expand_parts_kernel<2, 4>, 64 * kExpandWaves)
+  : steps == 3 ? run(lora_expand_parts_kernel<3, 4>, 64 * kExpandWaves)
+               : run(lora_expand_parts_kernel<4, 4>, 64 * kExpandWaves);
 }
 
 // The largest rank of the one launch (64 spills registers: 64 x 896 x 896 16.3 us, in two
@@ -686,10 +840,10 @@ void launch_lora(LoraArgs a, hipStream_t stream) {
       hipLaunchKernelGGL(kernel, dim3(units, (all + tiles - 1) / tiles, kSet / kTile),
                          dim3(kShrinkWaves * kWave), lds + kSet * sizeof(int), stream, a);
     };
-    all == 1   ? shrink(lora_shrink_kernel<1, true>, 1, sizeof(Stage<1>))
-    : all == 2 ? shrink(lora_shrink_kernel<2, true>, 2, sizeof(Stage<2>))
-               : shrink(lora_shrink_kernel<4, true>, 4, sizeof(Stage<4>));
-    launch_expand<true>(a, units, 0, stream);
+    all == 1   ? shrink(lora_shrink_kernel<1>, 1, sizeof(Stage<1>))
+    : all == 2 ? shrink(lora_shrink_kernel<2>, 2, sizeof(Stage<2>))
+               : shrink(lora_shrink_kernel<4>, 4, sizeof(Stage<4>));
+    launch_expand(a, units, stream);
     return;
   }
   a.by_token = a.adapters + 1 > a.tokens;
@@ -698,10 +852,7 @@ void launch_lora(LoraArgs a, hipStream_t stream) {
   const int tiles = (a.tokens + kTile - 1) / kTile;
   const int slots = std::min(tiles, 1 + a.tokens / (kTile * a.units));
   if (launch_fused(a, slots, stream)) return;
-  hipLaunchKernelGGL((lora_shrink_kernel<1, false>),
-                     dim3(a.units, a.targets * rank_tiles, slots), dim3(kShrinkWaves * kWave),
-                     sizeof(Stage<1>) + kGather * sizeof(int), stream, a);
-  launch_expand<false>(a, a.units, slots, stream);
+  launch_parts(a, slots, stream);
 }
 
 }  // namespace qlin
