@@ -36,6 +36,7 @@ constexpr int kSet = 64;        // tokens of a unit then, at most
 constexpr int kExpandWaves = 4;
 constexpr int kMostParts = 4;     // of K
 constexpr int kPartColumns = 768;
+constexpr int kCus = 256;
 
 // Words of a token's high (and low) part in the workspace: whole steps of the MFMA's K.
 __host__ __device__ constexpr int rank_pitch(int max_rank) { return (max_rank + 31) / 32 * 32; }
@@ -108,6 +109,11 @@ __device__ __forceinline__ Unit grouped_tokens(const LoraArgs& a, int unit, int*
   if (t < v.z) list[t] = token;
   __syncthreads();
   return u;
+}
+
+template <bool GROUPED>
+__device__ __forceinline__ Unit tokens_of(const LoraArgs& a, int unit, int* list) {
+  return GROUPED ? grouped_tokens(a, unit, list) : gather_tokens(a, unit, list);
 }
 
 // A chunk's tokens by adapter: a table of the chunk's adapters in LDS (twice as many
@@ -318,14 +324,14 @@ __device__ __forceinline__ void stage_rows(const uint16_t* (&rows)[RT + 1], cons
   }
 }
 
-template <int RT>
+template <int RT, bool GROUPED>
 __global__ __launch_bounds__(kShrinkWaves * kWave) void lora_shrink_kernel(LoraArgs a) {
   extern __shared__ __align__(16) char shared[];
   Stage<RT>& stage = *reinterpret_cast<Stage<RT>*>(shared);
   int* const list = reinterpret_cast<int*>(shared + sizeof(Stage<RT>));
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const Unit u = grouped_tokens(a, blockIdx.x, list);
+  const Unit u = tokens_of<GROUPED>(a, blockIdx.x, list);
   if (u.count == 0 || u.rank == 0) return;
   const int tiles = (a.max_rank + kTile - 1) / kTile, first = blockIdx.y * RT;
   const int pitch = rank_pitch(a.max_rank);
@@ -499,14 +505,14 @@ __device__ __forceinline__ int target_of(const LoraArgs& a, int columns, int& bl
   return -1;
 }
 
-template <int KS, int J, bool ONCE>
+template <int KS, int J, bool GROUPED, bool ONCE>
 __global__ __launch_bounds__(kExpandWaves * kWave) void lora_expand_kernel(LoraArgs a) {
-  __shared__ int list[kSet];
+  __shared__ int list[GROUPED ? kSet : kGather];
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int m = lane & 15, g = lane >> 4;
   // neighbouring workgroups have neighbouring columns, where they can be counted so
-  const Unit u = grouped_tokens(a, a.blocks ? blockIdx.x / a.blocks : blockIdx.x, list);
+  const Unit u = tokens_of<GROUPED>(a, a.blocks ? blockIdx.x / a.blocks : blockIdx.x, list);
   if (u.count == 0) return;
   int block = (a.blocks ? blockIdx.x % a.blocks : blockIdx.y) * kExpandWaves + wave;
   const int c = target_of(a, J * 16, block);
@@ -750,7 +756,8 @@ size_t lora_workspace_bytes(int tokens, int max_rank, int targets) {
 constexpr long long kStreamBytes = 192ll << 20;
 constexpr long long kMostWorkgroups = (1ll << 32) / (kExpandWaves * kWave) - 1;
 
-static void launch_expand(LoraArgs a, int units, hipStream_t stream) {
+template <bool GROUPED>
+static void launch_expand(LoraArgs a, int units, int slots, hipStream_t stream) {
   const int steps = rank_pitch(a.max_rank) / 32;
   long long bytes = 0;
   for (int i = 0; i < a.targets; ++i) bytes += 4ll * a.tokens * a.target[i].n;
@@ -760,33 +767,47 @@ static void launch_expand(LoraArgs a, int units, hipStream_t stream) {
     blocks = (blocks + kExpandWaves - 1) / kExpandWaves;
     // a unit's four tiles side by side where there would be few workgroups
     const long long few = static_cast<long long>((a.tokens + kSet - 1) / kSet) * blocks;
-    const int z = few >= 1024 ? 1 : few >= 512 ? 2 : kSet / kTile;
+    const int z = !GROUPED ? slots : few >= 1024 ? 1 : few >= 512 ? 2 : kSet / kTile;
     const bool flat = static_cast<long long>(units) * blocks <= kMostWorkgroups;
     a.blocks = flat ? blocks : 0;
     hipLaunchKernelGGL(kernel, flat ? dim3(units * blocks, 1, z) : dim3(units, blocks, z),
                        dim3(kExpandWaves * kWave), 0, stream, a);
   };
-  if (bytes > kStreamBytes) {
-    steps == 1   ? run(lora_expand_kernel<1, 8, true>, 128)
-    : steps == 2 ? run(lora_expand_kernel<2, 8, true>, 128)
-    : steps == 3 ? run(lora_expand_kernel<3, 4, true>, 64)
-                 : run(lora_expand_kernel<4, 4, true>, 64);
-    return;
+  if constexpr (GROUPED) {
+    if (bytes > kStreamBytes) {
+      steps == 1   ? run(lora_expand_kernel<1, 8, true, true>, 128)
+      : steps == 2 ? run(lora_expand_kernel<2, 8, true, true>, 128)
+      : steps == 3 ? run(lora_expand_kernel<3, 4, true, true>, 64)
+                   : run(lora_expand_kernel<4, 4, true, true>, 64);
+      return;
+    }
   }
-  steps == 1   ? run(lora_expand_kernel<1, 8, false>, 128)
-  : steps == 2 ? run(lora_expand_kernel<2, 4, false>, 64)
-  : steps == 3 ? run(lora_expand_kernel<3, 4, false>, 64)
-               : run(lora_expand_kernel<4, 4, false>, 64);
+  steps == 1   ? run(lora_expand_kernel<1, 8, GROUPED, false>, 128)
+  : steps == 2 ? run(lora_expand_kernel<2, 4, GROUPED, false>, 64)
+  : steps == 3 ? run(lora_expand_kernel<3, 4, GROUPED, false>, 64)
+               : run(lora_expand_kernel<4, 4, GROUPED, false>, 64);
 }
 
-static void launch_parts(LoraArgs a, int slots, hipStream_t stream) {
+static void launch_two(LoraArgs a, int slots, hipStream_t stream) {
   const int rows = a.targets * ((a.max_rank + kTile - 1) / kTile);
   // as long as a part has kPartColumns and the workgroups all run at once
   const long long units = std::min(a.units, a.tokens);
   a.parts = 1;
   while (a.parts < kMostParts && a.k >= 2 * a.parts * kPartColumns &&
-         2 * a.parts * units * rows * slots <= 256) {
+         2 * a.parts * units * rows * slots <= kCus) {
     a.parts *= 2;
+  }
+  if (a.parts == 1) {
+    auto shrink = [&](auto* kernel, int tiles, size_t lds) {
+      hipLaunchKernelGGL(kernel, dim3(a.units, (rows + tiles - 1) / tiles, slots),
+                         dim3(kShrinkWaves * kWave), lds + kGather * sizeof(int), stream, a);
+    };
+    const long long ones = units * rows * slots;
+    ones <= kCus       ? shrink(lora_shrink_kernel<1, false>, 1, sizeof(Stage<1>))
+    : ones <= 2 * kCus ? shrink(lora_shrink_kernel<2, false>, 2, sizeof(Stage<2>))
+                       : shrink(lora_shrink_kernel<4, false>, 4, sizeof(Stage<4>));
+    launch_expand<false>(a, a.units, slots, stream);
+    return;
   }
   hipLaunchKernelGGL(lora_shrink_part_kernel, dim3(a.units, rows * a.parts, slots),
                      dim3(kShrinkWaves * kWave), sizeof(Stage<1>) + kGather * sizeof(int), stream,
@@ -807,7 +828,7 @@ static void launch_parts(LoraArgs a, int slots, hipStream_t stream) {
 // The largest rank of the one launch (64 spills registers: 64 x 896 x 896 16.3 us, in two
 // launches 8.5; 32 33 tokens' q, k and v of 1536 9.5, 9.6), and A's bytes that it may read
 // over all its workgroups (64 x 3584 x 3584 at rank 16, 22 MB, 10.9 us, 12.2).
-constexpr int kFusedRank = 32;
+constexpr int kFusedRank = 32, kFusedRows = 1 << 16;
 constexpr long long kFusedBytes = 24ll << 20;
 
 static bool launch_fused(const LoraArgs& a, int slots, hipStream_t stream) {
@@ -815,7 +836,10 @@ static bool launch_fused(const LoraArgs& a, int slots, hipStream_t stream) {
   int blocks = 0;
   for (int i = 0; i < a.targets; ++i) blocks += (a.target[i].n + kColumns - 1) / kColumns;
   const long long units = std::min(a.units, a.tokens);
-  if (a.max_rank > kFusedRank || 2ll * units * blocks * a.max_rank * a.k > kFusedBytes) return false;
+  if (a.max_rank > kFusedRank || (a.max_rank + kTile - 1) / kTile * kTile * a.k > kFusedRows ||
+      2ll * units * blocks * a.max_rank * a.k > kFusedBytes) {
+    return false;
+  }
   auto run = [&](auto* kernel, size_t lds) {
     hipLaunchKernelGGL(kernel, dim3(a.units, blocks, slots), dim3(kShrinkWaves * kWave),
                        lds + kGather * sizeof(int), stream, a);
@@ -840,10 +864,10 @@ void launch_lora(LoraArgs a, hipStream_t stream) {
       hipLaunchKernelGGL(kernel, dim3(units, (all + tiles - 1) / tiles, kSet / kTile),
                          dim3(kShrinkWaves * kWave), lds + kSet * sizeof(int), stream, a);
     };
-    all == 1   ? shrink(lora_shrink_kernel<1>, 1, sizeof(Stage<1>))
-    : all == 2 ? shrink(lora_shrink_kernel<2>, 2, sizeof(Stage<2>))
-               : shrink(lora_shrink_kernel<4>, 4, sizeof(Stage<4>));
-    launch_expand(a, units, stream);
+    all == 1   ? shrink(lora_shrink_kernel<1, true>, 1, sizeof(Stage<1>))
+    : all == 2 ? shrink(lora_shrink_kernel<2, true>, 2, sizeof(Stage<2>))
+               : shrink(lora_shrink_kernel<4, true>, 4, sizeof(Stage<4>));
+    launch_expand<true>(a, units, 0, stream);
     return;
   }
   a.by_token = a.adapters + 1 > a.tokens;
@@ -852,7 +876,7 @@ void launch_lora(LoraArgs a, hipStream_t stream) {
   const int tiles = (a.tokens + kTile - 1) / kTile;
   const int slots = std::min(tiles, 1 + a.tokens / (kTile * a.units));
   if (launch_fused(a, slots, stream)) return;
-  launch_parts(a, slots, stream);
+  launch_two(a, slots, stream);
 }
 
 }  // namespace qlin

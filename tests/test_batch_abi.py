@@ -190,6 +190,13 @@ def test_sample_binding_refuses_cpu_tensors(hip, batch):
         batch.sample(x, torch.zeros(2), torch.zeros(2, dtype=torch.int32), x)
 
 
+@pytest.mark.parametrize("rank,targets", [(8, 1), (40, 2), (128, 3)])
+def test_a_workspace_serves_calls_of_fewer_tokens(batch, rank, targets):
+    bytes_of = [batch.lora_workspace_bytes(t, rank, targets) for t in
+                (1, 2, 16, 255, 256, 257, 300, 1024, 1025, 5000, 1 << 20)]
+    assert bytes_of[0] > 0 and bytes_of == sorted(bytes_of)
+
+
 # ------------------------------------------------------------------ bindings --
 
 class Accepts:

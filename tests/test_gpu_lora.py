@@ -74,7 +74,12 @@ CASES = [
     (3, 1024, [1025], 16, 2), (3, 1032, [1023], 32, 2), (7, 512, [65], 40, 2),
     (256, 520, [70], 32, 1), (256, 2056, [40, 50, 60], 24, 255), (300, 64, [40, 41, 42], 24, 5),
     (700, 1544, [24, 300], 56, 3), (513, 504, [33, 8, 9], 128, 2), (290, 4096, [128], 32, 1),
-    (2050, 8, [16], 8, 700)]
+    (2050, 8, [16], 8, 700),
+    # up to 256 tokens in two launches: K in two and four parts, several tiles of a unit one
+    # after the other; two and four tiles of rows of A at a time
+    (3, 1544, [100], 40, 2), (5, 3080, [40, 70], 128, 2), (9, 4104, [1030], 24, 3),
+    (20, 3592, [257], 72, 1), (256, 4104, [65], 16, 1), (70, 1600, [40, 9, 300], 56, 1),
+    (60, 128, [40], 80, 60), (100, 72, [40, 50], 64, 90), (120, 64, [20, 21, 22], 120, 119)]
 
 
 @pytest.mark.parametrize("runs", [False, True])
@@ -254,9 +259,10 @@ def test_an_adapter_past_2_32_elements(batch, dev):
     assert ((out.cpu().double() - want).abs() <= tol).all()
 
 
-@pytest.mark.parametrize("tokens,rank", [(30, 16), (100, 64), (400, 16)])
+@pytest.mark.parametrize("tokens,rank", [(30, 16), (100, 64), (400, 16), (60, 128)])
 def test_captured_calls_follow_the_ids(batch, dev, tokens, rank):
-    s = make(tokens, 256, [300, 40], rank, 6, 16)
+    k = 1600 if rank == 128 else 256  # in parts
+    s = make(tokens, k, [300, 40], rank, 6, 16)
     d = on(s, dev)
     ws = workspace(batch, tokens, rank, 2, dev)
     out = [torch.empty_like(y) for y in d["base"]]
@@ -268,7 +274,7 @@ def test_captured_calls_follow_the_ids(batch, dev, tokens, rank):
             batch.lora(d["x"], d["ids"], targets, ws, ranks=d["ranks"], scales=d["scales"])
     for step in range(4):
         s["ids"] = torch.randint(-1, 6, (tokens,), generator=gen(step), dtype=torch.int32)
-        s["x"] = bf16((tokens, 256), gen(step + 50))
+        s["x"] = bf16((tokens, k), gen(step + 50))
         d["ids"].copy_(s["ids"])
         d["x"].copy_(s["x"])
         graph.replay()
