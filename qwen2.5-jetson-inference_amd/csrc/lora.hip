@@ -217,10 +217,12 @@ constexpr int kShrinkWaves = 16;
 
 template <int RT>
 struct Stage {
-  // of a row's chunk: room for two workgroups a CU (one at RT 4)
+  // of a row's chunk: room for two workgroups a CU (one at RT 4), whose registers at RT 2 are
+  // few enough for both too (three chunks on their way, and one workgroup, are faster where
+  // workgroups are few: 3000 tokens by 896 38.1 us, 39.3; 12000 by 1536 49.3, 42.8)
   static constexpr int kLoads = RT == 1 ? 2 : 1;
   static constexpr int kColumns = 512 * kLoads;
-  static constexpr int kDepth = RT == 1 ? 4 : RT == 2 ? 3 : 2;
+  static constexpr int kDepth = RT == 1 ? 4 : 2;
   static constexpr int kSteps = kColumns / 32 / kShrinkWaves;  // of a wave
   static constexpr int kPitch = kColumns + 8;
   union {
@@ -325,7 +327,7 @@ __device__ __forceinline__ void stage_rows(const uint16_t* (&rows)[RT + 1], cons
 }
 
 template <int RT, bool GROUPED>
-__global__ __launch_bounds__(kShrinkWaves * kWave) void lora_shrink_kernel(LoraArgs a) {
+__global__ __launch_bounds__(kShrinkWaves * kWave, RT == 2 ? 8 : 4) void lora_shrink_kernel(LoraArgs a) {
   extern __shared__ __align__(16) char shared[];
   Stage<RT>& stage = *reinterpret_cast<Stage<RT>*>(shared);
   int* const list = reinterpret_cast<int*>(shared + sizeof(Stage<RT>));
