@@ -209,20 +209,19 @@ __device__ __forceinline__ uint4 cut_words(uint4 v, int k, int rank) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// h of RT tiles of rows of A by a tile's tokens, by 16 waves.  Each wave loads whole rows, a
-// KB in a row (as operands, 16 rows side by side, they would cost the CU's address unit
-// four times as much), into LDS, a chunk of columns at a time with kDepth of them on their
-// way; there it takes its steps of the chunk for all rows.
+// h of RT (1 or 2) tiles of rows of A by a tile's tokens, by 16 waves.  Each wave loads whole
+// rows, a KB in a row (as operands, 16 rows side by side, they would cost the CU's address
+// unit four times as much), into LDS, a chunk of columns at a time with kDepth of them on
+// their way; there it takes its steps of the chunk for all rows.  Two workgroups share a
+// CU, by LDS and by registers (12000 x 1536 at rank 32: one 49.3 us with all of the call,
+// two 42.8; four tiles at a time, one to a CU, 2000 x 3584 at rank 128 51.1 us, 43.8).
 constexpr int kShrinkWaves = 16;
 
 template <int RT>
 struct Stage {
-  // of a row's chunk: room for two workgroups a CU (one at RT 4), whose registers at RT 2 are
-  // few enough for both too (three chunks on their way, and one workgroup, are faster where
-  // workgroups are few: 3000 tokens by 896 38.1 us, 39.3; 12000 by 1536 49.3, 42.8)
-  static constexpr int kLoads = RT == 1 ? 2 : 1;
+  static constexpr int kLoads = RT == 1 ? 2 : 1;  // of a row's chunk
   static constexpr int kColumns = 512 * kLoads;
-  static constexpr int kDepth = RT == 1 ? 4 : 2;
+  static constexpr int kDepth = 2;
   static constexpr int kSteps = kColumns / 32 / kShrinkWaves;  // of a wave
   static constexpr int kPitch = kColumns + 8;
   union {
@@ -327,7 +326,7 @@ __device__ __forceinline__ void stage_rows(const uint16_t* (&rows)[RT + 1], cons
 }
 
 template <int RT, bool GROUPED>
-__global__ __launch_bounds__(kShrinkWaves * kWave, RT == 2 ? 8 : 4) void lora_shrink_kernel(LoraArgs a) {
+__global__ __launch_bounds__(kShrinkWaves * kWave, 8) void lora_shrink_kernel(LoraArgs a) {
   extern __shared__ __align__(16) char shared[];
   Stage<RT>& stage = *reinterpret_cast<Stage<RT>*>(shared);
   int* const list = reinterpret_cast<int*>(shared + sizeof(Stage<RT>));
@@ -804,10 +803,10 @@ static void launch_two(LoraArgs a, int slots, hipStream_t stream) {
       hipLaunchKernelGGL(kernel, dim3(a.units, (rows + tiles - 1) / tiles, slots),
                          dim3(kShrinkWaves * kWave), lds + kGather * sizeof(int), stream, a);
     };
-    const long long ones = units * rows * slots;
-    ones <= kCus       ? shrink(lora_shrink_kernel<1, false>, 1, sizeof(Stage<1>))
-    : ones <= 2 * kCus ? shrink(lora_shrink_kernel<2, false>, 2, sizeof(Stage<2>))
-                       : shrink(lora_shrink_kernel<4, false>, 4, sizeof(Stage<4>));
+    // x for two tiles of rows where there are many (33 tokens' q, k and v of 1536 at rank 64
+    // 15.1 us, 12.2)
+    units * rows * slots <= kCus ? shrink(lora_shrink_kernel<1, false>, 1, sizeof(Stage<1>))
+                                 : shrink(lora_shrink_kernel<2, false>, 2, sizeof(Stage<2>));
     launch_expand<false>(a, a.units, slots, stream);
     return;
   }
@@ -859,16 +858,13 @@ void launch_lora(LoraArgs a, hipStream_t stream) {
     a.units = units_of(a.tokens, a.adapters);
     const int chunks = chunks_of(a.tokens), units = chunks * a.units;
     hipLaunchKernelGGL(lora_group_kernel, dim3(chunks), dim3(kChunk), 0, stream, a);
-    // x once for all rows of A, up to four tiles of them (6001 x 1536 at rank 64: in twos
-    // 21.2 us, in fours 15.4)
     const int all = a.targets * rank_tiles;
     auto shrink = [&](auto* kernel, int tiles, size_t lds) {
       hipLaunchKernelGGL(kernel, dim3(units, (all + tiles - 1) / tiles, kSet / kTile),
                          dim3(kShrinkWaves * kWave), lds + kSet * sizeof(int), stream, a);
     };
-    all == 1   ? shrink(lora_shrink_kernel<1, true>, 1, sizeof(Stage<1>))
-    : all == 2 ? shrink(lora_shrink_kernel<2, true>, 2, sizeof(Stage<2>))
-               : shrink(lora_shrink_kernel<4, true>, 4, sizeof(Stage<4>));
+    all == 1 ? shrink(lora_shrink_kernel<1, true>, 1, sizeof(Stage<1>))
+             : shrink(lora_shrink_kernel<2, true>, 2, sizeof(Stage<2>));
     launch_expand<true>(a, units, 0, stream);
     return;
   }
