@@ -99,7 +99,9 @@ int infer_hip_lora_bf16(const uint16_t* x, long long x_stride, const int* ids, i
  * -1 and probability NaN.
  *
  * logits at least 2-byte aligned (rows that are 16-byte aligned are faster),
- * vocab up to 2^20, rows up to 2^20, the workspace 16-byte aligned. */
+ * vocab up to 2^20, rows up to 2^20, the workspace 16-byte aligned.  A row in which
+ * two values or more have 32768 tokens each takes some 50 times as long (one may, as
+ * a mask's does). */
 /* Bytes for calls of up to `rows` rows of `vocab` (0: refused shapes). */
 size_t infer_hip_sample_workspace_bytes(int rows, int vocab);
 int infer_hip_sample_bf16(const uint16_t* logits, long long stride, int rows, int vocab,

@@ -159,7 +159,7 @@ int infer_hip_attention_paged_decode(const infer_hip_kv_pages* pages,
  * the launch, and read everything on the device when the work runs.
  *
  * infer_hip_kv_pages_assign: sequence s holds lengths[s] positions and gets
- * added[s] more (negative: 0), over a block table [num_sequences][max_pages]
+ * added[s] more (negative: 0, for both), over a block table [num_sequences][max_pages]
  * with `stride` entries between rows, at most 65535 sequences and 2^30
  * positions, page_size as a pool's.  It needs
  *   need[s] = ceil((lengths[s] + added[s]) / page_size) - ceil(lengths[s] / page_size)

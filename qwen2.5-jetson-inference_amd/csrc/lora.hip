@@ -26,17 +26,25 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 // captured graph follows ids that change.
 //
 // h = s A x: 16 rows of A by 16 tokens a tile, K split over a workgroup's 16 waves and
-// joined in LDS in the order of the waves.  h is kept as high + low BF16 (2^-16 of it;
-// one BF16 number alone would add as much error as the output's rounding), and B h takes
-// two products.
+// joined in LDS in the order of the waves, and over up to kMostParts workgroups where there
+// are few.  h is kept as high + low BF16 (2^-16 of it; one BF16 number alone would add as
+// much error as the output's rounding), and B h takes two products.
+//
+// Small calls take one launch, up to kGather tokens two, more three.  What bounds them, in
+// us: one launch its reads one behind the other (ids, rows, then the join; 1 x 896 x 896 at
+// rank 8 6.7 of which 1.7 an empty launch, 33 tokens' q, k and v of 1536 at rank 16 7.8);
+// A x the same and a CU's loads (128 x 3584 by 2 x 64 rows 7.6; 6001 x 1536 by 32 8.6); B h
+// its bytes (128 x 2 x 18944 at rank 64 18.0 for 75 MB, 4.2 TB/s; 6001 x 8960 at rank 32
+// 46.4 for 216 MB, 4.7, a copy 5.07); grouping 3.2-4.7, a launch and LDS atomics.
 constexpr int kTile = 16;       // tokens, and rows of A
 constexpr int kGather = 256;    // tokens
 constexpr int kChunk = 1024;    // tokens grouped together beyond
 constexpr int kSet = 64;        // tokens of a unit then, at most
 constexpr int kExpandWaves = 4;
-constexpr int kMostParts = 4;     // of K
-constexpr int kPartColumns = 768;
 constexpr int kCus = 256;
+// A part's columns, at least: a workgroup's chunk is 1024, and 64 x 896 at rank 64 took 9.7
+// us in two parts, 8.9 in one.
+constexpr int kMostParts = 4, kPartColumns = 768;
 
 // Words of a token's high (and low) part in the workspace: whole steps of the MFMA's K.
 __host__ __device__ constexpr int rank_pitch(int max_rank) { return (max_rank + 31) / 32 * 32; }
@@ -387,7 +395,8 @@ __global__ __launch_bounds__(kShrinkWaves * kWave) void lora_shrink_part_kernel(
     shrink_tile<1>(sum, columns, rows, stage, wave, lane);
     const int e = threadIdx.x, at = tile * kTile + token_of(e);
     if (e < kTile * kTile && at < u.count) {
-      h[static_cast<size_t>(list[at]) * pitch + q % tiles * kTile + row_of(e)] = joined<1>(stage, e);
+      h[static_cast<size_t>(list[at]) * pitch + q % tiles * kTile + row_of(e)] =
+          joined<1>(stage, e);
     }
   }
 }
@@ -639,7 +648,8 @@ __global__ __launch_bounds__(kExpandWaves * kWave) void lora_expand_parts_kernel
       }
       if (kFours % kThreads == 0 || e < kFours) {
         uint16_t* to = &h[turn][0][e / (kPitch / 4)][row];
-        *reinterpret_cast<uint2*>(to) = make_uint2(high[0] | high[1] << 16, high[2] | high[3] << 16);
+        *reinterpret_cast<uint2*>(to) =
+            make_uint2(high[0] | high[1] << 16, high[2] | high[3] << 16);
         *reinterpret_cast<uint2*>(to + kTile * (kPitch + 8)) =
             make_uint2(low[0] | low[1] << 16, low[2] | low[3] << 16);
       }
@@ -791,7 +801,8 @@ static void launch_expand(LoraArgs a, int units, int slots, hipStream_t stream) 
 
 static void launch_two(LoraArgs a, int slots, hipStream_t stream) {
   const int rows = a.targets * ((a.max_rank + kTile - 1) / kTile);
-  // as long as a part has kPartColumns and the workgroups all run at once
+  // as long as a part has kPartColumns and the workgroups run at once, one to a CU (128 x
+  // 3584 x 2 x 18944 at rank 64 26.4 us in one part, 23.6 in two, 24.2 in four on 416)
   const long long units = std::min(a.units, a.tokens);
   a.parts = 1;
   while (a.parts < kMostParts && a.k >= 2 * a.parts * kPartColumns &&
@@ -826,11 +837,14 @@ static void launch_two(LoraArgs a, int slots, hipStream_t stream) {
                : run(lora_expand_parts_kernel<4, 4>, 64 * kExpandWaves);
 }
 
-// The largest rank of the one launch (64 spills registers: 64 x 896 x 896 16.3 us, in two
-// launches 8.5; 32 33 tokens' q, k and v of 1536 9.5, 9.6), and A's bytes that it may read
-// over all its workgroups (64 x 3584 x 3584 at rank 16, 22 MB, 10.9 us, 12.2).
+// The one launch's largest rank (64 spills registers: 64 x 896 x 896 16.3 us, in two launches
+// 8.8; 32 33 tokens' q, k and v of 1536 9.1, in two 10.1), rows of A by columns that each of
+// its workgroups takes (5 x 8960 x 1536 at rank 32 19.0 us, in two launches 11.0; 40 x 2048
+// x 2048 9.4, 9.7), and A's bytes that all of them may read (100 tokens' 60 adapters by
+// 2048 x 2048 at rank 32, 16 MB, 10.6 us, 11.1; 200's 200 by 1536 x 1536 at rank 16, 20 MB, 15.1,
+// 13.7; 128's 120 by 896 x 2 x 4864, 34 MB, 24.7, 17.3).
 constexpr int kFusedRank = 32, kFusedRows = 1 << 16;
-constexpr long long kFusedBytes = 24ll << 20;
+constexpr long long kFusedBytes = 16ll << 20;
 
 static bool launch_fused(const LoraArgs& a, int slots, hipStream_t stream) {
   constexpr int kColumns = kShrinkWaves * 64;

@@ -92,7 +92,8 @@ __device__ __forceinline__ Setting setting_of(const SampleArgs& a, int row) {
   const float m = a.min_p ? a.min_p[row] : 0.0f;
   const float u = a.uniform[row];
   const int k = a.top_k ? a.top_k[row] : 0;
-  Setting s{t, p, m, 0.0, k > 0 ? static_cast<unsigned>(k) : 0u, t != t || p != p || m != m || u != u};
+  Setting s{t, p, m, 0.0, k > 0 ? static_cast<unsigned>(k) : 0u,
+            t != t || p != p || m != m || u != u};
   // 1 - 2^-24, the last number under 1: a target under the sum of all
   s.uniform = fminf(fmaxf(u, 0.0f), 0x1.fffffep-1f);
   if (!(t > 0.0f)) s = Setting{1.0, 1.0, 0.0, 0.0, 1u, s.bad};
@@ -213,7 +214,8 @@ struct Lds {
   int low, high;
 };
 
-// A row that is read again for every question: 16 passes a border.
+// A row that is read again for every question, 16 passes a border: 16 rows of 151936 that
+// have two values with half of the tokens each 1880 us, where the count takes 21 to 116.
 struct ReadRow {
   const uint16_t* logits;
   int vocab;
@@ -277,14 +279,16 @@ struct ReadRow {
   }
 };
 
-__device__ __forceinline__ void finish(const SampleArgs& a, int row, int token, double probability) {
+__device__ __forceinline__ void finish(const SampleArgs& a, int row, int token,
+                                       double probability) {
   a.tokens[row] = token;
   if (a.probabilities) a.probabilities[row] = static_cast<float>(probability);
 }
 
 // The row's answer by bisection, for a row whose counts do not fit the other
 // kernel's.
-__device__ __forceinline__ void sample_by_bisection(const SampleArgs& a, int row, const Setting& s, Lds& lds) {
+__device__ __forceinline__ void sample_by_bisection(const SampleArgs& a, int row,
+                                                    const Setting& s, Lds& lds) {
   const int wave = threadIdx.x / kWave, lane = threadIdx.x & (kWave - 1);
   const uint16_t* logits = a.logits + row * a.stride;
   if (threadIdx.x == 0) {
@@ -348,6 +352,15 @@ __device__ __forceinline__ void sample_by_bisection(const SampleArgs& a, int row
 // weights are a geometric series, w q^l, and its sum a polynomial in q of the
 // counts: two exponentials a group, and 8 lanes for the polynomial.  One wave then asks
 // its questions of the sums of the groups with tokens, some 50 to 90 of a model's row.
+//
+// Bound: chains within one workgroup, as a row's counts meet in one CU's LDS.  Of the 46000
+// cycles of a row of 151936 (19.9 us with a launch) the count takes 22000, 8 LDS additions a
+// 16-byte piece at some 8 cycles a wave; the groups' sums 7000; the questions, one wave's
+// dependent 64-bit steps, 6000; the token's place 5000-7000 over the row in registers.  256
+// such rows take 26.5 us (78 MB, 2.9 TB/s), 17 of 32003 12.7, of which the counts are 5000
+// cycles.  Parts of a row counted by several workgroups need a launch to add them up: 1 x
+// 151936 24.7 us, 1 x 40000 22 for 12.4.  512 threads, so that the row stays in registers
+// beside the work.
 constexpr int kBins = 32768, kGroups = 1024;
 constexpr int kInfBin = 0x7F80;
 constexpr int kLastGroup = (0xFFFF - kKeyLowest) / kWave;  // with tokens that count
@@ -378,8 +391,8 @@ typedef __attribute__((address_space(3))) unsigned LdsWord;
 __device__ __forceinline__ void add_shifted(uint32_t shifted, unsigned times) {
   // `shifted` has the word's 16 bits from bit 2 on
   const unsigned one = (shifted & (1u << kBinShift)) | 1u;
-  __hip_atomic_fetch_add((LdsWord*)static_cast<uintptr_t>(shifted & (4u * (kBins - 1))), one * times, __ATOMIC_RELAXED,
-                         __HIP_MEMORY_SCOPE_WORKGROUP);
+  __hip_atomic_fetch_add((LdsWord*)static_cast<uintptr_t>(shifted & (4u * (kBins - 1))),
+                         one * times, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
 }
 __device__ __forceinline__ void add_word(uint32_t word, unsigned times) {
   add_shifted(word << 2, times);
@@ -682,8 +695,8 @@ __device__ __forceinline__ double group_mass(const Counted& c, const Weight& w, 
 
 // Everything after the bins: the token's value, and its place among those that have it,
 // in lds.pick.  False where the row has been answered.
-__device__ __forceinline__ bool choose_value(const SampleArgs& a, int row, const Setting& s, const Heavy& heavy,
-                             CountLds& lds) {
+__device__ __forceinline__ bool choose_value(const SampleArgs& a, int row, const Setting& s,
+                                             const Heavy& heavy, CountLds& lds) {
   const int t = threadIdx.x, lane = t & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(t / kWave);
   // Thread t's 64 dwords are groups 511 - t and 512 + t; 16 bytes at a time in an order
@@ -876,7 +889,9 @@ __device__ __forceinline__ bool locate(const SampleArgs& a, int row, const RowSp
       const u32x4 x = p.get(i);
       uint32_t others = 0;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) others = add_words(others, smaller_words(v.differs(x[j]), 0x10001u));
+      for (int j = 0; j < 4; ++j) {
+        others = add_words(others, smaller_words(v.differs(x[j]), 0x10001u));
+      }
       const unsigned n = 8 - (others & 0xFFFFu) - (others >> 16);
       if (n && live(i)) {
         atomicAdd(&lds.found[i], n);
