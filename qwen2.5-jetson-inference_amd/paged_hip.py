@@ -321,13 +321,25 @@ def kv_pages_release(table, page_size: int, free, free_count, lengths, finished,
     onto free (infer_hip_kv_pages_release); the other arguments are
     kv_pages_assign's."""
     index, on, tp, n, width, stride = _plan_table(table, stream)
-    fc, ln = (_flat(free_count, _I32, 1, index, "free_count"),
-              _flat(lengths, _I32, n, index, "lengths"))
+    if lengths_out is None:
+        lengths_out = lengths
+    if free_count_out is None:
+        free_count_out = free_count
+    if not (lengths.dtype is _I32 and lengths.get_device() == index and lengths.numel() == n
+            and lengths.is_contiguous() and finished.dtype is _I32
+            and finished.get_device() == index and finished.numel() == n
+            and finished.is_contiguous() and lengths_out.dtype is _I32
+            and lengths_out.get_device() == index and lengths_out.numel() == n
+            and lengths_out.is_contiguous() and free.dtype is _I32
+            and free.get_device() == index and free.is_contiguous()):
+        for t, count, name in ((lengths, n, "lengths"), (finished, n, "finished"),
+                               (lengths_out, n, "lengths_out"), (free, None, "free")):
+            _flat(t, _I32, count, index, name)
     status = load().infer_hip_kv_pages_release(
-        tp, n, width, stride, page_size, _flat(free, _I32, None, index, "free"), free.numel(), fc,
-        fc if free_count_out is None else _flat(free_count_out, _I32, 1, index, "free_count_out"),
-        ln, _flat(finished, _I32, n, index, "finished"),
-        ln if lengths_out is None else _flat(lengths_out, _I32, n, index, "lengths_out"),
+        tp, n, width, stride, page_size, free.data_ptr(), free.numel(),
+        _flat(free_count, _I32, 1, index, "free_count"),
+        _flat(free_count_out, _I32, 1, index, "free_count_out"), lengths.data_ptr(),
+        finished.data_ptr(), lengths_out.data_ptr(),
         _flat(workspace, _U8, None, index, "workspace"), workspace.numel(), on)
     if status:
         _check(status)
