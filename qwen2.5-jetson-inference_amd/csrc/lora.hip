@@ -35,12 +35,14 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 // rank 8 6.7 of which 1.7 an empty launch, 33 tokens' q, k and v of 1536 at rank 16 7.8);
 // A x the same and a CU's loads (128 x 3584 by 2 x 64 rows 7.6; 6001 x 1536 by 32 8.6); B h
 // its bytes (128 x 2 x 18944 at rank 64 18.0 for 75 MB, 4.2 TB/s; 6001 x 8960 at rank 32
-// 46.4 for 216 MB, 4.7, a copy 5.07); grouping 3.2-4.7, a launch and LDS atomics.
+// 46.4 for 216 MB, 4.7, a copy 5.07), from rank 64 on also h, which each wave reads (6001 x
+// 8960 at rank 64 69 with all of the call, at 128 113); grouping 3.2-4.7, a launch and LDS
+// atomics.
 constexpr int kTile = 16;       // tokens, and rows of A
 constexpr int kGather = 256;    // tokens
 constexpr int kChunk = 1024;    // tokens grouped together beyond
 constexpr int kSet = 64;        // tokens of a unit then, at most
-constexpr int kExpandWaves = 4;
+constexpr int kPartWaves = 4;
 constexpr int kCus = 256;
 // A part's columns, at least: a workgroup's chunk is 1024, and 64 x 896 at rank 64 took 9.7
 // us in two parts, 8.9 in one.
@@ -79,19 +81,19 @@ __device__ __forceinline__ Unit gather_tokens(const LoraArgs& a, int unit, int* 
     if (i * kWave < a.tokens && t < a.tokens) id[i] = adapter_of(a, a.ids[t]);
   }
   const int mine = a.by_token ? adapter_of(a, a.ids[unit]) : unit - 1;
-  int count = 0, first = -1;
+  Unit u = unit_of(a, mine, 0);  // on its way while the ids are compared
+  int first = -1;
 #pragma unroll
   for (int i = 0; i < kGather / kWave; ++i) {
     if (i * kWave >= a.tokens) break;
     const unsigned long long mask = __ballot(id[i] == mine);
     if (first < 0 && mask) first = i * kWave + __builtin_ctzll(mask);
     if (id[i] == mine && wave == 0) {
-      list[count + __popcll(mask & ((1ull << lane) - 1))] = i * kWave + lane;
+      list[u.count + __popcll(mask & ((1ull << lane) - 1))] = i * kWave + lane;
     }
-    count += __popcll(mask);
+    u.count += __popcll(mask);
   }
-  if (a.by_token && first != unit) return unit_of(a, -1, 0);
-  const Unit u = unit_of(a, mine, count);
+  if (a.by_token && first != unit) return Unit{-1, 0, 0, 1.0f};
   __syncthreads();
   return u;
 }
@@ -515,8 +517,8 @@ __device__ __forceinline__ int target_of(const LoraArgs& a, int columns, int& bl
   return -1;
 }
 
-template <int KS, int J, bool GROUPED, bool ONCE>
-__global__ __launch_bounds__(kExpandWaves * kWave) void lora_expand_kernel(LoraArgs a) {
+template <int KS, int J, int WAVES, bool GROUPED, bool ONCE>
+__global__ __launch_bounds__(WAVES * kWave) void lora_expand_kernel(LoraArgs a) {
   __shared__ int list[GROUPED ? kSet : kGather];
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -524,7 +526,7 @@ __global__ __launch_bounds__(kExpandWaves * kWave) void lora_expand_kernel(LoraA
   // neighbouring workgroups have neighbouring columns, where they can be counted so
   const Unit u = tokens_of<GROUPED>(a, a.blocks ? blockIdx.x / a.blocks : blockIdx.x, list);
   if (u.count == 0) return;
-  int block = (a.blocks ? blockIdx.x % a.blocks : blockIdx.y) * kExpandWaves + wave;
+  int block = (a.blocks ? blockIdx.x % a.blocks : blockIdx.y) * WAVES + wave;
   const int c = target_of(a, J * 16, block);
   if (c < 0) return;
   const LoraTarget& t = a.target[c];
@@ -575,8 +577,8 @@ __global__ __launch_bounds__(kExpandWaves * kWave) void lora_expand_kernel(LoraA
 // B h from the parts of h: a workgroup's waves add them up in the order of the parts, once
 // for all, into LDS.
 template <int KS, int J>
-__global__ __launch_bounds__(kExpandWaves * kWave) void lora_expand_parts_kernel(LoraArgs a) {
-  constexpr int kPitch = 32 * KS, kThreads = kExpandWaves * kWave;
+__global__ __launch_bounds__(kPartWaves * kWave) void lora_expand_parts_kernel(LoraArgs a) {
+  constexpr int kPitch = 32 * KS, kThreads = kPartWaves * kWave;
   constexpr int kFours = kTile * kPitch / 4, kMine = (kFours + kThreads - 1) / kThreads;
   __shared__ int list[kGather];
   __shared__ __align__(16) uint16_t h[2][2][kTile][kPitch + 8];
@@ -586,10 +588,10 @@ __global__ __launch_bounds__(kExpandWaves * kWave) void lora_expand_parts_kernel
   const Unit u = gather_tokens(a, blockIdx.x / a.blocks, list);
   if (u.count == 0) return;
   int block = blockIdx.x % a.blocks;
-  const int c = target_of(a, kExpandWaves * J * 16, block);
+  const int c = target_of(a, kPartWaves * J * 16, block);
   const LoraTarget& t = a.target[c];
   if (u.adapter < 0 && t.base == t.out) return;
-  block = block * kExpandWaves + wave;
+  block = block * kPartWaves + wave;
   const bool has = block * J * 16 < t.n;
   // A tile's parts and bases are loaded while the one before it is computed.
   struct Tile {
@@ -761,42 +763,54 @@ size_t lora_workspace_bytes(int tokens, int max_rank, int targets) {
                              16 * chunks * units_of(tokens, kChunk));
 }
 
-// Bytes of bases and outputs beyond which they are not left in the caches (6001 tokens by
-// 8960, 215 MB, 67.1 -> 64.1 us; 3000 by 2 x 4864, 117 MB, whose bases still are there, 31.6 ->
-// 36.7).
+// Bytes of bases and outputs beyond which four waves take 512 columns side by side, and beyond
+// which they are not left in the caches (6001 tokens by 8960, 215 MB, 67.1 -> 64.1 us; 3000 by
+// 2 x 4864, 117 MB, whose bases still are there, 31.6 -> 36.7).  Below, a wave is a workgroup, of
+// 64 columns beyond rank 32, that starts as soon as it finds room (2000 x 3584 x 3584 at rank
+// 128 43.6 us in fours, 37.3; 250 x 3584 x 3584 of 200 adapters 66.9, 64.6; but 3000 x 896 x 2 x
+// 4864 at rank 64 56.6 for 49.7, at rank 8 40.3 for 38.6).
+constexpr long long kManyBytes = 70ll << 20;
 constexpr long long kStreamBytes = 192ll << 20;
-constexpr long long kMostWorkgroups = (1ll << 32) / (kExpandWaves * kWave) - 1;
+constexpr long long kMostThreads = (1ll << 32) - 1;  // of a launch, along x
 
 template <bool GROUPED>
 static void launch_expand(LoraArgs a, int units, int slots, hipStream_t stream) {
   const int steps = rank_pitch(a.max_rank) / 32;
+  const int sets = (a.tokens + kSet - 1) / kSet;
   long long bytes = 0;
   for (int i = 0; i < a.targets; ++i) bytes += 4ll * a.tokens * a.target[i].n;
-  auto run = [&](auto* kernel, int columns) {
-    int blocks = 0;
-    for (int i = 0; i < a.targets; ++i) blocks += (a.target[i].n + columns - 1) / columns;
-    blocks = (blocks + kExpandWaves - 1) / kExpandWaves;
+  auto run = [&](auto* kernel, int columns, int waves) {
+    long long all = 0;
+    for (int i = 0; i < a.targets; ++i) all += (a.target[i].n + columns - 1) / columns;
+    const int blocks = static_cast<int>((all + waves - 1) / waves);
     // a unit's four tiles side by side where there would be few workgroups
-    const long long few = static_cast<long long>((a.tokens + kSet - 1) / kSet) * blocks;
-    const int z = !GROUPED ? slots : few >= 1024 ? 1 : few >= 512 ? 2 : kSet / kTile;
-    const bool flat = static_cast<long long>(units) * blocks <= kMostWorkgroups;
+    const long long few = static_cast<long long>(sets) * blocks;
+    const int z = !GROUPED ? slots : waves > 1 || few >= 1024 ? 1 : few >= 512 ? 2 : kSet / kTile;
+    const bool flat = static_cast<long long>(units) * blocks * waves * kWave <= kMostThreads;
     a.blocks = flat ? blocks : 0;
     hipLaunchKernelGGL(kernel, flat ? dim3(units * blocks, 1, z) : dim3(units, blocks, z),
-                       dim3(kExpandWaves * kWave), 0, stream, a);
+                       dim3(waves * kWave), 0, stream, a);
   };
   if constexpr (GROUPED) {
     if (bytes > kStreamBytes) {
-      steps == 1   ? run(lora_expand_kernel<1, 8, true, true>, 128)
-      : steps == 2 ? run(lora_expand_kernel<2, 8, true, true>, 128)
-      : steps == 3 ? run(lora_expand_kernel<3, 4, true, true>, 64)
-                   : run(lora_expand_kernel<4, 4, true, true>, 64);
+      steps == 1   ? run(lora_expand_kernel<1, 8, 4, true, true>, 128, 4)
+      : steps == 2 ? run(lora_expand_kernel<2, 8, 4, true, true>, 128, 4)
+      : steps == 3 ? run(lora_expand_kernel<3, 8, 4, true, true>, 128, 4)
+                   : run(lora_expand_kernel<4, 8, 4, true, true>, 128, 4);
+      return;
+    }
+    if (bytes > kManyBytes) {
+      steps == 1   ? run(lora_expand_kernel<1, 8, 4, true, false>, 128, 4)
+      : steps == 2 ? run(lora_expand_kernel<2, 8, 4, true, false>, 128, 4)
+      : steps == 3 ? run(lora_expand_kernel<3, 8, 4, true, false>, 128, 4)
+                   : run(lora_expand_kernel<4, 8, 4, true, false>, 128, 4);
       return;
     }
   }
-  steps == 1   ? run(lora_expand_kernel<1, 8, GROUPED, false>, 128)
-  : steps == 2 ? run(lora_expand_kernel<2, 4, GROUPED, false>, 64)
-  : steps == 3 ? run(lora_expand_kernel<3, 4, GROUPED, false>, 64)
-               : run(lora_expand_kernel<4, 4, GROUPED, false>, 64);
+  steps == 1   ? run(lora_expand_kernel<1, 8, 1, GROUPED, false>, 128, 1)
+  : steps == 2 ? run(lora_expand_kernel<2, 4, 1, GROUPED, false>, 64, 1)
+  : steps == 3 ? run(lora_expand_kernel<3, 4, 1, GROUPED, false>, 64, 1)
+               : run(lora_expand_kernel<4, 4, 1, GROUPED, false>, 64, 1);
 }
 
 static void launch_two(LoraArgs a, int slots, hipStream_t stream) {
@@ -827,14 +841,14 @@ static void launch_two(LoraArgs a, int slots, hipStream_t stream) {
   auto run = [&](auto* kernel, int columns) {
     a.blocks = 0;
     for (int i = 0; i < a.targets; ++i) a.blocks += (a.target[i].n + columns - 1) / columns;
-    hipLaunchKernelGGL(kernel, dim3(a.units * a.blocks, 1, slots), dim3(kExpandWaves * kWave), 0,
+    hipLaunchKernelGGL(kernel, dim3(a.units * a.blocks, 1, slots), dim3(kPartWaves * kWave), 0,
                        stream, a);
   };
   const int steps = rank_pitch(a.max_rank) / 32;
-  steps == 1   ? run(lora_expand_parts_kernel<1, 8>, 128 * kExpandWaves)
-  : steps == 2 ? run(lora_expand_parts_kernel<2, 4>, 64 * kExpandWaves)
-  : steps == 3 ? run(lora_expand_parts_kernel<3, 4>, 64 * kExpandWaves)
-               : run(lora_expand_parts_kernel<4, 4>, 64 * kExpandWaves);
+  steps == 1   ? run(lora_expand_parts_kernel<1, 8>, 128 * kPartWaves)
+  : steps == 2 ? run(lora_expand_parts_kernel<2, 4>, 64 * kPartWaves)
+  : steps == 3 ? run(lora_expand_parts_kernel<3, 4>, 64 * kPartWaves)
+               : run(lora_expand_parts_kernel<4, 4>, 64 * kPartWaves);
 }
 
 // The one launch's largest rank (64 spills registers: 64 x 896 x 896 16.3 us, in two launches

@@ -212,10 +212,10 @@ def test_thousands_of_tokens(batch, dev):
     check(out, s, 0)
 
 
+@pytest.mark.parametrize("tokens", [2301, 6001])
 @pytest.mark.parametrize("n,rank", [(9000, 8), (9001, 64), (8999, 72), (9008, 128)])
-def test_outputs_too_large_for_the_caches(batch, dev, n, rank):
-    """Beyond 192 MiB of bases and outputs; every 37th token is looked at."""
-    tokens = 6001
+def test_outputs_too_large_for_the_caches(batch, dev, n, rank, tokens):
+    """Beyond 70 and 192 MiB of bases and outputs; every 37th token is looked at."""
     s = make(tokens, 72, [n], rank, 5, n, runs=True)
     d, out = on(s, dev), torch.empty((tokens, n), dtype=torch.bfloat16, device=dev)
     batch.lora(d["x"], d["ids"], [(d["a"][0], d["b"][0], d["base"][0], out)],
