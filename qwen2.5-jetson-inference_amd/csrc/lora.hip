@@ -411,27 +411,27 @@ struct Words;
 template <>
 struct Words<8> {
   typedef u32x4 type;
+  typedef uint32_t memory __attribute__((ext_vector_type(4), aligned(2)));
 };
 template <>
 struct Words<4> {
   typedef uint32_t type __attribute__((ext_vector_type(2)));
+  typedef uint32_t memory __attribute__((ext_vector_type(2), aligned(2)));
 };
 
 template <int KS, int J, bool ONCE>
 struct Columns {
   typedef typename Words<J>::type words;
+  typedef typename Words<J>::memory memory;
   const LoraTarget& t;
   int n0, rank;
-  bool wide;  // whole, and aligned
+  bool whole;
   bf16x8_t w[KS][J];
 
   __device__ __forceinline__ Columns(const LoraArgs& a, const LoraTarget& target, int block,
                                      const Unit& u, int lane)
       : t(target), n0(block * J * 16 + J * (lane & 15)), rank(u.rank) {
-    wide = n0 + J <= t.n && (t.out_stride & 7) == 0 &&
-           (reinterpret_cast<uintptr_t>(t.out) & 15) == 0 &&
-           (!t.base ||
-            ((t.base_stride & 7) == 0 && (reinterpret_cast<uintptr_t>(t.base) & 15) == 0));
+    whole = n0 + J <= t.n;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       const int k = 32 * s + 8 * (lane >> 4);
@@ -459,9 +459,9 @@ struct Columns {
     }
   }
   __device__ __forceinline__ words base_of(int token) const {
-    if (!wide || !t.base) return words(0u);
-    const QLIN_GLOBAL words* p =
-        (const QLIN_GLOBAL words*)(t.base + token * t.base_stride + n0);
+    if (!whole || !t.base) return words(0u);
+    const QLIN_GLOBAL memory* p =
+        (const QLIN_GLOBAL memory*)(t.base + token * t.base_stride + n0);
     return ONCE ? __builtin_nontemporal_load(p) : *p;
   }
   __device__ __forceinline__ void multiply(f32x4_t (&sum)[J], const uint4 (&high)[KS],
@@ -481,16 +481,16 @@ struct Columns {
   // Row i of the sums is the token's.
   __device__ __forceinline__ void store(int token, const f32x4_t (&sum)[J], int i, words b) const {
     uint16_t* out = t.out + token * t.out_stride + n0;
-    if (wide) {
+    if (whole) {
       if (rank) {
 #pragma unroll
         for (int j = 0; j < J; j += 2) {
           b[j / 2] = pack2_bf16(bf16_lo(b[j / 2]) + sum[j][i], bf16_hi(b[j / 2]) + sum[j + 1][i]);
         }
       }
-      QLIN_GLOBAL words* p = (QLIN_GLOBAL words*)out;
+      QLIN_GLOBAL memory* p = (QLIN_GLOBAL memory*)out;
       if (ONCE) {
-        __builtin_nontemporal_store(b, p);
+        __builtin_nontemporal_store(memory(b), p);
       } else {
         *p = b;
       }
