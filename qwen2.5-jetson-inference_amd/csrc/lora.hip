@@ -765,10 +765,11 @@ size_t lora_workspace_bytes(int tokens, int max_rank, int targets) {
 
 // Bytes of bases and outputs beyond which four waves take 512 columns side by side, and beyond
 // which they are not left in the caches (6001 tokens by 8960, 215 MB, 67.1 -> 64.1 us; 3000 by
-// 2 x 4864, 117 MB, whose bases still are there, 31.6 -> 36.7).  Below, a wave is a workgroup, of
-// 64 columns beyond rank 32, that starts as soon as it finds room (2000 x 3584 x 3584 at rank
-// 128 43.6 us in fours, 37.3; 250 x 3584 x 3584 of 200 adapters 66.9, 64.6; but 3000 x 896 x 2 x
-// 4864 at rank 64 56.6 for 49.7, at rank 8 40.3 for 38.6).
+// 2 x 4864, 117 MB, whose bases still are there, 31.6 -> 36.7; 6001 by 8959, whose lines are
+// written in parts, 89 -> 102).  Below, a wave is a workgroup, of 64 columns beyond rank 32,
+// that starts as soon as it finds room (2000 x 3584 x 3584 at rank 128 43.6 us in fours, 37.3;
+// 250 x 3584 x 3584 of 200 adapters 66.9, 64.6; but 3000 x 896 x 2 x 4864 at rank 64 56.6 for
+// 49.7, at rank 8 40.3 for 38.6).
 constexpr long long kManyBytes = 70ll << 20;
 constexpr long long kStreamBytes = 192ll << 20;
 constexpr long long kMostThreads = (1ll << 32) - 1;  // of a launch, along x
@@ -778,7 +779,13 @@ static void launch_expand(LoraArgs a, int units, int slots, hipStream_t stream) 
   const int steps = rank_pitch(a.max_rank) / 32;
   const int sets = (a.tokens + kSet - 1) / kSet;
   long long bytes = 0;
-  for (int i = 0; i < a.targets; ++i) bytes += 4ll * a.tokens * a.target[i].n;
+  bool aligned = true;
+  for (int i = 0; i < a.targets; ++i) {
+    const LoraTarget& t = a.target[i];
+    bytes += 4ll * a.tokens * t.n;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(t.out) | reinterpret_cast<uintptr_t>(t.base);
+    aligned = aligned && (t.out_stride | t.base_stride) % 8 == 0 && at % 16 == 0;
+  }
   auto run = [&](auto* kernel, int columns, int waves) {
     long long all = 0;
     for (int i = 0; i < a.targets; ++i) all += (a.target[i].n + columns - 1) / columns;
@@ -792,7 +799,7 @@ static void launch_expand(LoraArgs a, int units, int slots, hipStream_t stream) 
                        dim3(waves * kWave), 0, stream, a);
   };
   if constexpr (GROUPED) {
-    if (bytes > kStreamBytes) {
+    if (bytes > kStreamBytes && aligned) {
       steps == 1   ? run(lora_expand_kernel<1, 8, 4, true, true>, 128, 4)
       : steps == 2 ? run(lora_expand_kernel<2, 8, 4, true, true>, 128, 4)
       : steps == 3 ? run(lora_expand_kernel<3, 8, 4, true, true>, 128, 4)

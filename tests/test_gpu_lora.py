@@ -213,7 +213,8 @@ def test_thousands_of_tokens(batch, dev):
 
 
 @pytest.mark.parametrize("tokens", [2301, 6001])
-@pytest.mark.parametrize("n,rank", [(9000, 8), (9001, 64), (8999, 72), (9008, 128)])
+@pytest.mark.parametrize("n,rank", [(9000, 8), (9001, 64), (8999, 72), (9008, 128), (9008, 64),
+                                    (9000, 72)])
 def test_outputs_too_large_for_the_caches(batch, dev, n, rank, tokens):
     """Beyond 70 and 192 MiB of bases and outputs; every 37th token is looked at."""
     s = make(tokens, 72, [n], rank, 5, n, runs=True)
