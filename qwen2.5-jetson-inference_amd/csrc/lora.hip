@@ -35,9 +35,7 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 // rank 8 6.7 of which 1.7 an empty launch, 33 tokens' q, k and v of 1536 at rank 16 7.8);
 // A x the same and a CU's loads (128 x 3584 by 2 x 64 rows 7.6; 6001 x 1536 by 32 8.6); B h
 // its bytes (128 x 2 x 18944 at rank 64 18.0 for 75 MB, 4.2 TB/s; 6001 x 8960 at rank 32
-// 46.4 for 216 MB, 4.7, a copy 5.07), from rank 64 on also h, which each wave reads (6001 x
-// 8960 at rank 64 69 with all of the call, at 128 113); grouping 3.2-4.7, a launch and LDS
-// atomics.
+// 45 for 216 MB, 4.8, a copy 5.07); grouping 3.2-4.7, a launch and LDS atomics.
 constexpr int kTile = 16;       // tokens, and rows of A
 constexpr int kGather = 256;    // tokens
 constexpr int kChunk = 1024;    // tokens grouped together beyond
@@ -517,37 +515,57 @@ __device__ __forceinline__ int target_of(const LoraArgs& a, int columns, int& bl
   return -1;
 }
 
+// Workgroups of several waves hold their unit's h in LDS, read once for all (6001 x 1536 x 8960
+// at rank 32 58.6 -> 57.2 us, at 128, where registers leave room for one more wave, 112 -> 90).
 template <int KS, int J, int WAVES, bool GROUPED, bool ONCE>
 __global__ __launch_bounds__(WAVES * kWave) void lora_expand_kernel(LoraArgs a) {
+  constexpr bool kShared = WAVES > 1;
+  constexpr int kWords = 64 * KS;  // of a token's h
   __shared__ int list[GROUPED ? kSet : kGather];
+  __shared__ __align__(16) uint16_t shared[kShared ? kSet : 1][kShared ? kWords + 8 : 8];
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int m = lane & 15, g = lane >> 4;
   // neighbouring workgroups have neighbouring columns, where they can be counted so
   const Unit u = tokens_of<GROUPED>(a, a.blocks ? blockIdx.x / a.blocks : blockIdx.x, list);
   if (u.count == 0) return;
-  int block = (a.blocks ? blockIdx.x % a.blocks : blockIdx.y) * WAVES + wave;
-  const int c = target_of(a, J * 16, block);
-  if (c < 0) return;
+  int block = a.blocks ? blockIdx.x % a.blocks : blockIdx.y;
+  const int c = target_of(a, WAVES * J * 16, block);
   const LoraTarget& t = a.target[c];
   if (u.adapter < 0 && t.base == t.out) return;
-  Columns<KS, J, ONCE> columns(a, t, block, u, lane);
-  const int rank = u.rank, pitch = rank_pitch(a.max_rank);
-  // A tile's h and bases are loaded while the one before it is computed.
+  const int rank = u.rank;
+  const uint16_t* const all_h = a.h + static_cast<size_t>(c) * a.tokens * kWords;
+  uint4 mine[kShared ? kSet * kWords / 8 / (WAVES * kWave) : 1];
+  if constexpr (kShared) {
+#pragma unroll
+    for (int i = 0; i < kSet * kWords / 8 / (WAVES * kWave); ++i) {
+      const int e = i * WAVES * kWave + threadIdx.x;
+      const int at = e / (kWords / 8), w = e % (kWords / 8) * 8;
+      mine[i] = make_uint4(0, 0, 0, 0);
+      if (at < u.count && w % (kWords / 2) < rank) {
+        mine[i] = load_global16(all_h + static_cast<size_t>(list[at]) * kWords + w);
+      }
+    }
+  }
+  block = block * WAVES + wave;
+  Columns<KS, J, ONCE> columns(a, t, block * J * 16 < t.n ? block : 0, u, lane);
+  // A tile's bases, and h, are loaded while the one before it is computed.
   struct Tile {
     uint4 high[KS], low[KS];
     typename Words<J>::type base[4];
   };
   auto load = [&](Tile& v, int tile) {
-    const int token = list[min(tile * kTile + m, u.count - 1)];
-    const uint16_t* h = a.h + (static_cast<size_t>(c) * a.tokens + token) * 2 * pitch;
+    if constexpr (!kShared) {
+      const uint16_t* h =
+          all_h + static_cast<size_t>(list[min(tile * kTile + m, u.count - 1)]) * kWords;
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const int k = 32 * s + 8 * g;
-      v.high[s] = v.low[s] = make_uint4(0, 0, 0, 0);
-      if (k < rank) {
-        v.high[s] = load_global16(h + k);
-        v.low[s] = load_global16(h + pitch + k);
+      for (int s = 0; s < KS; ++s) {
+        const int k = 32 * s + 8 * g;
+        v.high[s] = v.low[s] = make_uint4(0, 0, 0, 0);
+        if (k < rank) {
+          v.high[s] = load_global16(h + k);
+          v.low[s] = load_global16(h + kWords / 2 + k);
+        }
       }
     }
 #pragma unroll
@@ -560,10 +578,27 @@ __global__ __launch_bounds__(WAVES * kWave) void lora_expand_kernel(LoraArgs a) 
   if (tile * kTile >= u.count) return;
   Tile now, next;
   load(next, tile);
+  if constexpr (kShared) {
+#pragma unroll
+    for (int i = 0; i < kSet * kWords / 8 / (WAVES * kWave); ++i) {
+      const int e = i * WAVES * kWave + threadIdx.x;
+      *reinterpret_cast<uint4*>(&shared[e / (kWords / 8)][e % (kWords / 8) * 8]) = mine[i];
+    }
+    lds_barrier();
+    if (block * J * 16 >= t.n) return;
+  }
   columns.cut(lane);
   for (; tile * kTile < u.count; tile += step) {
     now = next;
     if ((tile + step) * kTile < u.count) load(next, tile + step);
+    if constexpr (kShared) {
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const uint16_t* h = &shared[tile * kTile + m][32 * s + 8 * g];
+        now.high[s] = *reinterpret_cast<const uint4*>(h);
+        now.low[s] = *reinterpret_cast<const uint4*>(h + kWords / 2);
+      }
+    }
     f32x4_t sum[J];
     columns.multiply(sum, now.high, now.low);
 #pragma unroll
@@ -787,9 +822,10 @@ static void launch_expand(LoraArgs a, int units, int slots, hipStream_t stream) 
     aligned = aligned && (t.out_stride | t.base_stride) % 8 == 0 && at % 16 == 0;
   }
   auto run = [&](auto* kernel, int columns, int waves) {
-    long long all = 0;
-    for (int i = 0; i < a.targets; ++i) all += (a.target[i].n + columns - 1) / columns;
-    const int blocks = static_cast<int>((all + waves - 1) / waves);
+    int blocks = 0;
+    for (int i = 0; i < a.targets; ++i) {
+      blocks += (a.target[i].n + columns * waves - 1) / (columns * waves);
+    }
     // a unit's four tiles side by side where there would be few workgroups
     const long long few = static_cast<long long>(sets) * blocks;
     const int z = !GROUPED ? slots : waves > 1 || few >= 1024 ? 1 : few >= 512 ? 2 : kSet / kTile;
