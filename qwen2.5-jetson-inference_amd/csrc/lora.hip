@@ -804,7 +804,7 @@ size_t lora_workspace_bytes(int tokens, int max_rank, int targets) {
 // written in parts, 89 -> 102).  Below, a wave is a workgroup, of 64 columns beyond rank 32,
 // that starts as soon as it finds room (2000 x 3584 x 3584 at rank 128 43.6 us in fours, 37.3;
 // 250 x 3584 x 3584 of 200 adapters 66.9, 64.6; but 3000 x 896 x 2 x 4864 at rank 64 56.6 for
-// 49.7, at rank 8 40.3 for 38.6).
+// 47.8, at rank 8 40.3 for 38.6).
 constexpr long long kManyBytes = 70ll << 20;
 constexpr long long kStreamBytes = 192ll << 20;
 constexpr long long kMostThreads = (1ll << 32) - 1;  // of a launch, along x
