@@ -102,7 +102,8 @@ int infer_hip_lora_bf16(const uint16_t* x, long long x_stride, const int* ids, i
  * vocab up to 2^20, rows up to 2^20, the workspace 16-byte aligned.  A row in which
  * two values or more have 32768 tokens each takes some 50 times as long (one may, as
  * a mask's does). */
-/* Bytes for calls of up to `rows` rows of `vocab` (0: refused shapes). */
+/* Bytes for calls of up to `rows` rows of `vocab` (0: refused shapes).  16 now,
+ * which nothing is written to: a row's state lies in its workgroup. */
 size_t infer_hip_sample_workspace_bytes(int rows, int vocab);
 int infer_hip_sample_bf16(const uint16_t* logits, long long stride, int rows, int vocab,
                           const float* temperature, const int* top_k, const float* top_p,

@@ -48,7 +48,6 @@ struct SampleArgs {
   const float* uniform;
   int* tokens;
   float* probabilities;
-  void* workspace;
 };
 
 size_t lora_workspace_bytes(int tokens, int max_rank, int targets);

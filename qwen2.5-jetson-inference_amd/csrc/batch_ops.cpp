@@ -139,7 +139,7 @@ extern "C" int infer_hip_sample_bf16(const uint16_t* logits, long long stride, i
                                  what);
   if (rc != INFER_HIP_OK) return rc;
   launch_sample(SampleArgs{logits, stride, rows, vocab, temperature, top_k, top_p, min_p, uniform,
-                           tokens, probabilities, workspace},
+                           tokens, probabilities},
                 stream);
   return check_launch(what);
 }
