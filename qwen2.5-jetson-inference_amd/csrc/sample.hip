@@ -525,7 +525,9 @@ struct RowSpan {
   }
 };
 
-// NR pieces of a thread, 512 apart, of those in [first, last).  Past them they are 0.
+// NR pieces of a thread, 512 apart, of those in [first, last).  Past them they are 0, by the
+// loads' own bounds check: a piece's place goes into their vector offset, which is sure to
+// be in it, also beyond the row.
 template <int NR>
 struct Pieces {
   u32x4 x[NR];
@@ -537,8 +539,8 @@ struct Pieces {
         const_cast<uint16_t*>(span.body), 0, 16 * last, 0x00020000);
 #pragma unroll
     for (int i = from; i < to && i < NR; ++i) {
-      x[i] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, 16 * threadIdx.x,
-                                                   16 * (first + i * kThreads), 0);
+      x[i] = __builtin_amdgcn_raw_buffer_load_b128(
+          rsrc, 16 * (first + i * kThreads + static_cast<int>(threadIdx.x)), 0, 0);
     }
   }
   // Piece i as a copy of its own, made here: what is computed of it is not computed
