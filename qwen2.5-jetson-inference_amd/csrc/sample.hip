@@ -603,7 +603,7 @@ struct Counting {
 
   template <int NR>
   __device__ __forceinline__ void add(Pieces<NR>& p, int first, int last) {
-    if (heavy.word == 0) {
+    if (heavy.word == 0 && heavy.count == 0) {  // zeros that were counted stay zeros
       unsigned most = 0;
 #pragma unroll
       for (int i = 0; i < kAhead && i < NR; ++i) most = max(most, largest(p.x[i]));
