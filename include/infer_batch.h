@@ -99,9 +99,10 @@ int infer_hip_lora_bf16(const uint16_t* x, long long x_stride, const int* ids, i
  * -1 and probability NaN.
  *
  * logits at least 2-byte aligned (rows that are 16-byte aligned are faster),
- * vocab up to 2^20, rows up to 2^20, the workspace 16-byte aligned.  A row in which
- * two values or more have 32768 tokens each takes some 50 times as long (one may, as
- * a mask's does). */
+ * vocab up to 2^20, rows up to 2^20, the workspace 16-byte aligned.  A row takes some 50
+ * times as long where 32768 tokens or more have one magnitude (both signs counted
+ * together), other than those of one value, a mask's: the lowest, or a low one that more
+ * tokens have than any below it. */
 /* Bytes for calls of up to `rows` rows of `vocab` (0: refused shapes).  16 now,
  * which nothing is written to: a row's state lies in its workgroup. */
 size_t infer_hip_sample_workspace_bytes(int rows, int vocab);

@@ -342,10 +342,11 @@ __device__ __forceinline__ void sample_by_bisection(const SampleArgs& a, int row
 
 // A workgroup counts a row's values in LDS.  Dword v & 0x7FFF counts the words of both
 // signs in 17 bits and those with the sign in the 15 above: its address and what is added
-// to it are two instructions from a shifted word.  Where one value has 32768 tokens or more,
-// which its total shows, the row is taken by bisection; but for one value, the row's
-// lowest as far as a wave has seen it (the largest word: that of a mask, as a rule), whose
-// tokens a wave counts in a register, as they would also meet at one address.
+// to it are two instructions from a shifted word.  Where 32768 tokens or more have one
+// magnitude, which a dword's total shows, the row is taken by bisection; but for those of
+// one value, a mask's: a low one, the row's lowest or one of more tokens than those below it,
+// as far as a wave has seen.  A wave counts them in a register, as they would also meet at one
+// address.
 //
 // Groups of 64 values are ordered from the largest down: 0 to 511 the positive ones,
 // 512 to 1023 the negative ones.  A group's values are equally far apart, so that its
@@ -566,18 +567,23 @@ struct Pieces {
 // The words of the pieces into the bins.  The first kAhead pieces are loaded before;
 // the others in the loop, so that counting begins while they are on their way (all of a
 // thread's loads at once wait for room: 256 rows of 151936 36 -> 30 us).  A piece in which
-// kHeavyLanes lanes of a wave or more have a word as low as the lowest of those kAhead is
-// left for later: it is read again, and its heavy words, a mask's, are counted in a
-// register.  A value of fewer lanes has at most 1 / 16 of the tokens.
-constexpr int kAhead = 6, kHeavyLanes = 5;
+// kHeavyLanes lanes of a wave or more have a word as low as the heavy one, a low one of
+// those kAhead, is left for later: it is read again, and its heavy words, a mask's, are
+// counted in a register.  A value of fewer lanes has at most 1 / 16 of the tokens.
+constexpr int kAhead = 6, kHeavyLanes = 5, kManyLanes = 16;
 struct Counting {
   const RowSpan& span;
   Heavy heavy{0u, 0u};  // of the wave
+  unsigned lead = 0;    // tokens that have it beyond those that were counted against it
 
   __device__ __forceinline__ static unsigned largest(const u32x4& x) {
     const uint32_t pair =
         larger_words(larger_words(x[0], x[1]), larger_words(x[2], x[3]));
     return max(pair & 0xFFFFu, pair >> 16);
+  }
+
+  __device__ __forceinline__ static uint32_t word_of(const u32x4& x, int j) {
+    return j & 1 ? x[j / 2] >> 16 : x[j / 2] & 0xFFFFu;
   }
 
   template <int NR, int I = 0>
@@ -607,7 +613,16 @@ struct Counting {
       unsigned most = 0;
 #pragma unroll
       for (int i = 0; i < kAhead && i < NR; ++i) most = max(most, largest(p.x[i]));
+      // the lowest, or where that is far below what many more lanes have, as -infinity in few
+      // places is below a mask, theirs
       heavy.word = lanes_max(most);
+      const unsigned some = min(min(at_lane(most, 0), at_lane(most, 21)), at_lane(most, 42));
+      if (heavy.word - some >= 256) {  // twice the exponent's step: ordinary rows end here
+        const int lanes = __popcll(__ballot(most == some));
+        if (lanes >= kManyLanes && lanes > __popcll(__ballot(most == heavy.word))) {
+          heavy.word = some;
+        }
+      }
     }
     unsigned long long later = 0;
     add_pieces(p, first, last, later);
@@ -618,18 +633,39 @@ struct Counting {
       const bool live = piece < last;
       const u32x4 x = live ? *(const QLIN_GLOBAL u32x4*)(span.body + 8ll * piece)
                            : u32x4{0, 0, 0, 0};
-      const unsigned most = lanes_max(largest(x));
-      if (most > heavy.word) {  // a lower value becomes the one that is counted here
-        if (heavy.count && (threadIdx.x & (kWave - 1)) == 0) add_word(heavy.word, heavy.count);
-        heavy = Heavy{most, 0u};
+      // The piece's lowest value, or the next if more lanes have that, takes the heavy one's
+      // place when more tokens have it than the heavy one leads by (a lower value alone did:
+      // 16 rows of 151936 at -10^4 but for 300 -infinities each took 1260 us, now 38).
+      const unsigned low = largest(x);
+      unsigned word = lanes_max(low);
+      const int lanes = __popcll(__ballot(low == word));
+      if (word != heavy.word || lanes < kWave / 2) {
+        const unsigned other = lanes_max(low == word ? 0u : low);
+        if (other && __popcll(__ballot(low == other)) > lanes) word = other;
+        if (word != heavy.word) {
+          unsigned n = 0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) n += __popcll(__ballot(live && word_of(x, j) == word));
+          if (n > lead) {
+            if (heavy.count && (threadIdx.x & (kWave - 1)) == 0) {
+              add_word(heavy.word, heavy.count);
+            }
+            heavy = Heavy{word, 0u};
+            lead = 0;
+          } else {
+            lead -= n;
+          }
+        }
       }
+      unsigned count = 0;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const uint32_t word = j & 1 ? x[j / 2] >> 16 : x[j / 2] & 0xFFFFu;
-        const bool is_heavy = word == heavy.word;
-        heavy.count += __popcll(__ballot(live && is_heavy));
-        if (live && !is_heavy) add_word(word, 1);
+        const bool is_heavy = word_of(x, j) == heavy.word;
+        count += __popcll(__ballot(live && is_heavy));
+        if (live && !is_heavy) add_word(word_of(x, j), 1);
       }
+      heavy.count += count;
+      lead += count;
     }
   }
 };
@@ -644,12 +680,15 @@ __device__ __forceinline__ void clear_bins(CountLds& lds) {
   if (threadIdx.x == 0) lds.total = lds.many = lds.nan = 0;
 }
 
-// One heavy value of `n` (up to 64) waves' or parts', from the lane that holds each; the
-// others go into the bins.
+// One heavy value of the waves', from the lane that holds each: the lowest of those of
+// which a wave has kManyHeavy tokens, or else of all.  The others go into the bins.
+constexpr unsigned kManyHeavy = 1024;
 __device__ __forceinline__ Heavy join_heavy(CountLds& lds, Heavy h, bool has, bool adds) {
-  const unsigned word = lanes_max(has && h.count ? h.word : 0u);
+  has = has && h.count;
+  const unsigned many = h.count >= kManyHeavy ? 0x10000u : 0u;
+  const unsigned word = lanes_max(has ? h.word | many : 0u) & 0xFFFFu;
   const bool same = has && h.word == word;
-  if (adds && has && !same && h.count) add_word(h.word, h.count);
+  if (adds && has && !same) add_word(h.word, h.count);
   return Heavy{word, wave_total(same ? h.count : 0u)};
 }
 
