@@ -387,17 +387,25 @@ struct CountLds {
   Lds bisect;
 };
 
-// The bins are the first of the workgroup's LDS, so that an offset is an address.
 typedef __attribute__((address_space(3))) unsigned LdsWord;
-__device__ __forceinline__ void add_shifted(uint32_t shifted, unsigned times) {
-  // `shifted` has the word's 16 bits from bit 2 on
-  const unsigned one = (shifted & (1u << kBinShift)) | 1u;
-  __hip_atomic_fetch_add((LdsWord*)static_cast<uintptr_t>(shifted & (4u * (kBins - 1))),
-                         one * times, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-}
-__device__ __forceinline__ void add_word(uint32_t word, unsigned times) {
-  add_shifted(word << 2, times);
-}
+typedef __attribute__((address_space(3))) char LdsByte;
+
+// The bins lie in static LDS: the compiler knows their address, so that a shifted word needs
+// no addition (of dynamic LDS it takes one a word).
+struct Bins {
+  LdsByte* first;
+
+  __device__ explicit Bins(unsigned* bins) : first((LdsByte*)bins) {}
+  // `shifted` has the word's 16 bits from bit 2 on.
+  __device__ __forceinline__ void add_shifted(uint32_t shifted, unsigned times) const {
+    const unsigned one = (shifted & (1u << kBinShift)) | 1u;
+    __hip_atomic_fetch_add((LdsWord*)(first + (shifted & (4u * (kBins - 1)))), one * times,
+                           __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+  }
+  __device__ __forceinline__ void add_word(uint32_t word, unsigned times) const {
+    add_shifted(word << 2, times);
+  }
+};
 
 __device__ __forceinline__ int key_of_lane(int group, int lane) {
   return 0xFFFF - (group * kWave + lane);
@@ -573,6 +581,7 @@ struct Pieces {
 constexpr int kAhead = 6, kHeavyLanes = 5, kManyLanes = 16;
 struct Counting {
   const RowSpan& span;
+  const Bins bins;
   Heavy heavy{0u, 0u};  // of the wave
   unsigned lead = 0;    // tokens that have it beyond those that were counted against it
 
@@ -598,8 +607,8 @@ struct Counting {
         } else if (first + I * kThreads + static_cast<int>(threadIdx.x) < last) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            add_shifted(x[j] << 2, 1);
-            add_shifted(x[j] >> 14, 1);
+            bins.add_shifted(x[j] << 2, 1);
+            bins.add_shifted(x[j] >> 14, 1);
           }
         }
       }
@@ -648,7 +657,7 @@ struct Counting {
           for (int j = 0; j < 8; ++j) n += __popcll(__ballot(live && word_of(x, j) == word));
           if (n > lead) {
             if (heavy.count && (threadIdx.x & (kWave - 1)) == 0) {
-              add_word(heavy.word, heavy.count);
+              bins.add_word(heavy.word, heavy.count);
             }
             heavy = Heavy{word, 0u};
             lead = 0;
@@ -662,7 +671,7 @@ struct Counting {
       for (int j = 0; j < 8; ++j) {
         const bool is_heavy = word_of(x, j) == heavy.word;
         count += __popcll(__ballot(live && is_heavy));
-        if (live && !is_heavy) add_word(word_of(x, j), 1);
+        if (live && !is_heavy) bins.add_word(word_of(x, j), 1);
       }
       heavy.count += count;
       lead += count;
@@ -688,7 +697,7 @@ __device__ __forceinline__ Heavy join_heavy(CountLds& lds, Heavy h, bool has, bo
   const unsigned many = h.count >= kManyHeavy ? 0x10000u : 0u;
   const unsigned word = lanes_max(has ? h.word | many : 0u) & 0xFFFFu;
   const bool same = has && h.word == word;
-  if (adds && has && !same) add_word(h.word, h.count);
+  if (adds && has && !same) Bins(lds.bins).add_word(h.word, h.count);
   return Heavy{word, wave_total(same ? h.count : 0u)};
 }
 
@@ -971,8 +980,7 @@ __device__ __forceinline__ bool locate(const SampleArgs& a, int row, const RowSp
 // NR: pieces a thread takes at a time; HELD: that is the row, kept in registers.
 template <int NR, bool HELD>
 __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
-  extern __shared__ __align__(16) char shared[];
-  CountLds& lds = *reinterpret_cast<CountLds*>(shared);
+  __shared__ __align__(16) CountLds lds;
   const int row = blockIdx.x, lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const RowSpan span(a.logits + row * a.stride, a.vocab);
@@ -986,12 +994,13 @@ __global__ __launch_bounds__(kThreads) void sample_kernel(SampleArgs a) {
   const bool has_edge = span.edge(lane, edge_word, edge_index);
   lds_barrier();
 
-  Counting counting{span};
+  const Bins bins(lds.bins);
+  Counting counting{span, bins};
   for (int base = 0; base < span.pieces; base += kStep) {
     if (!HELD && base) p.template load<0, kAhead>(span, base, span.pieces);
     counting.add(p, base, span.pieces);
   }
-  if (wave == 0 && has_edge) add_word(edge_word, 1);
+  if (wave == 0 && has_edge) bins.add_word(edge_word, 1);
   if (lane == 0) lds.heavy[wave] = counting.heavy;
   lds_barrier();
   const Heavy heavy = join_heavy(lds, lds.heavy[lane & (kWaves - 1)], lane < kWaves, wave == 0);
@@ -1039,7 +1048,7 @@ size_t sample_workspace_bytes(int rows, int vocab) {
 void launch_sample(const SampleArgs& a, hipStream_t stream) {
   const int pieces = (a.vocab + 7) / 8, each = (pieces + kThreads - 1) / kThreads;
   auto run = [&](auto* kernel) {
-    hipLaunchKernelGGL(kernel, dim3(a.rows), dim3(kThreads), sizeof(CountLds), stream, a);
+    hipLaunchKernelGGL(kernel, dim3(a.rows), dim3(kThreads), 0, stream, a);
   };
   each <= 2    ? run(sample_kernel<2, true>)
   : each <= 4  ? run(sample_kernel<4, true>)

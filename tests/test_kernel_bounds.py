@@ -30,3 +30,14 @@ def test_a_rows_pieces_are_bounded_by_the_vector_offset():
     for at in calls:
         _, vector, scalar, _ = arguments(text, at)
         assert scalar == "0" and "threadIdx.x" in vector and "first" in vector
+
+
+def test_no_lds_address_is_made_from_a_number():
+    """The bins of sampling's counts are reached from the object that they lie in, wherever
+    the compiler puts that, and not as the first bytes of the workgroup's LDS."""
+    text = open(os.path.join(CSRC, "sample.hip")).read()
+    names = re.findall(r"address_space\(3\)\)\)[\w ]*?(\w+);", text)
+    assert names
+    for name in names:
+        assert not re.search(rf"\({name}\s*\*\)\s*(static_cast<uintptr_t>|\d|\(uintptr_t\))", text)
+        assert not re.search(rf"reinterpret_cast<{name}\s*\*>\(\s*(static_cast<uintptr_t>|\d)", text)
