@@ -312,9 +312,11 @@ __device__ __forceinline__ float joined(const Stage<RT>& stage, int e) {
 __device__ __forceinline__ int row_of(int e) { return e / 256 * kTile + e / 64 % 4 * 4 + e % 4; }
 __device__ __forceinline__ int token_of(int e) { return e / 4 % 16; }
 
-// h as high + low BF16; an infinity has no remainder.
+// h as high + low BF16; an infinity has no remainder, and where h rounds to one the largest
+// number is high.
 __device__ __forceinline__ void split_word(float h, uint16_t& high, uint16_t& low) {
   high = f32_to_bf16(h);
+  if ((high & 0x7FFFu) == 0x7F80u && fabsf(h) < INFINITY) --high;
   low = (high & 0x7F80u) == 0x7F80u ? 0 : f32_to_bf16(h - bf16_to_f32(high));
 }
 
