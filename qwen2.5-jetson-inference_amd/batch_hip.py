@@ -15,7 +15,7 @@ import struct
 import torch
 
 import linear_hip
-from linear_hip import INVALID_ARGUMENT, InferError, _check, _flat, _here
+from linear_hip import INVALID_ARGUMENT, InferError, _check, _flat, _here, _too_large
 
 # Every symbol include/infer_batch.h declares.
 EXPORTED_SYMBOLS = (
@@ -99,9 +99,10 @@ def lora(x, ids, targets, workspace, ranks=None, scales=None, stream=None) -> No
     if len(shape) != 3 or shape[2] != k:
         _bad(f"a must be [adapters, max_rank, {k}] (got {list(shape)})")
     adapters, rank = shape[0], shape[1]
-    made = []
+    made, sizes = [], tokens | k | adapters
     for a, b, base, output in targets:
         n = output.shape[-1]
+        sizes |= n
         # contiguous, as a rule: looked at without a call for each
         if (base is not None and a.dtype is _BF16 and a.get_device() == index and a.shape == shape
                 and a.is_contiguous() and b.dtype is _BF16 and b.get_device() == index
@@ -119,6 +120,8 @@ def lora(x, ids, targets, workspace, ranks=None, scales=None, stream=None) -> No
         bp, bs = (0, 0) if base is None else _rows(base, tokens, n, index, "base")
         made += (_flat(a, _BF16, None, index, "a"), _flat(b, _BF16, None, index, "b"), bp, op, n,
                  bs, os_)
+    if sizes >> 31:  # ctypes would pass the low half
+        _too_large("lora")
     status = load().infer_hip_lora_bf16(
         xp, xs, _flat(ids, _I32, tokens, index, "ids"), tokens, k, _PACK[len(targets)](*made),
         len(targets), adapters, rank,
@@ -145,6 +148,8 @@ def sample(logits, uniform, tokens, workspace, temperature=None, top_k=None, top
         _bad(f"logits must be [rows, vocab] (got {list(logits.shape)})")
     rows, vocab = logits.shape
     lp, stride = _rows(logits, rows, vocab, index, "logits")
+    if (rows | vocab) >> 31:  # ctypes would pass the low half
+        _too_large("sample")
 
     def setting(t, dtype, name):
         return None if t is None else _flat(t, dtype, rows, index, name)

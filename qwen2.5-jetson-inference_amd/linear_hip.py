@@ -251,6 +251,10 @@ def _here(t, name, stream):
     return index, _stream(stream)
 
 
+def _too_large(what):
+    raise InferError(INVALID_ARGUMENT, f"{what}: a size of 2^31 or more")
+
+
 def _check(status: int) -> None:
     if status != OK:
         msg = load().infer_hip_last_error().decode("utf-8", "replace")

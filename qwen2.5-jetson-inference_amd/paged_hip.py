@@ -14,7 +14,7 @@ import ctypes
 import torch
 
 import linear_hip
-from linear_hip import INVALID_ARGUMENT, InferError, _check, _flat, _here, _stream
+from linear_hip import INVALID_ARGUMENT, InferError, _check, _flat, _here, _stream, _too_large
 
 # Every symbol include/infer_paged.h declares.
 EXPORTED_SYMBOLS = (
@@ -302,8 +302,11 @@ def kv_pages_assign(table, page_size: int, free, free_count, lengths, added, wor
                                (lengths_out, n, "lengths_out"), (positions, None, "positions"),
                                (free, None, "free")):
             _flat(t, _I32, count, index, name)
+    pool = free.numel()
+    if (n | width | stride | pool | tokens) >> 31:  # ctypes would pass the low half
+        _too_large("kv_pages_assign")
     status = load().infer_hip_kv_pages_assign(
-        tp, n, width, stride, page_size, free.data_ptr(), free.numel(),
+        tp, n, width, stride, page_size, free.data_ptr(), pool,
         _flat(free_count, _I32, 1, index, "free_count"),
         _flat(free_count_out, _I32, 1, index, "free_count_out"), lengths.data_ptr(),
         added.data_ptr(), lengths_out.data_ptr(), tokens, positions.data_ptr(),
@@ -335,8 +338,11 @@ def kv_pages_release(table, page_size: int, free, free_count, lengths, finished,
         for t, count, name in ((lengths, n, "lengths"), (finished, n, "finished"),
                                (lengths_out, n, "lengths_out"), (free, None, "free")):
             _flat(t, _I32, count, index, name)
+    pool = free.numel()
+    if (n | width | stride | pool) >> 31:
+        _too_large("kv_pages_release")
     status = load().infer_hip_kv_pages_release(
-        tp, n, width, stride, page_size, free.data_ptr(), free.numel(),
+        tp, n, width, stride, page_size, free.data_ptr(), pool,
         _flat(free_count, _I32, 1, index, "free_count"),
         _flat(free_count_out, _I32, 1, index, "free_count_out"), lengths.data_ptr(),
         finished.data_ptr(), lengths_out.data_ptr(),
