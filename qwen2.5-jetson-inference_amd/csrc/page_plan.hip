@@ -294,73 +294,64 @@ __device__ __forceinline__ unsigned ended_pages(const ReleaseArgs& a, int s, int
              static_cast<unsigned>(p.max_pages));
 }
 
-// Sequence s's pages to the entries down from `top`.
-__device__ __forceinline__ void give_back(const ReleaseArgs& a, int s, int pages, int top) {
+// Sequence s's pages to the entries above `above`, the unused ones and the pages that go
+// back after its own, its last page first.  Such a sum is right, or so large that its
+// entries lie past the list.
+__device__ __forceinline__ void give_back(const ReleaseArgs& a, int s, int pages,
+                                          unsigned above) {
   const PagePlan& p = a.plan;
+  const int top = static_cast<int>(add_sat(above, pages)) - 1;
   const int* row = p.table + static_cast<size_t>(s) * p.stride;
   for (int i = threadIdx.x; i < pages; i += blockDim.x) {
     const int place = top - i;
-    if (place >= 0 && place < p.num_pages) a.free_pages[place] = row[i];
+    if (place < p.num_pages) a.free_pages[place] = row[i];
   }
 }
 
 // Up to kReleaseHere sequences, nothing in place: a workgroup of each adds up the pages
-// that go back before its own, and all of them.  Otherwise one workgroup writes each
-// sequence's place into the workspace, and a second launch copies.
+// that go back after its own, the first's so all of them.  Otherwise one workgroup writes
+// each sequence's place into the workspace, and a second launch copies.
 //
 // Bound: as above; 64 sequences 2.4 us, 750 000 pages of 1350 sequences 5.0 for 6 MB.
 constexpr int kReleaseHere = 4096;
 
 __global__ __launch_bounds__(256) void release_kernel(ReleaseArgs a) {
   constexpr int kWaves = 256 / kWave;
-  __shared__ unsigned before_wave[kWaves], all_wave[kWaves];
+  __shared__ unsigned after_wave[kWaves];
   const PagePlan& p = a.plan;
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave, s = blockIdx.x;
   const int length = p.lengths[s];
   const unsigned mine = ended_pages(a, s, length);
-  unsigned before = 0, all = 0;
-  if (mine || s == 0) {
-    for (int i = threadIdx.x; i < p.sequences; i += 256) {
-      const unsigned pages = ended_pages(a, i, p.lengths[i]);
-      all = add_sat(all, pages);
-      if (i < s) before = add_sat(before, pages);
-    }
-    before = scan_sat(before);
-    all = scan_sat(all);
-    if (lane == kWave - 1) {
-      before_wave[wave] = before;
-      all_wave[wave] = all;
-    }
-  }
   if (threadIdx.x == 0) p.lengths_out[s] = a.finished[s] ? 0 : length;
   if (!mine && s) return;  // the same in all threads
+  unsigned after = 0;
+  for (int i = s + 1 + threadIdx.x; i < p.sequences; i += 256) {
+    after = add_sat(after, ended_pages(a, i, p.lengths[i]));
+  }
+  after = scan_sat(after);
+  if (lane == kWave - 1) after_wave[wave] = after;
   __syncthreads();
-  before = all = 0;
-  for (int i = 0; i < kWaves; ++i) {
-    before = add_sat(before, before_wave[i]);
-    all = add_sat(all, all_wave[i]);
-  }
-  const unsigned end = add_sat(unused_pages(p), all);
+  unsigned above = unused_pages(p);
+  for (int i = 0; i < kWaves; ++i) above = add_sat(above, after_wave[i]);
   if (s == 0 && threadIdx.x == 0) {
-    *p.free_count_out = min(end, static_cast<unsigned>(p.num_pages));
+    *p.free_count_out = min(add_sat(above, mine), static_cast<unsigned>(p.num_pages));
   }
-  give_back(a, s, mine, static_cast<int>(end) - 1 - static_cast<int>(before));
+  give_back(a, s, mine, above);
 }
 
-// Where the pages of each ended sequence go: share.first[s] pages lie before its first one,
-// share.held[s] how many there are, share.starts[0] where the places end.
+// Where the pages of each ended sequence go: share.first[s] entries lie below its last one,
+// share.held[s] how many there are.  From the last sequence down.
 __global__ __launch_bounds__(kWide) void release_scan_kernel(ReleaseArgs a, int* workspace) {
   __shared__ ScanLds lds;
   const PagePlan& p = a.plan;
   const Share share = share_of(workspace, p.sequences);
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int count = unused_pages(p);
-  unsigned before = 0;
+  unsigned below = unused_pages(p);
   for (int base = 0; base < p.sequences; base += kWide) {
-    const int s = base + threadIdx.x;
+    const int s = p.sequences - 1 - base - static_cast<int>(threadIdx.x);
     unsigned pages = 0;
-    if (s < p.sequences) {
+    if (s >= 0) {
       const int length = p.lengths[s];
       pages = ended_pages(a, s, length);
       p.lengths_out[s] = a.finished[s] ? 0 : length;
@@ -368,28 +359,24 @@ __global__ __launch_bounds__(kWide) void release_scan_kernel(ReleaseArgs a, int*
     const unsigned in = scan_sat(pages);
     if (lane == kWave - 1) lds.need[wave] = in;
     __syncthreads();
-    const SumPair sums = sums_before(lds.need, wave, kWide / kWave, before);
+    const SumPair sums = sums_before(lds.need, wave, kWide / kWave, below);
     const unsigned mine = sums.before;
     unsigned first = __shfl_up(in, 1);
     first = lane ? add_sat(mine, first) : mine;
-    if (s < p.sequences) {
+    if (s >= 0) {
       share.held[s] = pages;
       share.first[s] = first;
     }
-    before = sums.all;
+    below = sums.all;
     __syncthreads();
   }
-  if (threadIdx.x == 0) {
-    const unsigned end = add_sat(count, before);
-    share.starts[0] = end;
-    *p.free_count_out = min(end, static_cast<unsigned>(p.num_pages));
-  }
+  if (threadIdx.x == 0) *p.free_count_out = min(below, static_cast<unsigned>(p.num_pages));
 }
 
 __global__ __launch_bounds__(256) void release_copy_kernel(ReleaseArgs a, int* workspace) {
   const Share share = share_of(workspace, a.plan.sequences);
   const int s = blockIdx.x;
-  give_back(a, s, share.held[s], share.starts[0] - 1 - share.first[s]);
+  give_back(a, s, share.held[s], share.first[s]);
 }
 
 }  // namespace
