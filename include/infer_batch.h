@@ -52,9 +52,9 @@ extern "C" {
  * faster.
  *
  * A[i] x[t] times the scale is kept as the sum of two BF16 numbers (a relative
- * 2^-16) between the products.  An infinite element of B gives an infinity or
- * NaN in its row of the tokens with that adapter, and no other.  Results do not
- * change from run to run. */
+ * 2^-16, up to FP32's largest number) between the products.  An infinite element of
+ * B gives an infinity or NaN in its row of the tokens with that adapter, and no
+ * other.  Results do not change from run to run. */
 #define INFER_HIP_LORA_TARGETS 3
 
 typedef struct infer_hip_lora_target {

@@ -215,7 +215,7 @@ struct Lds {
 };
 
 // A row that is read again for every question, 16 passes a border: 16 rows of 151936 that
-// have two values with half of the tokens each 1880 us, where the count takes 21 to 116.
+// have two values with half of the tokens each 1880 us, where the count takes 21 to 111.
 struct ReadRow {
   const uint16_t* logits;
   int vocab;
@@ -358,7 +358,7 @@ __device__ __forceinline__ void sample_by_bisection(const SampleArgs& a, int row
 // cycles of a row of 151936 (19.9 us with a launch) the count takes 22000, 8 LDS additions a
 // 16-byte piece at some 8 cycles a wave; the groups' sums 7000; the questions, one wave's
 // dependent 64-bit steps, 6000; the token's place 5000-7000 over the row in registers.  256
-// such rows take 26.5 us (78 MB, 2.9 TB/s), 17 of 32003 12.7, of which the counts are 5000
+// such rows take 26.2 us (78 MB, 3.0 TB/s), 17 of 32003 12.7, of which the counts are 5000
 // cycles.  Parts of a row counted by several workgroups need a launch to add them up: 1 x
 // 151936 24.7 us, 1 x 40000 22 for 12.4.  512 threads, so that the row stays in registers
 // beside the work.

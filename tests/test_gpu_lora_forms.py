@@ -44,7 +44,8 @@ def make(tokens, k, outs, rank, adapters, seed, runs=False):
 def exact(s, i, rows=slice(None), base=True):
     """Target i's output for those tokens, rounded once."""
     x, ids = s["x"][rows].double(), s["ids"][rows]
-    out = s["base"][i][rows].double() if base else torch.zeros((len(x), s["b"][i].shape[1])).double()
+    zeros = torch.zeros((len(x), s["b"][i].shape[1]), dtype=torch.float64)
+    out = s["base"][i][rows].double() if base else zeros
     for j in set(ids.tolist()) - {-1}:
         mine = (ids == j).nonzero()[:, 0]
         h = x[mine] @ s["a"][i][j].double().t()
@@ -68,7 +69,8 @@ FORMS = [
     (6000, 264, [700], 16, 3), (9000, 264, [520, 520], 40, 7)]
 # beyond 70 and 192 MiB of bases and outputs, rows of both alignments
 LARGE = [(2301, 1544, [9000], 32, 5), (2301, 1544, [8999], 72, 5), (6001, 1536, [8960], 32, 6),
-         (6001, 1536, [8959], 32, 6), (6001, 1544, [9008], 128, 4), (6001, 264, [4500, 4600], 64, 3)]
+         (6001, 1536, [8959], 32, 6), (6001, 1544, [9008], 128, 4),
+         (6001, 264, [4500, 4600], 64, 3)]
 
 
 @pytest.mark.parametrize("where", ["apart", "in place", "no base"])

@@ -39,5 +39,5 @@ def test_no_lds_address_is_made_from_a_number():
     names = re.findall(r"address_space\(3\)\)\)[\w ]*?(\w+);", text)
     assert names
     for name in names:
-        assert not re.search(rf"\({name}\s*\*\)\s*(static_cast<uintptr_t>|\d|\(uintptr_t\))", text)
-        assert not re.search(rf"reinterpret_cast<{name}\s*\*>\(\s*(static_cast<uintptr_t>|\d)", text)
+        cast = rf"(\({name}\s*\*\)|reinterpret_cast<{name}\s*\*>\()\s*"
+        assert not re.search(cast + r"(static_cast<uintptr_t>|\(uintptr_t\)|\d)", text)
