@@ -309,8 +309,8 @@ __device__ __forceinline__ void give_back(const ReleaseArgs& a, int s, int pages
 }
 
 // Up to kReleaseHere sequences, nothing in place: a workgroup of each adds up the pages
-// that go back after its own, the first's so all of them.  Otherwise one workgroup writes
-// each sequence's place into the workspace, and a second launch copies.
+// that go back after its own; the first sequence's has the whole count so.  Otherwise one
+// workgroup writes each sequence's place into the workspace, and a second launch copies.
 //
 // Bound: as above; 64 sequences 2.4 us, 860 000 pages of 1350 sequences 3.9 for 6.9 MB.
 constexpr int kReleaseHere = 4096;
